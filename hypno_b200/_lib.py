@@ -53,6 +53,48 @@ class HcConfig(ctypes.Structure):
     ]
 
 
+class HcPagedKV(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_page_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("k_pos_stride", ctypes.c_int64),
+        ("v_page_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("v_pos_stride", ctypes.c_int64),
+        ("kv_dtype", ctypes.c_int32),
+        ("n_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class HcPagedBatch(ctypes.Structure):
+    _fields_ = [
+        ("block_table", ctypes.c_void_p),
+        ("q_start", ctypes.c_void_p),
+        ("kv_len", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("n_seqs", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("n_rows", ctypes.c_int32),
+        ("max_q_len", ctypes.c_int32),
+        ("max_kv_len", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class HcRows(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("row_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
 _U8P = ctypes.POINTER(ctypes.c_uint8)
@@ -101,6 +143,11 @@ SIGNATURES = {
     "hc_phase_count": (_I, []),
     "hc_sample_dev": (_I, [_P, _SZ, _I, _I, _P, _P, _P, _P, _P, _P]),
     "hc_argmax_dev": (_I, [_P, _SZ, _I, _I, _I, _P, _P, _P]),
+    "hc_sample_uniform_dev": (_I, [_P, _SZ, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "hc_paged_append_dev": (_I, [_P, _P, HcRows, HcRows, HcRows, HcRows, _I, _U32, _P, _I, _I, _I, _P]),
+    "hc_paged_attention_workspace": (_I, [_P, _P, _I, _U32, _I, ctypes.POINTER(_SZ)]),
+    "hc_paged_attention_dev": (_I, [_P, _P, HcRows, HcRows, _P, _I, _U32, _F, _I, _P, _SZ, _P]),
+    "hc_rope_table_host": (_I, [_SZ, _SZ, _F, _P]),
     "hc_phase_name": (ctypes.c_char_p, [_I]),
     "hc_comm_unique_id": (_I, [_P]),
     "hc_comm_init": (_I, [_P, _P, _I, _I, ctypes.c_double]),

@@ -1,0 +1,99 @@
+// Paged KV cache: arguments and device helpers shared by the append kernel
+// and the attention kernels (hc_paged.cu, hc_paged_split.cu, hc_paged_tc.cu).
+#pragma once
+
+#include "hc_common.cuh"
+#include "hc_internal.h"
+
+namespace hc {
+
+// The pool of one layer and the step's batch, as the kernels take them.
+struct PagedArgs {
+    void* k;
+    void* v;
+    int64_t kps, khs, kss;  // page / head / position strides of k, in elements
+    int64_t vps, vhs, vss;
+    const int32_t* table;
+    const int32_t* q_start;
+    const int32_t* kv_len;
+    int64_t table_stride;
+    int n_pages, page_size, page_shift;  // page_shift >= 0: page_size = 1 << page_shift
+    int nkv, hd;
+    int n_seqs, max_pages, n_rows;
+};
+
+struct PagedAttnArgs {
+    PagedArgs p;
+    const void* q;
+    void* out;
+    int64_t q_rs, q_hs, o_rs, o_hs;  // row / head strides, in elements
+    float* lse;                      // [n_rows][nh], may be null
+    int nh, G;                       // query heads, query heads per KV head
+    int window;                      // > 0: only the last `window` positions
+    float scale;
+    int qvec, ovec;                  // 16-byte aligned rows of q / out
+};
+
+__device__ __forceinline__ int page_of(const PagedArgs& P, int pos) {
+    return P.page_shift >= 0 ? (pos >> P.page_shift) : pos / P.page_size;
+}
+
+// Page of position pos (>= 0) of sequence seq, -1 for a hole; slot = the
+// position's place in it.
+__device__ __forceinline__ int lookup(const PagedArgs& P, int seq, int pos, int& slot) {
+    const int i = page_of(P, pos);
+    slot = pos - i * P.page_size;
+    if (i >= P.max_pages) return -1;
+    const int g = __ldg(P.table + (int64_t)seq * P.table_stride + i);
+    return (unsigned)g < (unsigned)P.n_pages ? g : -1;
+}
+
+// Rows [r0, r1) of sequence b, held to the packed rows that exist.
+__device__ __forceinline__ void seq_rows(const PagedArgs& P, int b, int& r0, int& r1) {
+    r0 = min(max(__ldg(P.q_start + b), 0), P.n_rows);
+    r1 = min(max(__ldg(P.q_start + b + 1), r0), P.n_rows);
+}
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// The tile-th tile of BM packed (token, query head of the group) rows, over
+// the sequences in order; executed by a whole warp.  Returns false past the
+// last tile.
+__device__ __forceinline__ bool find_tile(const PagedArgs& P, int G, int BM, int tile, int& seq, int& in_seq) {
+    const int lane = threadIdx.x & 31;
+    int base = 0;
+    for (int b0 = 0; b0 < P.n_seqs; b0 += 32) {
+        int n = 0;
+        if (b0 + lane < P.n_seqs) {
+            int r0, r1;
+            seq_rows(P, b0 + lane, r0, r1);
+            n = (int)(((int64_t)(r1 - r0) * G + BM - 1) / BM);
+        }
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += t;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, base + incl > tile);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            seq = b0 + l;
+            in_seq = tile - base - (__shfl_sync(0xffffffffu, incl, l) - __shfl_sync(0xffffffffu, n, l));
+            return true;
+        }
+        base += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return false;
+}
+
+int launch_paged_generic(const PagedAttnArgs& A, int q16, int c16, cudaStream_t s);
+
+}  // namespace hc

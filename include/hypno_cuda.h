@@ -238,6 +238,101 @@ int hc_sample_dev(const float* logits_dev, size_t ld, int B, int V, const float*
 int hc_argmax_dev(const float* logits_dev, size_t ld, int B, int V, int shards, float* pairs_dev, uint32_t* out_dev,
                   void* stream);
 
+/* The next token of B rows of device logits (row stride ld floats, V entries
+ * each) from the caller's uniform numbers; no counterpart in the reference
+ * (hc_sample_dev is its sampler).  Tokens are ordered by logit, largest first,
+ * equal ones by index; NaN counts as -inf.  With w = exp((l - max) / T), held
+ * as a whole multiple of 2^-40 so that every sum is exact in any order, a row
+ * keeps the first top_k tokens (0 or less: all), of these every token with
+ * less than top_p of their mass before it (1 or more: all), of these the ones
+ * with w >= min_p (0: all); the first token is always kept.  A temperature
+ * that is not above 0 keeps the first token alone.  out_dev[b] is the first
+ * kept index at which the running mass, by index, exceeds
+ * floor(u * kept mass), and logprob_dev[b] (may be NULL) the log of its share
+ * of the kept mass; a row without a logit above -inf gives -1 and -inf.
+ * u (in [0, 1)), temperature, top_k, top_p and min_p are device arrays of B.
+ * V <= 2^22.  Stream-ordered, no synchronization, no scratch. */
+int hc_sample_uniform_dev(const float* logits_dev, size_t ld, int B, int V, const float* u_dev,
+                          const float* temperature_dev, const int* top_k_dev, const float* top_p_dev,
+                          const float* min_p_dev, int32_t* out_dev, float* logprob_dev, void* stream);
+
+/* ---- paged KV cache (no counterpart in the reference) -------------------- */
+
+/* One layer's pool of pages.  Position s of page g of KV head h lies at
+ * k + g * k_page_stride + h * k_head_stride + s * k_pos_stride (elements; the
+ * head_dim elements of a position are contiguous); v likewise. */
+typedef struct hc_paged_kv {
+    void* k;
+    void* v;
+    int64_t k_page_stride, k_head_stride, k_pos_stride;
+    int64_t v_page_stride, v_head_stride, v_pos_stride;
+    int32_t kv_dtype; /* HC_KV_FP32 or HC_KV_FP16 */
+    int32_t n_pages, page_size, n_kv_heads, head_dim;
+    int32_t reserved;
+} hc_paged_kv;
+
+/* The new tokens of a step, packed: sequence b owns the rows q_start[b] ..
+ * q_start[b + 1] - 1 (q_start[0] = 0, non-decreasing, q_start[n_seqs] =
+ * n_rows), and its kv_len[b] positions end with them, so its i-th row stands
+ * at position kv_len[b] - (q_start[b + 1] - q_start[b]) + i.  Position p of
+ * sequence b lives in page block_table[b * table_stride + p / page_size]; an
+ * entry outside [0, n_pages) and a position beyond max_pages * page_size is a
+ * hole.  All arrays are device memory.  max_q_len and max_kv_len are the
+ * caller's upper bounds on the rows and positions of a sequence; they choose
+ * launches and hold off no work (a larger sequence is served all the same,
+ * more slowly). */
+typedef struct hc_paged_batch {
+    const int32_t* block_table;
+    const int32_t* q_start;
+    const int32_t* kv_len;
+    int64_t table_stride;
+    int32_t n_seqs, max_pages, n_rows, max_q_len, max_kv_len;
+    int32_t reserved;
+} hc_paged_batch;
+
+/* Rows of heads in device memory: head h of row r at
+ * data + r * row_stride + h * head_stride (elements; head_dim contiguous). */
+typedef struct hc_rows {
+    void* data;
+    int64_t row_stride, head_stride;
+} hc_rows;
+
+/* Writes the new tokens' keys and values into their pages and rotates keys
+ * and queries on the way: with (c, s) = rope[p][j] (rope_rows x rot_dim / 2
+ * pairs of floats; NULL: no rotation), pair j of the first rot_dim elements
+ * becomes (a c - b s, a s + b c); half_pairs 0: (a, b) = elements (2j, 2j + 1),
+ * the reference's pairs (transformer.rs:317-343); 1: elements
+ * (j, j + rot_dim / 2).  q (n_heads heads per row; q.data NULL: none) goes to
+ * q_out, which may be q itself.  q, k, v and q_out are `dtype`
+ * (HC_DTYPE_FP32 or HC_DTYPE_FP16); arithmetic is f32, rounded once.  A row at
+ * a hole stores nothing.  A position at or past rope_rows is refused on the
+ * host where max_kv_len shows it; the kernel takes the last row otherwise. */
+int hc_paged_append_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, hc_rows k, hc_rows v, hc_rows q,
+                        hc_rows q_out, int n_heads, uint32_t dtype, const float* rope, int rope_rows, int rot_dim,
+                        int half_pairs, void* stream);
+
+/* out[r][h] = sum_j softmax_j(scale * q[r][h] . k_j) v_j over the positions
+ * j <= p of the row's sequence (p the row's own position; window > 0: only
+ * j > p - window), holes left out; a row that sees nothing gives zeros.  Query
+ * head h reads KV head h / (n_heads / n_kv_heads).  The softmax is the exact
+ * exponential's (the flat-cache forward passes keep the reference's
+ * polynomial).  q and out are `dtype`; lse (may be NULL) receives the natural
+ * log of each row's sum of exponentials, [n_rows][n_heads], -inf for a row
+ * that sees nothing.  The call needs hc_paged_attention_workspace bytes of
+ * device memory (16-byte aligned; contents do not matter, and calls on
+ * different streams need one each).  Stream-ordered, no synchronization.
+ * head_dim <= 256. */
+int hc_paged_attention_workspace(const hc_paged_kv* kv, const hc_paged_batch* batch, int n_heads, uint32_t dtype,
+                                 int window, size_t* bytes);
+int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, hc_rows q, hc_rows out, float* lse,
+                           int n_heads, uint32_t dtype, float scale, int window, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* The cos/sin table of the model's rotation (transformer.rs:317-343):
+ * out[p][j] = (cos, sin)(p * theta^(-2j / head_dim)) for p < rows, j <
+ * head_dim / 2, computed on the host like the model's own. */
+int hc_rope_table_host(size_t rows, size_t head_dim, float theta, float* out);
+
 /* ---- tensor parallelism (new in this backend; the reference is single-CPU) */
 
 /* Writes a fresh 128-byte NCCL unique id (rank 0 creates it and shares it
