@@ -200,8 +200,8 @@ __global__ void __launch_bounds__(GT) k_paged_generic(PagedAttnArgs A) {
     T* out = (T*)A.out + row * A.o_rs + head * A.o_hs;
 #pragma unroll
     for (int i = 0; i < HDMAX / 8; i++)
-        if (t + 8 * i < hd) out[t + 8 * i] = from_f32<T>(mx == -INFINITY ? 0.0f : o[i] * inv);
-    if (A.lse && t == 0) A.lse[(int64_t)row * A.nh + head] = mx == -INFINITY ? -INFINITY : mx + logf(l);
+        if (t + 8 * i < hd) out[t + 8 * i] = from_f32<T>(l == 0.0f ? 0.0f : o[i] * inv);
+    if (A.lse && t == 0) A.lse[(int64_t)row * A.nh + head] = l == 0.0f ? -INFINITY : mx + logf(l);
 }
 
 template <typename T, typename C>
@@ -353,12 +353,25 @@ static int attn_checks(const char* who, const hc_paged_kv* kv, const hc_paged_ba
     return HC_OK;
 }
 
+namespace {
+struct AttnPlan {
+    bool split;
+    size_t bytes;
+};
+AttnPlan attn_plan(const hc::PagedAttnArgs& A, const hc_paged_batch* b, int c16) {
+    AttnPlan plan = {};
+    plan.split = hc::paged_split_ok(A.p, c16) && (int64_t)b->max_q_len * A.G <= 64;
+    if (plan.split) plan.bytes = hc::paged_split_bytes(A, b->max_kv_len);
+    return plan;
+}
+}  // namespace
+
 HC_EXPORT int hc_paged_attention_workspace(const hc_paged_kv* kv, const hc_paged_batch* batch, int n_heads,
                                            uint32_t dtype, int window, size_t* bytes) {
     hc::PagedAttnArgs A;
     HC_CHECK(bytes, HC_ERR_INVALID, "hc_paged_attention_workspace: NULL bytes");
     HC_TRY(attn_checks("hc_paged_attention_workspace", kv, batch, n_heads, dtype, window, A));
-    *bytes = 0;
+    *bytes = batch->n_rows == 0 ? 0 : attn_plan(A, batch, kv->kv_dtype == HC_KV_FP16).bytes;
     return HC_OK;
 }
 
@@ -379,7 +392,16 @@ HC_EXPORT int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch
     A.o_hs = out.head_stride;
     A.lse = lse;
     A.scale = scale;
-    return hc::launch_paged_generic(A, dtype == HC_DTYPE_FP16, kv->kv_dtype == HC_KV_FP16, (cudaStream_t)stream);
+    const int q16 = dtype == HC_DTYPE_FP16, c16 = kv->kv_dtype == HC_KV_FP16;
+    const int64_t e = q16 ? 8 : 4;
+    A.qvec = (uintptr_t)q.data % 16 == 0 && (q.row_stride | q.head_stride) % e == 0;
+    A.ovec = (uintptr_t)out.data % 16 == 0 && (out.row_stride | out.head_stride) % e == 0;
+    const AttnPlan plan = attn_plan(A, batch, c16);
+    HC_CHECK(workspace_bytes >= plan.bytes && (plan.bytes == 0 || (workspace && (uintptr_t)workspace % 16 == 0)),
+             HC_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, plan.bytes,
+             workspace_bytes);
+    if (plan.split) return hc::launch_paged_split(A, q16, c16, batch->max_kv_len, workspace, (cudaStream_t)stream);
+    return hc::launch_paged_generic(A, q16, c16, (cudaStream_t)stream);
 }
 
 HC_EXPORT int hc_rope_table_host(size_t rows, size_t head_dim, float theta, float* out) {

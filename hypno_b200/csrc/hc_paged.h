@@ -5,6 +5,8 @@
 #include "hc_common.cuh"
 #include "hc_internal.h"
 
+#include <algorithm>
+
 namespace hc {
 
 // The pool of one layer and the step's batch, as the kernels take them.
@@ -94,6 +96,37 @@ __device__ __forceinline__ bool find_tile(const PagedArgs& P, int G, int BM, int
     return false;
 }
 
+// Four columns of a finished row: v / l, zeros for a row that saw nothing (l = 0).
+template <typename T>
+__device__ __forceinline__ void store_row4(const PagedAttnArgs& A, int row, int head, int d, float l, float4 v) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = (T*)A.out + row * A.o_rs + head * A.o_hs + d;
+    if constexpr (sizeof(T) == 4) {
+        if (A.ovec) {
+            *reinterpret_cast<float4*>(out) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            return;
+        }
+    } else {
+        if (A.ovec) {
+            const __half2 a = __floats2half2_rn(v.x * inv, v.y * inv), b = __floats2half2_rn(v.z * inv, v.w * inv);
+            *reinterpret_cast<uint2*>(out) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+            return;
+        }
+    }
+    out[0] = from_f32<T>(v.x * inv);
+    out[1] = from_f32<T>(v.y * inv);
+    out[2] = from_f32<T>(v.z * inv);
+    out[3] = from_f32<T>(v.w * inv);
+}
+
+// Few rows per sequence (hc_paged_split.cu): the keys split over CTAs.
+bool paged_split_ok(const PagedArgs& P, int c16);
+bool paged_split_whole(const PagedAttnArgs& A, int max_kv_len);
+size_t paged_split_bytes(const PagedAttnArgs& A, int max_kv_len);  // workspace
+int launch_paged_split(const PagedAttnArgs& A, int q16, int c16, int max_kv_len, void* ws, cudaStream_t s);
+
+// Any shape (hc_paged.cu).
 int launch_paged_generic(const PagedAttnArgs& A, int q16, int c16, cudaStream_t s);
 
 }  // namespace hc
