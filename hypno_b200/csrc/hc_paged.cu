@@ -400,7 +400,7 @@ HC_EXPORT int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch
     HC_CHECK(workspace_bytes >= plan.bytes && (plan.bytes == 0 || (workspace && (uintptr_t)workspace % 16 == 0)),
              HC_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, plan.bytes,
              workspace_bytes);
-    if (plan.split) return hc::launch_paged_split(A, q16, c16, batch->max_kv_len, workspace, (cudaStream_t)stream);
+    if (plan.split) return hc::launch_paged_split(A, q16, c16, batch->max_q_len, batch->max_kv_len, workspace, (cudaStream_t)stream);
     return hc::launch_paged_generic(A, q16, c16, (cudaStream_t)stream);
 }
 

@@ -124,7 +124,8 @@ __device__ __forceinline__ void store_row4(const PagedAttnArgs& A, int row, int 
 bool paged_split_ok(const PagedArgs& P, int c16);
 bool paged_split_whole(const PagedAttnArgs& A, int max_kv_len);
 size_t paged_split_bytes(const PagedAttnArgs& A, int max_kv_len);  // workspace
-int launch_paged_split(const PagedAttnArgs& A, int q16, int c16, int max_kv_len, void* ws, cudaStream_t s);
+int launch_paged_split(const PagedAttnArgs& A, int q16, int c16, int max_q_len, int max_kv_len, void* ws,
+                       cudaStream_t s);
 
 // Any shape (hc_paged.cu).
 int launch_paged_generic(const PagedAttnArgs& A, int q16, int c16, cudaStream_t s);
