@@ -354,14 +354,26 @@ static int attn_checks(const char* who, const hc_paged_kv* kv, const hc_paged_ba
 }
 
 namespace {
+// Which kernel takes a call.  Up to 64 packed rows a sequence (single tokens,
+// short runs) read the keys once for 8 or 16 rows; more rows pay for the
+// 256-row tiles of the tcgen05 kernel where the cache is FP16, and stay with
+// the 16-row one where it is FP32.  Unaligned or odd heads take the kernel
+// for any shape.
+enum AttnKernel { ATTN_ANY, ATTN_SPLIT, ATTN_TC };
 struct AttnPlan {
-    bool split;
+    AttnKernel kernel;
     size_t bytes;
 };
 AttnPlan attn_plan(const hc::PagedAttnArgs& A, const hc_paged_batch* b, int c16) {
-    AttnPlan plan = {};
-    plan.split = hc::paged_split_ok(A.p, c16) && (int64_t)b->max_q_len * A.G <= 64;
-    if (plan.split) plan.bytes = hc::paged_split_bytes(A, b->max_kv_len);
+    AttnPlan plan = {ATTN_ANY, 0};
+    if (!hc::paged_split_ok(A.p, c16)) return plan;
+    if ((int64_t)b->max_q_len * A.G > 64 && hc::paged_tc_ok(A, c16)) {
+        plan.kernel = ATTN_TC;
+        plan.bytes = hc::paged_tc_bytes(A, b->max_kv_len);
+    } else {
+        plan.kernel = ATTN_SPLIT;
+        plan.bytes = hc::paged_split_bytes(A, b->max_kv_len);
+    }
     return plan;
 }
 }  // namespace
@@ -396,11 +408,16 @@ HC_EXPORT int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch
     const int64_t e = q16 ? 8 : 4;
     A.qvec = (uintptr_t)q.data % 16 == 0 && (q.row_stride | q.head_stride) % e == 0;
     A.ovec = (uintptr_t)out.data % 16 == 0 && (out.row_stride | out.head_stride) % e == 0;
-    const AttnPlan plan = attn_plan(A, batch, c16);
+    AttnPlan plan = attn_plan(A, batch, c16);
     HC_CHECK(workspace_bytes >= plan.bytes && (plan.bytes == 0 || (workspace && (uintptr_t)workspace % 16 == 0)),
              HC_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, plan.bytes,
              workspace_bytes);
-    if (plan.split) return hc::launch_paged_split(A, q16, c16, batch->max_q_len, batch->max_kv_len, workspace, (cudaStream_t)stream);
+    // the tcgen05 kernel takes row maxima before it applies the scale; the
+    // workspace does not know the scale, so another one goes to the kernel without one
+    if (plan.kernel == ATTN_TC && !(scale > 0.0f)) plan.kernel = ATTN_ANY;
+    if (plan.kernel == ATTN_TC)
+        return hc::launch_paged_tc(A, q16, batch->max_kv_len, workspace, (cudaStream_t)stream);
+    if (plan.kernel == ATTN_SPLIT) return hc::launch_paged_split(A, q16, c16, batch->max_q_len, batch->max_kv_len, workspace, (cudaStream_t)stream);
     return hc::launch_paged_generic(A, q16, c16, (cudaStream_t)stream);
 }
 

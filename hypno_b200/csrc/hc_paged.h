@@ -96,6 +96,44 @@ __device__ __forceinline__ bool find_tile(const PagedArgs& P, int G, int BM, int
     return false;
 }
 
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float lds_f32(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ __half lds_f16(uint32_t a) {
+    unsigned short v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+    return __ushort_as_half(v);
+}
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// x = hi + lo with both in fp16 (two values)
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = pack(a - f.x, b - f.y);
+}
+// Visible positions of packed rows [m0, m0 + n) of a sequence: [begin, end).
+__device__ __forceinline__ void visible(const PagedAttnArgs& A, int first, int m0, int n, int& begin, int& end) {
+    end = max(0, first + (m0 + n - 1) / A.G + 1);
+    begin = A.window > 0 ? max(0, first + m0 / A.G - A.window + 1) : 0;
+    begin = min(begin, end);
+}
+
 // Four columns of a finished row: v / l, zeros for a row that saw nothing (l = 0).
 template <typename T>
 __device__ __forceinline__ void store_row4(const PagedAttnArgs& A, int row, int head, int d, float l, float4 v) {
@@ -119,6 +157,11 @@ __device__ __forceinline__ void store_row4(const PagedAttnArgs& A, int row, int 
     out[2] = from_f32<T>(v.z * inv);
     out[3] = from_f32<T>(v.w * inv);
 }
+
+// Many rows per sequence (hc_paged_tc.cu): tcgen05 products over 256-row tiles.
+bool paged_tc_ok(const PagedAttnArgs& A, int c16);
+size_t paged_tc_bytes(const PagedAttnArgs& A, int max_kv_len);  // workspace
+int launch_paged_tc(const PagedAttnArgs& A, int q16, int max_kv_len, void* ws, cudaStream_t s);
 
 // Few rows per sequence (hc_paged_split.cu): the keys split over CTAs.
 bool paged_split_ok(const PagedArgs& P, int c16);

@@ -28,16 +28,6 @@ namespace hc {
 namespace {
 
 constexpr int SP_TK = 16, SP_WARPS = 4, SP_THREADS = 128;
-constexpr float LOG2E = 1.4426950408889634f;
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -62,32 +52,11 @@ __device__ __forceinline__ void mma8(float* d, const uint32_t* a, uint32_t b0, u
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float lds_f32(uint32_t a) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ __half lds_f16(uint32_t a) {
-    unsigned short v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-    return __ushort_as_half(v);
-}
-__device__ __forceinline__ uint32_t pack(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
 // Transposes an 8 x 8 matrix of 16-bit values held by the warp.
 __device__ __forceinline__ uint32_t mov_trans(uint32_t a) {
     uint32_t d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
-}
-// x = hi + lo with both in fp16 (two values)
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = pack(a - f.x, b - f.y);
 }
 // x = hi + lo with both in tf32 (10 mantissa bits, rounded)
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
@@ -113,13 +82,6 @@ struct SplitArgs {
     float* po;    // [slot][R][hd] partial outputs, slot = 2 CTA + (0: its first pair, 1: its last)
     float2* pml;  // [slot][R] (maximum in log2 units, sum)
 };
-
-// Visible positions of packed rows [m0, m0 + n) of a sequence: [begin, end).
-__device__ __forceinline__ void visible(const PagedAttnArgs& A, int first, int m0, int n, int& begin, int& end) {
-    end = max(0, first + (m0 + n - 1) / A.G + 1);
-    begin = A.window > 0 ? max(0, first + m0 / A.G - A.window + 1) : 0;
-    begin = min(begin, end);
-}
 
 struct SeqWork {
     int r0, r1, first;  // rows, position of the first row
