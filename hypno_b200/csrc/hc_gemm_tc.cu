@@ -895,6 +895,21 @@ int encode_2d(CUtensorMap* map, CUtensorMapDataType dt, void* base, uint64_t inn
     return HC_OK;
 }
 
+// Four dimensions (the innermost contiguous, strides in bytes of the others).
+int encode_4d(CUtensorMap* map, CUtensorMapDataType dt, void* base, const uint64_t dims[4], const uint64_t strides[3],
+              uint32_t box0, uint32_t box1, CUtensorMapSwizzle sw) {
+    auto fn = get_encode();
+    HC_CHECK(fn, HC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
+    const cuuint64_t st[3] = {strides[0], strides[1], strides[2]};
+    const cuuint32_t box[4] = {box0, box1, 1, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = fn(map, dt, 4, base, d, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    HC_CHECK(r == CUDA_SUCCESS, HC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return HC_OK;
+}
+
 // Nibble plane as [n][k/2] bytes in 128-row x 64-byte boxes (64-byte swizzle);
 // scale plane as [n][k/32] fp16 in 128-row x 8-scale boxes (16 bytes: the
 // scales of a pair of 128-wide K stages, so every box starts 16-byte aligned).

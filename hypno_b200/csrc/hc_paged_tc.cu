@@ -9,21 +9,40 @@
 //   O_h += P_h V           tcgen05.mma, P in tensor memory over S, V in shared memory
 // While one half's threads work on their weights the tensor core works on
 // the other half's products; S, P and O of both halves fill the 512 columns.
-// The running maximum m moves only when a row's maximum passes it by more
-// than 2^TAU (the weights are held times 2^BIAS and stay below 2^15, so that
-// one of 2^-25 of the largest still has 11 bits): O is rescaled in tensor
-// memory in the first tiles and rarely after them.
+// The products start on the first 64 keys' weights while the others' are made.
+//
+// 16-bit queries: O adds up in tensor memory, so the running maximum m moves
+// only when a row's maximum passes it by more than 2^TAU (the weights are held
+// times 2^BIAS and stay below 2^15, so that one of 2^-25 of the largest still
+// has 11 bits); O is rescaled in the first tiles and rarely after them.
+// Bound by the exponentials as much as by the products (128 x 128 of them take
+// 1024 cycles of the SM's special function units, the two products 1024 of the
+// tensor core), so part of them is a polynomial on the multiply-add units.
 //
 // f32 queries enter as q = 2^e (hi + lo), fp16 each, e the row's own, and their
-// weights as hi + lo: twice the products, results to f32's precision.
+// weights as hi + lo: twice the products.  The tensor core cuts (does not
+// round) the low bits of its running sums, which over many tiles is a bias
+// of several f32 ulps, so a tile's outputs start from zero and the running
+// ones are 128 registers of the row's thread, added to in f32.
 //
-// Warps: 0-3 and 4-7 the halves' rows (load Q, softmax, output; a row of S stays
+// Warps: 0-3 and 4-7 the halves' rows (load Q, softmax, output; a row of S or O is
 // in registers, so these take most of the register file), 8 issues the
-// products, 9 and 10 copy (11 is idle) K and V tiles by cp.async through the block table
-// (any page size; 16-byte pieces, whose issue the tensor work hides, instead
-// of tiled copies, which a page that ends inside a tile would cut).
+// products, 9 (or 9-11) copy K and V tiles.  Pages of a multiple of eight
+// positions come by TMA, in boxes of as many positions (8 to 128) as divide the
+// page: a lane looks up one box's page.  Pages of other sizes are looked up key
+// by key and come by cp.async, 16 bytes a thread; that took 4,400 to 6,000
+// cycles a tile pair, where the products of a pair take 2,048.  (TMA gathers of
+// four rows an instruction took 78 cycles each, 10,000 a pair.)  Keys without a
+// page are zeros; keys of a box that no row sees are zeroed by the rows' threads.
+//
+// The loops of the rows' warps are kept short (masked scores are rewritten in
+// tensor memory by a loop of its own, values that are not finite have one too):
+// the instruction fetch of code unrolled for every case cost more than its
+// arithmetic.
 #include "hc_paged.h"
 #include "hc_tc.cuh"
+
+#include <type_traits>
 
 namespace hc {
 
@@ -31,12 +50,16 @@ namespace {
 
 constexpr int TC_HALF = 128, TC_ROWS = 256, TC_KEYS = 128;
 constexpr int TC_THREADS = 384;
+constexpr int TC_COPY = 3;       // copying warps, every third group of eight keys each
 constexpr int REG_ROW = 208, REG_CTRL = 88;  // 256 x 208 + 128 x 88 = 384 x 168, what the launch holds
 constexpr int TC_MASKS = 8;      // ring of the tiles' key bits
-constexpr float TAU = 4.0f, BIAS = 11.0f;
+constexpr float TAU = 4.0f, BIAS = 11.0f, BIAS_EXACT = 15.0f;
+constexpr int POLY_OF_8 = 2;     // of eight pairs of weights, those by the polynomial
 
 struct TcArgs {
     PagedAttnArgs a;
+    CUtensorMap kmap, vmap;  // the pools as [page][head][position][64 elements] (TMA only)
+    int box;                 // positions of a box, 0: copies key by key
     int nsplit;   // runs of key tiles per row tile
     float* po;    // [(tile * nkv + kvh) * nsplit + run][256][hd]
     float2* pml;  // [..][256] (maximum in log2 units, sum)
@@ -45,6 +68,7 @@ struct TcArgs {
 template <int HD, bool HILO>
 struct TcShape {
     static constexpr int QH = TC_HALF * HD * 2 * (HILO ? 2 : 1);   // bytes of a half's queries: hi, lo
+    static constexpr int QG = (HILO ? 2 : 1) * (HD / 64) * 1024;   // bytes of eight rows: 128-byte pieces, hi then lo
     static constexpr int TILE = TC_KEYS * HD * 2;
     static constexpr int NS = HD == 64 ? 6 : (HILO ? 3 : 5);       // key / value tiles in flight
     static constexpr int SMEM = 2 * QH + NS * TILE + 1024;
@@ -52,7 +76,8 @@ struct TcShape {
 
 struct TcBarriers {
     uint64_t full[6], empty[6];
-    uint64_t q_ready[2], s_full[2], p_ready[2], o_full[2], vote[2];
+    uint64_t q_ready[2], s_full[2], o_full[2], vote[2];
+    uint64_t p_ready[2][2];  // [half][keys 0-63, keys 64-127]
     uint64_t drain;
 };
 
@@ -65,6 +90,31 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t* v) {
           "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
           "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(taddr)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+
+// Waits for tensor-memory loads; the registers named are used only after it.
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
+                   "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+                 :
+                 : "memory");
+}
+
+// A box of a 4-D tensor map into this CTA's shared memory.
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int pos, int head, int page) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+        "[%2];" ::"r"(dst),
+        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(pos), "r"(head), "r"(page)
         : "memory");
 }
 
@@ -97,19 +147,73 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Largest of three, NaN if any is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// Pairs of f32 in one instruction.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 two(float a, float b) {
+    f2 y;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ void untwo(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+    return y;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 y;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+// 2^x of a pair without the special function unit: x = n + r with n the nearest
+// integer (read from the low bits of x + 1.5 2^23), 2^r by the polynomial of
+// degree 5 with the least relative error on [-1/2, 1/2] (Remez exchange:
+// 7.5e-8; degree 3 would do for fp16 weights but not for the sums), n added
+// to the exponent.  x below -126 counts as -126.
+__device__ __forceinline__ void ex2_poly(f2 x, float& y0, float& y1) {
+    float a, b;
+    untwo(x, a, b);
+    x = two(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    const f2 t = add2(x, two(12582912.0f, 12582912.0f));
+    const f2 n = add2(t, two(-12582912.0f, -12582912.0f));
+    const f2 r = fma2(n, two(-1.0f, -1.0f), x);
+    f2 p = fma2(r, two(0.0013276472f, 0.0013276472f), two(0.009675541f, 0.009675541f));
+    p = fma2(p, r, two(0.05550713f, 0.05550713f));
+    p = fma2(p, r, two(0.2402212f, 0.2402212f));
+    p = fma2(p, r, two(0.69314694f, 0.69314694f));
+    p = fma2(p, r, two(1.0000001f, 1.0000001f));
+    float ta, tb;
+    untwo(t, ta, tb);
+    untwo(p, a, b);
+    y0 = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23));
+    y1 = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
+}
 
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // The key tiles of a CTA: positions begin + 128 j for j in [ja, jb), of which
 // half h is active in [ha[h], hb[h]).
 struct TcRange {
-    int begin, end;
+    int begin, end;    // begin: a multiple of the box
+    int seen;          // first position that any row sees
     int ja, jb;
     int ha[2], hb[2];
 };
-__device__ __forceinline__ TcRange tc_range(const PagedAttnArgs& A, int first, int m0, int mtot, int run, int nsplit) {
+__device__ __forceinline__ TcRange tc_range(const PagedAttnArgs& A, int first, int m0, int mtot, int run, int nsplit, int box) {
     TcRange r;
-    visible(A, first, m0, min(TC_ROWS, mtot - m0), r.begin, r.end);
+    visible(A, first, m0, min(TC_ROWS, mtot - m0), r.seen, r.end);
+    r.begin = box > 0 ? r.seen & ~(box - 1) : r.seen;
     const int n = (r.end - r.begin + TC_KEYS - 1) / TC_KEYS;
     const int per = (n + nsplit - 1) / nsplit;
     r.ja = min(n, run * per);
@@ -128,21 +232,20 @@ __device__ __forceinline__ TcRange tc_range(const PagedAttnArgs& A, int first, i
     return r;
 }
 
-template <typename QT, int HD>
+template <typename QT, int HD, bool TMA>
 __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constant__ TcArgs X) {
     constexpr bool HILO = sizeof(QT) == 4;
     using Sh = TcShape<HD, HILO>;
     constexpr int NS = Sh::NS, PL = HILO ? 2 : 1;
-    constexpr int QPLANE = TC_HALF * HD * 2;
     const PagedAttnArgs& A = X.a;
     const PagedArgs& P = A.p;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ TcBarriers B;
     __shared__ uint32_t s_tmem;
     __shared__ int abort_flag, s_skip[2], s_bad[2];
-    __shared__ int s_tile[3];
-    __shared__ float s_cf[TC_ROWS];               // score factor of each row
-    __shared__ uint32_t s_in[TC_MASKS][4];        // which keys of a tile exist
+    __shared__ int s_tile[6];
+    __shared__ float s_cf[TC_ROWS];               // 2^e of each f32 row
+    __shared__ uint32_t s_in[TC_MASKS][4];        // which keys of a tile exist (bytes of eight)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
@@ -153,31 +256,32 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         const int bound = gridDim.x / X.nsplit;
         // later tiles of a prompt see more keys: they go first
         const bool ok = find_tile(P, A.G, TC_ROWS, bound - 1 - (int)(blockIdx.x / X.nsplit), seq, tile);
-        if (lane == 0) {
-            s_tile[0] = ok;
+        if (ok && lane == 0) {
             s_tile[1] = seq;
             s_tile[2] = tile;
+            seq_rows(P, seq, s_tile[3], s_tile[4]);
+            s_tile[5] = __ldg(P.kv_len + seq);
         }
+        if (lane == 0) s_tile[0] = ok;
     }
     if (threadIdx.x == 32) {
         abort_flag = 0;
         s_bad[0] = s_bad[1] = 0;
         for (int i = 0; i < NS; i++) {
-            mbar_init(&B.full[i], 64);
+            mbar_init(&B.full[i], TMA ? 1 : TC_COPY);
             mbar_init(&B.empty[i], 1);
         }
         for (int h = 0; h < 2; h++) {
             mbar_init(&B.q_ready[h], 128);
             mbar_init(&B.s_full[h], 1);
-            mbar_init(&B.p_ready[h], 128);
+            mbar_init(&B.p_ready[h][0], 128);
+            mbar_init(&B.p_ready[h][1], 128);
             mbar_init(&B.o_full[h], 1);
             mbar_init(&B.vote[h], 128);
         }
         mbar_init(&B.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    __syncthreads();
-    if (!s_tile[0]) return;  // the grid is an upper bound
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -186,13 +290,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = s_tmem;
+    if (!s_tile[0]) {  // the grid is an upper bound
+        if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        return;
+    }
     const int run = blockIdx.x % X.nsplit, kvh = blockIdx.y;
     const int seq = s_tile[1], m0 = s_tile[2] * TC_ROWS;
-    int r0, r1;
-    seq_rows(P, seq, r0, r1);
-    const int first = __ldg(P.kv_len + seq) - (r1 - r0);
+    const int r0 = s_tile[3], r1 = s_tile[4], first = s_tile[5] - (r1 - r0);
     const int mtot = (int)min((int64_t)(r1 - r0) * A.G, (int64_t)m0 + TC_ROWS);  // rows up to this tile's end
-    const TcRange rg = tc_range(A, first, m0, mtot, run, X.nsplit);
+    const TcRange rg = tc_range(A, first, m0, mtot, run, X.nsplit, TMA ? X.box : 0);
 
     if (warp < 8) {
         // ================ the halves: queries, weights, outputs
@@ -203,56 +309,65 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         const uint32_t s_col = tmem + lane_off + (uint32_t)(h * 128), o_col = tmem + lane_off + 256u + (uint32_t)(h * 128);
         const uint32_t qs = q_s + h * Sh::QH;
         bool ok = true;
-        // ---- queries: whole rows per warp instruction, 16 bytes a lane
+        // ---- queries.  Eight rows are QG bytes, whether as they come (f32 or fp16
+        // rows one after the other) or as the products take them (128-byte pieces
+        // of the eight rows), so a warp copies its rows as they come and turns
+        // them over eight at a time in place.
         if (rg.hb[h] > rg.ha[h]) {
-            constexpr int EPL = HILO ? 4 : 8, LPR = HD / EPL, RPI = 32 / LPR, BATCH = 8;
+            constexpr int EPL = HILO ? 4 : 8, LPR = HD / EPL, RPI = 32 / LPR;  // elements a lane, lanes a row, rows at once
             const int d = (lane % LPR) * EPL;
+            const uint32_t mine = qs + (uint32_t)((warp & 3) * 4 * Sh::QG);
+#pragma unroll 4
+            for (int i = 0; i < 32 / RPI; i++) {
+                const int rr = i * RPI + lane / LPR, row = (warp & 3) * 32 + rr, m = mh + row;
+                const bool there = row < rows && d < P.hd;
+                const int t = there ? m / A.G : 0;
+                const QT* q = (const QT*)A.q + (there ? (int64_t)(r0 + t) * A.q_rs + (kvh * A.G + m - t * A.G) * A.q_hs + d : 0);
+                const uint32_t dst = mine + (HILO ? (uint32_t)(rr * HD * 4 + (lane % LPR) * 16)
+                                                  : (uint32_t)((rr >> 3) * Sh::QG + (d >> 6) * 1024 + (rr & 7) * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4)));
+                if (A.qvec || !there) {
+                    cp16(dst, there ? (const void*)q : P.k, there);
+                } else {
 #pragma unroll 1
-            for (int i0 = 0; i0 < 32 / RPI; i0 += BATCH) {
-                uint4 v[BATCH];
-#pragma unroll
-                for (int i = 0; i < BATCH; i++) {
-                    const int row = (warp & 3) * 32 + (i0 + i) * RPI + lane / LPR, m = mh + row;
-                    v[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (row < rows && d < P.hd) {
-                        const int t = m / A.G;
-                        const QT* q = (const QT*)A.q + (int64_t)(r0 + t) * A.q_rs + (kvh * A.G + m - t * A.G) * A.q_hs + d;
-                        if (A.qvec) {
-                            v[i] = *reinterpret_cast<const uint4*>(q);
-                        } else if constexpr (HILO) {
-                            v[i] = make_uint4(__float_as_uint(q[0]), __float_as_uint(q[1]), __float_as_uint(q[2]), __float_as_uint(q[3]));
-                        } else {
-                            const unsigned short* u = reinterpret_cast<const unsigned short*>(q);
-                            v[i] = make_uint4(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16, u[4] | (uint32_t)u[5] << 16,
-                                              u[6] | (uint32_t)u[7] << 16);
-                        }
+                    for (int e = 0; e < EPL; e++) {
+                        if constexpr (HILO) asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 4 * e), "f"(q[e]) : "memory");
+                        else asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + 2 * e), "h"(__half_as_ushort(q[e])) : "memory");
                     }
                 }
+            }
+            cp_commit();
+            cp_wait<0>();
+            __syncwarp();
+            if constexpr (HILO) {
+#pragma unroll 1
+                for (int g = 0; g < 4; g++) {
+                    constexpr int N = 8 / RPI;
+                    float f[N][4];
 #pragma unroll
-                for (int i = 0; i < BATCH; i++) {
-                    const int row = (warp & 3) * 32 + (i0 + i) * RPI + lane / LPR;
-                    const uint32_t dst = qs + (uint32_t)((d >> 6) * (TC_HALF * 128) + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 7) * 2);
-                    float c = A.scale * LOG2E;
-                    if constexpr (HILO) {
-                        const float f[4] = {__uint_as_float(v[i].x), __uint_as_float(v[i].y), __uint_as_float(v[i].z), __uint_as_float(v[i].w)};
-                        float mx = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
+                    for (int i = 0; i < N; i++)
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(f[i][0]), "=f"(f[i][1]), "=f"(f[i][2]), "=f"(f[i][3])
+                                     : "r"(mine + (uint32_t)(g * Sh::QG + (i * RPI + lane / LPR) * HD * 4 + (lane % LPR) * 16)));
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const int rr = i * RPI + lane / LPR;  // of the eight
+                        float mx = fmaxf(fmaxf(fabsf(f[i][0]), fabsf(f[i][1])), fmaxf(fabsf(f[i][2]), fabsf(f[i][3])));
 #pragma unroll
                         for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
                         const int e = min(max((int)(__float_as_uint(mx) >> 23), 2), 252);
                         const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-                        c *= __uint_as_float((uint32_t)e << 23);
                         uint32_t hi[2], lo[2];
-                        split2(f[0] * down, f[1] * down, hi[0], lo[0]);
-                        split2(f[2] * down, f[3] * down, hi[1], lo[1]);
+                        split2(f[i][0] * down, f[i][1] * down, hi[0], lo[0]);
+                        split2(f[i][2] * down, f[i][3] * down, hi[1], lo[1]);
+                        const uint32_t dst = mine + (uint32_t)(g * Sh::QG + (d >> 6) * 1024 + rr * 128 + ((((d & 63) >> 3) ^ rr) << 4) + (d & 7) * 2);
                         asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst), "r"(hi[0]), "r"(hi[1]) : "memory");
-                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst + QPLANE), "r"(lo[0]), "r"(lo[1]) : "memory");
-                    } else {
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w) : "memory");
+                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst + Sh::QG / 2), "r"(lo[0]), "r"(lo[1]) : "memory");
+                        if (lane % LPR == 0) s_cf[h * TC_HALF + (warp & 3) * 32 + g * 8 + rr] = __uint_as_float((uint32_t)e << 23);
                     }
-                    if (lane % LPR == 0) s_cf[h * TC_HALF + row] = c;
+                    __syncwarp();
                 }
             }
-            __syncwarp();
             fence_async_shared();
             mbar_arrive(&B.q_ready[h]);
         }
@@ -261,72 +376,121 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         const int lo_pos = A.window > 0 ? pos - A.window + 1 : 0;
         const int p_min = first + mh / A.G, l_max = A.window > 0 ? first + (mh + rows - 1) / A.G - A.window + 1 : 0;
         const bool one_token = rows > 0 && mh / A.G == (mh + rows - 1) / A.G;
-        const float cf = in ? s_cf[h * TC_HALF + r] : 1.0f;
+        const float cf = A.scale * LOG2E * (HILO && in && rg.hb[h] > rg.ha[h] ? s_cf[h * TC_HALF + r] : 1.0f);
         float m = -INFINITY, l = 0.0f;  // running maximum (log2 units), sum of weights
+        float acc[HILO ? HD : 1];       // f32 queries: the running outputs
+        if constexpr (HILO) {
+#pragma unroll
+            for (int i = 0; i < HD; i++) acc[i] = 0.0f;
+        }
+        bool tile_out = false;          // f32 queries: a tile's outputs are in tensor memory
+        auto add_tile = [&]() {
+            if constexpr (HILO) {
+                uint32_t o[2][16];  // the next 16 columns load while these are added
+                tmem_ld_x16(o_col, o[0]);
+#pragma unroll
+                for (int c = 0; c < HD / 16; c++) {
+                    uint32_t* u = o[c & 1];
+                    tmem_wait_ld16(u);
+                    if (c + 1 < HD / 16) tmem_ld_x16(o_col + 16u * (c + 1), o[(c + 1) & 1]);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2)
+                        untwo(add2(two(acc[16 * c + i], acc[16 * c + i + 1]), two(__uint_as_float(u[i]), __uint_as_float(u[i + 1]))),
+                              acc[16 * c + i], acc[16 * c + i + 1]);
+                }
+            }
+        };
+        // The maximum moves to `nm` (NaN and +inf make the row NaN); returns
+        // the factor of what was summed with the old one.
+        auto move_max = [&](float nm, bool raise) -> float {
+            float to = raise ? nm : m;
+            if (!(to < INFINITY) || m != m) to = __int_as_float(0x7fffffff);
+            const float f = to == m ? 1.0f : ex2(m - to);
+            m = to;
+            l *= f;
+            return f;
+        };
+        // A tile's products by the row's thread, masked keys left out: from the
+        // scores still in tensor memory into the half's outputs there.
+        auto careful = [&](float nb, bool add, uint32_t vt, int hi_c, int lo_c, const uint32_t* bits) {
+#pragma unroll 1
+            for (int c0 = 0; c0 < HD; c0 += 8) {
+                uint32_t u[8];
+                float o[8];
+                if (add) {
+                    tmem_ld_x8(o_col + c0, u);
+                    tmem_wait_ld();
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) o[i] = add ? __uint_as_float(u[i]) : 0.0f;
+#pragma unroll 1
+                for (int k = 0; k < TC_KEYS; k += 8) {
+                    tmem_ld_x8(s_col + (uint32_t)k, u);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int y = 0; y < 8; y++) {
+                        const int key = k + y;
+                        if (key > hi_c || key < lo_c || !((bits[key >> 5] >> (key & 31)) & 1u)) continue;
+                        const float p = ex2(fmaf(__uint_as_float(u[y]), cf, nb));
+                        uint32_t w[4];
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                                     : "r"(vt + (c0 >> 6) * (TC_KEYS * 128) + key * 128 + ((((c0 & 63) >> 3) ^ (key & 7)) << 4)));
+#pragma unroll
+                        for (int z = 0; z < 4; z++) {
+                            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[z]));
+                            o[2 * z] = fmaf(p, g.x, o[2 * z]);
+                            o[2 * z + 1] = fmaf(p, g.y, o[2 * z + 1]);
+                        }
+                    }
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) u[i] = __float_as_uint(o[i]);
+                tmem_st_x8(o_col + c0, u);
+            }
+            tmem_wait_st();
+        };
         uint32_t done = 0, votes = 0;
-        for (int j = rg.ha[h]; j < rg.hb[h] && ok; j++, done++) {
+        for (int j = rg.ha[h]; j < rg.hb[h]; j++, done++) {
             ok = mbar_wait(&B.s_full[h], done & 1u, &abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tmem_fence_after();
-            uint32_t sr[128];
-#pragma unroll
-            for (int c = 0; c < 4; c++) tmem_ld_x32(s_col + 32u * c, sr + 32 * c);
-            tmem_wait_ld();
             const int k0 = rg.begin + j * TC_KEYS;
             const uint32_t* bits = s_in[j % TC_MASKS];
             const bool whole = k0 + TC_KEYS - 1 <= p_min && k0 >= l_max && (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu;
-            if (!whole) {
-                const int hi_c = pos - k0, lo_c = lo_pos - k0;
-#pragma unroll
-                for (int c = 0; c < 128; c++)
-                    if (c > hi_c || c < lo_c || !((bits[c >> 5] >> (c & 31)) & 1u)) sr[c] = 0xff800000u;
-            }
-            float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < 128; c++) x[c & 3] = fmaxf(x[c & 3], __uint_as_float(sr[c]));
-            const float nm = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * cf;
-            const bool raise = nm > m + TAU || (m == -INFINITY && nm > m);
-            if (__any_sync(0xffffffffu, raise)) {
-                const float to = raise ? nm : m;
-                const float f = to == m ? 1.0f : ex2(m - to);
-                m = to;
-                l *= f;
-                if (done > 0) {
-                    // the products of the tile before are complete: this tile's
-                    // scores were committed after them
-#pragma unroll
-                    for (int c = 0; c < HD / 16; c++) {
-                        uint32_t o[16];
-                        tmem_ld_x16(o_col + 16u * c, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tmem_st_x16(o_col + 16u * c, o);
-                    }
-                }
-            }
-            const float nb = m == -INFINITY ? 0.0f : BIAS - m;
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int c = 0; c < 128; c++) {
-                const float p = ex2(fmaf(__uint_as_float(sr[c]), cf, nb));
-                sum[c & 3] += p;
-                sr[c] = __float_as_uint(p);
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            const int hi_c = pos - k0, lo_c = lo_pos - k0;
             // A key that some rows of the half see and others do not must not
             // reach the latter through 0 * v where v is not finite: such a tile
             // (rare) leaves the products to the row's thread, masked keys left out.
             bool skip = false;
-            if (!whole && !one_token) {
-                const int n = 2 * j + 1 - 2 * rg.ja, slot = n % NS;
+            uint32_t vt = 0;
+            // keys of the tile that no row sees: what their memory holds is nobody's
+            const bool strangers = TMA && (k0 < rg.seen || k0 + TC_KEYS > rg.end);
+            if ((!whole && !one_token) || strangers) {
+                const int n = 2 * (j - rg.ja) + 1, slot = n % NS;
                 ok = mbar_wait(&B.full[slot], (uint32_t)(n / NS) & 1u, &abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                const uint32_t vt = ring + slot * Sh::TILE;
+                vt = ring + slot * Sh::TILE;
+            }
+            if (strangers) {
+                // their values become zeros (by both halves, before either's products)
+                if (k0 + r < rg.seen || k0 + r >= rg.end)
+#pragma unroll 1
+                    for (int c = 0; c < HD / 64; c++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vt + (uint32_t)(c * (TC_KEYS * 128) + r * 128 + i * 16)), "r"(0) : "memory");
+                fence_async_shared();
+            }
+            if (!whole && !one_token) {
+                // (the other half may still be writing its zeros: a stranger is not looked at)
                 uint32_t bad = 0;
                 for (int i = r; i < Sh::TILE / 16; i += TC_HALF) {
+                    const int key = k0 + (i >> 3) % TC_KEYS;
+                    if (key < rg.seen || key >= rg.end) continue;
                     uint32_t w[4];
                     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
@@ -340,54 +504,148 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 skip = *(volatile int*)&s_bad[h] == j + 1;
-                if (skip) {
-                    const int hi_c = pos - k0, lo_c = lo_pos - k0;
+            }
+            if (r == 0) s_skip[h] = skip;
+
+            if (!whole) {
+                // masked scores become -inf where they stand
 #pragma unroll 1
-                    for (int c0 = 0; c0 < HD; c0 += 16) {
-                        float o[16];
-                        uint32_t u[16];
-                        if (done > 0) {
-                            tmem_ld_x16(o_col + c0, u);
-                            tmem_wait_ld();
-                        }
+                for (int c = 0; c < 4; c++) {
+                    // the visible keys of these 32, as bits
+                    const int up = min(hi_c - 32 * c, 31), dn = max(lo_c - 32 * c, 0);
+                    const uint32_t vis = up < dn ? 0u : bits[c] & (0xffffffffu >> (31 - up)) & (0xffffffffu << dn);
+#pragma unroll 1
+                    for (int y = 0; y < 32; y += 16) {
+                        uint32_t v[16];
+                        tmem_ld_x16(s_col + (uint32_t)(32 * c + y), v);
+                        tmem_wait_ld16(v);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) o[i] = done > 0 ? __uint_as_float(u[i]) : 0.0f;
-#pragma unroll
-                        for (int c = 0; c < 128; c++) {
-                            if (c > hi_c || c < lo_c || !((bits[c >> 5] >> (c & 31)) & 1u)) continue;
-#pragma unroll
-                            for (int i = 0; i < 16; i++) {
-                                const int d = c0 + i;
-                                const float v = __half2float(lds_f16(vt + (d >> 6) * (TC_KEYS * 128) + c * 128 + ((((d & 63) >> 3) ^ (c & 7)) << 4) + (d & 7) * 2));
-                                o[i] = fmaf(__uint_as_float(sr[c]), v, o[i]);
-                            }
-                        }
-                        __syncwarp();
-#pragma unroll
-                        for (int i = 0; i < 16; i++) u[i] = __float_as_uint(o[i]);
-                        tmem_st_x16(o_col + c0, u);
+                        for (int i = 0; i < 16; i++)
+                            if (!((vis >> y >> i) & 1u)) v[i] = 0xff800000u;
+                        tmem_st_x16(s_col + (uint32_t)(32 * c + y), v);
                     }
                 }
-                if (r == 0) s_skip[h] = skip;
-            } else if (r == 0) {
-                s_skip[h] = 0;
+                tmem_wait_st();
             }
-            // weights over the scores: hi in columns 0-63, lo in 64-127
+            float sum0 = 0.0f, sum1 = 0.0f;
+            if constexpr (HILO) {
+                if (tile_out) add_tile();
+                tile_out = true;
+                float x0 = -INFINITY, x1 = -INFINITY;
+                uint32_t vv[2][16];
+                tmem_ld_x16(s_col, vv[0]);
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t hi[16], lo[HILO ? 16 : 1];
+                for (int c = 0; c < 8; c++) {
+                    uint32_t* v = vv[c & 1];
+                    tmem_wait_ld16(v);
+                    tmem_ld_x16(s_col + 16u * ((c + 1) & 7), vv[(c + 1) & 1]);  // the last one: the first again, for the weights
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float a = __uint_as_float(sr[32 * c + 2 * i]), b = __uint_as_float(sr[32 * c + 2 * i + 1]);
-                    if constexpr (HILO) split2(a, b, hi[i], lo[i]);
-                    else hi[i] = pack(a, b);
+                    for (int i = 0; i < 16; i += 4) {
+                        x0 = max3(x0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                        x1 = max3(x1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+                    }
                 }
-                tmem_st_x16(s_col + 16u * c, hi);
-                if constexpr (HILO) tmem_st_x16(s_col + 64u + 16u * c, lo);
+                const float nm = max3(x0, x1, x1) * cf;
+                const bool raise = !(nm <= m);
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float f = move_max(nm, raise);
+                    const f2 ff = two(f, f);
+#pragma unroll
+                    for (int i = 0; i < HD; i += 2) untwo(mul2(two(acc[i], acc[i + 1]), ff), acc[i], acc[i + 1]);
+                }
+                const float nb = m == -INFINITY ? 0.0f : BIAS_EXACT - m;
+                if (skip) careful(nb, false, vt, hi_c, lo_c, bits);
+                const f2 cf2 = two(cf, cf), nb2 = two(nb, nb), minus = two(-1.0f, -1.0f);
+                f2 sum = 0;
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    uint32_t hi[8], lo[8];
+                    uint32_t* v = vv[c & 1];
+                    tmem_wait_ld16(v);
+                    if (c < 7) tmem_ld_x16(s_col + 16u * (c + 1), vv[(c + 1) & 1]);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        float a, b;
+                        untwo(fma2(two(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), cf2, nb2), a, b);
+                        const f2 w = two(ex2(a), ex2(b));
+                        sum = add2(sum, w);
+                        untwo(w, a, b);
+                        hi[i / 2] = pack(a, b);
+                        const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi[i / 2]));
+                        untwo(fma2(two(g.x, g.y), minus, w), a, b);
+                        lo[i / 2] = pack(a, b);
+                    }
+                    // weights over the scores just read: hi in 8 columns, lo in the next 8
+                    tmem_st_x8(s_col + 16u * c, hi);
+                    tmem_st_x8(s_col + 16u * c + 8u, lo);
+                    if (c == 3) {
+                        tmem_wait_st();
+                        tmem_fence_before();
+                        mbar_arrive(&B.p_ready[h][0]);
+                    }
+                }
+                untwo(sum, sum0, sum1);
+            } else {
+                uint32_t sr[128];
+#pragma unroll
+                for (int c = 0; c < 4; c++) tmem_ld_x32(s_col + 32u * c, sr + 32 * c);
+                tmem_wait_ld();
+                float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 128; c += 2) x[(c >> 1) & 3] = max3(x[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+                const float nm = max3(max3(x[0], x[1], x[2]), x[3], x[3]) * cf;
+                const bool raise = !(nm <= m + TAU);
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float f = move_max(nm, raise);
+                    if (done > 0) {
+                        // the products of the tile before are complete: this tile's
+                        // scores were committed after them
+#pragma unroll 1
+                        for (int c = 0; c < HD / 16; c++) {
+                            uint32_t o[16];
+                            tmem_ld_x16(o_col + 16u * c, o);
+                            tmem_wait_ld16(o);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st_x16(o_col + 16u * c, o);
+                        }
+                    }
+                }
+                const float nb = m == -INFINITY ? 0.0f : BIAS - m;
+                if (skip) careful(nb, done > 0, vt, hi_c, lo_c, bits);
+                const f2 cf2 = two(cf, cf), nb2 = two(nb, nb);
+                f2 sum[2] = {0, 0};
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int k = 32 * c + 2 * i;
+                        const f2 e = fma2(two(__uint_as_float(sr[k]), __uint_as_float(sr[k + 1])), cf2, nb2);
+                        float a, b;
+                        if ((i & 7) < POLY_OF_8) {
+                            ex2_poly(e, a, b);
+                        } else {
+                            untwo(e, a, b);
+                            a = ex2(a);
+                            b = ex2(b);
+                        }
+                        sum[i & 1] = add2(sum[i & 1], two(a, b));
+                        w[i] = pack(a, b);
+                    }
+                    tmem_st_x16(s_col + 16u * c, w);
+                    if (c == 1) {
+                        tmem_wait_st();
+                        tmem_fence_before();
+                        mbar_arrive(&B.p_ready[h][0]);
+                    }
+                }
+                untwo(add2(sum[0], sum[1]), sum0, sum1);
             }
+            l += m == -INFINITY ? 0.0f : sum0 + sum1;
             tmem_wait_st();
             tmem_fence_before();
-            mbar_arrive(&B.p_ready[h]);
+            mbar_arrive(&B.p_ready[h][1]);
         }
         // ---- outputs
         const bool any = rg.hb[h] > rg.ha[h];
@@ -395,36 +653,87 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             ok = mbar_wait(&B.o_full[h], 0, &abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             tmem_fence_after();
+            if (ok && tile_out) add_tile();
         }
-        if (rows > 0) {
-            const int t = (mh + r) / A.G, row = r0 + t, head = kvh * A.G + (mh + r) - t * A.G;
-            if (!ok) l = __int_as_float(0x7fffffff);  // a wait ran out: the row is NaN, not a wrong number
-            const int64_t slot = ((int64_t)(blockIdx.x / X.nsplit) * P.nkv + kvh) * X.nsplit + run;
-            const int64_t pr = slot * TC_ROWS + h * TC_HALF + r;
-#pragma unroll 1
-            for (int c = 0; c < HD / 16; c++) {
-                uint32_t o[16];
-                if (any && ok) {
-                    tmem_ld_x16(o_col + 16u * c, o);
-                    tmem_wait_ld();
+        if (!ok) l = __int_as_float(0x7fffffff);  // a wait ran out: the row is NaN, not a wrong number
+        const int64_t pr = (((int64_t)(blockIdx.x / X.nsplit) * P.nkv + kvh) * X.nsplit + run) * TC_ROWS + h * TC_HALF + r;
+        if (in) {
+            if (X.nsplit > 1) {
+                X.pml[pr] = make_float2(m == -INFINITY ? m : m - (HILO ? BIAS_EXACT : BIAS), l);
+            } else if (A.lse) {
+                const int t = (mh + r) / A.G;
+                A.lse[(int64_t)(r0 + t) * A.nh + kvh * A.G + (mh + r) - t * A.G] =
+                    l == 0.0f ? -INFINITY : (m - (HILO ? BIAS_EXACT : BIAS) + log2f(l)) / LOG2E;
+            }
+        }
+        const float inv = X.nsplit > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+        // 16 columns at a time: partial results straight to the workspace; results
+        // through the half's query memory (its products are done), so that a
+        // warp's stores are whole rows
+        const uint32_t stage = qs + (uint32_t)((warp & 3) * 32 * HD * (int)sizeof(QT));
+#pragma unroll(HILO ? HD / 16 : 1)
+        for (int c = 0; c < HD / 16; c++) {
+            uint32_t o[16];
+            if constexpr (HILO) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[i] = __float_as_uint(acc[16 * c + i]);
+            } else if (any && ok) {
+                tmem_ld_x16(o_col + 16u * c, o);
+                tmem_wait_ld();
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[i] = 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+            if (X.nsplit > 1) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    if (in && 16 * c + i < P.hd)
+                        *reinterpret_cast<uint4*>(X.po + pr * P.hd + 16 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            } else {
+                const uint32_t row_at = stage + (uint32_t)(lane * HD * (int)sizeof(QT));
+                if constexpr (HILO) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + (((4 * c + i) ^ (lane & 7)) << 4)),
+                                     "r"(o[4 * i]), "r"(o[4 * i + 1]), "r"(o[4 * i + 2]), "r"(o[4 * i + 3])
+                                     : "memory");
                 } else {
+                    uint32_t w[8];
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[i] = 0u;
-                }
-                if (in && 16 * c < P.hd) {
+                    for (int i = 0; i < 8; i++) w[i] = pack(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const int d = 16 * c + i;
-                        const float4 v = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-                        if (d >= P.hd) break;
-                        if (X.nsplit == 1) store_row4<QT>(A, row, head, d, l, v);
-                        else *reinterpret_cast<float4*>(X.po + pr * P.hd + d) = v;
-                    }
+                    for (int i = 0; i < 2; i++)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + (((2 * c + i) ^ (lane & 7)) << 4)),
+                                     "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3])
+                                     : "memory");
                 }
             }
-            if (in) {
-                if (X.nsplit > 1) X.pml[pr] = make_float2(m == -INFINITY ? m : m - BIAS, l);
-                else if (A.lse) A.lse[(int64_t)row * A.nh + head] = l == 0.0f ? -INFINITY : (m - BIAS + log2f(l)) / LOG2E;
+        }
+        if (X.nsplit == 1) {
+            __syncwarp();
+            constexpr int EPL = 16 / (int)sizeof(QT), LPR = HD / EPL, RPI = 32 / LPR;
+            const int d = (lane % LPR) * EPL;
+#pragma unroll 4
+            for (int i = 0; i < 32 / RPI; i++) {
+                const int rr = i * RPI + lane / LPR, row = (warp & 3) * 32 + rr;
+                if (row >= rows || d >= P.hd) continue;
+                uint32_t w[4];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                             : "r"(stage + (uint32_t)(rr * HD * (int)sizeof(QT)) + (((lane % LPR) ^ (rr & 7)) << 4)));
+                const int t = (mh + row) / A.G;
+                QT* out = (QT*)A.out + (int64_t)(r0 + t) * A.o_rs + (kvh * A.G + (mh + row) - t * A.G) * A.o_hs + d;
+                if (A.ovec) {
+                    *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+#pragma unroll
+                    for (int y = 0; y < EPL; y++) {
+                        if constexpr (HILO) out[y] = __uint_as_float(w[y]);
+                        else reinterpret_cast<unsigned short*>(out)[y] = (unsigned short)(w[y / 2] >> (16 * (y & 1)));
+                    }
+                }
             }
         }
         tmem_fence_before();
@@ -436,41 +745,50 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         constexpr uint32_t idesc_o = make_idesc_mn(128, HD) | (1u << 16);  // V is MN-major
         bool ok = true;
         uint32_t pdone[2] = {0, 0};
+        const uint64_t q_d = (sw128_desc(q_s) & ~((uint64_t)0x3FFF << 32)) | (uint64_t)(Sh::QG >> 4) << 32;  // eight rows are QG apart
         for (int j = rg.ja; j <= rg.jb && ok; j++) {
             const int nk = 2 * (j - rg.ja), nv = nk - 1;  // ring places of K_j and V_(j-1)
+            const uint64_t k_d = sw128_desc(ring + (nk % NS) * Sh::TILE), v_d = sw128_mn_desc(ring + (nv + NS) % NS * Sh::TILE);
+            if (j > rg.ja) ok = warp_wait(&B.full[nv % NS], (uint32_t)(nv / NS) & 1u, &abort_flag);
+            if (j < rg.jb) ok = ok && warp_wait(&B.full[nk % NS], (uint32_t)(nk / NS) & 1u, &abort_flag);
+            if (!ok) break;
             for (int h = 0; h < 2 && ok; h++) {
                 const uint32_t s_t = tmem + (uint32_t)(h * 128), o_t = tmem + 256u + (uint32_t)(h * 128);
-                if (j - 1 >= rg.ha[h] && j - 1 < rg.hb[h]) {  // O_h += P_h V_(j-1)
-                    ok = warp_wait(&B.p_ready[h], pdone[h] & 1u, &abort_flag) &&
-                         warp_wait(&B.full[nv % NS], (uint32_t)(nv / NS) & 1u, &abort_flag);
-                    if (!ok) break;
-                    tmem_fence_after();
-                    const int skip = *(volatile int*)&s_skip[h];
-                    const uint32_t vs = ring + (nv % NS) * Sh::TILE;
-                    if (!skip && elect_one()) {
+                const bool pv = j - 1 >= rg.ha[h] && j - 1 < rg.hb[h], sc = j >= rg.ha[h] && j < rg.hb[h];
+                if (pv) {  // O_h += P_h V_(j-1), the first 64 keys as soon as their weights are there
+                    for (int half = 0; half < 2; half++) {
+                        ok = warp_wait(&B.p_ready[h][half], pdone[h] & 1u, &abort_flag);
+                        if (!ok) break;
+                        tmem_fence_after();
+                        if (!*(volatile int*)&s_skip[h] && elect_one()) {
 #pragma unroll
-                        for (int p = PL - 1; p >= 0; p--)
+                            for (int p = PL - 1; p >= 0; p--)
 #pragma unroll
-                            for (int kk = 0; kk < TC_KEYS / 16; kk++)
-                                mma_f16_ts(o_t, s_t + (uint32_t)(p * 64 + kk * 8), sw128_mn_desc(vs + kk * 2048), idesc_o,
-                                           pdone[h] > 0 || kk > 0 || p < PL - 1);
+                                for (int k4 = 0; k4 < 4; k4++) {
+                                    const int kk = half * 4 + k4;
+                                    mma_f16_ts(o_t, s_t + (uint32_t)(HILO ? kk * 16 + p * 8 : kk * 8), v_d + (uint64_t)(kk * (2048 >> 4)), idesc_o,
+                                               (!HILO && pdone[h] > 0) || half > 0 || k4 > 0 || p < PL - 1);
+                                }
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    if (!ok) break;
                     pdone[h]++;
                 }
-                if (j >= rg.ha[h] && j < rg.hb[h]) {  // S_h = Q_h K_j^T
-                    if (j == rg.ha[h]) ok = warp_wait(&B.q_ready[h], 0, &abort_flag);
-                    ok = ok && warp_wait(&B.full[nk % NS], (uint32_t)(nk / NS) & 1u, &abort_flag);
-                    if (!ok) break;
+                if (sc) {  // S_h = Q_h K_j^T
+                    if (j == rg.ha[h]) {
+                        ok = warp_wait(&B.q_ready[h], 0, &abort_flag);
+                        if (!ok) break;
+                    }
                     tmem_fence_after();
-                    const uint32_t ks = ring + (nk % NS) * Sh::TILE, qs = q_s + h * Sh::QH;
                     if (elect_one()) {
 #pragma unroll
                         for (int p = PL - 1; p >= 0; p--)
 #pragma unroll
                             for (int kk = 0; kk < HD / 16; kk++) {
-                                const uint32_t off = (uint32_t)((kk >> 2) * (128 * 128) + (kk & 3) * 32);
-                                mma_f16_ss(s_t, sw128_desc(qs + p * QPLANE + off), sw128_desc(ks + off), idesc_s, kk > 0 || p < PL - 1);
+                                const uint32_t qo = (uint32_t)(h * Sh::QH + (p * (HD / 64) + (kk >> 2)) * 1024 + (kk & 3) * 32);
+                                const uint32_t ko = (uint32_t)((kk >> 2) * (TC_KEYS * 128) + (kk & 3) * 32);
+                                mma_f16_ss(s_t, q_d + (uint64_t)(qo >> 4), k_d + (uint64_t)(ko >> 4), idesc_s, kk > 0 || p < PL - 1);
                             }
                         mma_commit(&B.s_full[h]);
                     }
@@ -495,78 +813,124 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             mbar_wait(&B.drain, 0, &none);
         }
         tmem_fence_before();
-      } else if (warp < 11) {
-        // ================ the copies: warp lw takes keys 64 lw .. 64 lw + 63 of each tile
-        const int lw = warp - 9;
-        constexpr int CPL = HD / 32;  // 16-byte chunks of a row per lane (four lanes copy a row)
+      } else if (TMA && warp == 9) {
+        // ================ the copies: lane l takes the tile's l-th box
         bool ok = true;
-        int waiting = -1;             // tile copied but not yet announced
-        auto announce = [&]() {
-            if (waiting >= 0) {
-                fence_async_shared();
-                mbar_arrive(&B.full[waiting % NS]);
-            }
-            waiting = -1;
+        int copied = 0;
+        const int box = X.box, nbox = TC_KEYS / box;
+        int page, slot;
+        auto look = [&](int j) {
+            const int p = rg.begin + j * TC_KEYS + lane * box;
+            page = -1;
+            slot = 0;
+            if (lane < nbox && j < rg.jb && p < rg.end) page = lookup(P, seq, p, slot);
         };
-        int page[2], slot[2];
+        look(rg.ja);
+        for (int j = rg.ja; j < rg.jb && ok; j++) {
+            const int pg = page >= 0 ? page : P.n_pages, sl = slot;  // no page: outside the pool, read as zeros
+            const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+            look(j + 1);
+            if (lane < 4) {  // the mask of keys 32 lane ..: bit by bit of the boxes
+                uint32_t w = 0;
+                if (box >= 32) w = (there >> (32 * lane / box)) & 1u ? 0xffffffffu : 0u;
+                else
+                    for (int i = 0; i < 32 / box; i++)
+                        if ((there >> (32 / box * lane + i)) & 1u) w |= ((1u << box) - 1u) << (i * box);
+                s_in[j % TC_MASKS][lane] = w;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int kv = 0; kv < 2; kv++) {
+                const int n = 2 * (j - rg.ja) + kv;
+                if (n >= NS) ok = warp_wait(&B.empty[n % NS], (uint32_t)(n / NS - 1) & 1u, &abort_flag);
+                if (!ok) break;
+                if (lane == 0) mbar_expect_tx(&B.full[n % NS], (uint32_t)Sh::TILE);
+                __syncwarp();
+                if (lane < nbox) {
+#pragma unroll
+                    for (int c = 0; c < HD / 64; c++)
+                        tma_box(ring + (n % NS) * Sh::TILE + (uint32_t)(c * (TC_KEYS * 128) + lane * box * 128), kv ? &X.vmap : &X.kmap,
+                                &B.full[n % NS], c * 64, sl, kvh, pg);
+                }
+                copied = n + 1;
+            }
+        }
+        if (!ok) {  // let the copies in flight land
+            int none = 0;
+            for (int n = max(0, copied - NS); n < copied; n++) mbar_wait(&B.full[n % NS], (uint32_t)(n / NS) & 1u, &none);
+        }
+      } else if constexpr (!TMA) {
+        // ================ the copies: groups lw, lw + 3, ... of eight keys, four lanes a key
+        const int lw = warp - 9;
+        constexpr int CPL = HD / 32;     // 16-byte chunks of a row per lane
+        constexpr int NG = 6;            // groups of a warp: 6, 5 and 5 of the 16
+        bool ok = true;
+        int next = 0;                    // first tile not yet announced
+        auto announce = [&](int upto) {  // tiles below `upto` have landed
+            if (next >= upto) return;
+            fence_async_shared();
+            __syncwarp();
+            for (; next < upto; next++)
+                if (lane == 0) mbar_arrive(&B.full[next % NS]);
+        };
+        int page[NG], slot[NG];          // of key 8 (lw + 3 g) + lane / 4
         auto look = [&](int j) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int p = rg.begin + j * TC_KEYS + lw * 64 + i * 32 + lane;
-                page[i] = -1;
-                slot[i] = 0;
-                if (j < rg.jb && p < rg.end) page[i] = lookup(P, seq, p, slot[i]);
+            for (int g = 0; g < NG; g++) {
+                const int p = rg.begin + j * TC_KEYS + (lw + 3 * g) * 8 + (lane >> 2);
+                page[g] = -1;
+                slot[g] = 0;
+                if (lw + 3 * g < 16 && j < rg.jb && p < rg.end) page[g] = lookup(P, seq, p, slot[g]);
             }
         };
         look(rg.ja);
         for (int j = rg.ja; j < rg.jb && ok; j++) {
-            int64_t ko[2], vo[2];
-            uint32_t in[2];
+            int64_t ko[NG], vo[NG];      // element offsets of the keys, -1 for none
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                in[i] = __ballot_sync(0xffffffffu, page[i] >= 0);
-                ko[i] = page[i] >= 0 ? page[i] * P.kps + kvh * P.khs + slot[i] * P.kss : 0;
-                vo[i] = page[i] >= 0 ? page[i] * P.vps + kvh * P.vhs + slot[i] * P.vss : 0;
+            for (int g = 0; g < NG; g++) {
+                ko[g] = page[g] >= 0 ? page[g] * P.kps + kvh * P.khs + slot[g] * P.kss + (lane & 3) * 8 : -1;
+                vo[g] = page[g] >= 0 ? page[g] * P.vps + kvh * P.vhs + slot[g] * P.vss + (lane & 3) * 8 : -1;
             }
             look(j + 1);
-            for (int kv = 0; kv < 2 && ok; kv++) {
+#pragma unroll
+            for (int kv = 0; kv < 2; kv++) {
                 const int n = 2 * (j - rg.ja) + kv;
                 if (n >= NS) {
                     const uint32_t par = (uint32_t)(n / NS - 1) & 1u;
-                    if (!mbar_test_wait(&B.empty[n % NS], par)) {
-                        cp_wait<0>();  // nothing to copy yet: announce what has landed
-                        announce();
-                        ok = mbar_wait(&B.empty[n % NS], par, &abort_flag);
+                    if (!__all_sync(0xffffffffu, mbar_test_wait(&B.empty[n % NS], par))) {
+                        cp_wait<0>();  // no room for a copy yet: announce what has landed
+                        announce(n);
+                        ok = warp_wait(&B.empty[n % NS], par, &abort_flag);
                     }
-                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                 }
-                if (kv == 0 && lane < 2) s_in[j % TC_MASKS][lw * 2 + lane] = lane ? in[1] : in[0];
-                const __half* src = (const __half*)(kv ? P.v : P.k) + (lane & 3) * 8;
-                const uint32_t dst = ring + (n % NS) * Sh::TILE + (uint32_t)((lw * 64 + (lane >> 2)) * 128);
+                const uint32_t dst = ring + (n % NS) * Sh::TILE + (uint32_t)(lw * 1024 + (lane >> 2) * 128 + (((lane & 3) ^ (lane >> 2)) << 4));
 #pragma unroll
-                for (int g = 0; g < 8; g++) {  // rows 8 g + lane / 4
-                    const int row = (g * 8 + (lane >> 2)) & 31;
-                    const int64_t off = __shfl_sync(0xffffffffu, kv ? vo[g >> 2] : ko[g >> 2], row);
-                    const bool row_in = (in[g >> 2] >> row) & 1u;
+                for (int g = 0; g < NG; g++) {
+                    if (lw + 3 * g >= 16) break;
+                    const int64_t off = kv ? vo[g] : ko[g];
+                    const __half* src = (const __half*)(kv ? P.v : P.k) + off;
+                    if (kv == 0) {
+                        const uint32_t in = __ballot_sync(0xffffffffu, off >= 0);  // the lanes of a key agree
+                        uint32_t byte = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) byte |= ((in >> (4 * i)) & 1u) << i;
+                        if (lane == 0) reinterpret_cast<volatile uint8_t*>(s_in[j % TC_MASKS])[lw + 3 * g] = (uint8_t)byte;
+                    }
 #pragma unroll
                     for (int x = 0; x < CPL; x++) {
-                        const int c = (lane & 3) + 4 * x;
-                        const bool ok_c = row_in && c * 8 < P.hd;
-                        cp16(dst + (uint32_t)((c >> 3) * (TC_KEYS * 128) + g * 1024 + (((c & 7) ^ (lane >> 2)) << 4)),
-                             ok_c ? src + off + 32 * x : (const __half*)P.k, ok_c);
+                        const bool in = off >= 0 && (lane & 3) * 8 + 32 * x < P.hd;
+                        // chunk (lane % 4) + 4 x of the row: block x / 2, place ^ (row % 8)
+                        cp16((dst ^ (uint32_t)((x & 1) << 6)) + (uint32_t)((x >> 1) * (TC_KEYS * 128) + g * 3072), in ? src + 32 * x : (const __half*)P.k, in);
                     }
                 }
                 cp_commit();
-                if (waiting >= 0) {
-                    cp_wait<1>();
-                    announce();
-                }
-                waiting = n;
+                cp_wait<1>();
+                announce(n);
             }
         }
         cp_wait<0>();
-        if (ok) announce();
+        if (ok) announce(2 * (rg.jb - rg.ja));
       }
     }
     __syncthreads();
@@ -627,14 +991,14 @@ int tc_nsplit(const PagedAttnArgs& A, int max_kv_len) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(148 / pairs, units / 4));
 }
 
-template <typename QT, int HD>
+template <typename QT, int HD, bool TMA>
 int launch_tc_t(const TcArgs& X, cudaStream_t s) {
     using Sh = TcShape<HD, sizeof(QT) == 4>;
-    HC_CUDA(cudaFuncSetAttribute(k_paged_tc<QT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
+    HC_CUDA(cudaFuncSetAttribute(k_paged_tc<QT, HD, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
     const PagedArgs& P = X.a.p;
     const int64_t tiles = tc_tiles(X.a);
     HC_CHECK(tiles * X.nsplit <= 0x7fffffff, HC_ERR_INVALID, "paged attention: %d rows of %d heads", P.n_rows, X.a.nh);
-    k_paged_tc<QT, HD><<<dim3((unsigned)(tiles * X.nsplit), P.nkv), TC_THREADS, Sh::SMEM, s>>>(X);
+    k_paged_tc<QT, HD, TMA><<<dim3((unsigned)(tiles * X.nsplit), P.nkv), TC_THREADS, Sh::SMEM, s>>>(X);
     HC_LAUNCH_CHECK();
     if (X.nsplit > 1) {
         k_paged_tc_join<QT><<<dim3((unsigned)tiles, P.nkv, 8), 256, 0, s>>>(X);
@@ -643,10 +1007,31 @@ int launch_tc_t(const TcArgs& X, cudaStream_t s) {
     return HC_OK;
 }
 
+// A pool's tensor map; a dimension of one entry may have any stride.
+int pool_map(CUtensorMap* map, const PagedArgs& P, void* base, int64_t ps, int64_t hs, int64_t ss, int box) {
+    const uint64_t dims[4] = {(uint64_t)P.hd, (uint64_t)P.page_size, (uint64_t)P.nkv, (uint64_t)P.n_pages};
+    const uint64_t row = (uint64_t)((P.hd + 7) / 8 * 16);
+    const uint64_t strides[3] = {P.page_size > 1 ? (uint64_t)ss * 2 : row, P.nkv > 1 ? (uint64_t)hs * 2 : row,
+                                 P.n_pages > 1 ? (uint64_t)ps * 2 : row};
+    return encode_4d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, base, dims, strides, 64, (uint32_t)box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename QT, int HD>
+int launch_tc_copy(TcArgs& X, cudaStream_t s) {
+    const PagedArgs& P = X.a.p;
+    X.box = 0;
+    for (int b = 8; b <= TC_KEYS && P.page_size % b == 0; b *= 2) X.box = b;
+    const int64_t widest = std::max({P.kps, P.khs, P.kss, P.vps, P.vhs, P.vss});
+    if (X.box == 0 || widest >= (1ll << 38)) return launch_tc_t<QT, HD, false>(X, s);
+    HC_TRY(pool_map(&X.kmap, P, P.k, P.kps, P.khs, P.kss, X.box));
+    HC_TRY(pool_map(&X.vmap, P, P.v, P.vps, P.vhs, P.vss, X.box));
+    return launch_tc_t<QT, HD, true>(X, s);
+}
+
 }  // namespace
 
 // FP16 cache with 16-byte rows, head sizes the padded tiles hold, a positive
-// scale (the maximum is taken before it is applied), rows that fit 32 bits.
+// scale (the maximum is taken before it is applied), row indexes of 31 bits.
 bool paged_tc_ok(const PagedAttnArgs& A, int c16) {
     const PagedArgs& P = A.p;
     return c16 && P.hd <= 128 && P.hd % 8 == 0 && ((uintptr_t)P.k | (uintptr_t)P.v) % 16 == 0 &&
@@ -664,8 +1049,8 @@ int launch_paged_tc(const PagedAttnArgs& A, int q16, int max_kv_len, void* ws, c
     X.nsplit = tc_nsplit(A, max_kv_len);
     X.po = (float*)ws;
     X.pml = (float2*)((float*)ws + (size_t)tc_tiles(A) * A.p.nkv * X.nsplit * TC_ROWS * A.p.hd);
-    if (q16) return A.p.hd <= 64 ? launch_tc_t<__half, 64>(X, s) : launch_tc_t<__half, 128>(X, s);
-    return A.p.hd <= 64 ? launch_tc_t<float, 64>(X, s) : launch_tc_t<float, 128>(X, s);
+    if (q16) return A.p.hd <= 64 ? launch_tc_copy<__half, 64>(X, s) : launch_tc_copy<__half, 128>(X, s);
+    return A.p.hd <= 64 ? launch_tc_copy<float, 64>(X, s) : launch_tc_copy<float, 128>(X, s);
 }
 
 }  // namespace hc

@@ -121,6 +121,8 @@ __device__ __forceinline__ void named_arrive(int id, int n) {
 // ---- host side: tensor maps (hc_gemm_tc.cu)
 int encode_2d(CUtensorMap* map, CUtensorMapDataType dt, void* base, uint64_t inner, uint64_t outer,
               uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw);
+int encode_4d(CUtensorMap* map, CUtensorMapDataType dt, void* base, const uint64_t dims[4], const uint64_t strides[3],
+              uint32_t box0, uint32_t box1, CUtensorMapSwizzle sw);
 // Nibble plane as [n][k/2] bytes in 128-row x 64-byte boxes (64-byte swizzle);
 // scale plane as [n][k/32] fp16 in 128-row x 8-scale boxes (16 bytes: the
 // scales of a pair of 128-wide K stages).
