@@ -5,11 +5,15 @@
 // A CTA takes 256 packed (token, query head of the group) rows of one
 // (sequence, KV head) as two halves of 128, and walks key tiles of 128:
 //   S_h = Q_h K^T          tcgen05.mma, Q and K in shared memory (128 x 128 f32)
-//   P_h = 2^(c S_h - m)    one thread per row, S read from tensor memory
+//   P_h = 2^(c S_h - m)    two threads per row, 64 keys each, S read from tensor memory
 //   O_h += P_h V           tcgen05.mma, P in tensor memory over S, V in shared memory
 // While one half's threads work on their weights the tensor core works on
 // the other half's products; S, P and O of both halves fill the 512 columns.
-// The products start on the first 64 keys' weights while the others' are made.
+// A half's weights and its products wait for one another, so the time from
+// S_h to P_h counts in full: two threads a row (16 warps, four a scheduler)
+// halve it, where one thread a row left the schedulers idle for want of
+// independent work.  The products start when each thread has 32 of its 64
+// weights.
 //
 // 16-bit queries: O adds up in tensor memory, so the running maximum m moves
 // only when a row's maximum passes it by more than 2^TAU (the weights are held
@@ -23,11 +27,11 @@
 // weights as hi + lo: twice the products.  The tensor core cuts (does not
 // round) the low bits of its running sums, which over many tiles is a bias
 // of several f32 ulps, so a tile's outputs start from zero and the running
-// ones are 128 registers of the row's thread, added to in f32.
+// ones are in registers of the row's threads, 64 columns each, added to in f32.
 //
-// Warps: 0-3 and 4-7 the halves' rows (load Q, softmax, output; a row of S or O is
-// in registers, so these take most of the register file), 8 issues the
-// products, 9 (or 9-11) copy K and V tiles.  Pages of a multiple of eight
+// Warps: 0-7 and 8-15 the halves' rows (load Q, softmax, output; of a half's
+// eight, the first four take keys 0-63 and the low columns of O, the others the
+// rest), 16 issues the products, 17 (to 19) copy K and V tiles.  Pages of a multiple of eight
 // positions come by TMA, in boxes of as many positions (8 to 128) as divide the
 // page: a lane looks up one box's page.  Pages of other sizes are looked up key
 // by key and come by cp.async, 16 bytes a thread; that took 4,400 to 6,000
@@ -49,9 +53,8 @@ namespace hc {
 namespace {
 
 constexpr int TC_HALF = 128, TC_ROWS = 256, TC_KEYS = 128;
-constexpr int TC_THREADS = 384;
-constexpr int TC_COPY = 3;       // copying warps, every third group of eight keys each
-constexpr int REG_ROW = 208, REG_CTRL = 88;  // 256 x 208 + 128 x 88 = 384 x 168, what the launch holds
+constexpr int TC_THREADS = 640;  // 16 warps of rows (two threads a row), 4 of products and copies
+constexpr int TC_COPY = 3;       // copying warps where keys come one by one, every third group of eight each
 constexpr int TC_MASKS = 8;      // ring of the tiles' key bits
 constexpr float TAU = 4.0f, BIAS = 11.0f, BIAS_EXACT = 15.0f;
 constexpr int POLY_OF_8 = 2;     // of eight pairs of weights, those by the polynomial
@@ -65,21 +68,33 @@ struct TcArgs {
     float2* pml;  // [..][256] (maximum in log2 units, sum)
 };
 
+constexpr int TC_CTRL = 3072;    // shared memory before the queries and the ring, which begin on a 1024-byte boundary
+
 template <int HD, bool HILO>
 struct TcShape {
     static constexpr int QH = TC_HALF * HD * 2 * (HILO ? 2 : 1);   // bytes of a half's queries: hi, lo
     static constexpr int QG = (HILO ? 2 : 1) * (HD / 64) * 1024;   // bytes of eight rows: 128-byte pieces, hi then lo
     static constexpr int TILE = TC_KEYS * HD * 2;
     static constexpr int NS = HD == 64 ? 6 : (HILO ? 3 : 5);       // key / value tiles in flight
-    static constexpr int SMEM = 2 * QH + NS * TILE + 1024;
+    static constexpr int SMEM = TC_CTRL + 2 * QH + NS * TILE;
 };
 
 struct TcBarriers {
     uint64_t full[6], empty[6];
     uint64_t q_ready[2], s_full[2], o_full[2], vote[2];
-    uint64_t p_ready[2][2];  // [half][keys 0-63, keys 64-127]
+    uint64_t p_ready[2][2];  // [half][keys 0-31 and 64-95, the others]
+    uint64_t fin[8];         // the pairs of warps of the same rows, at the end
     uint64_t drain;
 };
+
+struct TcControl {
+    TcBarriers bars;
+    __align__(16) uint32_t in[TC_MASKS][4];  // which keys of a tile exist (bytes of eight)
+    float pair[TC_ROWS][2];                  // what a row's two threads tell one another
+    uint32_t tmem;
+    int abort, skip[2], bad[2], tile[6];
+};
+static_assert(sizeof(TcControl) <= TC_CTRL, "the control block fits");
 
 __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t* v) {
     asm volatile(
@@ -200,6 +215,11 @@ __device__ __forceinline__ void ex2_poly(f2 x, float& y0, float& y1) {
     y1 = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
 }
 
+// A wait that mostly finds its phase complete: the bounded loop is off the path.
+__device__ __forceinline__ bool quick_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, abort_flag);
+}
+
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // The key tiles of a CTA: positions begin + 128 j for j in [ja, jb), of which
@@ -237,19 +257,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
     constexpr bool HILO = sizeof(QT) == 4;
     using Sh = TcShape<HD, HILO>;
     constexpr int NS = Sh::NS, PL = HILO ? 2 : 1;
+    // registers of a row's thread and of the others': 512 R + 128 C = 640 x 96, what the launch holds
+    constexpr int REG_ROW = 104, REG_CTRL = 64;
     const PagedAttnArgs& A = X.a;
     const PagedArgs& P = A.p;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    __shared__ TcBarriers B;
-    __shared__ uint32_t s_tmem;
-    __shared__ int abort_flag, s_skip[2], s_bad[2];
-    __shared__ int s_tile[6];
-    __shared__ float s_cf[TC_ROWS];               // 2^e of each f32 row
-    __shared__ uint32_t s_in[TC_MASKS][4];        // which keys of a tile exist (bytes of eight)
+    TcControl& C = *reinterpret_cast<TcControl*>(smem_raw);
+    TcBarriers& B = C.bars;
+    auto& s_in = C.in;
+    auto& s_pair = C.pair;
+    auto& s_skip = C.skip;
+    auto& s_bad = C.bad;
+    auto& s_tile = C.tile;
+    int& abort_flag = C.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t q_s = base, ring = base + 2 * Sh::QH;
+    const uint32_t q_s = smem_u32(smem_raw) + TC_CTRL, ring = q_s + 2 * Sh::QH;
 
     if (warp == 0) {
         int seq = 0, tile = 0;
@@ -272,26 +294,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             mbar_init(&B.empty[i], 1);
         }
         for (int h = 0; h < 2; h++) {
-            mbar_init(&B.q_ready[h], 128);
+            mbar_init(&B.q_ready[h], 256);
             mbar_init(&B.s_full[h], 1);
-            mbar_init(&B.p_ready[h][0], 128);
-            mbar_init(&B.p_ready[h][1], 128);
+            mbar_init(&B.p_ready[h][0], 256);
+            mbar_init(&B.p_ready[h][1], 256);
             mbar_init(&B.o_full[h], 1);
-            mbar_init(&B.vote[h], 128);
+            mbar_init(&B.vote[h], 256);
         }
+        for (int i = 0; i < 8; i++) mbar_init(&B.fin[i], 64);
         mbar_init(&B.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
+    if (warp == 16) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&C.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = C.tmem;
     if (!s_tile[0]) {  // the grid is an upper bound
-        if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
         return;
     }
     const int run = blockIdx.x % X.nsplit, kvh = blockIdx.y;
@@ -300,15 +323,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
     const int mtot = (int)min((int64_t)(r1 - r0) * A.G, (int64_t)m0 + TC_ROWS);  // rows up to this tile's end
     const TcRange rg = tc_range(A, first, m0, mtot, run, X.nsplit, TMA ? X.box : 0);
 
-    if (warp < 8) {
+    if (warp < 16) {
         // ================ the halves: queries, weights, outputs
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_ROW));
-        const int h = warp >> 2, r = (warp & 3) * 32 + lane;
+        const int h = warp >> 3, g = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;  // half, key half, row
         const int mh = m0 + h * TC_HALF, rows = min(max(mtot - mh, 0), TC_HALF);
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s_col = tmem + lane_off + (uint32_t)(h * 128), o_col = tmem + lane_off + 256u + (uint32_t)(h * 128);
+        // this thread's 64 score columns and HD / 2 output columns
+        constexpr int HO = HD / 2;
+        const uint32_t s_col = tmem + lane_off + (uint32_t)(h * 128 + g * 64), o_col = tmem + lane_off + 256u + (uint32_t)(h * 128 + g * HO);
         const uint32_t qs = q_s + h * Sh::QH;
+        // the other warp of these rows (one that gives up arrives once more, so that nobody is left waiting)
+        const int pair_id = 1 + h * 4 + (warp & 3);
+        auto pair_sync = [&]() { named_sync(pair_id, 64); };
         bool ok = true;
+        float up = 1.0f;  // 2^e of an f32 row
         // ---- queries.  Eight rows are QG bytes, whether as they come (f32 or fp16
         // rows one after the other) or as the products take them (128-byte pieces
         // of the eight rows), so a warp copies its rows as they come and turns
@@ -316,10 +345,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         if (rg.hb[h] > rg.ha[h]) {
             constexpr int EPL = HILO ? 4 : 8, LPR = HD / EPL, RPI = 32 / LPR;  // elements a lane, lanes a row, rows at once
             const int d = (lane % LPR) * EPL;
-            const uint32_t mine = qs + (uint32_t)((warp & 3) * 4 * Sh::QG);
+            const uint32_t mine = qs + (uint32_t)(((warp & 3) * 4 + g * 2) * Sh::QG);  // 16 rows
+            const int row0 = (warp & 3) * 32 + g * 16;
 #pragma unroll 4
-            for (int i = 0; i < 32 / RPI; i++) {
-                const int rr = i * RPI + lane / LPR, row = (warp & 3) * 32 + rr, m = mh + row;
+            for (int i = 0; i < 16 / RPI; i++) {
+                const int rr = i * RPI + lane / LPR, row = row0 + rr, m = mh + row;
                 const bool there = row < rows && d < P.hd;
                 const int t = there ? m / A.G : 0;
                 const QT* q = (const QT*)A.q + (there ? (int64_t)(r0 + t) * A.q_rs + (kvh * A.G + m - t * A.G) * A.q_hs + d : 0);
@@ -340,14 +370,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             __syncwarp();
             if constexpr (HILO) {
 #pragma unroll 1
-                for (int g = 0; g < 4; g++) {
+                for (int e8 = 0; e8 < 2; e8++) {
                     constexpr int N = 8 / RPI;
                     float f[N][4];
 #pragma unroll
                     for (int i = 0; i < N; i++)
                         asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
                                      : "=f"(f[i][0]), "=f"(f[i][1]), "=f"(f[i][2]), "=f"(f[i][3])
-                                     : "r"(mine + (uint32_t)(g * Sh::QG + (i * RPI + lane / LPR) * HD * 4 + (lane % LPR) * 16)));
+                                     : "r"(mine + (uint32_t)(e8 * Sh::QG + (i * RPI + lane / LPR) * HD * 4 + (lane % LPR) * 16)));
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < N; i++) {
@@ -360,39 +390,42 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                         uint32_t hi[2], lo[2];
                         split2(f[i][0] * down, f[i][1] * down, hi[0], lo[0]);
                         split2(f[i][2] * down, f[i][3] * down, hi[1], lo[1]);
-                        const uint32_t dst = mine + (uint32_t)(g * Sh::QG + (d >> 6) * 1024 + rr * 128 + ((((d & 63) >> 3) ^ rr) << 4) + (d & 7) * 2);
+                        const uint32_t dst = mine + (uint32_t)(e8 * Sh::QG + (d >> 6) * 1024 + rr * 128 + ((((d & 63) >> 3) ^ rr) << 4) + (d & 7) * 2);
                         asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst), "r"(hi[0]), "r"(hi[1]) : "memory");
                         asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst + Sh::QG / 2), "r"(lo[0]), "r"(lo[1]) : "memory");
-                        if (lane % LPR == 0) s_cf[h * TC_HALF + (warp & 3) * 32 + g * 8 + rr] = __uint_as_float((uint32_t)e << 23);
+                        if (lane % LPR == 0) s_pair[h * TC_HALF + row0 + e8 * 8 + rr][0] = __uint_as_float((uint32_t)e << 23);
                     }
                     __syncwarp();
                 }
             }
             fence_async_shared();
-            mbar_arrive(&B.q_ready[h]);
+            if constexpr (HILO) {
+                pair_sync();
+                up = s_pair[h * TC_HALF + r][0];
+                __syncwarp();
+            }
+            mbar_arrive(&B.q_ready[h]);  // (no scores, so nobody's next word in s_pair, before all have read it)
         }
         const bool in = r < rows;
         const int pos = in ? first + (mh + r) / A.G : -1;
         const int lo_pos = A.window > 0 ? pos - A.window + 1 : 0;
         const int p_min = first + mh / A.G, l_max = A.window > 0 ? first + (mh + rows - 1) / A.G - A.window + 1 : 0;
         const bool one_token = rows > 0 && mh / A.G == (mh + rows - 1) / A.G;
-        const float cf = A.scale * LOG2E * (HILO && in && rg.hb[h] > rg.ha[h] ? s_cf[h * TC_HALF + r] : 1.0f);
+        const float cf = A.scale * LOG2E * up;
         float m = -INFINITY, l = 0.0f;  // running maximum (log2 units), sum of weights
-        float acc[HILO ? HD : 1];       // f32 queries: the running outputs
+        float acc[HILO ? HO : 1];       // f32 queries: the running outputs
         if constexpr (HILO) {
 #pragma unroll
-            for (int i = 0; i < HD; i++) acc[i] = 0.0f;
+            for (int i = 0; i < HO; i++) acc[i] = 0.0f;
         }
         bool tile_out = false;          // f32 queries: a tile's outputs are in tensor memory
         auto add_tile = [&]() {
             if constexpr (HILO) {
-                uint32_t o[2][16];  // the next 16 columns load while these are added
-                tmem_ld_x16(o_col, o[0]);
 #pragma unroll
-                for (int c = 0; c < HD / 16; c++) {
-                    uint32_t* u = o[c & 1];
+                for (int c = 0; c < HO / 16; c++) {
+                    uint32_t u[16];
+                    tmem_ld_x16(o_col + 16u * c, u);
                     tmem_wait_ld16(u);
-                    if (c + 1 < HD / 16) tmem_ld_x16(o_col + 16u * (c + 1), o[(c + 1) & 1]);
 #pragma unroll
                     for (int i = 0; i < 16; i += 2)
                         untwo(add2(two(acc[16 * c + i], acc[16 * c + i + 1]), two(__uint_as_float(u[i]), __uint_as_float(u[i + 1]))),
@@ -410,22 +443,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             l *= f;
             return f;
         };
-        // A tile's products by the row's thread, masked keys left out: from the
-        // scores still in tensor memory into the half's outputs there.
+        // A tile's products by the row's threads, masked keys left out: from the
+        // scores still in tensor memory into the half's outputs there, this
+        // thread's columns of them.
         auto careful = [&](float nb, bool add, uint32_t vt, int hi_c, int lo_c, const uint32_t* bits) {
 #pragma unroll 1
-            for (int c0 = 0; c0 < HD; c0 += 8) {
+            for (int c1 = 0; c1 < HO; c1 += 8) {
+                const int c0 = g * HO + c1;
                 uint32_t u[8];
                 float o[8];
                 if (add) {
-                    tmem_ld_x8(o_col + c0, u);
+                    tmem_ld_x8(o_col + c1, u);
                     tmem_wait_ld();
                 }
 #pragma unroll
                 for (int i = 0; i < 8; i++) o[i] = add ? __uint_as_float(u[i]) : 0.0f;
 #pragma unroll 1
                 for (int k = 0; k < TC_KEYS; k += 8) {
-                    tmem_ld_x8(s_col + (uint32_t)k, u);
+                    tmem_ld_x8(s_col - (uint32_t)(g * 64) + (uint32_t)k, u);
                     tmem_wait_ld();
 #pragma unroll
                     for (int y = 0; y < 8; y++) {
@@ -447,19 +482,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                 }
 #pragma unroll
                 for (int i = 0; i < 8; i++) u[i] = __float_as_uint(o[i]);
-                tmem_st_x8(o_col + c0, u);
+                tmem_st_x8(o_col + c1, u);
             }
             tmem_wait_st();
+            pair_sync();  // both have read the scores that the weights will overwrite
         };
         uint32_t done = 0, votes = 0;
         for (int j = rg.ha[h]; j < rg.hb[h]; j++, done++) {
-            ok = mbar_wait(&B.s_full[h], done & 1u, &abort_flag);
+            ok = quick_wait(&B.s_full[h], done & 1u, &abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tmem_fence_after();
             const int k0 = rg.begin + j * TC_KEYS;
             const uint32_t* bits = s_in[j % TC_MASKS];
-            const bool whole = k0 + TC_KEYS - 1 <= p_min && k0 >= l_max && (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu;
+            const uint4 b4 = *reinterpret_cast<const uint4*>(bits);
+            const bool whole = k0 + TC_KEYS - 1 <= p_min && k0 >= l_max && (b4.x & b4.y & b4.z & b4.w) == 0xffffffffu;
             const int hi_c = pos - k0, lo_c = lo_pos - k0;
             // A key that some rows of the half see and others do not must not
             // reach the latter through 0 * v where v is not finite: such a tile
@@ -479,7 +516,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                 // their values become zeros (by both halves, before either's products)
                 if (k0 + r < rg.seen || k0 + r >= rg.end)
 #pragma unroll 1
-                    for (int c = 0; c < HD / 64; c++)
+                    for (int c = g; c < HD / 64; c += 2)
 #pragma unroll
                         for (int i = 0; i < 8; i++)
                             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vt + (uint32_t)(c * (TC_KEYS * 128) + r * 128 + i * 16)), "r"(0) : "memory");
@@ -488,7 +525,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             if (!whole && !one_token) {
                 // (the other half may still be writing its zeros: a stranger is not looked at)
                 uint32_t bad = 0;
-                for (int i = r; i < Sh::TILE / 16; i += TC_HALF) {
+                for (int i = r + g * TC_HALF; i < Sh::TILE / 16; i += 2 * TC_HALF) {
                     const int key = k0 + (i >> 3) % TC_KEYS;
                     if (key < rg.seen || key >= rg.end) continue;
                     uint32_t w[4];
@@ -505,15 +542,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                 if (!ok) break;
                 skip = *(volatile int*)&s_bad[h] == j + 1;
             }
-            if (r == 0) s_skip[h] = skip;
+            if (r == 0 && g == 0) s_skip[h] = skip;
 
             if (!whole) {
                 // masked scores become -inf where they stand
 #pragma unroll 1
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < 2; c++) {
                     // the visible keys of these 32, as bits
-                    const int up = min(hi_c - 32 * c, 31), dn = max(lo_c - 32 * c, 0);
-                    const uint32_t vis = up < dn ? 0u : bits[c] & (0xffffffffu >> (31 - up)) & (0xffffffffu << dn);
+                    const int up = min(hi_c - 64 * g - 32 * c, 31), dn = max(lo_c - 64 * g - 32 * c, 0);
+                    const uint32_t vis = up < dn ? 0u : bits[2 * g + c] & (0xffffffffu >> (31 - up)) & (0xffffffffu << dn);
 #pragma unroll 1
                     for (int y = 0; y < 32; y += 16) {
                         uint32_t v[16];
@@ -528,41 +565,44 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                 tmem_wait_st();
             }
             float sum0 = 0.0f, sum1 = 0.0f;
+            // the row's maximum: this thread's 64 keys and the other's
+            auto row_max = [&](float x) -> float {
+                s_pair[h * TC_HALF + r][g] = x;
+                pair_sync();
+                return max3(x, s_pair[h * TC_HALF + r][g ^ 1], x) * cf;
+            };
             if constexpr (HILO) {
                 if (tile_out) add_tile();
                 tile_out = true;
                 float x0 = -INFINITY, x1 = -INFINITY;
-                uint32_t vv[2][16];
-                tmem_ld_x16(s_col, vv[0]);
 #pragma unroll
-                for (int c = 0; c < 8; c++) {
-                    uint32_t* v = vv[c & 1];
+                for (int c = 0; c < 4; c++) {
+                    uint32_t v[16];
+                    tmem_ld_x16(s_col + 16u * c, v);
                     tmem_wait_ld16(v);
-                    tmem_ld_x16(s_col + 16u * ((c + 1) & 7), vv[(c + 1) & 1]);  // the last one: the first again, for the weights
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         x0 = max3(x0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
                         x1 = max3(x1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
                     }
                 }
-                const float nm = max3(x0, x1, x1) * cf;
+                const float nm = row_max(max3(x0, x1, x1));
                 const bool raise = !(nm <= m);
                 if (__any_sync(0xffffffffu, raise)) {
                     const float f = move_max(nm, raise);
                     const f2 ff = two(f, f);
 #pragma unroll
-                    for (int i = 0; i < HD; i += 2) untwo(mul2(two(acc[i], acc[i + 1]), ff), acc[i], acc[i + 1]);
+                    for (int i = 0; i < HO; i += 2) untwo(mul2(two(acc[i], acc[i + 1]), ff), acc[i], acc[i + 1]);
                 }
                 const float nb = m == -INFINITY ? 0.0f : BIAS_EXACT - m;
                 if (skip) careful(nb, false, vt, hi_c, lo_c, bits);
                 const f2 cf2 = two(cf, cf), nb2 = two(nb, nb), minus = two(-1.0f, -1.0f);
                 f2 sum = 0;
 #pragma unroll
-                for (int c = 0; c < 8; c++) {
-                    uint32_t hi[8], lo[8];
-                    uint32_t* v = vv[c & 1];
+                for (int c = 0; c < 4; c++) {
+                    uint32_t v[16], hi[8], lo[8];
+                    tmem_ld_x16(s_col + 16u * c, v);
                     tmem_wait_ld16(v);
-                    if (c < 7) tmem_ld_x16(s_col + 16u * (c + 1), vv[(c + 1) & 1]);
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
                         float a, b;
@@ -571,14 +611,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                         sum = add2(sum, w);
                         untwo(w, a, b);
                         hi[i / 2] = pack(a, b);
-                        const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi[i / 2]));
-                        untwo(fma2(two(g.x, g.y), minus, w), a, b);
+                        const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&hi[i / 2]));
+                        untwo(fma2(two(q.x, q.y), minus, w), a, b);
                         lo[i / 2] = pack(a, b);
                     }
                     // weights over the scores just read: hi in 8 columns, lo in the next 8
                     tmem_st_x8(s_col + 16u * c, hi);
                     tmem_st_x8(s_col + 16u * c + 8u, lo);
-                    if (c == 3) {
+                    if (c == 1) {
                         tmem_wait_st();
                         tmem_fence_before();
                         mbar_arrive(&B.p_ready[h][0]);
@@ -586,14 +626,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                 }
                 untwo(sum, sum0, sum1);
             } else {
-                uint32_t sr[128];
-#pragma unroll
-                for (int c = 0; c < 4; c++) tmem_ld_x32(s_col + 32u * c, sr + 32 * c);
+                uint32_t sr[64];
+                tmem_ld_x32(s_col, sr);
+                tmem_ld_x32(s_col + 32u, sr + 32);
                 tmem_wait_ld();
                 float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 128; c += 2) x[(c >> 1) & 3] = max3(x[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
-                const float nm = max3(max3(x[0], x[1], x[2]), x[3], x[3]) * cf;
+                for (int c = 0; c < 64; c += 2) x[(c >> 1) & 3] = max3(x[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+                const float nm = row_max(max3(max3(x[0], x[1], x[2]), x[3], x[3]));
                 const bool raise = !(nm <= m + TAU);
                 if (__any_sync(0xffffffffu, raise)) {
                     const float f = move_max(nm, raise);
@@ -601,7 +641,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                         // the products of the tile before are complete: this tile's
                         // scores were committed after them
 #pragma unroll 1
-                        for (int c = 0; c < HD / 16; c++) {
+                        for (int c = 0; c < HO / 16; c++) {
                             uint32_t o[16];
                             tmem_ld_x16(o_col + 16u * c, o);
                             tmem_wait_ld16(o);
@@ -616,7 +656,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                 const f2 cf2 = two(cf, cf), nb2 = two(nb, nb);
                 f2 sum[2] = {0, 0};
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < 2; c++) {
                     uint32_t w[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
@@ -633,8 +673,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                         sum[i & 1] = add2(sum[i & 1], two(a, b));
                         w[i] = pack(a, b);
                     }
+                    // weights over this thread's own scores: 64 in 32 columns
                     tmem_st_x16(s_col + 16u * c, w);
-                    if (c == 1) {
+                    if (c == 0) {
                         tmem_wait_st();
                         tmem_fence_before();
                         mbar_arrive(&B.p_ready[h][0]);
@@ -655,9 +696,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             tmem_fence_after();
             if (ok && tile_out) add_tile();
         }
+        if (!ok) named_arrive(pair_id, 64);
+        auto fin_sync = [&](uint32_t parity) -> bool {  // bounded: the other warp may have given up
+            mbar_arrive(&B.fin[pair_id - 1]);
+            return mbar_wait(&B.fin[pair_id - 1], parity, &abort_flag);
+        };
+        // the row's sum: this thread's keys and the other's
+        if (rows > 0) {
+            s_pair[h * TC_HALF + r][g] = l;
+            ok = __all_sync(0xffffffffu, fin_sync(0) && ok && !*(volatile int*)&abort_flag);
+            l += s_pair[h * TC_HALF + r][g ^ 1];
+        }
         if (!ok) l = __int_as_float(0x7fffffff);  // a wait ran out: the row is NaN, not a wrong number
         const int64_t pr = (((int64_t)(blockIdx.x / X.nsplit) * P.nkv + kvh) * X.nsplit + run) * TC_ROWS + h * TC_HALF + r;
-        if (in) {
+        if (in && g == 0) {
             if (X.nsplit > 1) {
                 X.pml[pr] = make_float2(m == -INFINITY ? m : m - (HILO ? BIAS_EXACT : BIAS), l);
             } else if (A.lse) {
@@ -671,8 +723,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         // through the half's query memory (its products are done), so that a
         // warp's stores are whole rows
         const uint32_t stage = qs + (uint32_t)((warp & 3) * 32 * HD * (int)sizeof(QT));
-#pragma unroll(HILO ? HD / 16 : 1)
-        for (int c = 0; c < HD / 16; c++) {
+#pragma unroll(HILO ? HO / 16 : 1)
+        for (int c = 0; c < HO / 16; c++) {
+            const int cc = g * (HO / 16) + c;
             uint32_t o[16];
             if constexpr (HILO) {
 #pragma unroll
@@ -689,14 +742,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             if (X.nsplit > 1) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
-                    if (in && 16 * c + i < P.hd)
-                        *reinterpret_cast<uint4*>(X.po + pr * P.hd + 16 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    if (in && 16 * cc + i < P.hd)
+                        *reinterpret_cast<uint4*>(X.po + pr * P.hd + 16 * cc + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
             } else {
                 const uint32_t row_at = stage + (uint32_t)(lane * HD * (int)sizeof(QT));
                 if constexpr (HILO) {
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + (((4 * c + i) ^ (lane & 7)) << 4)),
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + (((4 * cc + i) ^ (lane & 7)) << 4)),
                                      "r"(o[4 * i]), "r"(o[4 * i + 1]), "r"(o[4 * i + 2]), "r"(o[4 * i + 3])
                                      : "memory");
                 } else {
@@ -705,19 +758,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                     for (int i = 0; i < 8; i++) w[i] = pack(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
 #pragma unroll
                     for (int i = 0; i < 2; i++)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + (((2 * c + i) ^ (lane & 7)) << 4)),
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + (((2 * cc + i) ^ (lane & 7)) << 4)),
                                      "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3])
                                      : "memory");
                 }
             }
         }
-        if (X.nsplit == 1) {
-            __syncwarp();
+        if (X.nsplit == 1 && rows > 0) {
+            fin_sync(1);
             constexpr int EPL = 16 / (int)sizeof(QT), LPR = HD / EPL, RPI = 32 / LPR;
             const int d = (lane % LPR) * EPL;
 #pragma unroll 4
-            for (int i = 0; i < 32 / RPI; i++) {
-                const int rr = i * RPI + lane / LPR, row = (warp & 3) * 32 + rr;
+            for (int i = 0; i < 16 / RPI; i++) {
+                const int rr = g * 16 + i * RPI + lane / LPR, row = (warp & 3) * 32 + rr;
                 if (row >= rows || d >= P.hd) continue;
                 uint32_t w[4];
                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -739,72 +792,83 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         tmem_fence_before();
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_CTRL));
-      if (warp == 8) {
-        // ================ the products
+      if (warp == 16) {
+        // ================ the products.  What addresses them is the same in all
+        // lanes and said to be so: issued from ordinary registers a product took 90
+        // to 110 cycles of the issuing warp, where the tensor core takes 64.
         constexpr uint32_t idesc_s = make_idesc_mn(128, 128);
         constexpr uint32_t idesc_o = make_idesc_mn(128, HD) | (1u << 16);  // V is MN-major
+        const int ja = __shfl_sync(0xffffffffu, rg.ja, 0), jb = __shfl_sync(0xffffffffu, rg.jb, 0);
+        const int ha0 = __shfl_sync(0xffffffffu, rg.ha[0], 0), hb0 = __shfl_sync(0xffffffffu, rg.hb[0], 0);
+        const int ha1 = __shfl_sync(0xffffffffu, rg.ha[1], 0), hb1 = __shfl_sync(0xffffffffu, rg.hb[1], 0);
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        // eight rows of queries are QG apart
+        const uint64_t q_d = (sw128_desc(q_s) & ~((uint64_t)0x3FFF << 32)) | (uint64_t)(Sh::QG >> 4) << 32;
+        const uint64_t k_d0 = sw128_desc(ring), v_d0 = sw128_mn_desc(ring);
         bool ok = true;
         uint32_t pdone[2] = {0, 0};
-        const uint64_t q_d = (sw128_desc(q_s) & ~((uint64_t)0x3FFF << 32)) | (uint64_t)(Sh::QG >> 4) << 32;  // eight rows are QG apart
-        for (int j = rg.ja; j <= rg.jb && ok; j++) {
-            const int nk = 2 * (j - rg.ja), nv = nk - 1;  // ring places of K_j and V_(j-1)
-            const uint64_t k_d = sw128_desc(ring + (nk % NS) * Sh::TILE), v_d = sw128_mn_desc(ring + (nv + NS) % NS * Sh::TILE);
-            if (j > rg.ja) ok = warp_wait(&B.full[nv % NS], (uint32_t)(nv / NS) & 1u, &abort_flag);
-            if (j < rg.jb) ok = ok && warp_wait(&B.full[nk % NS], (uint32_t)(nk / NS) & 1u, &abort_flag);
-            if (!ok) break;
-            for (int h = 0; h < 2 && ok; h++) {
-                const uint32_t s_t = tmem + (uint32_t)(h * 128), o_t = tmem + 256u + (uint32_t)(h * 128);
-                const bool pv = j - 1 >= rg.ha[h] && j - 1 < rg.hb[h], sc = j >= rg.ha[h] && j < rg.hb[h];
-                if (pv) {  // O_h += P_h V_(j-1), the first 64 keys as soon as their weights are there
-                    for (int half = 0; half < 2; half++) {
-                        ok = warp_wait(&B.p_ready[h][half], pdone[h] & 1u, &abort_flag);
-                        if (!ok) break;
-                        tmem_fence_after();
-                        if (!*(volatile int*)&s_skip[h] && elect_one()) {
+        int ks = 0, vs = NS - 1;          // ring slots of K_j and V_(j-1), with their phases
+        uint32_t kph = 0, vph = 1;
+        for (int j = ja; j <= jb && ok; j++) {
+            const uint64_t k_d = k_d0 + (uint64_t)(ks * (Sh::TILE >> 4)), v_d = v_d0 + (uint64_t)(vs * (Sh::TILE >> 4));
+            int vs2 = vs + 2;             // V_j
+            uint32_t vph2 = vph;
+            if (vs2 >= NS) vs2 -= NS, vph2 ^= 1u;
 #pragma unroll
-                            for (int p = PL - 1; p >= 0; p--)
+            for (int h = 0; h < 2; h++) {
+                const uint32_t s_t = tm + (uint32_t)(h * 128), o_t = tm + 256u + (uint32_t)(h * 128);
+                const int ha = h ? ha1 : ha0, hb = h ? hb1 : hb0;
+                const bool pv = j - 1 >= ha && j - 1 < hb, sc = j >= ha && j < hb;
+                bool mul = false;  // O_h += P_h V_(j-1), half of the keys as soon as their weights are there
+                auto add_pv = [&](int part) {
 #pragma unroll
-                                for (int k4 = 0; k4 < 4; k4++) {
-                                    const int kk = half * 4 + k4;
-                                    mma_f16_ts(o_t, s_t + (uint32_t)(HILO ? kk * 16 + p * 8 : kk * 8), v_d + (uint64_t)(kk * (2048 >> 4)), idesc_o,
-                                               (!HILO && pdone[h] > 0) || half > 0 || k4 > 0 || p < PL - 1);
-                                }
+                    for (int p = PL - 1; p >= 0; p--)
+#pragma unroll
+                        for (int k4 = 0; k4 < 4; k4++) {
+                            const int kk = (k4 >> 1) * 4 + part * 2 + (k4 & 1);  // of the eight steps of 16 keys
+                            mma_f16_ts(o_t, s_t + (uint32_t)(HILO ? kk * 16 + p * 8 : (kk >> 2) * 64 + (kk & 3) * 8), v_d + (uint64_t)(kk * (2048 >> 4)),
+                                       idesc_o, (!HILO && pdone[h] > 0) || part > 0 || k4 > 0 || p < PL - 1);
                         }
-                        __syncwarp();
-                    }
-                    if (!ok) break;
-                    pdone[h]++;
-                }
-                if (sc) {  // S_h = Q_h K_j^T
-                    if (j == rg.ha[h]) {
-                        ok = warp_wait(&B.q_ready[h], 0, &abort_flag);
-                        if (!ok) break;
-                    }
+                };
+                if (pv) {
+                    ok = quick_wait(&B.p_ready[h][0], pdone[h] & 1u, &abort_flag);
                     tmem_fence_after();
-                    if (elect_one()) {
+                    mul = !*(volatile int*)&s_skip[h];
+                    if (mul && elect_one()) add_pv(0);
+                    __syncwarp();
+                }
+                // the copies, while the other weights are made: K_j before its first use, V_j before the next step
+                if (h == 0 && j < jb) ok = ok && quick_wait(&B.full[ks], kph, &abort_flag);
+                if (h == 1 && j < jb) ok = ok && quick_wait(&B.full[vs2], vph2, &abort_flag);
+                if (sc && j == ha) ok = ok && quick_wait(&B.q_ready[h], 0, &abort_flag);
+                if (pv) ok = ok && quick_wait(&B.p_ready[h][1], pdone[h] & 1u, &abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tmem_fence_after();
+                if (elect_one()) {
+                    if (mul) add_pv(1);
+                    if (h == 1 && j > ja) mma_commit(&B.empty[vs]);
+                    if (sc) {  // S_h = Q_h K_j^T
 #pragma unroll
                         for (int p = PL - 1; p >= 0; p--)
 #pragma unroll
                             for (int kk = 0; kk < HD / 16; kk++) {
-                                const uint32_t qo = (uint32_t)(h * Sh::QH + (p * (HD / 64) + (kk >> 2)) * 1024 + (kk & 3) * 32);
+                                const uint32_t qo = (uint32_t)((p * (HD / 64) + (kk >> 2)) * 1024 + (kk & 3) * 32);
                                 const uint32_t ko = (uint32_t)((kk >> 2) * (TC_KEYS * 128) + (kk & 3) * 32);
-                                mma_f16_ss(s_t, q_d + (uint64_t)(qo >> 4), k_d + (uint64_t)(ko >> 4), idesc_s, kk > 0 || p < PL - 1);
+                                mma_f16_ss(s_t, q_d + (uint64_t)((h * Sh::QH + qo) >> 4), k_d + (uint64_t)(ko >> 4), idesc_s, kk > 0 || p < PL - 1);
                             }
                         mma_commit(&B.s_full[h]);
                     }
-                    __syncwarp();
+                    if (h == 1 && j < jb) mma_commit(&B.empty[ks]);
+                    if (j == hb && hb > ha) mma_commit(&B.o_full[h]);
                 }
-                if (j == rg.hb[h] && rg.hb[h] > rg.ha[h]) {
-                    if (elect_one()) mma_commit(&B.o_full[h]);
-                    __syncwarp();
-                }
+                __syncwarp();
+                if (pv) pdone[h]++;
             }
-            if (!ok) break;
-            if (elect_one()) {
-                if (j > rg.ja) mma_commit(&B.empty[nv % NS]);
-                if (j < rg.jb) mma_commit(&B.empty[nk % NS]);
-            }
-            __syncwarp();
+            ks += 2;
+            if (ks >= NS) ks -= NS, kph ^= 1u;
+            vs = vs2;
+            vph = vph2;
         }
         if (!ok) {  // let what is in flight end before tensor memory is given back
             if (elect_one()) mma_commit(&B.drain);
@@ -813,7 +877,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             mbar_wait(&B.drain, 0, &none);
         }
         tmem_fence_before();
-      } else if (TMA && warp == 9) {
+      } else if (TMA && warp == 17) {
         // ================ the copies: lane l takes the tile's l-th box
         bool ok = true;
         int copied = 0;
@@ -861,7 +925,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         }
       } else if constexpr (!TMA) {
         // ================ the copies: groups lw, lw + 3, ... of eight keys, four lanes a key
-        const int lw = warp - 9;
+        const int lw = warp - 17;
         constexpr int CPL = HD / 32;     // 16-byte chunks of a row per lane
         constexpr int NG = 6;            // groups of a warp: 6, 5 and 5 of the 16
         bool ok = true;
@@ -934,7 +998,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
       }
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 16) {
         tmem_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
