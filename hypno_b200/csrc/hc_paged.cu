@@ -29,8 +29,103 @@ __device__ __forceinline__ int seq_of_row(const PagedArgs& P, int r) {
     return lo;
 }
 
-// One thread per pair of a head: (x0, x1) -> (x0 c - x1 s, x0 s + x1 c) for
-// the pairs of the first rot elements, copies for the others and for v.
+// 16-byte groups.  A unit is eight elements of a head: four pairs, which lie
+// side by side (adjacent) or in two runs of four (halves), or eight elements
+// past rot or of v, which pass through.  A block takes one row, its threads up
+// to NU units each: all loads of a thread are in flight before the row's
+// place in the cache (three dependent loads: row start, length, page) is known.
+// Bound by its bytes: q is read and written, k and v are read and stored.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float* v) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 x = __ldcs(reinterpret_cast<const float4*>(p));
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+        const uint2 x = __ldcs(reinterpret_cast<const uint2*>(p));
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&x.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&x.y));
+        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float* v) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+        *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+}
+
+constexpr int AP_THREADS = 256;
+
+template <typename T, typename C, int NU>
+__global__ void __launch_bounds__(AP_THREADS) k_paged_append_vec(AppendArgs A) {
+    const PagedArgs& P = A.p;
+    const int row = blockIdx.x, hu = P.hd >> 3, half = A.rot >> 1;
+    const int units = (A.nh + 2 * P.nkv) * hu;
+    const int first = blockIdx.y * (AP_THREADS * NU) + threadIdx.x;
+    float v[NU][8];
+    int head[NU], i0[NU], i1[NU];  // first elements of the two runs of four
+#pragma unroll
+    for (int n = 0; n < NU; n++) {
+        const int unit = first + n * AP_THREADS;
+        head[n] = unit < units ? unit / hu : -1;
+        if (head[n] < 0) continue;
+        const int u = unit - head[n] * hu;
+        i0[n] = 8 * u;
+        i1[n] = i0[n] + 4;
+        if (A.halves && i0[n] < A.rot) {
+            i0[n] = 4 * u;
+            i1[n] = i0[n] + half;
+        }
+        const T* src = head[n] < A.nh             ? (const T*)A.q + row * A.q_rs + head[n] * A.q_hs
+                       : head[n] < A.nh + P.nkv ? (const T*)A.k + row * A.k_rs + (head[n] - A.nh) * A.k_hs
+                                                  : (const T*)A.v + row * A.v_rs + (head[n] - A.nh - P.nkv) * A.v_hs;
+        load4(src + i0[n], v[n]);
+        load4(src + i1[n], v[n] + 4);
+    }
+    const int seq = seq_of_row(P, row);
+    int r0, r1;
+    seq_rows(P, seq, r0, r1);
+    if (row < r0 || row >= r1) return;
+    const int pos = __ldg(P.kv_len + seq) - (r1 - r0) + (row - r0);
+    const float2* cs = A.rope + (int64_t)min(max(pos, 0), A.rope_rows - 1) * half;
+    int slot = 0;
+    const int page = pos >= 0 ? lookup(P, seq, pos, slot) : -1;
+#pragma unroll
+    for (int n = 0; n < NU; n++) {
+        if (head[n] < 0) continue;
+        const bool is_q = head[n] < A.nh, is_v = head[n] >= A.nh + P.nkv;
+        float* x = v[n];
+        if (i0[n] < A.rot && !is_v) {
+            const int j = A.halves ? i0[n] : i0[n] >> 1;  // first pair
+            const float4 c01 = __ldg(reinterpret_cast<const float4*>(cs + j)), c23 = __ldg(reinterpret_cast<const float4*>(cs + j + 2));
+            const float c[4] = {c01.x, c01.z, c23.x, c23.z}, s[4] = {c01.y, c01.w, c23.y, c23.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                // static places: a pair is (i, i + 4) or (2 i, 2 i + 1)
+                const float a = A.halves ? x[i] : x[2 * i], b = A.halves ? x[i + 4] : x[2 * i + 1];
+                const float ra = a * c[i] - b * s[i], rb = a * s[i] + b * c[i];
+                if (A.halves) x[i] = ra, x[i + 4] = rb;
+                else x[2 * i] = ra, x[2 * i + 1] = rb;
+            }
+        }
+        if (is_q) {
+            T* dst = (T*)A.qo + row * A.o_rs + head[n] * A.o_hs;
+            store4(dst + i0[n], x);
+            store4(dst + i1[n], x + 4);
+        } else if (page >= 0) {
+            C* dst = is_v ? (C*)P.v + page * P.vps + (head[n] - A.nh - P.nkv) * P.vhs + slot * P.vss
+                          : (C*)P.k + page * P.kps + (head[n] - A.nh) * P.khs + slot * P.kss;
+            store4(dst + i0[n], x);
+            store4(dst + i1[n], x + 4);
+        }
+    }
+}
+
+// Any head size and alignment: one thread per pair of a head,
+// (x0, x1) -> (x0 c - x1 s, x0 s + x1 c) for the pairs of the first rot
+// elements, copies for the others and for v.
 template <typename T, typename C>
 __global__ void __launch_bounds__(256) k_paged_append(AppendArgs A) {
     const PagedArgs& P = A.p;
@@ -122,14 +217,14 @@ __global__ void __launch_bounds__(GT) k_paged_generic(PagedAttnArgs A) {
     const int T_b = r1 - r0, m0 = s_tile * GM, mrows = min(GM, T_b * A.G - m0);
     const int first = __ldg(P.kv_len + seq) - T_b;  // position of the sequence's first row
     for (int i = threadIdx.x; i < mrows * hd; i += GT) {
-        const int m = i / hd, d = i - m * hd, row = (m0 + m) / A.G, g = (m0 + m) - row * A.G;
+        const int m = i / hd, d = i - m * hd, row = token_of(A, m0 + m), g = (m0 + m) - row * A.G;
         Q[m * ldk + d] = to_f32(((const T*)A.q)[(r0 + row) * A.q_rs + (kvh * A.G + g) * A.q_hs + d]) * A.scale;
     }
     const int m = threadIdx.x >> 3, t = threadIdx.x & 7;
-    const int pos = m < mrows ? first + (m0 + m) / A.G : -1;
+    const int pos = m < mrows ? first + token_of(A, m0 + m) : -1;
     const int lo = A.window > 0 ? max(0, pos - A.window + 1) : 0;
-    const int last = first + (m0 + mrows - 1) / A.G;                      // last position seen by the tile
-    const int p0 = first + m0 / A.G;
+    const int last = first + token_of(A, m0 + mrows - 1);                      // last position seen by the tile
+    const int p0 = first + token_of(A, m0);
     const int begin = A.window > 0 ? max(0, p0 - A.window + 1) / GN * GN : 0;
     float o[HDMAX / 8];
 #pragma unroll
@@ -195,7 +290,7 @@ __global__ void __launch_bounds__(GT) k_paged_generic(PagedAttnArgs A) {
         __syncwarp();
     }
     if (m >= mrows) return;
-    const int row = r0 + (m0 + m) / A.G, head = kvh * A.G + (m0 + m) % A.G;
+    const int row = r0 + token_of(A, m0 + m), head = kvh * A.G + (m0 + m) % A.G;
     const float inv = 1.0f / l;
     T* out = (T*)A.out + row * A.o_rs + head * A.o_hs;
 #pragma unroll
@@ -283,9 +378,25 @@ int rows_ok(const char* who, const char* what, const hc_rows& r, uint32_t dtype)
 
 template <typename T, typename C>
 int launch_append(const hc::AppendArgs& A, cudaStream_t s) {
-    const int64_t units = (int64_t)(A.nh + 2 * A.p.nkv) * ((A.p.hd + 1) / 2);
-    HC_CHECK(units <= 65535 * 256ll, HC_ERR_INVALID, "hc_paged_append_dev: %d + %d heads of %d", A.nh, A.p.nkv, A.p.hd);
-    hc::k_paged_append<T, C><<<dim3((unsigned)A.p.n_rows, (unsigned)((units + 255) / 256)), 256, 0, s>>>(A);
+    const hc::PagedArgs& P = A.p;
+    // 16-byte groups: whole eights of elements and pairs, rows and pools aligned
+    const int64_t et = 16 / (int64_t)sizeof(T), ec = 16 / (int64_t)sizeof(C);
+    const bool vec = P.hd % 8 == 0 && A.rot % 8 == 0 &&
+                     ((uintptr_t)A.k | (uintptr_t)A.v | (uintptr_t)A.q | (uintptr_t)A.qo | (uintptr_t)A.rope | (uintptr_t)P.k | (uintptr_t)P.v) % 16 == 0 &&
+                     (A.k_rs | A.k_hs | A.v_rs | A.v_hs | (A.nh ? A.q_rs | A.q_hs | A.o_rs | A.o_hs : 0)) % et == 0 &&
+                     (P.kps | P.khs | P.kss | P.vps | P.vhs | P.vss) % ec == 0;
+    const int64_t units = vec ? (int64_t)(A.nh + 2 * P.nkv) * (P.hd / 8) : (int64_t)(A.nh + 2 * P.nkv) * ((P.hd + 1) / 2);
+    HC_CHECK(units <= 65535 * 256ll, HC_ERR_INVALID, "hc_paged_append_dev: %d + %d heads of %d", A.nh, P.nkv, P.hd);
+    // Few rows: one unit a thread, blocks over the row (the latency of one chain
+    // counts).  Many: three units a thread, as many loads in flight and a third
+    // of the chains.
+    if (vec && (int64_t)P.n_rows * units < 148 * 8 * 256) {
+        hc::k_paged_append_vec<T, C, 1><<<dim3((unsigned)P.n_rows, (unsigned)((units + 255) / 256)), 256, 0, s>>>(A);
+    } else if (vec) {
+        hc::k_paged_append_vec<T, C, 3><<<dim3((unsigned)P.n_rows, (unsigned)((units + 767) / 768)), 256, 0, s>>>(A);
+    } else {
+        hc::k_paged_append<T, C><<<dim3((unsigned)P.n_rows, (unsigned)((units + 255) / 256)), 256, 0, s>>>(A);
+    }
     HC_LAUNCH_CHECK();
     return HC_OK;
 }
@@ -349,6 +460,9 @@ static int attn_checks(const char* who, const hc_paged_kv* kv, const hc_paged_ba
     HC_CHECK(window >= 0, HC_ERR_INVALID, "%s: window %d", who, window);
     A.nh = n_heads;
     A.G = n_heads / A.p.nkv;
+    A.g_shift = -1;
+    for (int i = 0; i < 31; i++)
+        if (A.G == (1 << i)) A.g_shift = i;
     A.window = window;
     return HC_OK;
 }

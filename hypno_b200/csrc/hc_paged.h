@@ -31,6 +31,7 @@ struct PagedAttnArgs {
     int64_t q_rs, q_hs, o_rs, o_hs;  // row / head strides, in elements
     float* lse;                      // [n_rows][nh], may be null
     int nh, G;                       // query heads, query heads per KV head
+    int g_shift;                     // >= 0: G = 1 << g_shift
     int window;                      // > 0: only the last `window` positions
     float scale;
     int qvec, ovec;                  // 16-byte aligned rows of q / out
@@ -39,6 +40,9 @@ struct PagedAttnArgs {
 __device__ __forceinline__ int page_of(const PagedArgs& P, int pos) {
     return P.page_shift >= 0 ? (pos >> P.page_shift) : pos / P.page_size;
 }
+
+// Token of packed row m (within its sequence).
+__device__ __forceinline__ int token_of(const PagedAttnArgs& A, int m) { return A.g_shift >= 0 ? m >> A.g_shift : m / A.G; }
 
 // Page of position pos (>= 0) of sequence seq, -1 for a hole; slot = the
 // position's place in it.
@@ -129,8 +133,8 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 }
 // Visible positions of packed rows [m0, m0 + n) of a sequence: [begin, end).
 __device__ __forceinline__ void visible(const PagedAttnArgs& A, int first, int m0, int n, int& begin, int& end) {
-    end = max(0, first + (m0 + n - 1) / A.G + 1);
-    begin = A.window > 0 ? max(0, first + m0 / A.G - A.window + 1) : 0;
+    end = max(0, first + token_of(A, m0 + n - 1) + 1);
+    begin = A.window > 0 ? max(0, first + token_of(A, m0) - A.window + 1) : 0;
     begin = min(begin, end);
 }
 

@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
         for (int n = 0; n < NQ; n++) {
             const int m = n * 8 + (lane >> 2);
             const bool in = m < mrows;
-            const int t = (m0 + m) / A.G;
+            const int t = token_of(A, m0 + m);
             const QT* q = (const QT*)A.q + (in ? (int64_t)(r0 + t) * A.q_rs + (kvh * A.G + (m0 + m) - t * A.G) * A.q_hs : 0);
             float c = A.scale * LOG2E;
             if constexpr (C16) {
@@ -328,13 +328,13 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
             for (int x = 0; x < 2; x++) {
                 cf[n][x] = __shfl_sync(0xffffffffu, c, (col + x) * 4);
                 const int mm = n * 8 + col + x;
-                ps[n][x] = mm < mrows ? first + (m0 + mm) / A.G : -1;
+                ps[n][x] = mm < mrows ? first + token_of(A, m0 + mm) : -1;
                 lo[n][x] = A.window > 0 ? ps[n][x] - A.window + 1 : 0;
             }
         }
         // keys that every row of the tile sees
-        const int p_min = first + m0 / A.G, l_max = A.window > 0 ? first + (m0 + mrows - 1) / A.G - A.window + 1 : 0;
-        const bool one_token = m0 / A.G == (m0 + mrows - 1) / A.G;
+        const int p_min = first + token_of(A, m0), l_max = A.window > 0 ? first + token_of(A, m0 + mrows - 1) - A.window + 1 : 0;
+        const bool one_token = token_of(A, m0) == token_of(A, m0 + mrows - 1);
 
         float o[NQ][DT][4];
         float mx[NQ][2], sum[NQ][2];  // running maximum; sum of this thread's keys only
@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
                 v.w = fmaf(f, y.w, v.w);
             }
             if (!cut) {
-                const int t = (m0 + m) / A.G, row = r0 + t, head = kvh * A.G + (m0 + m) - t * A.G;
+                const int t = token_of(A, m0 + m), row = r0 + t, head = kvh * A.G + (m0 + m) - t * A.G;
                 store_row4<QT>(A, row, head, d, l, v);
                 if (A.lse && d == 0)
                     A.lse[(int64_t)row * A.nh + head] = l == 0.0f ? -INFINITY : (mm - BIAS + log2f(l)) / LOG2E;
@@ -671,7 +671,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_join(const __grid_constant
             v.z = fmaf(f, y.z, v.z);
             v.w = fmaf(f, y.w, v.w);
         }
-        const int t = (m0 + m) / A.G, row = r0 + t, head = kvh * A.G + (m0 + m) - t * A.G;
+        const int t = token_of(A, m0 + m), row = r0 + t, head = kvh * A.G + (m0 + m) - t * A.G;
         store_row4<QT>(A, row, head, d, l, v);
         if (A.lse && d == 0)
             A.lse[(int64_t)row * A.nh + head] = l == 0.0f ? -INFINITY : (mx + log2f(l)) / LOG2E;

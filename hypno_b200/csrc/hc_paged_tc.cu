@@ -39,10 +39,9 @@
 // four rows an instruction took 78 cycles each, 10,000 a pair.)  Keys without a
 // page are zeros; keys of a box that no row sees are zeroed by the rows' threads.
 //
-// The loops of the rows' warps are kept short (masked scores are rewritten in
-// tensor memory by a loop of its own, values that are not finite have one too):
-// the instruction fetch of code unrolled for every case cost more than its
-// arithmetic.
+// The loop of the rows' warps is kept short (values that are not finite have a
+// loop of their own): the instruction fetch of code unrolled for every case cost
+// more than its arithmetic.
 #include "hc_paged.h"
 #include "hc_tc.cuh"
 
@@ -351,7 +350,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             for (int i = 0; i < 16 / RPI; i++) {
                 const int rr = i * RPI + lane / LPR, row = row0 + rr, m = mh + row;
                 const bool there = row < rows && d < P.hd;
-                const int t = there ? m / A.G : 0;
+                const int t = there ? token_of(A, m) : 0;
                 const QT* q = (const QT*)A.q + (there ? (int64_t)(r0 + t) * A.q_rs + (kvh * A.G + m - t * A.G) * A.q_hs + d : 0);
                 const uint32_t dst = mine + (HILO ? (uint32_t)(rr * HD * 4 + (lane % LPR) * 16)
                                                   : (uint32_t)((rr >> 3) * Sh::QG + (d >> 6) * 1024 + (rr & 7) * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4)));
@@ -383,8 +382,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                     for (int i = 0; i < N; i++) {
                         const int rr = i * RPI + lane / LPR;  // of the eight
                         float mx = fmaxf(fmaxf(fabsf(f[i][0]), fabsf(f[i][1])), fmaxf(fabsf(f[i][2]), fabsf(f[i][3])));
+                        if constexpr (LPR == 32) {  // |q| orders like its bits
+                            mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+                        } else {
 #pragma unroll
-                        for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                            for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        }
                         const int e = min(max((int)(__float_as_uint(mx) >> 23), 2), 252);
                         const float down = __uint_as_float((uint32_t)(254 - e) << 23);
                         uint32_t hi[2], lo[2];
@@ -407,10 +410,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             mbar_arrive(&B.q_ready[h]);  // (no scores, so nobody's next word in s_pair, before all have read it)
         }
         const bool in = r < rows;
-        const int pos = in ? first + (mh + r) / A.G : -1;
+        const int pos = in ? first + token_of(A, mh + r) : -1;
         const int lo_pos = A.window > 0 ? pos - A.window + 1 : 0;
-        const int p_min = first + mh / A.G, l_max = A.window > 0 ? first + (mh + rows - 1) / A.G - A.window + 1 : 0;
-        const bool one_token = rows > 0 && mh / A.G == (mh + rows - 1) / A.G;
+        const int p_min = first + token_of(A, mh), l_max = A.window > 0 ? first + token_of(A, mh + rows - 1) - A.window + 1 : 0;
+        const bool one_token = rows > 0 && token_of(A, mh) == token_of(A, mh + rows - 1);
         const float cf = A.scale * LOG2E * up;
         float m = -INFINITY, l = 0.0f;  // running maximum (log2 units), sum of weights
         float acc[HILO ? HO : 1];       // f32 queries: the running outputs
@@ -527,7 +530,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                 uint32_t bad = 0;
                 for (int i = r + g * TC_HALF; i < Sh::TILE / 16; i += 2 * TC_HALF) {
                     const int key = k0 + (i >> 3) % TC_KEYS;
-                    if (key < rg.seen || key >= rg.end) continue;
+                    if (key < rg.seen || key >= rg.end || (key <= p_min && key >= l_max)) continue;  // nobody's, or everybody's
                     uint32_t w[4];
                     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
@@ -544,25 +547,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             }
             if (r == 0 && g == 0) s_skip[h] = skip;
 
+            uint32_t vis[2] = {0u, 0u};  // the visible ones of this thread's keys, as bits
             if (!whole) {
-                // masked scores become -inf where they stand
-#pragma unroll 1
-                for (int c = 0; c < 2; c++) {
-                    // the visible keys of these 32, as bits
-                    const int up = min(hi_c - 64 * g - 32 * c, 31), dn = max(lo_c - 64 * g - 32 * c, 0);
-                    const uint32_t vis = up < dn ? 0u : bits[2 * g + c] & (0xffffffffu >> (31 - up)) & (0xffffffffu << dn);
-#pragma unroll 1
-                    for (int y = 0; y < 32; y += 16) {
-                        uint32_t v[16];
-                        tmem_ld_x16(s_col + (uint32_t)(32 * c + y), v);
-                        tmem_wait_ld16(v);
 #pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            if (!((vis >> y >> i) & 1u)) v[i] = 0xff800000u;
-                        tmem_st_x16(s_col + (uint32_t)(32 * c + y), v);
-                    }
+                for (int c = 0; c < 2; c++) {
+                    const int up = min(hi_c - 64 * g - 32 * c, 31), dn = max(lo_c - 64 * g - 32 * c, 0);
+                    if (up >= dn) vis[c] = bits[2 * g + c] & (0xffffffffu >> (31 - up)) & (0xffffffffu << dn);
                 }
-                tmem_wait_st();
             }
             float sum0 = 0.0f, sum1 = 0.0f;
             // the row's maximum: this thread's 64 keys and the other's
@@ -580,12 +571,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                     uint32_t v[16];
                     tmem_ld_x16(s_col + 16u * c, v);
                     tmem_wait_ld16(v);
+                    if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (!((vis[c >> 1] >> (16 * (c & 1) + i)) & 1u)) v[i] = 0xff800000u;
+                        tmem_st_x16(s_col + 16u * c, v);  // they are read again
+                    }
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         x0 = max3(x0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
                         x1 = max3(x1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
                     }
                 }
+                if (!whole) tmem_wait_st();
                 const float nm = row_max(max3(x0, x1, x1));
                 const bool raise = !(nm <= m);
                 if (__any_sync(0xffffffffu, raise)) {
@@ -630,6 +628,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                 tmem_ld_x32(s_col, sr);
                 tmem_ld_x32(s_col + 32u, sr + 32);
                 tmem_wait_ld();
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 64; i++)
+                        if (!((vis[i >> 5] >> (i & 31)) & 1u)) sr[i] = 0xff800000u;
+                }
                 float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int c = 0; c < 64; c += 2) x[(c >> 1) & 3] = max3(x[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
@@ -713,7 +716,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             if (X.nsplit > 1) {
                 X.pml[pr] = make_float2(m == -INFINITY ? m : m - (HILO ? BIAS_EXACT : BIAS), l);
             } else if (A.lse) {
-                const int t = (mh + r) / A.G;
+                const int t = token_of(A, mh + r);
                 A.lse[(int64_t)(r0 + t) * A.nh + kvh * A.G + (mh + r) - t * A.G] =
                     l == 0.0f ? -INFINITY : (m - (HILO ? BIAS_EXACT : BIAS) + log2f(l)) / LOG2E;
             }
@@ -776,7 +779,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                              : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                              : "r"(stage + (uint32_t)(rr * HD * (int)sizeof(QT)) + (((lane % LPR) ^ (rr & 7)) << 4)));
-                const int t = (mh + row) / A.G;
+                const int t = token_of(A, mh + row);
                 QT* out = (QT*)A.out + (int64_t)(r0 + t) * A.o_rs + (kvh * A.G + (mh + row) - t * A.G) * A.o_hs + d;
                 if (A.ovec) {
                     *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -1036,7 +1039,7 @@ __global__ void __launch_bounds__(256) k_paged_tc_join(const __grid_constant__ T
             v.z = fmaf(f, y.z, v.z);
             v.w = fmaf(f, y.w, v.w);
         }
-        const int t = (m0 + m) / A.G, row = r0 + t, head = kvh * A.G + (m0 + m) - t * A.G;
+        const int t = token_of(A, m0 + m), row = r0 + t, head = kvh * A.G + (m0 + m) - t * A.G;
         store_row4<QT>(A, row, head, d, l, v);
         if (A.lse && d == 0)
             A.lse[(int64_t)row * A.nh + head] = l == 0.0f ? -INFINITY : (mx + log2f(l)) / LOG2E;
