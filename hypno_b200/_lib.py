@@ -5,6 +5,7 @@ the library is missing or cannot be loaded, every entry point raises.
 """
 import ctypes
 import os
+import struct
 import threading
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libhypno_cuda.so")
@@ -72,28 +73,9 @@ class HcPagedKV(ctypes.Structure):
     ]
 
 
-class HcPagedBatch(ctypes.Structure):
-    _fields_ = [
-        ("block_table", ctypes.c_void_p),
-        ("q_start", ctypes.c_void_p),
-        ("kv_len", ctypes.c_void_p),
-        ("table_stride", ctypes.c_int64),
-        ("n_seqs", ctypes.c_int32),
-        ("max_pages", ctypes.c_int32),
-        ("n_rows", ctypes.c_int32),
-        ("max_q_len", ctypes.c_int32),
-        ("max_kv_len", ctypes.c_int32),
-        ("reserved", ctypes.c_int32),
-    ]
-
-
-class HcRows(ctypes.Structure):
-    _fields_ = [
-        ("data", ctypes.c_void_p),
-        ("row_stride", ctypes.c_int64),
-        ("head_stride", ctypes.c_int64),
-    ]
-
+# hc_paged_batch and hc_rows, in the order of their fields: passed by address as packed bytes
+HC_PAGED_BATCH = struct.Struct("PPPq6i")
+HC_ROWS = struct.Struct("Pqq")
 
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
@@ -144,9 +126,9 @@ SIGNATURES = {
     "hc_sample_dev": (_I, [_P, _SZ, _I, _I, _P, _P, _P, _P, _P, _P]),
     "hc_argmax_dev": (_I, [_P, _SZ, _I, _I, _I, _P, _P, _P]),
     "hc_sample_uniform_dev": (_I, [_P, _SZ, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P]),
-    "hc_paged_append_dev": (_I, [_P, _P, HcRows, HcRows, HcRows, HcRows, _I, _U32, _P, _I, _I, _I, _P]),
+    "hc_paged_append_dev": (_I, [_P, _P, _P, _P, _P, _P, _I, _U32, _P, _I, _I, _I, _P]),
     "hc_paged_attention_workspace": (_I, [_P, _P, _I, _U32, _I, ctypes.POINTER(_SZ)]),
-    "hc_paged_attention_dev": (_I, [_P, _P, HcRows, HcRows, _P, _I, _U32, _F, _I, _P, _SZ, _P]),
+    "hc_paged_attention_dev": (_I, [_P, _P, _P, _P, _P, _I, _U32, _F, _I, _P, _SZ, _P]),
     "hc_rope_table_host": (_I, [_SZ, _SZ, _F, _P]),
     "hc_phase_name": (ctypes.c_char_p, [_I]),
     "hc_comm_unique_id": (_I, [_P]),
@@ -191,3 +173,10 @@ def check(rc):
 def call(name, *args):
     """Calls an int-returning entry point and raises on failure."""
     return check(getattr(load(), name)(*args))
+
+
+def raw_stream(index):
+    """torch's current stream of a CUDA device, as the integer the C ABI takes."""
+    import torch
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return get(index) if get is not None else torch.cuda.current_stream(index).cuda_stream

@@ -370,9 +370,9 @@ int paged_args(const char* who, const hc_paged_kv* kv, const hc_paged_batch* b, 
     return HC_OK;
 }
 
-int rows_ok(const char* who, const char* what, const hc_rows& r, uint32_t dtype) {
-    HC_CHECK(r.data, HC_ERR_INVALID, "%s: NULL %s", who, what);
-    HC_CHECK((uintptr_t)r.data % (dtype == HC_DTYPE_FP16 ? 2 : 4) == 0, HC_ERR_INVALID, "%s: misaligned %s", who, what);
+int rows_ok(const char* who, const char* what, const hc_rows* r, uint32_t dtype) {
+    HC_CHECK(r && r->data, HC_ERR_INVALID, "%s: NULL %s", who, what);
+    HC_CHECK((uintptr_t)r->data % (dtype == HC_DTYPE_FP16 ? 2 : 4) == 0, HC_ERR_INVALID, "%s: misaligned %s", who, what);
     return HC_OK;
 }
 
@@ -403,8 +403,8 @@ int launch_append(const hc::AppendArgs& A, cudaStream_t s) {
 
 }  // namespace
 
-HC_EXPORT int hc_paged_append_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, hc_rows k, hc_rows v, hc_rows q,
-                                  hc_rows q_out, int n_heads, uint32_t dtype, const float* rope, int rope_rows,
+HC_EXPORT int hc_paged_append_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_rows* k, const hc_rows* v,
+                                  const hc_rows* q, const hc_rows* q_out, int n_heads, uint32_t dtype, const float* rope, int rope_rows,
                                   int rot_dim, int half_pairs, void* stream) {
     const char* who = "hc_paged_append_dev";
     hc::AppendArgs A;
@@ -422,28 +422,30 @@ HC_EXPORT int hc_paged_append_dev(const hc_paged_kv* kv, const hc_paged_batch* b
     if (batch->n_rows == 0) return HC_OK;
     HC_TRY(rows_ok(who, "k", k, dtype));
     HC_TRY(rows_ok(who, "v", v, dtype));
-    if (q.data) {
+    if (q) {
         HC_CHECK(n_heads > 0, HC_ERR_INVALID, "%s: q without heads", who);
         HC_TRY(rows_ok(who, "q", q, dtype));
         HC_TRY(rows_ok(who, "q_out", q_out, dtype));
     }
-    A.k = k.data;
-    A.k_rs = k.row_stride;
-    A.k_hs = k.head_stride;
-    A.v = v.data;
-    A.v_rs = v.row_stride;
-    A.v_hs = v.head_stride;
-    A.q = q.data;
-    A.q_rs = q.row_stride;
-    A.q_hs = q.head_stride;
-    A.qo = q_out.data;
-    A.o_rs = q_out.row_stride;
-    A.o_hs = q_out.head_stride;
+    const hc_rows none = {nullptr, 0, 0};
+    if (!q) q = q_out = &none;
+    A.k = k->data;
+    A.k_rs = k->row_stride;
+    A.k_hs = k->head_stride;
+    A.v = v->data;
+    A.v_rs = v->row_stride;
+    A.v_hs = v->head_stride;
+    A.q = q->data;
+    A.q_rs = q->row_stride;
+    A.q_hs = q->head_stride;
+    A.qo = q_out->data;
+    A.o_rs = q_out->row_stride;
+    A.o_hs = q_out->head_stride;
     A.rope = (const float2*)rope;
     A.rope_rows = rope_rows;
     A.rot = rope ? rot_dim : 0;
     A.halves = half_pairs;
-    A.nh = q.data ? n_heads : 0;
+    A.nh = q->data ? n_heads : 0;
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == HC_DTYPE_FP16)
         return kv->kv_dtype == HC_KV_FP16 ? launch_append<__half, __half>(A, s) : launch_append<__half, float>(A, s);
@@ -501,8 +503,8 @@ HC_EXPORT int hc_paged_attention_workspace(const hc_paged_kv* kv, const hc_paged
     return HC_OK;
 }
 
-HC_EXPORT int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, hc_rows q, hc_rows out,
-                                     float* lse, int n_heads, uint32_t dtype, float scale, int window, void* workspace,
+HC_EXPORT int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_rows* q,
+                                     const hc_rows* out, float* lse, int n_heads, uint32_t dtype, float scale, int window, void* workspace,
                                      size_t workspace_bytes, void* stream) {
     const char* who = "hc_paged_attention_dev";
     hc::PagedAttnArgs A;
@@ -510,18 +512,18 @@ HC_EXPORT int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch
     if (batch->n_rows == 0) return HC_OK;
     HC_TRY(rows_ok(who, "q", q, dtype));
     HC_TRY(rows_ok(who, "out", out, dtype));
-    A.q = q.data;
-    A.q_rs = q.row_stride;
-    A.q_hs = q.head_stride;
-    A.out = out.data;
-    A.o_rs = out.row_stride;
-    A.o_hs = out.head_stride;
+    A.q = q->data;
+    A.q_rs = q->row_stride;
+    A.q_hs = q->head_stride;
+    A.out = out->data;
+    A.o_rs = out->row_stride;
+    A.o_hs = out->head_stride;
     A.lse = lse;
     A.scale = scale;
     const int q16 = dtype == HC_DTYPE_FP16, c16 = kv->kv_dtype == HC_KV_FP16;
     const int64_t e = q16 ? 8 : 4;
-    A.qvec = (uintptr_t)q.data % 16 == 0 && (q.row_stride | q.head_stride) % e == 0;
-    A.ovec = (uintptr_t)out.data % 16 == 0 && (out.row_stride | out.head_stride) % e == 0;
+    A.qvec = (uintptr_t)q->data % 16 == 0 && (q->row_stride | q->head_stride) % e == 0;
+    A.ovec = (uintptr_t)out->data % 16 == 0 && (out->row_stride | out->head_stride) % e == 0;
     AttnPlan plan = attn_plan(A, batch, c16);
     HC_CHECK(workspace_bytes >= plan.bytes && (plan.bytes == 0 || (workspace && (uintptr_t)workspace % 16 == 0)),
              HC_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, plan.bytes,

@@ -26,13 +26,13 @@ import ctypes
 import numpy as np
 import torch
 
-from ._lib import (DTYPE_FP16, DTYPE_FP32, KV_FP16, KV_FP32, HcPagedBatch, HcPagedKV, HcRows, call, check, load)
+from ._lib import (DTYPE_FP16, DTYPE_FP32, HC_PAGED_BATCH, HC_ROWS, KV_FP16, KV_FP32, HcPagedKV, call, check, load, raw_stream)
 
 __all__ = ["PagedKV", "PagedBatch", "append", "attention", "rope_table", "PageTable"]
 
 _DTYPE = {torch.float32: DTYPE_FP32, torch.float16: DTYPE_FP16}
 _KV = {torch.float32: KV_FP32, torch.float16: KV_FP16}
-_NO_ROWS = HcRows(None, 0, 0)
+_pack = HC_ROWS.pack
 
 
 class PagedKV:
@@ -67,12 +67,12 @@ class PagedKV:
         return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
 
 
-def _int32(t, name, dim, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dim or t.device != device:
-        raise TypeError(f"{name} must be a {dim}-dimensional int32 tensor on {device}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+def _int32(t, name, dim, index):
+    """Raises for what PagedBatch does not take."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.dim() != dim or t.get_device() != index or index < 0:
+        raise TypeError(f"{name} must be a {dim}-dimensional int32 CUDA tensor on the device of kv_len")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name} must be contiguous along its last dimension")
-    return t.data_ptr()
 
 
 class PagedBatch:
@@ -83,48 +83,49 @@ class PagedBatch:
     max_q_len and max_kv_len are the host's upper bounds on a sequence's rows
     and positions: they choose launches, not results."""
 
-    __slots__ = ("block_table", "q_start", "kv_len", "n_seqs", "max_q_len", "max_kv_len", "device", "struct", "ref",
-                 "n_rows")
+    __slots__ = ("block_table", "q_start", "kv_len", "max_q_len", "max_kv_len", "index", "n_rows", "blob")
 
     def __init__(self, block_table, q_start, kv_len, max_q_len, max_kv_len):
-        device = kv_len.device
-        table = _int32(block_table, "block_table", 2, device)
-        start = _int32(q_start, "q_start", 1, device)
-        length = _int32(kv_len, "kv_len", 1, device)
-        n = kv_len.shape[0]
-        if block_table.shape[0] != n or q_start.shape[0] != n + 1:
-            raise ValueError(f"{n} sequences need a block_table of {n} rows and {n + 1} row starts")
+        index = kv_len.get_device()
+        _int32(kv_len, "kv_len", 1, index)
+        _int32(block_table, "block_table", 2, index)
+        _int32(q_start, "q_start", 1, index)
+        n = block_table.shape[0]
+        if kv_len.shape[0] != n or q_start.shape[0] != n + 1:
+            raise ValueError(f"a block_table of {n} rows needs {n} lengths and {n + 1} row starts")
         if max_q_len < 0 or max_kv_len < 0:
             raise ValueError("max_q_len and max_kv_len must not be negative")
         self.block_table, self.q_start, self.kv_len = block_table, q_start, kv_len
-        self.n_seqs, self.max_q_len, self.max_kv_len, self.device = n, int(max_q_len), int(max_kv_len), device
+        self.max_q_len, self.max_kv_len, self.index = max_q_len, max_kv_len, index
         self.n_rows = -1
-        self.struct = HcPagedBatch(table, start, length, block_table.stride(0), n, block_table.shape[1], 0,
-                                   self.max_q_len, self.max_kv_len, 0)
-        self.ref = ctypes.addressof(self.struct)
 
-    def _rows(self, n):
-        if n != self.n_rows:
-            self.n_rows = self.struct.n_rows = n
-        return self.ref
+    def pack(self, n_rows):
+        """The batch with so many rows as the C ABI takes it."""
+        if n_rows != self.n_rows:
+            t = self.block_table
+            n, pages = t.shape
+            self.blob = HC_PAGED_BATCH.pack(t.data_ptr(), self.q_start.data_ptr(), self.kv_len.data_ptr(), t.stride(0), n,
+                                            pages, n_rows, self.max_q_len, self.max_kv_len, 0)
+            self.n_rows = n_rows
+        return self.blob
 
 
-def _rows(t, name, kv, dtype, n_rows=None):
-    if t.dim() != 3 or t.dtype != dtype or t.device != kv.device:
+def _rows(t, name, kv, dtype, n):
+    shape = t.shape
+    if len(shape) != 3 or t.dtype is not dtype or t.get_device() != kv.index:
         raise TypeError(f"{name} must be a 3-dimensional {dtype} tensor on {kv.device}")
-    r, h, d = t.shape
-    if d != kv.head_dim or (n_rows is not None and r != n_rows):
-        raise ValueError(f"{name} of shape {tuple(t.shape)}: the cache has heads of {kv.head_dim}"
-                         + (f", the batch {n_rows} rows" if n_rows is not None else ""))
     rs, hs, ds = t.stride()
+    d = shape[2]
+    if d != kv.head_dim or shape[0] != n:
+        raise ValueError(f"{name} of shape {tuple(shape)}: the cache has heads of {kv.head_dim}, the call {n} rows")
     if ds != 1 and d > 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
-    return HcRows(t.data_ptr(), rs, hs)
+    return _pack(t.data_ptr(), rs, hs)
 
 
 def _same_device(kv, batch):
-    if batch.device != kv.device:
-        raise ValueError(f"the batch is on {batch.device}, the pool on {kv.device}")
+    if batch.index != kv.index:
+        raise ValueError(f"the batch is on cuda:{batch.index}, the pool on {kv.device}")
 
 
 def append(kv, batch, k, v, q=None, rope=None, pairs="adjacent", q_out=None):
@@ -138,21 +139,22 @@ def append(kv, batch, k, v, q=None, rope=None, pairs="adjacent", q_out=None):
     strides; no two rows of one call may name the same position."""
     _same_device(kv, batch)
     dtype = k.dtype
-    if dtype not in _DTYPE:
+    code = _DTYPE.get(dtype)
+    if code is None:
         raise TypeError(f"k must be float32 or float16, not {dtype}")
     n = k.shape[0]
-    ks, vs = _rows(k, "k", kv, dtype), _rows(v, "v", kv, dtype, n)
+    ks, vs = _rows(k, "k", kv, dtype, n), _rows(v, "v", kv, dtype, n)
     if k.shape[1] != kv.n_kv_heads or v.shape[1] != kv.n_kv_heads:
         raise ValueError(f"k and v need the cache's {kv.n_kv_heads} heads")
     if pairs != "adjacent" and pairs != "halves":
         raise ValueError(f"pairs must be 'adjacent' or 'halves', not {pairs!r}")
-    qs = os_ = _NO_ROWS
+    qs = os_ = None
     heads = 0
     if q is not None:
         qs = _rows(q, "q", kv, dtype, n)
         heads = q.shape[1]
         if q_out is None:
-            q_out = torch.empty((n, heads, kv.head_dim), dtype=dtype, device=kv.device)
+            q_out = q.new_empty(q.shape)
         elif q_out.shape != q.shape:
             raise ValueError("q_out must have the shape of q")
         os_ = _rows(q_out, "q_out", kv, dtype, n)
@@ -160,13 +162,14 @@ def append(kv, batch, k, v, q=None, rope=None, pairs="adjacent", q_out=None):
         raise ValueError("q_out without q")
     table, table_rows, rot = None, 0, 0
     if rope is not None:
-        if rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[2] != 2 or rope.device != kv.device:
+        shape = rope.shape
+        if rope.dtype is not torch.float32 or len(shape) != 3 or shape[2] != 2 or rope.get_device() != kv.index:
             raise TypeError(f"rope must be a [positions, rot / 2, 2] float32 tensor on {kv.device}")
         if not rope.is_contiguous():
             raise ValueError("rope must be contiguous")
-        table, table_rows, rot = rope.data_ptr(), rope.shape[0], 2 * rope.shape[1]
-    check(load().hc_paged_append_dev(kv.ref, batch._rows(n), ks, vs, qs, os_, heads, _DTYPE[dtype], table, table_rows, rot,
-                                     pairs == "halves", torch.cuda.current_stream(kv.device).cuda_stream))
+        table, table_rows, rot = rope.data_ptr(), shape[0], 2 * shape[1]
+    check(load().hc_paged_append_dev(kv.ref, batch.pack(n), ks, vs, qs, os_, heads, code, table, table_rows, rot,
+                                     pairs == "halves", raw_stream(kv.index)))
     return q_out
 
 
@@ -180,12 +183,13 @@ def attention(kv, batch, q, out=None, scale=None, window=0, lse=None):
     flat-cache forward passes keep the reference's polynomial)."""
     _same_device(kv, batch)
     dtype = q.dtype
-    if dtype not in _DTYPE:
+    code = _DTYPE.get(dtype)
+    if code is None:
         raise TypeError(f"q must be float32 or float16, not {dtype}")
-    qs = _rows(q, "q", kv, dtype)
     n, heads, dim = q.shape
+    qs = _rows(q, "q", kv, dtype, n)
     if out is None:
-        out = torch.empty((n, heads, dim), dtype=dtype, device=kv.device)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape:
         raise ValueError("out must have the shape of q")
     os_ = _rows(out, "out", kv, dtype, n)
@@ -194,15 +198,13 @@ def attention(kv, batch, q, out=None, scale=None, window=0, lse=None):
         if lse.dtype != torch.float32 or lse.shape != (n, heads) or not lse.is_contiguous() or lse.device != kv.device:
             raise TypeError(f"lse must be a contiguous [{n}, {heads}] float32 tensor on {kv.device}")
         lse_ptr = lse.data_ptr()
-    lib, ref = load(), batch._rows(n)
+    lib, ref = load(), batch.pack(n)
     need = ctypes.c_size_t()
-    check(lib.hc_paged_attention_workspace(kv.ref, ref, heads, _DTYPE[dtype], window, ctypes.byref(need)))
+    check(lib.hc_paged_attention_workspace(kv.ref, ref, heads, code, window, ctypes.byref(need)))
     # the workspace lives until the stream's later allocations reuse it: torch orders them after this call
     ws = torch.empty(need.value, dtype=torch.uint8, device=kv.device) if need.value else None
-    check(lib.hc_paged_attention_dev(kv.ref, ref, qs, os_, lse_ptr, heads, _DTYPE[dtype],
-                                     dim ** -0.5 if scale is None else scale, window,
-                                     ws.data_ptr() if ws is not None else None, need.value,
-                                     torch.cuda.current_stream(kv.device).cuda_stream))
+    check(lib.hc_paged_attention_dev(kv.ref, ref, qs, os_, lse_ptr, heads, code, dim ** -0.5 if scale is None else scale,
+                                     window, ws.data_ptr() if ws is not None else None, need.value, raw_stream(kv.index)))
     return out
 
 

@@ -6,7 +6,7 @@ its XorShift64 states is engine.DeviceSampler.
 """
 import torch
 
-from ._lib import check, load
+from ._lib import check, load, raw_stream
 
 __all__ = ["sample"]
 
@@ -14,9 +14,9 @@ __all__ = ["sample"]
 def _per_row(x, name, dtype, rows, device):
     if not isinstance(x, torch.Tensor):
         return torch.full((rows,), x, dtype=dtype, device=device)
-    if x.dtype != dtype or x.shape != (rows,) or x.device != device:
+    if x.dtype is not dtype or x.dim() != 1 or x.shape[0] != rows or x.get_device() != device.index:
         raise TypeError(f"{name} must be a number or a [{rows}] {dtype} tensor on {device}")
-    if rows > 1 and x.stride(0) != 1:
+    if x.stride(0) != 1 and rows > 1:
         raise ValueError(f"{name} must be contiguous")
     return x
 
@@ -47,12 +47,12 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
     k = _per_row(top_k, "top_k", i, rows, dev)
     p = _per_row(top_p, "top_p", f, rows, dev)
     m = _per_row(min_p, "min_p", f, rows, dev)
-    out = torch.empty(rows, dtype=i, device=dev) if out is None else _per_row(out, "out", i, rows, dev)
-    logprob = torch.empty(rows, dtype=f, device=dev) if logprob is None else _per_row(logprob, "logprob", f, rows, dev)
+    out = torch.empty_like(k) if out is None else _per_row(out, "out", i, rows, dev)
+    logprob = torch.empty_like(t) if logprob is None else _per_row(logprob, "logprob", f, rows, dev)
     ld = logits.stride(0) if rows > 1 else vocab
     if ld < vocab:
         raise ValueError("the rows of logits overlap")
     check(load().hc_sample_uniform_dev(logits.data_ptr(), ld, rows, vocab, u.data_ptr(), t.data_ptr(), k.data_ptr(),
                                        p.data_ptr(), m.data_ptr(), out.data_ptr(), logprob.data_ptr(),
-                                       torch.cuda.current_stream(dev).cuda_stream))
+                                       raw_stream(dev.index)))
     return out, logprob

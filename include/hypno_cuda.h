@@ -302,13 +302,13 @@ typedef struct hc_rows {
  * pairs of floats; NULL: no rotation), pair j of the first rot_dim elements
  * becomes (a c - b s, a s + b c); half_pairs 0: (a, b) = elements (2j, 2j + 1),
  * the reference's pairs (transformer.rs:317-343); 1: elements
- * (j, j + rot_dim / 2).  q (n_heads heads per row; q.data NULL: none) goes to
+ * (j, j + rot_dim / 2).  q (n_heads heads per row; NULL: none) goes to
  * q_out, which may be q itself.  q, k, v and q_out are `dtype`
  * (HC_DTYPE_FP32 or HC_DTYPE_FP16); arithmetic is f32, rounded once.  A row at
  * a hole stores nothing.  A position at or past rope_rows is refused on the
  * host where max_kv_len shows it; the kernel takes the last row otherwise. */
-int hc_paged_append_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, hc_rows k, hc_rows v, hc_rows q,
-                        hc_rows q_out, int n_heads, uint32_t dtype, const float* rope, int rope_rows, int rot_dim,
+int hc_paged_append_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_rows* k, const hc_rows* v,
+                        const hc_rows* q, const hc_rows* q_out, int n_heads, uint32_t dtype, const float* rope, int rope_rows, int rot_dim,
                         int half_pairs, void* stream);
 
 /* out[r][h] = sum_j softmax_j(scale * q[r][h] . k_j) v_j over the positions
@@ -324,7 +324,8 @@ int hc_paged_append_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, hc_r
  * head_dim <= 256. */
 int hc_paged_attention_workspace(const hc_paged_kv* kv, const hc_paged_batch* batch, int n_heads, uint32_t dtype,
                                  int window, size_t* bytes);
-int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, hc_rows q, hc_rows out, float* lse,
+int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_rows* q, const hc_rows* out,
+                           float* lse,
                            int n_heads, uint32_t dtype, float scale, int window, void* workspace, size_t workspace_bytes,
                            void* stream);
 

@@ -334,18 +334,20 @@ def test_refusals(cuda_device):
 
 
 def test_refusals_at_the_c_entry(cuda_device):
-    from hypno_b200._lib import HcRows, load
+    from hypno_b200._lib import HC_ROWS, load
     c = ref.Case([2, 1], [30, 7], 4, 2, 64, 16, 24)
     kv, batch, q, kn, vn = on_device(c, cuda_device)
-    r, none = HcRows(q.data_ptr(), 256, 64), HcRows(None, 0, 0)
+    r, none = HC_ROWS.pack(q.data_ptr(), 256, 64), HC_ROWS.pack(0, 0, 0)
     lib = load()
-    ref_b = batch._rows(3)
+    ref_b = batch.pack(3)
     assert lib.hc_paged_attention_dev(None, ref_b, r, r, None, 4, 0, 0.1, 0, None, 0, None) == -1
     assert lib.hc_paged_attention_dev(kv.ref, None, r, r, None, 4, 0, 0.1, 0, None, 0, None) == -1
     assert lib.hc_paged_attention_dev(kv.ref, ref_b, none, r, None, 4, 0, 0.1, 0, None, 0, None) == -1
     assert lib.hc_paged_attention_dev(kv.ref, ref_b, r, none, None, 4, 0, 0.1, 0, None, 0, None) == -1
     assert lib.hc_paged_attention_dev(kv.ref, ref_b, r, r, None, 4, 2, 0.1, 0, None, 0, None) == -3
-    assert lib.hc_paged_append_dev(kv.ref, ref_b, none, r, none, none, 0, 0, None, 0, 0, 0, None) == -1
+    assert lib.hc_paged_append_dev(kv.ref, ref_b, none, r, None, None, 0, 0, None, 0, 0, 0, None) == -1
+    assert lib.hc_paged_append_dev(kv.ref, ref_b, r, None, None, None, 0, 0, None, 0, 0, 0, None) == -1
+    assert lib.hc_paged_append_dev(kv.ref, ref_b, r, r, r, None, 4, 0, None, 0, 0, 0, None) == -1
     assert lib.hc_paged_attention_workspace(kv.ref, ref_b, 4, 0, 0, None) == -1
     kv.struct.page_size = 0
     assert lib.hc_paged_attention_dev(kv.ref, ref_b, r, r, None, 4, 0, 0.1, 0, None, 0, None) == -1
