@@ -8,18 +8,21 @@
 // drawn.  The kept set is a head of the order (logit descending, index
 // ascending), so one (key, index) pair cuts it off.
 //
-// k_sample_cluster: a cluster of up to 8 CTAs takes a row, each CTA a slice that
-// it reads once into shared memory.  Passes over the slice: the maximum; the
-// mass, with a histogram (count and mass) of the tokens within HEAD of the
-// maximum in units of T; the tokens of the bucket in which the head of the
-// order ends, gathered by the first CTA and sorted there; the kept mass of each
-// warp's run, in which the draw is then found.  A row whose order ends beyond
-// the histogram, or in a bucket too full to sort (flat rows), is left to the
-// first CTA and the kernel's slow path: a radix search over the logits' keys.
-// Bound by the latency of the cluster barriers for few rows, by the passes
-// over shared memory (not by the one read of the logits) for many.
+// k_sample_cluster: a cluster of up to 16 CTAs takes a row, each CTA a slice that
+// it reads once into shared memory.  Passes over the slice: the maximum; for
+// top-k a histogram (counts) of the tokens within HEAD of the maximum in units
+// of T, or beyond it where that has fewer than k; the tokens of the bucket in
+// which the order ends, gathered by the first CTA and sorted there; for top-p
+// the same by mass, over what top-k kept; the kept mass of each warp's run, in
+// which the draw is then found.  A bucket too full to sort (flat rows) is left
+// to the first CTA and the kernel's slow path: a radix search over the logits'
+// keys.  Bound by the latency of the cluster barriers for few rows, by the
+// instructions of the passes (not by the one read of the logits) for many: a
+// weight is some 30 of them.
 #include "hc_internal.h"
 #include "hc_common.cuh"
+
+#include <cfloat>
 
 namespace hc {
 
@@ -40,6 +43,10 @@ __device__ __forceinline__ float ukey_value(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
 
+// floor(2^40 w) for w in [0, 1].  (Moving the mantissa to its place by shifts
+// took a fifth longer than the conversion.)
+__device__ __forceinline__ u64 mass_of(float w) { return __float2ull_rz(__fmul_rn(w, 1099511627776.0f)); }
+
 struct URow {
     const float* l;
     int V;
@@ -48,7 +55,7 @@ struct URow {
         return f == mx ? 1.0f : expf(__fmul_rn(__fsub_rn(f, mx), inv));
     }
     __device__ __forceinline__ u64 mass(float f) const {
-        return f > -INFINITY ? __float2ull_rz(__fmul_rn(weight(f), 1099511627776.0f)) : 0ull;
+        return f > -INFINITY ? mass_of(weight(f)) : 0ull;
     }
 };
 
@@ -239,7 +246,7 @@ __device__ __noinline__ void sample_row(URow R, URowArgs P, UShared& S, int32_t*
 
 // ============================================================ the cluster kernel
 
-constexpr int UC_MAX = 8;          // CTAs of a cluster
+constexpr int UC_MAX = 16;         // CTAs of a cluster (above 8 for few long rows only)
 constexpr int HB2 = 1024;          // buckets of a histogram
 // Distances (max - l) / T that the two histograms cover: weights from 1 to 6e-6,
 // where most orders end and few tokens are, and from there to below 2^-40.
@@ -259,7 +266,7 @@ struct __align__(16) CShared {
     u64 red[32];
     uint32_t redu[32];
     // what the CTAs of the cluster tell one another, one word for each (all have the same copy)
-    uint32_t c_max[UC_MAX];
+    uint32_t c_max[UC_MAX], c_at[UC_MAX];
     u64 c_mass[UC_MAX];            // mass (pass 2), kept mass (pass 4)
     // what the first CTA tells all
     int n_list;
@@ -268,6 +275,9 @@ struct __align__(16) CShared {
     // the first CTA's own
     u64 sel_mass, head_mass;       // mass before the bucket; of the first histogram
     uint32_t sel_cnt, head_cnt;    // likewise tokens
+    u64 w_mass[UW];                // of the warps' buckets
+    uint32_t w_cnt[UW];
+    u64 sorted[256];
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -300,9 +310,20 @@ __device__ __forceinline__ u64 remote_ld64(const void* p, uint32_t rank) {
     return v;
 }
 
-// Descending bitonic sort of the first CTA's list.
-__device__ void sort_list(CShared& S, int n) {
-    int m = 1;
+// Descending sort of the first CTA's list: places by counting for short lists,
+// bitonic for long ones.  Returns where the sorted list is.
+__device__ u64* sort_list(CShared& S, int n) {
+    if (n <= 256) {
+        if ((int)threadIdx.x < n) {
+            const u64 e = S.h.list[threadIdx.x];
+            int at = 0;
+            for (int j = 0; j < n; j++) at += S.h.list[j] > e;
+            S.sorted[at] = e;
+        }
+        __syncthreads();
+        return S.sorted;
+    }
+    int m = 512;
     while (m < n) m <<= 1;
     for (int j = n + (int)threadIdx.x; j < m; j += UT) S.h.list[j] = 0ull;
     __syncthreads();
@@ -320,9 +341,10 @@ __device__ void sort_list(CShared& S, int n) {
             }
             __syncthreads();
         }
+    return S.h.list;
 }
 
-__global__ void __launch_bounds__(UT) k_sample_cluster(const float* __restrict__ logits, size_t ld, int V, int slice,
+__global__ void __launch_bounds__(UT, 2) k_sample_cluster(const float* __restrict__ logits, size_t ld, int V, int slice,
                                                        const float* __restrict__ u, const float* __restrict__ temp,
                                                        const int* __restrict__ top_k, const float* __restrict__ top_p,
                                                        const float* __restrict__ min_p, int32_t* __restrict__ out,
@@ -349,7 +371,7 @@ __global__ void __launch_bounds__(UT) k_sample_cluster(const float* __restrict__
     R.inv = T > 0.0f ? __fdiv_rn(1.0f, T) : 1.0f;
 
     // ---- 1: the slice and the maximum
-    uint32_t kmax = 0;
+    float top = -INFINITY;  // (NaN never wins)
     const float* src = R.l + base;
     const int head = min(n, (int)((16 - ((uintptr_t)src & 15)) & 15) / 4), n4 = (n - head) >> 2;  // 16-byte loads in between
     float* L = reinterpret_cast<float*>(smem + sizeof(CShared)) + ((4 - head) & 3);  // and 16-byte stores
@@ -357,15 +379,11 @@ __global__ void __launch_bounds__(UT) k_sample_cluster(const float* __restrict__
     for (int i = threadIdx.x; i < n4; i += UT) {
         const float4 v = __ldcs(reinterpret_cast<const float4*>(src + head) + i);
         *reinterpret_cast<float4*>(L + head + 4 * i) = v;
-        kmax = max(max(max(kmax, ukey(v.x)), max(ukey(v.y), ukey(v.z))), ukey(v.w));
+        top = fmaxf(fmaxf(fmaxf(top, v.x), fmaxf(v.y, v.z)), v.w);
     }
-    for (int i = threadIdx.x; i < n; i += UT)
-        if (i < head || i >= head + 4 * n4) {
-            const float v = src[i];
-            L[i] = v;
-            kmax = max(kmax, ukey(v));
-        }
-    kmax = __reduce_max_sync(0xffffffffu, kmax);
+    for (int i = threadIdx.x; i < head; i += UT) top = fmaxf(top, L[i] = src[i]);
+    for (int i = head + 4 * n4 + threadIdx.x; i < n; i += UT) top = fmaxf(top, L[i] = src[i]);
+    uint32_t kmax = __reduce_max_sync(0xffffffffu, ukey(top));
     if (lane == 0) S.redu[warp] = kmax;
     if (threadIdx.x == 0) S.cut = 1ull << 32;  // keys from 1 on: every token
     __syncthreads();
@@ -381,6 +399,25 @@ __global__ void __launch_bounds__(UT) k_sample_cluster(const float* __restrict__
         return;
     }
     R.mx = ukey_value(kmax);
+
+    if (P.tk == 1) {  // the first of the maxima
+        uint32_t at = 0xffffffffu;
+        for (int i = threadIdx.x; i < n; i += UT)
+            if (L[i] == R.mx) at = min(at, (uint32_t)(base + i));
+        at = __reduce_min_sync(0xffffffffu, at);
+        __syncthreads();  // (S.redu has been read)
+        if (lane == 0) S.redu[warp] = at;
+        __syncthreads();
+        at = __reduce_min_sync(0xffffffffu, lane < UW ? S.redu[lane] : 0xffffffffu);
+        if (threadIdx.x == 0) remote_st32(&S.c_at[rank], 0, at);
+        sync_all();
+        if (rank == 0 && threadIdx.x == 0) {
+            for (int c = 0; c < CS; c++) at = min(at, S.c_at[c]);
+            out[row] = (int)at;
+            if (logprob) logprob[row] = 0.0f;
+        }
+        return;
+    }
 
     auto block_sum = [&](u64 v) -> u64 {
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -402,98 +439,117 @@ __global__ void __launch_bounds__(UT) k_sample_cluster(const float* __restrict__
     u64 cut = 1ull << 32;
     if (by_k || by_p) {
         u64 held = 0;      // (first CTA) the mass of which top_p is a share
-        int have = -1;     // the histogram at hand
+        float kf = -FLT_MAX;               // top-k's end: logits above it, and equal ones up to index ki
+        uint32_t ki = 0xffffffffu;
         // Two ends may have to be found: top-k's by count, then top-p's by mass.
         for (int pass = by_k ? 0 : 1; pass < (by_p ? 2 : 1); pass++) {
             int level = 0;
             for (;; level++) {
-                if (have != level) {
-                    // ---- 2: the histogram, and (once) the mass
-                    for (int b = threadIdx.x; b < HB2; b += UT) {
-                        S.h.sum[b] = 0ull;
-                        S.h.cnt[b] = 0u;
+                // ---- 2: the histogram: counts, and for top-p masses
+                for (int b = threadIdx.x; b < HB2; b += UT) {
+                    S.h.sum[b] = 0ull;
+                    S.h.cnt[b] = 0u;
+                }
+                __syncthreads();
+                u64 mass = 0;
+                if (pass == 0) {
+                    for (int i = threadIdx.x; i < n; i += UT) {
+                        const int b = bucket_of(L[i], level);
+                        if (b >= 0) atomicAdd(&S.h.cnt[b], 1u);
                     }
-                    __syncthreads();
-                    u64 mass = 0;
+                } else {
                     for (int i = threadIdx.x; i < n; i += UT) {
                         const float f = L[i];
-                        if (!(f > -INFINITY)) continue;
+                        if (!(f >= kf) || (f == kf && (uint32_t)(base + i) > ki)) continue;
                         const int b = bucket_of(f, level);
-                        if (b < 0 && have >= 0) continue;
-                        const u64 m = R.mass(f);
+                        if (b < 0 && level == 1) continue;
+                        const u64 m = mass_of(R.weight(f));
                         mass += m;
                         if (b >= 0) {
                             atomicAdd(&S.h.cnt[b], 1u);
                             atomicAdd(&S.h.sum[b], m);
                         }
                     }
-                    if (have < 0) {
+                    if (level == 0) {
                         mass = block_sum(mass);
-                        if (threadIdx.x < CS) remote_st64(&S.c_mass[rank], threadIdx.x, mass);
+                        if (threadIdx.x == 0) remote_st64(&S.c_mass[rank], 0, mass);
                     }
-                    sync_all();
-                    if (rank == 0) {  // the first CTA adds the histograms up
-                        if (have < 0)
-                            for (int c = 0; c < CS; c++) held += S.c_mass[c];
-                        for (int b = threadIdx.x; b < HB2; b += UT) {
-                            uint32_t nc = S.h.cnt[b];
-                            u64 ms = S.h.sum[b];
-                            for (int c = 1; c < CS; c++) {
-                                nc += remote_ld32(&S.h.cnt[b], c);
-                                ms += remote_ld64(&S.h.sum[b], c);
-                            }
-                            S.h.cnt[b] = nc;
-                            S.h.sum[b] = ms;
-                        }
-                        __syncthreads();
-                    }
-                    have = level;
                 }
-                if (rank == 0 && warp == 0) {
-                    // warp 0: the last bucket that holds a token of the order's head
-                    const double goal = (double)P.tp * (double)held;
-                    u64 be = level ? S.head_mass : 0ull, sel_be = 0;
-                    uint32_t nb = level ? S.head_cnt : 0u, sel_nb = 0;
-                    int sel = -1;
-                    bool over = false;
-                    for (int b0 = 0; b0 < HB2 && !over; b0 += 32) {
-                        const uint32_t c = S.h.cnt[b0 + lane];
-                        const u64 m = S.h.sum[b0 + lane];
-                        uint32_t ci = c;
-                        u64 mi = m;
-                        for (int o = 1; o < 32; o <<= 1) {
-                            const uint32_t tc = __shfl_up_sync(0xffffffffu, ci, o);
-                            const u64 tm = __shfl_up_sync(0xffffffffu, mi, o);
-                            if (lane >= o) {
-                                ci += tc;
-                                mi += tm;
-                            }
+                sync_all();
+                if (rank == 0) {  // the first CTA adds the histograms up
+                    if (pass == 1 && level == 0)
+                        for (int c = 0; c < CS; c++) held += S.c_mass[c];
+                    for (int b = threadIdx.x; b < HB2; b += UT) {
+                        uint32_t nc[UC_MAX];
+                        u64 ms[UC_MAX];
+#pragma unroll
+                        for (int c = 1; c < UC_MAX; c++) {  // all on their way before the first is added
+                            nc[c] = c < CS ? remote_ld32(&S.h.cnt[b], c) : 0u;
+                            ms[c] = c < CS && pass == 1 ? remote_ld64(&S.h.sum[b], c) : 0ull;
                         }
-                        const uint32_t nb_l = nb + ci - c;
-                        const u64 be_l = be + mi - m;
-                        const bool in = c > 0 && (pass == 0 ? nb_l < (uint32_t)P.tk : (double)be_l < goal);
-                        const bool end = pass == 0 ? nb + ci >= (uint32_t)P.tk : !((double)(be + mi) < goal);
-                        const unsigned has = __ballot_sync(0xffffffffu, in);
-                        if (has) {
-                            const int l = 31 - __clz(has);
-                            sel = b0 + l;
-                            sel_nb = __shfl_sync(0xffffffffu, nb_l, l);
-                            sel_be = __shfl_sync(0xffffffffu, be_l, l);
+#pragma unroll
+                        for (int c = 1; c < UC_MAX; c++) {
+                            S.h.cnt[b] += nc[c];
+                            S.h.sum[b] += ms[c];
                         }
-                        over = __any_sync(0xffffffffu, end);
-                        nb += __shfl_sync(0xffffffffu, ci, 31);
-                        be += __shfl_sync(0xffffffffu, mi, 31);
                     }
-                    if (lane == 0) {
-                        // not over: the order ends further on, or (top-k) it keeps every token with a mass
-                        int b = over && sel >= 0 ? (S.h.cnt[sel] <= (uint32_t)CAP ? sel : SLOW) : level == 0 ? GO_ON : pass == 0 ? ALL : SLOW;
-                        S.bucket = b;
-                        S.sel_mass = sel_be;
-                        S.sel_cnt = sel_nb;
+                    __syncthreads();
+                }
+                if (rank == 0) {
+                    // the last bucket that holds a token of the order's head: two buckets a thread
+                    const double goal = (double)P.tp * (double)held;
+                    const int b0 = 2 * threadIdx.x;
+                    const uint32_t c0 = S.h.cnt[b0], c1 = S.h.cnt[b0 + 1];
+                    const u64 m0 = S.h.sum[b0], m1 = S.h.sum[b0 + 1];
+                    uint32_t ci = c0 + c1;
+                    u64 mi = m0 + m1;
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const uint32_t tc = __shfl_up_sync(0xffffffffu, ci, o);
+                        const u64 tm = __shfl_up_sync(0xffffffffu, mi, o);
+                        if (lane >= o) {
+                            ci += tc;
+                            mi += tm;
+                        }
+                    }
+                    if (lane == 31) {
+                        S.w_cnt[warp] = ci;
+                        S.w_mass[warp] = mi;
+                    }
+                    if (threadIdx.x == 0) {
+                        S.bucket = -1;
                         S.n_list = 0;
+                    }
+                    __syncthreads();
+                    uint32_t nb = level ? S.head_cnt : 0u, all_n = nb;
+                    u64 be = level ? S.head_mass : 0ull, all_m = be;
+                    for (int w = 0; w < UW; w++) {
+                        if (w < warp) {
+                            nb += S.w_cnt[w];
+                            be += S.w_mass[w];
+                        }
+                        all_n += S.w_cnt[w];
+                        all_m += S.w_mass[w];
+                    }
+                    nb += ci - c0 - c1;
+                    be += mi - m0 - m1;
+                    const bool over = pass == 0 ? all_n >= (uint32_t)P.tk : !((double)all_m < goal);
+                    const bool in0 = c0 > 0 && (pass == 0 ? nb < (uint32_t)P.tk : (double)be < goal);
+                    const bool in1 = c1 > 0 && (pass == 0 ? nb + c0 < (uint32_t)P.tk : (double)(be + m0) < goal);
+                    const int mine = in1 ? b0 + 1 : in0 ? b0 : -1;
+                    const int top = __reduce_max_sync(0xffffffffu, mine);
+                    if (lane == 0 && top >= 0) atomicMax(&S.bucket, top);
+                    __syncthreads();
+                    const int sel = S.bucket;
+                    __syncthreads();
+                    if (over && sel >= 0 ? mine == sel : threadIdx.x == 0) {
+                        // not over: the order ends further on, or (top-k) it keeps every token with a mass
+                        const int b = over && sel >= 0 ? ((in1 ? c1 : c0) <= (uint32_t)CAP ? sel : SLOW) : level == 0 ? GO_ON : pass == 0 ? ALL : SLOW;
+                        S.bucket = b;
+                        S.sel_mass = in1 ? be + m0 : be;
+                        S.sel_cnt = in1 ? nb + c0 : nb;
                         if (b == GO_ON) {
-                            S.head_mass = be;
-                            S.head_cnt = nb;
+                            S.head_mass = all_m;
+                            S.head_cnt = all_n;
                         }
                         for (int c = 1; c < CS; c++) remote_st32(&S.bucket, c, (uint32_t)b);
                     }
@@ -514,7 +570,7 @@ __global__ void __launch_bounds__(UT) k_sample_cluster(const float* __restrict__
             // ---- 3: the bucket's tokens, to the first CTA
             for (int i = threadIdx.x; i < n; i += UT) {
                 const float f = L[i];
-                if (!(f > -INFINITY) || bucket_of(f, level) != sel) continue;
+                if (!(f >= kf) || bucket_of(f, level) != sel || (f == kf && (uint32_t)(base + i) > ki)) continue;
                 uint32_t at;
                 asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(CS > 1 ? remote(&S.n_list, 0) : smem_u32(&S.n_list)) : "memory");
                 if (at >= (uint32_t)CAP) continue;
@@ -525,41 +581,50 @@ __global__ void __launch_bounds__(UT) k_sample_cluster(const float* __restrict__
             sync_all();
             if (rank == 0) {
                 const int ln = S.n_list;
-                sort_list(S, ln);
-                if (threadIdx.x == 0) {
-                    u64 before = S.sel_mass;
+                const u64* list = sort_list(S, ln);
+                if (warp == 0) {
+                    // 32 tokens at a time: the masses before them, and the last one kept
+                    u64 before = S.sel_mass, c = 0;
                     const double goal = (double)P.tp * (double)held;
-                    u64 c = 0;
-                    for (int i = 0; i < ln; i++) {
-                        const u64 e = S.h.list[i];
-                        if (pass == 0 ? S.sel_cnt + i >= (uint32_t)P.tk : (!((double)before < goal) || e < cut)) break;
-                        c = e;
-                        before += R.mass(ukey_value((uint32_t)(e >> 32)));
+                    for (int i0 = 0; i0 < ln; i0 += 32) {
+                        const u64 e = i0 + lane < ln ? list[i0 + lane] : 0ull;
+                        const u64 m = e ? R.mass(ukey_value((uint32_t)(e >> 32))) : 0ull;
+                        u64 incl = m;
+                        for (int o = 1; o < 32; o <<= 1) {
+                            const u64 t = __shfl_up_sync(0xffffffffu, incl, o);
+                            if (lane >= o) incl += t;
+                        }
+                        const bool in = e && (pass == 0 ? S.sel_cnt + i0 + lane < (uint32_t)P.tk : (double)(before + incl - m) < goal);
+                        const unsigned b = __ballot_sync(0xffffffffu, in);  // a run of low lanes
+                        if (b) {
+                            const int l = 31 - __clz(b);
+                            c = __shfl_sync(0xffffffffu, e, l);
+                            before += __shfl_sync(0xffffffffu, incl, l);
+                        }
+                        if (b != 0xffffffffu) break;
                     }
-                    if (c < cut) c = cut;  // (no token: the end that top-k gave)
-                    S.cut = c;
-                    S.sel_mass = before;
-                    for (int q = 1; q < CS; q++) remote_st64(&S.cut, q, c);
+                    if (lane == 0) {
+                        S.cut = c;
+                        for (int q = 1; q < CS; q++) remote_st64(&S.cut, q, c);
+                    }
                 }
-                __syncthreads();
-                if (pass == 0) held = S.sel_mass;  // the mass of what top-k kept
-                cut = S.cut;
-                __syncthreads();
             }
+            sync_all();
+            cut = S.cut;
+            kf = ukey_value((uint32_t)(cut >> 32));
+            ki = ~(uint32_t)cut;
         }
-        sync_all();
-        cut = S.cut;
     }
 
     // ---- 4: the kept mass of each warp's run of tokens, and the draw
-    const uint32_t ck = (uint32_t)(cut >> 32), ci = ~(uint32_t)cut;
-    const bool minp = P.mp > 0.0f && P.mp <= 1.0f;
+    const float cf = cut == 1ull << 32 ? -FLT_MAX : ukey_value((uint32_t)(cut >> 32));
+    const uint32_t ci = ~(uint32_t)cut;
+    const float least = P.mp <= 1.0f ? P.mp : 0.0f;
     auto kept = [&](int i) -> u64 {
         const float f = L[i];
-        const uint32_t k = ukey(f);
-        if (k < ck || (k == ck && (uint32_t)(base + i) > ci)) return 0ull;
+        if (!(f >= cf) || (f == cf && (uint32_t)(base + i) > ci)) return 0ull;
         const float w = R.weight(f);
-        return minp && !(w >= P.mp) ? 0ull : __float2ull_rz(__fmul_rn(w, 1099511627776.0f));
+        return w >= least ? mass_of(w) : 0ull;
     };
     const int per = ((n + UW - 1) / UW + 31) & ~31, w0 = min(warp * per, n), w1 = min(w0 + per, n);
     u64 mine = 0;
@@ -650,9 +715,10 @@ HC_EXPORT int hc_sample_uniform_dev(const float* logits_dev, size_t ld, int B, i
              HC_ERR_INVALID, "hc_sample_uniform_dev: NULL argument");
     if (B == 0) return HC_OK;
     cudaStream_t s = (cudaStream_t)stream;
-    // CTAs a row: slices of 4,096 logits or more, up to eight; a slice fits shared memory
+    // CTAs a row: slices of 4,096 logits or more, up to eight CTAs; a slice fits shared memory
     int cs = 1;
-    while (cs < hc::UC_MAX && V > cs * 4096) cs *= 2;
+    while (cs < 8 && V > cs * 4096) cs *= 2;
+    if ((int64_t)B * 16 <= 148 && V >= 16 * 4096) cs = 16;  // few long rows: shorter passes
     const int slice = (V + cs - 1) / cs;
     const size_t smem = sizeof(hc::CShared) + ((size_t)slice + 8) * sizeof(float);
     if (smem > 227 * 1024) {
@@ -663,6 +729,7 @@ HC_EXPORT int hc_sample_uniform_dev(const float* logits_dev, size_t ld, int B, i
     }
     HC_CHECK((int64_t)B * cs <= 0x7fffffff, HC_ERR_INVALID, "hc_sample_uniform_dev: %d rows", B);
     HC_CUDA(cudaFuncSetAttribute(hc::k_sample_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (cs > 8) HC_CUDA(cudaFuncSetAttribute(hc::k_sample_cluster, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(B * cs));
     cfg.blockDim = dim3(hc::UT);
