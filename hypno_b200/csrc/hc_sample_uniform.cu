@@ -8,15 +8,20 @@
 // drawn.  The kept set is a head of the order (logit descending, index
 // ascending), so one (key, index) pair cuts it off.
 //
-// k_sample_cluster: a cluster of up to 16 CTAs takes a row, each CTA a slice that
-// it reads once into shared memory.  Passes over the slice: the maximum; for
-// top-k a histogram (counts) of the tokens within HEAD of the maximum in units
-// of T, or beyond it where that has fewer than k; the tokens of the bucket in
-// which the order ends, gathered by the first CTA and sorted there; for top-p
-// the same by mass, over what top-k kept; the kept mass of each warp's run, in
-// which the draw is then found.  A bucket too full to sort (flat rows) is left
-// to the first CTA and the kernel's slow path: a radix search over the logits'
-// keys.  Bound by the latency of the cluster barriers for few rows, by the
+// k_sample_cluster: a cluster of up to 16 CTAs takes a row, each CTA a slice,
+// each warp a run of it.  Passes over the logits (the first from memory, the
+// others from L2): the maximum; the tokens near it (the head),
+// where most orders end and few tokens are, into a list of each warp, by index
+// (for top-p alone also the mass of all).  Then, from the lists: a histogram (for
+// top-k by count, for top-p by mass over what top-k kept), the tokens of the
+// bucket in which the order ends, gathered by the first CTA and sorted there,
+// the kept mass of each warp, and the draw.  Where an order ends beyond the head, or
+// keeps every token, the passes go over the logits instead of the lists; a
+// bucket too full to sort (flat rows) is left to the first CTA and the kernel's
+// slow path, a radix search over the logits' keys.  Nothing of a row stays in
+// shared memory but the lists, so that several rows share an SM and one's
+// serial parts (barriers, the first CTA's work) hide behind another's passes.
+// Bound by the latency of the cluster barriers for few rows, by the
 // instructions of the passes (not by the one read of the logits) for many: a
 // weight is some 30 of them.
 #include "hc_internal.h"
@@ -28,7 +33,7 @@ namespace hc {
 
 namespace {
 
-constexpr int UT = 512;    // threads
+constexpr int UT = 256;    // threads
 constexpr int UB = 2048;   // buckets of a radix pass
 constexpr int UW = UT / 32;
 typedef unsigned long long u64;
@@ -248,10 +253,14 @@ __device__ __noinline__ void sample_row(URow R, URowArgs P, UShared& S, int32_t*
 
 constexpr int UC_MAX = 16;         // CTAs of a cluster (above 8 for few long rows only)
 constexpr int HB2 = 1024;          // buckets of a histogram
-// Distances (max - l) / T that the two histograms cover: weights from 1 to 6e-6,
-// where most orders end and few tokens are, and from there to below 2^-40.
-constexpr float HEAD = 12.0f, TAIL = 28.0f;
+constexpr int HBT = HB2 / UT;      // a thread's
+// Distances (max - l) / T that the two histograms cover: up to the head's end and
+// from there to TAIL, where weights are below 2^-40.  The head ends NEAR below the
+// maximum in logits (a language model has some thousands of tokens there), and
+// between weights of 3e-4 and 2e-12.
+constexpr float NEAR = 12.0f, HEAD_MIN = 8.0f, HEAD_MAX = 27.0f, TAIL = 28.0f;
 constexpr int CAP = 1024;          // tokens of a bucket that are sorted
+constexpr int WCAP = 512;          // tokens of a warp's list
 constexpr int GO_ON = -2, ALL = -1, SLOW = HB2;  // instead of a bucket
 
 struct __align__(16) CShared {
@@ -261,13 +270,16 @@ struct __align__(16) CShared {
             u64 sum[HB2];
             uint32_t cnt[HB2];
             u64 list[CAP];         // gathered tokens, key above ~index (first CTA)
+            u64 sorted[UT];
+            float near_l[UW][WCAP];  // the warps' lists: logits, indices
+            uint32_t near_i[UW][WCAP];
         } h;
     };
     u64 red[32];
     uint32_t redu[32];
-    // what the CTAs of the cluster tell one another, one word for each (all have the same copy)
+    // what the CTAs of the cluster tell one another, one word for each
     uint32_t c_max[UC_MAX], c_at[UC_MAX];
-    u64 c_mass[UC_MAX];            // mass (pass 2), kept mass (pass 4)
+    u64 c_mass[UC_MAX];
     // what the first CTA tells all
     int n_list;
     int bucket;
@@ -277,7 +289,6 @@ struct __align__(16) CShared {
     uint32_t sel_cnt, head_cnt;    // likewise tokens
     u64 w_mass[UW];                // of the warps' buckets
     uint32_t w_cnt[UW];
-    u64 sorted[256];
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -313,17 +324,17 @@ __device__ __forceinline__ u64 remote_ld64(const void* p, uint32_t rank) {
 // Descending sort of the first CTA's list: places by counting for short lists,
 // bitonic for long ones.  Returns where the sorted list is.
 __device__ u64* sort_list(CShared& S, int n) {
-    if (n <= 256) {
+    if (n <= UT) {
         if ((int)threadIdx.x < n) {
             const u64 e = S.h.list[threadIdx.x];
             int at = 0;
             for (int j = 0; j < n; j++) at += S.h.list[j] > e;
-            S.sorted[at] = e;
+            S.h.sorted[at] = e;
         }
         __syncthreads();
-        return S.sorted;
+        return S.h.sorted;
     }
-    int m = 512;
+    int m = 2 * UT;
     while (m < n) m <<= 1;
     for (int j = n + (int)threadIdx.x; j < m; j += UT) S.h.list[j] = 0ull;
     __syncthreads();
@@ -344,16 +355,17 @@ __device__ u64* sort_list(CShared& S, int n) {
     return S.h.list;
 }
 
-__global__ void __launch_bounds__(UT, 2) k_sample_cluster(const float* __restrict__ logits, size_t ld, int V, int slice,
-                                                       const float* __restrict__ u, const float* __restrict__ temp,
-                                                       const int* __restrict__ top_k, const float* __restrict__ top_p,
-                                                       const float* __restrict__ min_p, int32_t* __restrict__ out,
-                                                       float* __restrict__ logprob, int CS) {
+static_assert(4 * (sizeof(CShared) + 1024) <= 228 * 1024, "four CTAs an SM");
+
+__global__ void __launch_bounds__(UT, 4) k_sample_cluster(const float* __restrict__ logits, size_t ld, int V, int slice,
+                                                          const float* __restrict__ u, const float* __restrict__ temp,
+                                                          const int* __restrict__ top_k, const float* __restrict__ top_p,
+                                                          const float* __restrict__ min_p, int32_t* __restrict__ out,
+                                                          float* __restrict__ logprob, int CS) {
     extern __shared__ __align__(16) uint8_t smem[];
     CShared& S = *reinterpret_cast<CShared*>(smem);
     const int rank = CS > 1 ? (int)cluster_rank() : 0, row = blockIdx.x / CS;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int base = rank * slice, n = max(0, min(slice, V - base));
     auto sync_all = [&]() {
         if (CS > 1) cluster_barrier();
         else __syncthreads();
@@ -370,19 +382,51 @@ __global__ void __launch_bounds__(UT, 2) k_sample_cluster(const float* __restric
     R.V = V;
     R.inv = T > 0.0f ? __fdiv_rn(1.0f, T) : 1.0f;
 
-    // ---- 1: the slice and the maximum
-    float top = -INFINITY;  // (NaN never wins)
-    const float* src = R.l + base;
-    const int head = min(n, (int)((16 - ((uintptr_t)src & 15)) & 15) / 4), n4 = (n - head) >> 2;  // 16-byte loads in between
-    float* L = reinterpret_cast<float*>(smem + sizeof(CShared)) + ((4 - head) & 3);  // and 16-byte stores
-#pragma unroll 4
-    for (int i = threadIdx.x; i < n4; i += UT) {
-        const float4 v = __ldcs(reinterpret_cast<const float4*>(src + head) + i);
-        *reinterpret_cast<float4*>(L + head + 4 * i) = v;
-        top = fmaxf(fmaxf(fmaxf(top, v.x), fmaxf(v.y, v.z)), v.w);
+    // Places are counted from the 16-byte boundary at or before the row's first
+    // logit: place = index + off.  A warp has the run [w0, w1) of places, 128 at
+    // a time, four a lane.
+    const int off = (int)(((uintptr_t)R.l & 15) >> 2), places = V + off;
+    const int per = slice / UW;  // (a multiple of 128)
+    const int w0 = min(rank * slice + warp * per, places), w1 = min(w0 + per, places);
+    const float* P0 = R.l - off;  // (never read below off)
+    auto get4 = [&](int j, float* v) {
+        if (j >= off && j + 4 <= places) {
+            const float4 x = *reinterpret_cast<const float4*>(P0 + j);
+            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+        } else {
+#pragma unroll
+            for (int y = 0; y < 4; y++) v[y] = j + y >= off && j + y < places ? P0[j + y] : -INFINITY;
+        }
+    };
+
+    // A later cluster's slice on its way to L2 while this one is worked on: the
+    // one that will follow when four CTAs an SM have gone by.
+    {
+        const int64_t later = (int64_t)blockIdx.x / CS + 148 * 4 / CS;
+        if (later < (int64_t)(gridDim.x / CS)) {
+            const float* q = logits + (size_t)later * ld - off;
+            for (int j = w0 + lane * 32; j < w1; j += 32 * 32)
+                if (j >= off) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + j));
+        }
     }
-    for (int i = threadIdx.x; i < head; i += UT) top = fmaxf(top, L[i] = src[i]);
-    for (int i = head + 4 * n4 + threadIdx.x; i < n; i += UT) top = fmaxf(top, L[i] = src[i]);
+
+    // ---- 1: the maximum
+    float top = -INFINITY;  // (NaN never wins)
+    {
+        int j = w0 + lane * 4;
+        for (; j + 3 * 128 < w1; j += 4 * 128) {
+            float v[4][4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) get4(j + x * 128, v[x]);
+#pragma unroll
+            for (int x = 0; x < 4; x++) top = fmaxf(fmaxf(fmaxf(top, v[x][0]), fmaxf(v[x][1], v[x][2])), v[x][3]);
+        }
+        for (; j < w1; j += 128) {
+            float v[4];
+            get4(j, v);
+            top = fmaxf(fmaxf(fmaxf(top, v[0]), fmaxf(v[1], v[2])), v[3]);
+        }
+    }
     uint32_t kmax = __reduce_max_sync(0xffffffffu, ukey(top));
     if (lane == 0) S.redu[warp] = kmax;
     if (threadIdx.x == 0) S.cut = 1ull << 32;  // keys from 1 on: every token
@@ -402,8 +446,15 @@ __global__ void __launch_bounds__(UT, 2) k_sample_cluster(const float* __restric
 
     if (P.tk == 1) {  // the first of the maxima
         uint32_t at = 0xffffffffu;
-        for (int i = threadIdx.x; i < n; i += UT)
-            if (L[i] == R.mx) at = min(at, (uint32_t)(base + i));
+        if (__any_sync(0xffffffffu, top == R.mx)) {
+            for (int j = w0 + lane * 4; j < w1; j += 128) {
+                float v[4];
+                get4(j, v);
+#pragma unroll
+                for (int y = 3; y >= 0; y--)
+                    if (v[y] == R.mx) at = min(at, (uint32_t)(j + y - off));
+            }
+        }
         at = __reduce_min_sync(0xffffffffu, at);
         __syncthreads();  // (S.redu has been read)
         if (lane == 0) S.redu[warp] = at;
@@ -428,52 +479,112 @@ __global__ void __launch_bounds__(UT, 2) k_sample_cluster(const float* __restric
         for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
         return t;
     };
-    // bucket of a logit in histogram 0 or 1, monotone in l; -1 outside it
-    auto bucket_of = [&](float f, int level) -> int {
-        const float d = f == R.mx ? 0.0f : __fmul_rn(__fsub_rn(R.mx, f), R.inv);
-        if (level == 0) return d < HEAD ? (int)(d * (HB2 / HEAD)) : -1;
-        return d >= HEAD && d < TAIL ? min((int)((d - HEAD) * (HB2 / (TAIL - HEAD))), HB2 - 1) : -1;
+    if (R.mx == INFINITY) {  // differences of infinities are left to the slow path
+        if (rank == 0) sample_row(R, P, S.slow, out + row, logprob ? logprob + row : nullptr);
+        return;
+    }
+    const float headd = fminf(fmaxf(NEAR * R.inv, HEAD_MIN), HEAD_MAX), step0 = HB2 / headd, step1 = HB2 / (TAIL - headd);
+    // -(max - l) / T, the exponent of a weight; its bucket in histogram 0 or 1,
+    // monotone in l, -1 outside it
+    auto expo = [&](float f) -> float { return __fmul_rn(__fsub_rn(f, R.mx), R.inv); };
+    auto bucket_at = [&](float x, int level) -> int {
+        if (level == 0) return -x < headd ? min((int)(-x * step0), HB2 - 1) : -1;
+        return -x >= headd && -x < TAIL ? min((int)((-x - headd) * step1), HB2 - 1) : -1;
     };
+    auto bucket_of = [&](float f, int level) -> int { return bucket_at(expo(f), level); };
 
     const bool by_k = P.tk > 0 && P.tk < V, by_p = P.tp < 1.0f && P.tk != 1;
     u64 cut = 1ull << 32;
+    // What is kept so far: logits above kf, and equal ones up to index ki.
+    float kf = -FLT_MAX;
+    uint32_t ki = 0xffffffffu;
+    auto in_head = [&](float f, uint32_t i) -> bool { return f >= kf && !(f == kf && i > ki); };
+    // fn(logit, index) for this warp's tokens, by index over a lane's own; from the
+    // list where all that matter are in it.
+    int listed = 0;       // tokens in the warp's list, WCAP + 1 for more than it holds
+    bool near = false;    // only tokens of the head matter
+    auto each = [&](auto fn) {
+        if (near && listed <= WCAP) {
+            for (int e = lane; e < listed; e += 32) fn(S.h.near_l[warp][e], S.h.near_i[warp][e]);
+        } else {
+            for (int j = w0 + lane * 4; j < w1; j += 128) {
+                float v[4];
+                get4(j, v);
+#pragma unroll
+                for (int y = 0; y < 4; y++) fn(v[y], (uint32_t)(j + y - off));
+            }
+        }
+    };
     if (by_k || by_p) {
-        u64 held = 0;      // (first CTA) the mass of which top_p is a share
-        float kf = -FLT_MAX;               // top-k's end: logits above it, and equal ones up to index ki
-        uint32_t ki = 0xffffffffu;
+        // ---- 2: the lists, and for top-p alone the mass
+        u64 mass = 0;
+        for (int j0 = w0; j0 < w1; j0 += 128) {
+            float v[4];
+            get4(j0 + lane * 4, v);
+            unsigned b[4];
+            bool any = false;
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const float x = expo(v[y]);
+                b[y] = __ballot_sync(0xffffffffu, -x < headd);
+                any = any || b[y];
+                if (!by_k) mass += v[y] >= -FLT_MAX ? mass_of(expf(x)) : 0ull;
+            }
+            if (any) {
+                const unsigned lt = (1u << lane) - 1u;
+                int at = listed + __popc(b[0] & lt) + __popc(b[1] & lt) + __popc(b[2] & lt) + __popc(b[3] & lt);
+#pragma unroll
+                for (int y = 0; y < 4; y++)
+                    if ((b[y] >> lane) & 1u) {
+                        if (at < WCAP) {
+                            S.h.near_l[warp][at] = v[y];
+                            S.h.near_i[warp][at] = (uint32_t)(j0 + lane * 4 + y - off);
+                        }
+                        at++;
+                    }
+                listed = min(listed + __popc(b[0]) + __popc(b[1]) + __popc(b[2]) + __popc(b[3]), WCAP + 1);
+                if (listed > WCAP && by_k) break;
+            }
+        }
+        __syncwarp();
+        if (!by_k) {
+            mass = block_sum(mass);
+            if (threadIdx.x == 0) remote_st64(&S.c_mass[rank], 0, mass);
+        }
+        u64 held = 0;          // (first CTA) the mass of which top_p is a share
+        bool cut_near = false; // the end found last is within the head
         // Two ends may have to be found: top-k's by count, then top-p's by mass.
         for (int pass = by_k ? 0 : 1; pass < (by_p ? 2 : 1); pass++) {
             int level = 0;
             for (;; level++) {
-                // ---- 2: the histogram: counts, and for top-p masses
+                // ---- 3: the histogram: counts, and for top-p masses
                 for (int b = threadIdx.x; b < HB2; b += UT) {
                     S.h.sum[b] = 0ull;
                     S.h.cnt[b] = 0u;
                 }
                 __syncthreads();
-                u64 mass = 0;
-                if (pass == 0) {
-                    for (int i = threadIdx.x; i < n; i += UT) {
-                        const int b = bucket_of(L[i], level);
+                // (what top-k kept has its mass taken here, near or not)
+                near = level == 0 && (pass == 0 || !by_k || cut_near);
+                u64 m2 = 0;
+                each([&](float f, uint32_t i) {
+                    if (!in_head(f, i)) return;
+                    const float x = expo(f);
+                    const int b = bucket_at(x, level);
+                    if (pass == 0) {
                         if (b >= 0) atomicAdd(&S.h.cnt[b], 1u);
+                        return;
                     }
-                } else {
-                    for (int i = threadIdx.x; i < n; i += UT) {
-                        const float f = L[i];
-                        if (!(f >= kf) || (f == kf && (uint32_t)(base + i) > ki)) continue;
-                        const int b = bucket_of(f, level);
-                        if (b < 0 && level == 1) continue;
-                        const u64 m = mass_of(R.weight(f));
-                        mass += m;
-                        if (b >= 0) {
-                            atomicAdd(&S.h.cnt[b], 1u);
-                            atomicAdd(&S.h.sum[b], m);
-                        }
+                    if (b < 0 && (level == 1 || !by_k)) return;
+                    const u64 m = mass_of(expf(x));
+                    m2 += m;
+                    if (b >= 0) {
+                        atomicAdd(&S.h.cnt[b], 1u);
+                        atomicAdd(&S.h.sum[b], m);
                     }
-                    if (level == 0) {
-                        mass = block_sum(mass);
-                        if (threadIdx.x == 0) remote_st64(&S.c_mass[rank], 0, mass);
-                    }
+                });
+                if (pass == 1 && level == 0 && by_k) {
+                    m2 = block_sum(m2);
+                    if (threadIdx.x == 0) remote_st64(&S.c_mass[rank], 0, m2);
                 }
                 sync_all();
                 if (rank == 0) {  // the first CTA adds the histograms up
@@ -496,13 +607,20 @@ __global__ void __launch_bounds__(UT, 2) k_sample_cluster(const float* __restric
                     __syncthreads();
                 }
                 if (rank == 0) {
-                    // the last bucket that holds a token of the order's head: two buckets a thread
+                    // the last bucket that holds a token of the order's head: HBT buckets a thread
                     const double goal = (double)P.tp * (double)held;
-                    const int b0 = 2 * threadIdx.x;
-                    const uint32_t c0 = S.h.cnt[b0], c1 = S.h.cnt[b0 + 1];
-                    const u64 m0 = S.h.sum[b0], m1 = S.h.sum[b0 + 1];
-                    uint32_t ci = c0 + c1;
-                    u64 mi = m0 + m1;
+                    const int b0 = HBT * threadIdx.x;
+                    uint32_t c[HBT], cs = 0;
+                    u64 m[HBT], ms = 0;
+#pragma unroll
+                    for (int i = 0; i < HBT; i++) {
+                        c[i] = S.h.cnt[b0 + i];
+                        m[i] = S.h.sum[b0 + i];
+                        cs += c[i];
+                        ms += m[i];
+                    }
+                    uint32_t ci = cs;
+                    u64 mi = ms;
                     for (int o = 1; o < 32; o <<= 1) {
                         const uint32_t tc = __shfl_up_sync(0xffffffffu, ci, o);
                         const u64 tm = __shfl_up_sync(0xffffffffu, mi, o);
@@ -530,28 +648,39 @@ __global__ void __launch_bounds__(UT, 2) k_sample_cluster(const float* __restric
                         all_n += S.w_cnt[w];
                         all_m += S.w_mass[w];
                     }
-                    nb += ci - c0 - c1;
-                    be += mi - m0 - m1;
+                    nb += ci - cs;
+                    be += mi - ms;
                     const bool over = pass == 0 ? all_n >= (uint32_t)P.tk : !((double)all_m < goal);
-                    const bool in0 = c0 > 0 && (pass == 0 ? nb < (uint32_t)P.tk : (double)be < goal);
-                    const bool in1 = c1 > 0 && (pass == 0 ? nb + c0 < (uint32_t)P.tk : (double)(be + m0) < goal);
-                    const int mine = in1 ? b0 + 1 : in0 ? b0 : -1;
-                    const int top = __reduce_max_sync(0xffffffffu, mine);
-                    if (lane == 0 && top >= 0) atomicMax(&S.bucket, top);
+                    int mine = -1;
+                    uint32_t my_nb = 0, my_c = 0;
+                    u64 my_be = 0;
+#pragma unroll
+                    for (int i = 0; i < HBT; i++) {
+                        if (c[i] > 0 && (pass == 0 ? nb < (uint32_t)P.tk : (double)be < goal)) {
+                            mine = b0 + i;
+                            my_nb = nb;
+                            my_be = be;
+                            my_c = c[i];
+                        }
+                        nb += c[i];
+                        be += m[i];
+                    }
+                    const int best = __reduce_max_sync(0xffffffffu, mine);
+                    if (lane == 0 && best >= 0) atomicMax(&S.bucket, best);
                     __syncthreads();
                     const int sel = S.bucket;
                     __syncthreads();
                     if (over && sel >= 0 ? mine == sel : threadIdx.x == 0) {
                         // not over: the order ends further on, or (top-k) it keeps every token with a mass
-                        const int b = over && sel >= 0 ? ((in1 ? c1 : c0) <= (uint32_t)CAP ? sel : SLOW) : level == 0 ? GO_ON : pass == 0 ? ALL : SLOW;
+                        const int b = over && sel >= 0 ? (my_c <= (uint32_t)CAP ? sel : SLOW) : level == 0 ? GO_ON : pass == 0 ? ALL : SLOW;
                         S.bucket = b;
-                        S.sel_mass = in1 ? be + m0 : be;
-                        S.sel_cnt = in1 ? nb + c0 : nb;
+                        S.sel_mass = my_be;
+                        S.sel_cnt = my_nb;
                         if (b == GO_ON) {
                             S.head_mass = all_m;
                             S.head_cnt = all_n;
                         }
-                        for (int c = 1; c < CS; c++) remote_st32(&S.bucket, c, (uint32_t)b);
+                        for (int q = 1; q < CS; q++) remote_st32(&S.bucket, q, (uint32_t)b);
                     }
                 }
                 sync_all();
@@ -567,17 +696,17 @@ __global__ void __launch_bounds__(UT, 2) k_sample_cluster(const float* __restric
                 sync_all();
                 continue;
             }
-            // ---- 3: the bucket's tokens, to the first CTA
-            for (int i = threadIdx.x; i < n; i += UT) {
-                const float f = L[i];
-                if (!(f >= kf) || bucket_of(f, level) != sel || (f == kf && (uint32_t)(base + i) > ki)) continue;
+            // ---- 4: the bucket's tokens, to the first CTA
+            near = level == 0;
+            each([&](float f, uint32_t i) {
+                if (!in_head(f, i) || bucket_of(f, level) != sel) return;
                 uint32_t at;
                 asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(CS > 1 ? remote(&S.n_list, 0) : smem_u32(&S.n_list)) : "memory");
-                if (at >= (uint32_t)CAP) continue;
-                const u64 e = (u64)ukey(f) << 32 | (uint32_t)~(base + i);
+                if (at >= (uint32_t)CAP) return;
+                const u64 e = (u64)ukey(f) << 32 | (uint32_t)~i;
                 if (CS > 1) remote_st64(&S.h.list[at], 0, e);
                 else S.h.list[at] = e;
-            }
+            });
             sync_all();
             if (rank == 0) {
                 const int ln = S.n_list;
@@ -613,22 +742,20 @@ __global__ void __launch_bounds__(UT, 2) k_sample_cluster(const float* __restric
             cut = S.cut;
             kf = ukey_value((uint32_t)(cut >> 32));
             ki = ~(uint32_t)cut;
+            cut_near = level == 0;
         }
+        near = cut_near;
     }
 
-    // ---- 4: the kept mass of each warp's run of tokens, and the draw
-    const float cf = cut == 1ull << 32 ? -FLT_MAX : ukey_value((uint32_t)(cut >> 32));
-    const uint32_t ci = ~(uint32_t)cut;
+    // ---- 5: the kept mass of each warp, and the draw
     const float least = P.mp <= 1.0f ? P.mp : 0.0f;
-    auto kept = [&](int i) -> u64 {
-        const float f = L[i];
-        if (!(f >= cf) || (f == cf && (uint32_t)(base + i) > ci)) return 0ull;
-        const float w = R.weight(f);
+    auto kept = [&](float f, uint32_t i) -> u64 {
+        if (!in_head(f, i)) return 0ull;
+        const float w = expf(expo(f));
         return w >= least ? mass_of(w) : 0ull;
     };
-    const int per = ((n + UW - 1) / UW + 31) & ~31, w0 = min(warp * per, n), w1 = min(w0 + per, n);
     u64 mine = 0;
-    for (int i = w0 + lane; i < w1; i += 32) mine += kept(i);
+    each([&](float f, uint32_t i) { mine += kept(f, i); });
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     __syncthreads();
     if (lane == 0) S.red[warp] = mine;
@@ -647,9 +774,27 @@ __global__ void __launch_bounds__(UT, 2) k_sample_cluster(const float* __restric
     }
     const u64 goal = draw_goal(P.u, total);
     if (goal < below || goal >= below + mine) return;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-        const u64 m = i0 + lane < w1 ? kept(i0 + lane) : 0ull;
-        u64 incl = m;
+    // this warp's: its tokens in order, one a lane from the list, four a lane from the logits
+    const bool list = near && listed <= WCAP;
+    const int end = list ? listed : w1, stride = list ? 32 : 128;
+    float v[4], next[4];
+    if (!list) get4(w0 + lane * 4, next);
+    for (int j0 = list ? 0 : w0; j0 < end; j0 += stride) {
+        u64 m[4] = {0, 0, 0, 0};
+        uint32_t i = 0;
+        if (list) {
+            if (j0 + lane < listed) m[0] = kept(S.h.near_l[warp][j0 + lane], i = S.h.near_i[warp][j0 + lane]);
+        } else {
+            const int j = j0 + lane * 4;
+            i = (uint32_t)(j - off);
+#pragma unroll
+            for (int y = 0; y < 4; y++) v[y] = next[y];
+            if (j0 + stride < end) get4(j + 128, next);
+#pragma unroll
+            for (int y = 0; y < 4; y++) m[y] = j + y < w1 ? kept(v[y], i + y) : 0ull;
+        }
+        const u64 sum = (m[0] + m[1]) + (m[2] + m[3]);
+        u64 incl = sum;
         for (int o = 1; o < 32; o <<= 1) {
             const u64 t = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += t;
@@ -657,49 +802,16 @@ __global__ void __launch_bounds__(UT, 2) k_sample_cluster(const float* __restric
         const unsigned hit = __ballot_sync(0xffffffffu, below + incl > goal);
         if (hit) {
             if (lane == __ffs(hit) - 1) {
-                out[row] = base + i0 + lane;
-                if (logprob) logprob[row] = logf((float)((double)m / (double)total));
+                u64 run = below + incl - sum;
+                int y = 0;
+                while (y < 3 && run + m[y] <= goal) run += m[y++];
+                out[row] = (int)(i + y);
+                if (logprob) logprob[row] = logf((float)((double)m[y] / (double)total));
             }
             return;
         }
         below += __shfl_sync(0xffffffffu, incl, 31);
     }
-}
-
-// Rows too long for the shared memory of a cluster.
-__global__ void __launch_bounds__(UT) k_sample_uniform(const float* __restrict__ logits, size_t ld, int V,
-                                                       const float* __restrict__ u, const float* __restrict__ temp,
-                                                       const int* __restrict__ top_k, const float* __restrict__ top_p,
-                                                       const float* __restrict__ min_p, int32_t* __restrict__ out,
-                                                       float* __restrict__ logprob) {
-    __shared__ UShared S;
-    const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float T = temp[row];
-    URowArgs P;
-    P.u = u[row];
-    P.tp = top_p[row];
-    P.mp = min_p[row];
-    P.tk = top_k[row];
-    if (!(T > 0.0f) || !(P.tp > 0.0f) || !(P.mp <= 1.0f)) P.tk = 1;  // only the first token can be kept
-    URow R;
-    R.l = logits + (size_t)row * ld;
-    R.V = V;
-    R.inv = T > 0.0f ? __fdiv_rn(1.0f, T) : 1.0f;
-    uint32_t kmax = 0;
-    for (int i = threadIdx.x; i < V; i += UT) kmax = max(kmax, ukey(R.l[i]));
-    kmax = __reduce_max_sync(0xffffffffu, kmax);
-    if (lane == 0) S.redu[warp] = kmax;
-    __syncthreads();
-    kmax = __reduce_max_sync(0xffffffffu, lane < UW ? S.redu[lane] : 0u);
-    if (kmax == 0) {  // nothing above -inf
-        if (threadIdx.x == 0) {
-            out[row] = -1;
-            if (logprob) logprob[row] = -INFINITY;
-        }
-        return;
-    }
-    R.mx = ukey_value(kmax);
-    sample_row(R, P, S, out + row, logprob ? logprob + row : nullptr);
 }
 
 }  // namespace
@@ -714,19 +826,17 @@ HC_EXPORT int hc_sample_uniform_dev(const float* logits_dev, size_t ld, int B, i
     HC_CHECK(B == 0 || (logits_dev && u_dev && temperature_dev && top_k_dev && top_p_dev && min_p_dev && out_dev),
              HC_ERR_INVALID, "hc_sample_uniform_dev: NULL argument");
     if (B == 0) return HC_OK;
+    HC_CHECK((uintptr_t)logits_dev % 4 == 0, HC_ERR_INVALID, "hc_sample_uniform_dev: misaligned logits");
     cudaStream_t s = (cudaStream_t)stream;
-    // CTAs a row: slices of 4,096 logits or more, up to eight CTAs; a slice fits shared memory
+    // CTAs a row: slices of 4,096 logits or more, up to eight CTAs (two a row, so
+    // that 256 rows are resident at once, took a third longer: the passes count);
+    // sixteen where the GPU holds them all on SMs of their own.
     int cs = 1;
     while (cs < 8 && V > cs * 4096) cs *= 2;
-    if ((int64_t)B * 16 <= 148 && V >= 16 * 4096) cs = 16;  // few long rows: shorter passes
-    const int slice = (V + cs - 1) / cs;
-    const size_t smem = sizeof(hc::CShared) + ((size_t)slice + 8) * sizeof(float);
-    if (smem > 227 * 1024) {
-        hc::k_sample_uniform<<<(unsigned)B, hc::UT, 0, s>>>(logits_dev, ld, V, u_dev, temperature_dev, top_k_dev, top_p_dev,
-                                                           min_p_dev, out_dev, logprob_dev);
-        HC_LAUNCH_CHECK();
-        return HC_OK;
-    }
+    if ((int64_t)B * 16 <= 148 && V > 8 * 4096) cs = 16;
+    const int runs = cs * hc::UW * 128;                       // a warp's run is a multiple of 128 places
+    const int slice = (int)(((int64_t)V + 3 + runs - 1) / runs) * hc::UW * 128;
+    const size_t smem = sizeof(hc::CShared);
     HC_CHECK((int64_t)B * cs <= 0x7fffffff, HC_ERR_INVALID, "hc_sample_uniform_dev: %d rows", B);
     HC_CUDA(cudaFuncSetAttribute(hc::k_sample_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     if (cs > 8) HC_CUDA(cudaFuncSetAttribute(hc::k_sample_cluster, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
