@@ -72,12 +72,13 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
 // leaves partial results to k_paged_join; a CTA cuts at most two (its first
 // and its last), so it has two slots.
 constexpr int UNIT = SP_WARPS * SP_TK;
-constexpr int SP_CTAS = 148 * 2;  // two CTAs per SM
+constexpr int SP_CTAS = 148 * 3;  // at most: CTAs of the cut line, as many as are resident at once
 constexpr int MIN_UNITS = 4;      // of a run: a CTA's start costs about as much as the stream of 256 keys
 
 struct SplitArgs {
     PagedAttnArgs a;
     int whole;
+    int ctas;     // CTAs of the line (cut)
     int rows;     // R, rows of a tile
     float* po;    // [slot][R][hd] partial outputs, slot = 2 CTA + (0: its first pair, 1: its last)
     float2* pml;  // [slot][R] (maximum in log2 units, sum)
@@ -149,15 +150,15 @@ __device__ __forceinline__ int64_t all_units(const PagedAttnArgs& A, int R) {
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     return n;
 }
-__device__ __forceinline__ int64_t run_of(int64_t units) {
-    return max((units + SP_CTAS - 1) / SP_CTAS, (int64_t)MIN_UNITS);
+__device__ __forceinline__ int64_t run_of(int64_t units, int ctas) {
+    return max((units + ctas - 1) / ctas, (int64_t)MIN_UNITS);
 }
 
 template <typename CT, int HD>
 struct SplitShape {
     static constexpr int ROWB = HD * (int)sizeof(CT);           // bytes of a key in shared memory
     static constexpr int STAGE = 2 * SP_TK * ROWB;              // K tile, V tile
-    static constexpr int STAGES = STAGE > 4096 ? 3 : 5;
+    static constexpr int STAGES = STAGE > 8192 ? 3 : (STAGE > 4096 ? 2 : 4);  // three CTAs an SM before a deeper ring
     static constexpr int WARPB = STAGES * STAGE;
     static constexpr int SMEM = SP_WARPS * WARPB + 512;         // 512: rows are aligned to their size
     static constexpr int LDO = HD + 4;                          // row of outputs: conflict-free column stores
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
         u = blockIdx.x;
         u_end = u + 1;
     } else {
-        const int64_t run = run_of(all_units(A, R));
+        const int64_t run = run_of(all_units(A, R), X.ctas);
         u = blockIdx.x * run;
         u_end = u + run;
     }
@@ -630,7 +631,7 @@ template <typename QT>
 __global__ void __launch_bounds__(SP_THREADS) k_paged_join(const __grid_constant__ SplitArgs X) {
     const PagedAttnArgs& A = X.a;
     const PagedArgs& P = A.p;
-    const int64_t run = run_of(all_units(A, X.rows));
+    const int64_t run = run_of(all_units(A, X.rows), X.ctas);
     Line at = {0, 0, {}};
     const bool any = advance(A, X.rows, blockIdx.x, true, at);  // pair blockIdx.x, counted in pairs
     pdl_wait();
@@ -684,13 +685,19 @@ int64_t pairs_bound(const SplitArgs& X) {
 }
 
 template <typename QT, typename CT, int HD, int NQ>
-int launch_split_t(const SplitArgs& X, cudaStream_t s) {
+int launch_split_t(SplitArgs& X, cudaStream_t s) {
     using Sh = SplitShape<CT, HD>;
     HC_CUDA(cudaFuncSetAttribute(k_paged_split<QT, CT, HD, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
     const PagedArgs& P = X.a.p;
+    static const int resident = [] {  // CTAs an SM holds: the kernel's registers and shared memory decide
+        int n = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_paged_split<QT, CT, HD, NQ>, SP_THREADS, Sh::SMEM) != cudaSuccess) n = 1;
+        return std::min(std::max(n, 1), SP_CTAS / 148);
+    }();
+    X.ctas = 148 * resident;
     const int64_t pairs = pairs_bound(X);
     HC_CHECK(pairs <= 0x7fffffff, HC_ERR_INVALID, "paged attention: %d rows of %d heads", P.n_rows, X.a.nh);
-    k_paged_split<QT, CT, HD, NQ><<<X.whole ? (unsigned)pairs : SP_CTAS, SP_THREADS, Sh::SMEM, s>>>(X);
+    k_paged_split<QT, CT, HD, NQ><<<X.whole ? (unsigned)pairs : (unsigned)X.ctas, SP_THREADS, Sh::SMEM, s>>>(X);
     HC_LAUNCH_CHECK();
     if (!X.whole) {
         const int y = (std::min(X.rows, X.a.G) * P.hd / 4 + SP_THREADS - 1) / SP_THREADS;
@@ -701,7 +708,7 @@ int launch_split_t(const SplitArgs& X, cudaStream_t s) {
 }
 
 template <typename QT, typename CT>
-int launch_split_hd(const SplitArgs& X, cudaStream_t s) {
+int launch_split_hd(SplitArgs& X, cudaStream_t s) {
     if (X.rows == 8) return X.a.p.hd <= 64 ? launch_split_t<QT, CT, 64, 1>(X, s) : launch_split_t<QT, CT, 128, 1>(X, s);
     return X.a.p.hd <= 64 ? launch_split_t<QT, CT, 64, 2>(X, s) : launch_split_t<QT, CT, 128, 2>(X, s);
 }
