@@ -488,7 +488,7 @@ AttnPlan attn_plan(const hc::PagedAttnArgs& A, const hc_paged_batch* b, int c16)
         plan.bytes = hc::paged_tc_bytes(A, b->max_kv_len);
     } else {
         plan.kernel = ATTN_SPLIT;
-        plan.bytes = hc::paged_split_bytes(A, b->max_kv_len);
+        plan.bytes = hc::paged_split_bytes(A, b->max_q_len, b->max_kv_len);
     }
     return plan;
 }

@@ -169,8 +169,8 @@ int launch_paged_tc(const PagedAttnArgs& A, int q16, int max_kv_len, void* ws, c
 
 // Few rows per sequence (hc_paged_split.cu): the keys split over CTAs.
 bool paged_split_ok(const PagedArgs& P, int c16);
-bool paged_split_whole(const PagedAttnArgs& A, int max_kv_len);
-size_t paged_split_bytes(const PagedAttnArgs& A, int max_kv_len);  // workspace
+bool paged_split_whole(const PagedAttnArgs& A, int max_q_len, int max_kv_len);
+size_t paged_split_bytes(const PagedAttnArgs& A, int max_q_len, int max_kv_len);  // workspace
 int launch_paged_split(const PagedAttnArgs& A, int q16, int c16, int max_q_len, int max_kv_len, void* ws,
                        cudaStream_t s);
 

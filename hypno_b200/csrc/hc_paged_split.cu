@@ -721,12 +721,16 @@ bool paged_split_ok(const PagedArgs& P, int c16) {
            (P.kps | P.khs | P.kss | P.vps | P.vhs | P.vss) % e == 0;
 }
 
-size_t paged_split_bytes(const PagedAttnArgs& A, int max_kv_len) {
-    return paged_split_whole(A, max_kv_len) ? 0 : (size_t)2 * SP_CTAS * 16 * ((size_t)A.p.hd * 4 + 8);
+size_t paged_split_bytes(const PagedAttnArgs& A, int max_q_len, int max_kv_len) {
+    return paged_split_whole(A, max_q_len, max_kv_len) ? 0 : (size_t)2 * SP_CTAS * 16 * ((size_t)A.p.hd * 4 + 8);
 }
 
-// One CTA per pair where no pair is long enough to be worth cutting.
-bool paged_split_whole(const PagedAttnArgs& A, int max_kv_len) {
+// One CTA per pair where no pair is long enough to be worth cutting, and for
+// chunks with many pairs: a chunk's early row tiles see fewer keys than the
+// line counts for them, and a CTA's pairs cost a start each (7 chunks of 264
+// tokens, 9 heads of 64, FP32 cache: 69 us cut, 51 whole).
+bool paged_split_whole(const PagedAttnArgs& A, int max_q_len, int max_kv_len) {
+    if ((int64_t)max_q_len * A.G > 64 && (int64_t)A.p.n_rows * A.G / 16 * A.p.nkv >= 2 * SP_CTAS) return true;
     const int64_t len = A.window > 0 ? std::min<int64_t>(max_kv_len, (int64_t)A.window + 16) : max_kv_len;
     return len <= MIN_UNITS * UNIT;
 }
@@ -735,7 +739,7 @@ int launch_paged_split(const PagedAttnArgs& A, int q16, int c16, int max_q_len, 
                        cudaStream_t s) {
     SplitArgs X;
     X.a = A;
-    X.whole = paged_split_whole(A, max_kv_len);
+    X.whole = paged_split_whole(A, max_q_len, max_kv_len);
     X.rows = (int64_t)max_q_len * A.G <= 8 ? 8 : 16;
     X.po = (float*)ws;
     X.pml = (float2*)((float*)ws + (size_t)2 * SP_CTAS * 16 * A.p.hd);

@@ -1,0 +1,107 @@
+"""The paged path end to end: a synthetic Q4_0 model through PagedModel against
+its forward pass in 64 bits on the host, and PagedGenerator's tokens whatever
+the schedule."""
+import importlib.util
+import os
+
+import numpy as np
+import pytest
+import torch
+
+from hypno_b200 import hypno_file as hf
+from hypno_b200 import ops, paged, synth
+from hypno_b200.paged_model import PagedGenerator, PagedModel
+
+pytestmark = pytest.mark.gpu
+CFG = dict(hidden=256, layers=2, heads=8, kv_heads=2, inter=384, vocab=700, theta=10000.0, max_pos=256)
+
+
+@pytest.fixture(scope="module")
+def image(cuda_device):
+    return synth.build_image(CFG, seed=5, std=0.08)
+
+
+def forward(image, ids):
+    """Logits after every token, in 64 bits."""
+    man = hf.Manifest(image)
+
+    def w(name):
+        shape, dt, _, _ = man.tensors[name]
+        raw, _ = man.tensor_bytes(name)
+        v = ops.dequantize_q4_0(bytes(raw)) if dt == hf.DT_Q4_0 else np.frombuffer(raw, np.float32)
+        return v[:int(np.prod(shape))].reshape(shape).astype(np.float64)
+
+    H, KH, D, n = CFG["heads"], CFG["kv_heads"], CFG["hidden"] // CFG["heads"], len(ids)
+    norm = lambda x, g: x / np.sqrt((x * x).mean(-1, keepdims=True) + 1e-5) * g  # noqa: E731
+    a = np.arange(n)[:, None] * CFG["theta"] ** (-2 * np.arange(D // 2) / D)
+    cs, sn = np.cos(a)[:, None], np.sin(a)[:, None]
+
+    def turn(x):
+        y = x.copy()
+        y[..., 0::2], y[..., 1::2] = x[..., 0::2] * cs - x[..., 1::2] * sn, x[..., 0::2] * sn + x[..., 1::2] * cs
+        return y
+
+    x = w("model.embed_tokens.weight")[ids]
+    for i in range(CFG["layers"]):
+        p = f"model.layers.{i}."
+        h = norm(x, w(p + "input_layernorm.weight"))
+        q, k, v = (h @ w(p + f"self_attn.{c}_proj.weight").T for c in "qkv")
+        q, k, v = turn(q.reshape(n, H, D)), turn(k.reshape(n, KH, D)), v.reshape(n, KH, D)
+        k, v = (np.repeat(t.astype(np.float16).astype(np.float64), H // KH, 1) for t in (k, v))
+        s = np.einsum("ihd,jhd->hij", q, k) / np.sqrt(D)
+        s = np.where(np.tril(np.ones((n, n), bool)), s, -np.inf)
+        e = np.exp(s - s.max(-1, keepdims=True))
+        x = x + np.einsum("hij,jhd->ihd", e / e.sum(-1, keepdims=True), v).reshape(n, -1) @ w(p + "self_attn.o_proj.weight").T
+        h = norm(x, w(p + "post_attention_layernorm.weight"))
+        g = h @ w(p + "mlp.gate_proj.weight").T
+        x = x + (g / (1 + np.exp(-g)) * (h @ w(p + "mlp.up_proj.weight").T)) @ w(p + "mlp.down_proj.weight").T
+    return norm(x, w("model.norm.weight")) @ w("model.embed_tokens.weight").T
+
+
+@pytest.mark.parametrize("sizes", [(40,), (17, 1, 1, 21), (1,) * 40])
+def test_logits(cuda_device, image, sizes):
+    """A prompt in one piece, in chunks, and token by token."""
+    ids = synth.prompt_ids(CFG["vocab"], 40, seed=3).astype(np.int64)
+    want = forward(image, ids)
+    m = PagedModel(image, n_pages=8, page_size=16)
+    t = paged.PageTable(8, 16, 1, 16)
+    i32 = dict(dtype=torch.int32, device=cuda_device)
+    at = 0
+    for n in sizes:
+        length = t.grow(0, n)
+        batch = paged.PagedBatch(torch.from_numpy(t.table[:, :3].copy()).to(cuda_device), torch.tensor([0, n], **i32), torch.tensor([length], **i32), n, length)
+        got = m.logits(torch.from_numpy(ids[at:at + n]).to(cuda_device), batch, torch.arange(n, device=cuda_device)).cpu().numpy()
+        # the framework's bar for logits (an FP16 cache rounds keys either way within it)
+        assert np.max(np.abs(got - want[at:at + n])) <= 1e-3 * max(1.0, np.abs(want).max())
+        at += n
+    m.close()
+
+
+def test_tokens_do_not_depend_on_the_schedule(cuda_device, image):
+    def tokens(max_seqs, budget):
+        m = PagedModel(image, n_pages=40, page_size=16)
+        gen = PagedGenerator(m, max_seqs=max_seqs, budget=budget)
+        g = np.random.default_rng(1)
+        for i in range(6):
+            gen.submit(g.integers(0, CFG["vocab"], size=int(g.integers(1, 90))), 12, temperature=[0.0, 0.7][i % 2], top_k=30, top_p=0.9, seed=i)
+        out = gen.run()
+        assert len(gen.pages.free) == 40
+        m.close()
+        return out
+
+    want = tokens(1, 1000)
+    assert all(len(v) == 12 for v in want.values())
+    for other in ((6, 1000), (4, 13)):
+        got = tokens(*other)
+        # a draw or a greedy pick may turn where two tokens lie within the logits' rounding
+        assert sum(got[k] != want[k] for k in want) <= 1
+
+
+def test_example_runs(cuda_device, capsys):
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_generate.py")
+    spec = importlib.util.spec_from_file_location("paged_generate", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    out = mod.main([path])
+    assert len(out) == 12 and all(len(v) == 24 for v in out.values())
+    assert "256 of 256 pages free" in capsys.readouterr().out
