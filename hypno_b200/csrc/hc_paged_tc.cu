@@ -86,12 +86,21 @@ struct TcBarriers {
     uint64_t drain;
 };
 
+// The key tiles of a CTA: positions begin + 128 j for j in [ja, jb), of which
+// half h is active in [ha[h], hb[h]).
+struct TcRange {
+    int begin, end;    // begin: a multiple of the box
+    int seen;          // first position that any row sees
+    int ja, jb;
+    int ha[2], hb[2];
+};
 struct TcControl {
     TcBarriers bars;
     __align__(16) uint32_t in[TC_MASKS][4];  // which keys of a tile exist (bytes of eight)
     float pair[TC_ROWS][2];                  // what a row's two threads tell one another
     uint32_t tmem;
     int abort, skip[2], bad[2], tile[6];
+    TcRange range;
 };
 static_assert(sizeof(TcControl) <= TC_CTRL, "the control block fits");
 
@@ -221,14 +230,6 @@ __device__ __forceinline__ bool quick_wait(uint64_t* bar, uint32_t parity, volat
 
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// The key tiles of a CTA: positions begin + 128 j for j in [ja, jb), of which
-// half h is active in [ha[h], hb[h]).
-struct TcRange {
-    int begin, end;    // begin: a multiple of the box
-    int seen;          // first position that any row sees
-    int ja, jb;
-    int ha[2], hb[2];
-};
 __device__ __forceinline__ TcRange tc_range(const PagedAttnArgs& A, int first, int m0, int mtot, int run, int nsplit, int box) {
     TcRange r;
     visible(A, first, m0, min(TC_ROWS, mtot - m0), r.seen, r.end);
@@ -278,10 +279,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         // later tiles of a prompt see more keys: they go first
         const bool ok = find_tile(P, A.G, TC_ROWS, bound - 1 - (int)(blockIdx.x / X.nsplit), seq, tile);
         if (ok && lane == 0) {
+            // once for all warps: everything that follows from the tile's place
+            int a, b;
+            seq_rows(P, seq, a, b);
+            const int at = __ldg(P.kv_len + seq) - (b - a), m = tile * TC_ROWS;
             s_tile[1] = seq;
-            s_tile[2] = tile;
-            seq_rows(P, seq, s_tile[3], s_tile[4]);
-            s_tile[5] = __ldg(P.kv_len + seq);
+            s_tile[2] = m;
+            s_tile[3] = a;
+            s_tile[4] = (int)min((int64_t)(b - a) * A.G, (int64_t)m + TC_ROWS);  // rows up to this tile's end
+            s_tile[5] = at;
+            C.range = tc_range(A, at, m, s_tile[4], blockIdx.x % X.nsplit, X.nsplit, TMA ? X.box : 0);
         }
         if (lane == 0) s_tile[0] = ok;
     }
@@ -317,10 +324,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         return;
     }
     const int run = blockIdx.x % X.nsplit, kvh = blockIdx.y;
-    const int seq = s_tile[1], m0 = s_tile[2] * TC_ROWS;
-    const int r0 = s_tile[3], r1 = s_tile[4], first = s_tile[5] - (r1 - r0);
-    const int mtot = (int)min((int64_t)(r1 - r0) * A.G, (int64_t)m0 + TC_ROWS);  // rows up to this tile's end
-    const TcRange rg = tc_range(A, first, m0, mtot, run, X.nsplit, TMA ? X.box : 0);
+    const int seq = s_tile[1], m0 = s_tile[2], r0 = s_tile[3], mtot = s_tile[4], first = s_tile[5];
+    const TcRange rg = C.range;
 
     if (warp < 16) {
         // ================ the halves: queries, weights, outputs
@@ -337,6 +342,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         auto pair_sync = [&]() { named_sync(pair_id, 64); };
         bool ok = true;
         float up = 1.0f;  // 2^e of an f32 row
+        auto row_offset = [&](int64_t rs, int64_t hs) -> int64_t {
+            const int t = token_of(A, mh + r);
+            return (int64_t)(r0 + t) * rs + (kvh * A.G + (mh + r) - t * A.G) * hs;
+        };
         // ---- queries.  Eight rows are QG bytes, whether as they come (f32 or fp16
         // rows one after the other) or as the products take them (128-byte pieces
         // of the eight rows), so a warp copies its rows as they come and turns
@@ -346,12 +355,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             const int d = (lane % LPR) * EPL;
             const uint32_t mine = qs + (uint32_t)(((warp & 3) * 4 + g * 2) * Sh::QG);  // 16 rows
             const int row0 = (warp & 3) * 32 + g * 16;
+            const int64_t at = r < rows ? row_offset(A.q_rs, A.q_hs) : 0;  // of this lane's row
 #pragma unroll 4
             for (int i = 0; i < 16 / RPI; i++) {
-                const int rr = i * RPI + lane / LPR, row = row0 + rr, m = mh + row;
+                const int rr = i * RPI + lane / LPR, row = row0 + rr;
                 const bool there = row < rows && d < P.hd;
-                const int t = there ? token_of(A, m) : 0;
-                const QT* q = (const QT*)A.q + (there ? (int64_t)(r0 + t) * A.q_rs + (kvh * A.G + m - t * A.G) * A.q_hs + d : 0);
+                const QT* q = (const QT*)A.q + __shfl_sync(0xffffffffu, at, g * 16 + rr) + (there ? d : 0);
                 const uint32_t dst = mine + (HILO ? (uint32_t)(rr * HD * 4 + (lane % LPR) * 16)
                                                   : (uint32_t)((rr >> 3) * Sh::QG + (d >> 6) * 1024 + (rr & 7) * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4)));
                 if (A.qvec || !there) {
@@ -768,19 +777,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             }
         }
         if (X.nsplit == 1 && rows > 0) {
+            const int64_t at = in ? row_offset(A.o_rs, A.o_hs) : 0;
             fin_sync(1);
             constexpr int EPL = 16 / (int)sizeof(QT), LPR = HD / EPL, RPI = 32 / LPR;
             const int d = (lane % LPR) * EPL;
 #pragma unroll 4
             for (int i = 0; i < 16 / RPI; i++) {
                 const int rr = g * 16 + i * RPI + lane / LPR, row = (warp & 3) * 32 + rr;
+                const int64_t off = __shfl_sync(0xffffffffu, at, rr);
                 if (row >= rows || d >= P.hd) continue;
                 uint32_t w[4];
                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                              : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                              : "r"(stage + (uint32_t)(rr * HD * (int)sizeof(QT)) + (((lane % LPR) ^ (rr & 7)) << 4)));
-                const int t = token_of(A, mh + row);
-                QT* out = (QT*)A.out + (int64_t)(r0 + t) * A.o_rs + (kvh * A.G + (mh + row) - t * A.G) * A.o_hs + d;
+                QT* out = (QT*)A.out + off + d;
                 if (A.ovec) {
                     *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
                 } else {
