@@ -252,8 +252,8 @@ __device__ __noinline__ void sample_row(URow R, URowArgs P, UShared& S, int32_t*
 // ============================================================ the cluster kernel
 
 constexpr int UC_MAX = 16;         // CTAs of a cluster (above 8 for few long rows only)
-constexpr int HB2 = 1024;          // buckets of a histogram
-constexpr int HBT = HB2 / UT;      // a thread's
+constexpr int HB2 = 256;           // buckets of a histogram (the first CTA reads everyone's)
+static_assert(HB2 == UT, "a bucket a thread");
 // Distances (max - l) / T that the two histograms cover: up to the head's end and
 // from there to TAIL, where weights are below 2^-40.  The head ends NEAR below the
 // maximum in logits (a language model has some thousands of tokens there), and
@@ -261,7 +261,7 @@ constexpr int HBT = HB2 / UT;      // a thread's
 constexpr float NEAR = 12.0f, HEAD_MIN = 8.0f, HEAD_MAX = 27.0f, TAIL = 28.0f;
 constexpr int CAP = 1024;          // tokens of a bucket that are sorted
 constexpr int WCAP = 512;          // tokens of a warp's list
-constexpr int GO_ON = -2, ALL = -1, SLOW = HB2;  // instead of a bucket
+constexpr int FINER = -3, GO_ON = -2, ALL = -1, SLOW = HB2;  // instead of a bucket
 
 struct __align__(16) CShared {
     union {
@@ -282,11 +282,11 @@ struct __align__(16) CShared {
     u64 c_mass[UC_MAX];
     // what the first CTA tells all
     int n_list;
-    int bucket;
+    int bucket, within;            // what the histogram gave; the bucket that a finer one divides
     u64 cut;                       // the last token kept: key above ~index
     // the first CTA's own
-    u64 sel_mass, head_mass;       // mass before the bucket; of the first histogram
-    uint32_t sel_cnt, head_cnt;    // likewise tokens
+    u64 sel_mass, base_mass;       // mass before the bucket; before the histogram
+    uint32_t sel_cnt, base_cnt;    // likewise tokens
     u64 w_mass[UW];                // of the warps' buckets
     uint32_t w_cnt[UW];
 };
@@ -296,8 +296,22 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
     return r;
 }
+// (Not the .aligned forms: they are undefined for a warp whose lanes have not met
+// again after a branch, which the compiler does not promise at inline assembly.)
 __device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+// The two halves apart: the first access of another CTA's shared memory comes
+// after that CTA has begun, which nothing else promises.
+__device__ __forceinline__ void cluster_begun() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_all_begun() {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
     uint32_t r;
@@ -370,6 +384,7 @@ __global__ void __launch_bounds__(UT, 4) k_sample_cluster(const float* __restric
         if (CS > 1) cluster_barrier();
         else __syncthreads();
     };
+    if (CS > 1) cluster_begun();
     const float T = temp[row];
     URowArgs P;
     P.u = u[row];
@@ -432,6 +447,7 @@ __global__ void __launch_bounds__(UT, 4) k_sample_cluster(const float* __restric
     if (threadIdx.x == 0) S.cut = 1ull << 32;  // keys from 1 on: every token
     __syncthreads();
     kmax = __reduce_max_sync(0xffffffffu, lane < UW ? S.redu[lane] : 0u);
+    if (CS > 1) cluster_all_begun();
     if (threadIdx.x < CS) remote_st32(&S.c_max[rank], threadIdx.x, kmax);
     sync_all();
     for (int c = 0; c < CS; c++) kmax = max(kmax, S.c_max[c]);
@@ -491,7 +507,14 @@ __global__ void __launch_bounds__(UT, 4) k_sample_cluster(const float* __restric
         if (level == 0) return -x < headd ? min((int)(-x * step0), HB2 - 1) : -1;
         return -x >= headd && -x < TAIL ? min((int)((-x - headd) * step1), HB2 - 1) : -1;
     };
-    auto bucket_of = [&](float f, int level) -> int { return bucket_at(expo(f), level); };
+    // within >= 0: the places in a finer histogram of that bucket, -1 outside it
+    auto place = [&](float x, int level, int within) -> int {
+        const int b = bucket_at(x, level);
+        if (within < 0) return b;
+        if (b != within) return -1;
+        const float step = level ? step1 : step0, lo = (level ? headd : 0.0f) + (float)within / step;
+        return min(max((int)((-x - lo) * step * HB2), 0), HB2 - 1);
+    };
 
     const bool by_k = P.tk > 0 && P.tk < V, by_p = P.tp < 1.0f && P.tk != 1;
     u64 cut = 1ull << 32;
@@ -555,8 +578,12 @@ __global__ void __launch_bounds__(UT, 4) k_sample_cluster(const float* __restric
         bool cut_near = false; // the end found last is within the head
         // Two ends may have to be found: top-k's by count, then top-p's by mass.
         for (int pass = by_k ? 0 : 1; pass < (by_p ? 2 : 1); pass++) {
-            int level = 0;
-            for (;; level++) {
+            int level = 0, within = -1;
+            if (rank == 0 && threadIdx.x == 0) {
+                S.base_mass = 0ull;
+                S.base_cnt = 0u;
+            }
+            for (int round = 0; round < 3; round++) {  // the head, the rest, a finer one
                 // ---- 3: the histogram: counts, and for top-p masses
                 for (int b = threadIdx.x; b < HB2; b += UT) {
                     S.h.sum[b] = 0ull;
@@ -564,17 +591,18 @@ __global__ void __launch_bounds__(UT, 4) k_sample_cluster(const float* __restric
                 }
                 __syncthreads();
                 // (what top-k kept has its mass taken here, near or not)
-                near = level == 0 && (pass == 0 || !by_k || cut_near);
+                const bool first = level == 0 && within < 0;
+                near = level == 0 && (pass == 0 || !by_k || cut_near || !first);
                 u64 m2 = 0;
                 each([&](float f, uint32_t i) {
                     if (!in_head(f, i)) return;
                     const float x = expo(f);
-                    const int b = bucket_at(x, level);
+                    const int b = place(x, level, within);
                     if (pass == 0) {
                         if (b >= 0) atomicAdd(&S.h.cnt[b], 1u);
                         return;
                     }
-                    if (b < 0 && (level == 1 || !by_k)) return;
+                    if (b < 0 && (!first || !by_k)) return;
                     const u64 m = mass_of(expf(x));
                     m2 += m;
                     if (b >= 0) {
@@ -582,15 +610,16 @@ __global__ void __launch_bounds__(UT, 4) k_sample_cluster(const float* __restric
                         atomicAdd(&S.h.sum[b], m);
                     }
                 });
-                if (pass == 1 && level == 0 && by_k) {
+                if (pass == 1 && first && by_k) {
                     m2 = block_sum(m2);
                     if (threadIdx.x == 0) remote_st64(&S.c_mass[rank], 0, m2);
                 }
                 sync_all();
                 if (rank == 0) {  // the first CTA adds the histograms up
-                    if (pass == 1 && level == 0)
+                    if (pass == 1 && first)
                         for (int c = 0; c < CS; c++) held += S.c_mass[c];
-                    for (int b = threadIdx.x; b < HB2; b += UT) {
+                    {
+                        const int b = threadIdx.x;
                         uint32_t nc[UC_MAX];
                         u64 ms[UC_MAX];
 #pragma unroll
@@ -607,20 +636,12 @@ __global__ void __launch_bounds__(UT, 4) k_sample_cluster(const float* __restric
                     __syncthreads();
                 }
                 if (rank == 0) {
-                    // the last bucket that holds a token of the order's head: HBT buckets a thread
+                    // the last bucket that holds a token of the order's head: a bucket a thread
                     const double goal = (double)P.tp * (double)held;
-                    const int b0 = HBT * threadIdx.x;
-                    uint32_t c[HBT], cs = 0;
-                    u64 m[HBT], ms = 0;
-#pragma unroll
-                    for (int i = 0; i < HBT; i++) {
-                        c[i] = S.h.cnt[b0 + i];
-                        m[i] = S.h.sum[b0 + i];
-                        cs += c[i];
-                        ms += m[i];
-                    }
-                    uint32_t ci = cs;
-                    u64 mi = ms;
+                    const uint32_t c = S.h.cnt[threadIdx.x];
+                    const u64 m = S.h.sum[threadIdx.x];
+                    uint32_t ci = c;
+                    u64 mi = m;
                     for (int o = 1; o < 32; o <<= 1) {
                         const uint32_t tc = __shfl_up_sync(0xffffffffu, ci, o);
                         const u64 tm = __shfl_up_sync(0xffffffffu, mi, o);
@@ -638,8 +659,8 @@ __global__ void __launch_bounds__(UT, 4) k_sample_cluster(const float* __restric
                         S.n_list = 0;
                     }
                     __syncthreads();
-                    uint32_t nb = level ? S.head_cnt : 0u, all_n = nb;
-                    u64 be = level ? S.head_mass : 0ull, all_m = be;
+                    uint32_t nb = S.base_cnt, all_n = nb;
+                    u64 be = S.base_mass, all_m = be;
                     for (int w = 0; w < UW; w++) {
                         if (w < warp) {
                             nb += S.w_cnt[w];
@@ -648,23 +669,10 @@ __global__ void __launch_bounds__(UT, 4) k_sample_cluster(const float* __restric
                         all_n += S.w_cnt[w];
                         all_m += S.w_mass[w];
                     }
-                    nb += ci - cs;
-                    be += mi - ms;
+                    nb += ci - c;
+                    be += mi - m;
                     const bool over = pass == 0 ? all_n >= (uint32_t)P.tk : !((double)all_m < goal);
-                    int mine = -1;
-                    uint32_t my_nb = 0, my_c = 0;
-                    u64 my_be = 0;
-#pragma unroll
-                    for (int i = 0; i < HBT; i++) {
-                        if (c[i] > 0 && (pass == 0 ? nb < (uint32_t)P.tk : (double)be < goal)) {
-                            mine = b0 + i;
-                            my_nb = nb;
-                            my_be = be;
-                            my_c = c[i];
-                        }
-                        nb += c[i];
-                        be += m[i];
-                    }
+                    const int mine = c > 0 && (pass == 0 ? nb < (uint32_t)P.tk : (double)be < goal) ? (int)threadIdx.x : -1;
                     const int best = __reduce_max_sync(0xffffffffu, mine);
                     if (lane == 0 && best >= 0) atomicMax(&S.bucket, best);
                     __syncthreads();
@@ -672,19 +680,33 @@ __global__ void __launch_bounds__(UT, 4) k_sample_cluster(const float* __restric
                     __syncthreads();
                     if (over && sel >= 0 ? mine == sel : threadIdx.x == 0) {
                         // not over: the order ends further on, or (top-k) it keeps every token with a mass
-                        const int b = over && sel >= 0 ? (my_c <= (uint32_t)CAP ? sel : SLOW) : level == 0 ? GO_ON : pass == 0 ? ALL : SLOW;
-                        S.bucket = b;
-                        S.sel_mass = my_be;
-                        S.sel_cnt = my_nb;
-                        if (b == GO_ON) {
-                            S.head_mass = all_m;
-                            S.head_cnt = all_n;
+                        int b;
+                        if (over && sel >= 0) {
+                            b = c <= (uint32_t)CAP ? sel : within < 0 ? FINER : SLOW;
+                            S.sel_mass = be;
+                            S.sel_cnt = nb;
+                            if (b == FINER) {
+                                S.base_mass = be;
+                                S.base_cnt = nb;
+                            }
+                        } else {
+                            b = level == 0 && within < 0 ? GO_ON : pass == 0 && within < 0 ? ALL : SLOW;
+                            if (b == GO_ON) {
+                                S.base_mass = all_m;
+                                S.base_cnt = all_n;
+                            }
                         }
+                        S.bucket = b;
+                        S.within = sel;
+                        for (int q = 1; q < CS; q++) remote_st32(&S.within, q, (uint32_t)sel);
                         for (int q = 1; q < CS; q++) remote_st32(&S.bucket, q, (uint32_t)b);
                     }
                 }
                 sync_all();
-                if (S.bucket != GO_ON) break;
+                const int got = S.bucket;
+                if (got != GO_ON && got != FINER) break;
+                if (got == GO_ON) level = 1;
+                else within = S.within;
                 sync_all();  // (all have read it)
             }
             const int sel = S.bucket;
@@ -699,7 +721,7 @@ __global__ void __launch_bounds__(UT, 4) k_sample_cluster(const float* __restric
             // ---- 4: the bucket's tokens, to the first CTA
             near = level == 0;
             each([&](float f, uint32_t i) {
-                if (!in_head(f, i) || bucket_of(f, level) != sel) return;
+                if (!in_head(f, i) || place(expo(f), level, within) != sel) return;
                 uint32_t at;
                 asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(CS > 1 ? remote(&S.n_list, 0) : smem_u32(&S.n_list)) : "memory");
                 if (at >= (uint32_t)CAP) return;

@@ -76,6 +76,21 @@ def test_ties_go_to_the_lowest_index(cuda_device, V):
     assert int(t) == int(np.ceil(0.25 * V)) - 1
 
 
+@pytest.mark.parametrize("V", [3000, 9000, 40001])
+@pytest.mark.parametrize("spread", [1e-3, 0.5, 30.0])
+def test_flat_and_steep_rows(cuda_device, V, spread):
+    """Ends of the order in buckets with thousands of distinct logits, far below the
+    maximum, and among ties of thousands."""
+    g = np.random.default_rng(V)
+    l = np.empty((4, V), np.float32)
+    l[0] = spread * g.random(V)                                   # evenly spread
+    l[1] = -spread * np.sqrt(g.random(V))                         # most of them at the far end
+    l[2] = np.where(g.random(V) < 0.5, -spread, 0.0)              # two values
+    l[3] = -spread * g.random(V) ** 8                             # most of them at the maximum
+    s = [(1.0, 0, 0.3, 0.0), (1.0, 0, 0.97, 0.0), (1.0, V // 2, 1.0, 0.0), (0.7, V - 7, 0.5, 0.2), (3.0, 1500, 0.9, 0.0), (0.05, 700, 0.999, 0.0)]
+    draws(cuda_device, l, s, g.random(4 * len(s)).astype(np.float32))
+
+
 def test_special_rows(cuda_device):
     """NaN and -inf are never drawn, +inf and -0 / +0 are handled, a row without a logit gives -1."""
     nan, inf = np.nan, np.inf
