@@ -730,6 +730,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                     l == 0.0f ? -INFINITY : (m - (HILO ? BIAS_EXACT : BIAS) + log2f(l)) / LOG2E;
             }
         }
+        __syncwarp();  // (the loads below are the warp's)
         const float inv = X.nsplit > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
         // 16 columns at a time: partial results straight to the workspace; results
         // through the half's query memory (its products are done), so that a
@@ -822,11 +823,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         uint32_t pdone[2] = {0, 0};
         int ks = 0, vs = NS - 1;          // ring slots of K_j and V_(j-1), with their phases
         uint32_t kph = 0, vph = 1;
+        if (NS > 3 && ja < jb) ok = quick_wait(&B.full[0], 0, &abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
         for (int j = ja; j <= jb && ok; j++) {
             const uint64_t k_d = k_d0 + (uint64_t)(ks * (Sh::TILE >> 4)), v_d = v_d0 + (uint64_t)(vs * (Sh::TILE >> 4));
-            int vs2 = vs + 2;             // V_j
-            uint32_t vph2 = vph;
+            int vs2 = vs + 2, ks2 = ks + 2;  // V_j, K_(j+1)
+            uint32_t vph2 = vph, kph2 = kph;
             if (vs2 >= NS) vs2 -= NS, vph2 ^= 1u;
+            if (ks2 >= NS) ks2 -= NS, kph2 ^= 1u;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const uint32_t s_t = tm + (uint32_t)(h * 128), o_t = tm + 256u + (uint32_t)(h * 128);
@@ -843,23 +847,30 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                                        idesc_o, (!HILO && pdone[h] > 0) || part > 0 || k4 > 0 || p < PL - 1);
                         }
                 };
+                bool both = false;
                 if (pv) {
-                    ok = quick_wait(&B.p_ready[h][0], pdone[h] & 1u, &abort_flag);
+                    ok = ok && quick_wait(&B.p_ready[h][0], pdone[h] & 1u, &abort_flag);
+                    __syncwarp();
+                    both = __all_sync(0xffffffffu, mbar_try_wait(&B.p_ready[h][1], pdone[h] & 1u));
                     tmem_fence_after();
                     mul = !*(volatile int*)&s_skip[h];
-                    if (mul && elect_one()) add_pv(0);
-                    __syncwarp();
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!both) {
+                        if (mul && ok && elect_one()) add_pv(0);
+                        __syncwarp();
+                        ok = ok && quick_wait(&B.p_ready[h][1], pdone[h] & 1u, &abort_flag);
+                    }
                 }
-                // the copies, while the other weights are made: K_j before its first use, V_j before the next step
-                if (h == 0 && j < jb) ok = ok && quick_wait(&B.full[ks], kph, &abort_flag);
-                if (h == 1 && j < jb) ok = ok && quick_wait(&B.full[vs2], vph2, &abort_flag);
+                if (NS == 3 && h == 0 && j < jb) ok = ok && quick_wait(&B.full[ks], kph, &abort_flag);  // (its slot was V_(j-2)'s)
                 if (sc && j == ha) ok = ok && quick_wait(&B.q_ready[h], 0, &abort_flag);
-                if (pv) ok = ok && quick_wait(&B.p_ready[h][1], pdone[h] & 1u, &abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tmem_fence_after();
                 if (elect_one()) {
-                    if (mul) add_pv(1);
+                    if (mul) {
+                        if (both) add_pv(0);
+                        add_pv(1);
+                    }
                     if (h == 1 && j > ja) mma_commit(&B.empty[vs]);
                     if (sc) {  // S_h = Q_h K_j^T
 #pragma unroll
@@ -877,9 +888,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                 }
                 __syncwarp();
                 if (pv) pdone[h]++;
+                // the copies that the next products need, while the tensor core is busy with these
+                if (h == 0 && j < jb) ok = ok && quick_wait(&B.full[vs2], vph2, &abort_flag);
+                if (NS > 3 && h == 1 && j + 1 < jb) ok = ok && quick_wait(&B.full[ks2], kph2, &abort_flag);
             }
-            ks += 2;
-            if (ks >= NS) ks -= NS, kph ^= 1u;
+            ks = ks2;
+            kph = kph2;
             vs = vs2;
             vph = vph2;
         }
