@@ -626,7 +626,11 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
 }
 
 // Joins the partial results of a pair that was cut: with M = max m_s, o = sum
-// 2^(m_s - M) o_s / sum 2^(m_s - M) l_s, in the order of the CTAs.
+// 2^(m_s - M) o_s / sum 2^(m_s - M) l_s, in the order of the CTAs.  Bound by
+// latency (a pair has a few KB of partial results), so what can be worked out
+// from the batch alone is done before the wait, and JOIN CTAs' results are
+// requested at once.
+constexpr int JOIN = 8;
 template <typename QT>
 __global__ void __launch_bounds__(SP_THREADS) k_paged_join(const __grid_constant__ SplitArgs X) {
     const PagedAttnArgs& A = X.a;
@@ -634,8 +638,6 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_join(const __grid_constant
     const int64_t run = run_of(all_units(A, X.rows), X.ctas);
     Line at = {0, 0, {}};
     const bool any = advance(A, X.rows, blockIdx.x, true, at);  // pair blockIdx.x, counted in pairs
-    pdl_wait();
-    if (!any) return;
     const int seq = at.b, pair = (int)(blockIdx.x - at.base);
     // units before this sequence
     int64_t before = 0;
@@ -647,7 +649,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_join(const __grid_constant
     for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
     const int64_t p0 = before + (int64_t)pair * at.w.units, p1 = p0 + at.w.units;
     const int c0 = (int)(p0 / run), c1 = (int)((p1 - 1) / run);
-    if (c0 == c1) return;  // one CTA took it whole
+    pdl_wait();  // (every CTA waits: the next kernel on the stream begins when this grid has ended)
+    if (!any || c0 == c1) return;  // c0 == c1: one CTA took it whole
     const int kvh = pair % P.nkv, m0 = pair / P.nkv * X.rows, r0 = at.w.r0;
     const int mrows = (int)min((int64_t)X.rows, (int64_t)(at.w.r1 - r0) * A.G - m0);
     const int hq = P.hd >> 2;
@@ -656,21 +659,40 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_join(const __grid_constant
     auto slot = [&](int c) -> int64_t { return c == c0 ? s0 : 2 * (int64_t)c; };
     for (int x = blockIdx.y * SP_THREADS + threadIdx.x; x < mrows * hq; x += SP_THREADS * gridDim.y) {
         const int m = x / hq, d = (x - m * hq) * 4;
-        float mx = -INFINITY;
-        for (int c = c0; c <= c1; c++) mx = fmaxf(mx, X.pml[slot(c) * X.rows + m].x);
-        float l = 0.0f;
+        float mx = -INFINITY, l = 0.0f;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int c = c0; c <= c1; c++) {
-            const float2 ml = X.pml[slot(c) * X.rows + m];
-            const float4 y = *reinterpret_cast<const float4*>(X.po + (slot(c) * X.rows + m) * P.hd + d);
-            if (ml.y == 0.0f) continue;  // saw nothing
-            const float f = exp2f(ml.x - mx);
-            l = fmaf(f, ml.y, l);
-            v.x = fmaf(f, y.x, v.x);
-            v.y = fmaf(f, y.y, v.y);
-            v.z = fmaf(f, y.z, v.z);
-            v.w = fmaf(f, y.w, v.w);
+        for (int cb = c0; cb <= c1; cb += JOIN) {
+            float2 ml[JOIN];
+            float4 y[JOIN];
+#pragma unroll
+            for (int i = 0; i < JOIN; i++) {
+                const int64_t at_row = slot(min(cb + i, c1)) * X.rows + m;
+                ml[i] = X.pml[at_row];
+                y[i] = *reinterpret_cast<const float4*>(X.po + at_row * P.hd + d);
+                if (cb + i > c1) ml[i] = make_float2(-INFINITY, 0.0f);
+            }
+            float top = mx;
+#pragma unroll
+            for (int i = 0; i < JOIN; i++) top = fmaxf(top, ml[i].x);
+            if (l != 0.0f) {
+                const float f = exp2f(mx - top);
+                l *= f;
+                v.x *= f;
+                v.y *= f;
+                v.z *= f;
+                v.w *= f;
+            }
+            mx = top;
+#pragma unroll
+            for (int i = 0; i < JOIN; i++) {
+                if (ml[i].y == 0.0f) continue;  // saw nothing
+                const float f = exp2f(ml[i].x - mx);
+                l = fmaf(f, ml[i].y, l);
+                v.x = fmaf(f, y[i].x, v.x);
+                v.y = fmaf(f, y[i].y, v.y);
+                v.z = fmaf(f, y[i].z, v.z);
+                v.w = fmaf(f, y[i].w, v.w);
+            }
         }
         const int t = token_of(A, m0 + m), row = r0 + t, head = kvh * A.G + (m0 + m) - t * A.G;
         store_row4<QT>(A, row, head, d, l, v);
