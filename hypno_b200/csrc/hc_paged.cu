@@ -31,10 +31,13 @@ __device__ __forceinline__ int seq_of_row(const PagedArgs& P, int r) {
 
 // 16-byte groups.  A unit is eight elements of a head: four pairs, which lie
 // side by side (adjacent) or in two runs of four (halves), or eight elements
-// past rot or of v, which pass through.  A block takes one row, its threads up
-// to NU units each: all loads of a thread are in flight before the row's
-// place in the cache (three dependent loads: row start, length, page) is known.
+// past rot or of v, which pass through.  A thread takes one unit, a row's units
+// are dealt over blocks; a thread's loads are in flight before the row's place
+// in the cache (three dependent loads: row start, length, page) is known.
 // Bound by its bytes: q is read and written, k and v are read and stored.
+// (Three units a thread, with as many loads in flight, took 63 us where one
+// takes 60: 8,192 rows of 32 + 8 + 8 heads of 128, f32 into FP16; 32 rows: 3.9
+// against 3.3.)
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, float* v) {
     if constexpr (sizeof(T) == 4) {
@@ -58,69 +61,59 @@ __device__ __forceinline__ void store4(T* p, const float* v) {
 
 constexpr int AP_THREADS = 256;
 
-template <typename T, typename C, int NU>
+template <typename T, typename C>
 __global__ void __launch_bounds__(AP_THREADS) k_paged_append_vec(AppendArgs A) {
     const PagedArgs& P = A.p;
     const int row = blockIdx.x, hu = P.hd >> 3, half = A.rot >> 1;
-    const int units = (A.nh + 2 * P.nkv) * hu;
-    const int first = blockIdx.y * (AP_THREADS * NU) + threadIdx.x;
-    float v[NU][8];
-    int head[NU], i0[NU], i1[NU];  // first elements of the two runs of four
-#pragma unroll
-    for (int n = 0; n < NU; n++) {
-        const int unit = first + n * AP_THREADS;
-        head[n] = unit < units ? unit / hu : -1;
-        if (head[n] < 0) continue;
-        const int u = unit - head[n] * hu;
-        i0[n] = 8 * u;
-        i1[n] = i0[n] + 4;
-        if (A.halves && i0[n] < A.rot) {
-            i0[n] = 4 * u;
-            i1[n] = i0[n] + half;
-        }
-        const T* src = head[n] < A.nh             ? (const T*)A.q + row * A.q_rs + head[n] * A.q_hs
-                       : head[n] < A.nh + P.nkv ? (const T*)A.k + row * A.k_rs + (head[n] - A.nh) * A.k_hs
-                                                  : (const T*)A.v + row * A.v_rs + (head[n] - A.nh - P.nkv) * A.v_hs;
-        load4(src + i0[n], v[n]);
-        load4(src + i1[n], v[n] + 4);
+    const int unit = blockIdx.y * AP_THREADS + threadIdx.x;
+    if (unit >= (A.nh + 2 * P.nkv) * hu) return;
+    int head = unit / hu;
+    const int u = unit - head * hu;
+    const bool is_q = head < A.nh, is_v = head >= A.nh + P.nkv;
+    if (!is_q) head -= is_v ? A.nh + P.nkv : A.nh;
+    const bool rotated = 8 * u < A.rot && !is_v;
+    int i0 = 8 * u, i1 = i0 + 4;  // first elements of the two runs of four
+    if (A.halves && i0 < A.rot) {
+        i0 = 4 * u;
+        i1 = i0 + half;
     }
+    const T* src = is_q   ? (const T*)A.q + row * A.q_rs + head * A.q_hs
+                   : is_v ? (const T*)A.v + row * A.v_rs + head * A.v_hs
+                          : (const T*)A.k + row * A.k_rs + head * A.k_hs;
+    float x[8];
+    load4(src + i0, x);
+    load4(src + i1, x + 4);
     const int seq = seq_of_row(P, row);
     int r0, r1;
     seq_rows(P, seq, r0, r1);
     if (row < r0 || row >= r1) return;
     const int pos = __ldg(P.kv_len + seq) - (r1 - r0) + (row - r0);
-    const float2* cs = A.rope + (int64_t)min(max(pos, 0), A.rope_rows - 1) * half;
-    int slot = 0;
-    const int page = pos >= 0 ? lookup(P, seq, pos, slot) : -1;
+    if (rotated) {
+        const float2* cs = A.rope + (int64_t)min(max(pos, 0), A.rope_rows - 1) * half + (A.halves ? i0 : i0 >> 1);
+        const float4 c01 = __ldg(reinterpret_cast<const float4*>(cs)), c23 = __ldg(reinterpret_cast<const float4*>(cs + 2));
+        const float c[4] = {c01.x, c01.z, c23.x, c23.z}, s[4] = {c01.y, c01.w, c23.y, c23.w};
 #pragma unroll
-    for (int n = 0; n < NU; n++) {
-        if (head[n] < 0) continue;
-        const bool is_q = head[n] < A.nh, is_v = head[n] >= A.nh + P.nkv;
-        float* x = v[n];
-        if (i0[n] < A.rot && !is_v) {
-            const int j = A.halves ? i0[n] : i0[n] >> 1;  // first pair
-            const float4 c01 = __ldg(reinterpret_cast<const float4*>(cs + j)), c23 = __ldg(reinterpret_cast<const float4*>(cs + j + 2));
-            const float c[4] = {c01.x, c01.z, c23.x, c23.z}, s[4] = {c01.y, c01.w, c23.y, c23.w};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                // static places: a pair is (i, i + 4) or (2 i, 2 i + 1)
-                const float a = A.halves ? x[i] : x[2 * i], b = A.halves ? x[i + 4] : x[2 * i + 1];
-                const float ra = a * c[i] - b * s[i], rb = a * s[i] + b * c[i];
-                if (A.halves) x[i] = ra, x[i + 4] = rb;
-                else x[2 * i] = ra, x[2 * i + 1] = rb;
-            }
-        }
-        if (is_q) {
-            T* dst = (T*)A.qo + row * A.o_rs + head[n] * A.o_hs;
-            store4(dst + i0[n], x);
-            store4(dst + i1[n], x + 4);
-        } else if (page >= 0) {
-            C* dst = is_v ? (C*)P.v + page * P.vps + (head[n] - A.nh - P.nkv) * P.vhs + slot * P.vss
-                          : (C*)P.k + page * P.kps + (head[n] - A.nh) * P.khs + slot * P.kss;
-            store4(dst + i0[n], x);
-            store4(dst + i1[n], x + 4);
+        for (int i = 0; i < 4; i++) {
+            // static places: a pair is (i, i + 4) or (2 i, 2 i + 1)
+            const float a = A.halves ? x[i] : x[2 * i], b = A.halves ? x[i + 4] : x[2 * i + 1];
+            const float ra = a * c[i] - b * s[i], rb = a * s[i] + b * c[i];
+            if (A.halves) x[i] = ra, x[i + 4] = rb;
+            else x[2 * i] = ra, x[2 * i + 1] = rb;
         }
     }
+    if (is_q) {
+        T* dst = (T*)A.qo + row * A.o_rs + head * A.o_hs;
+        store4(dst + i0, x);
+        store4(dst + i1, x + 4);
+        return;
+    }
+    if (pos < 0) return;
+    int slot;
+    const int page = lookup(P, seq, pos, slot);
+    if (page < 0) return;
+    C* dst = is_v ? (C*)P.v + page * P.vps + head * P.vhs + slot * P.vss : (C*)P.k + page * P.kps + head * P.khs + slot * P.kss;
+    store4(dst + i0, x);
+    store4(dst + i1, x + 4);
 }
 
 // Any head size and alignment: one thread per pair of a head,
@@ -387,13 +380,8 @@ int launch_append(const hc::AppendArgs& A, cudaStream_t s) {
                      (P.kps | P.khs | P.kss | P.vps | P.vhs | P.vss) % ec == 0;
     const int64_t units = vec ? (int64_t)(A.nh + 2 * P.nkv) * (P.hd / 8) : (int64_t)(A.nh + 2 * P.nkv) * ((P.hd + 1) / 2);
     HC_CHECK(units <= 65535 * 256ll, HC_ERR_INVALID, "hc_paged_append_dev: %d + %d heads of %d", A.nh, P.nkv, P.hd);
-    // Few rows: one unit a thread, blocks over the row (the latency of one chain
-    // counts).  Many: three units a thread, as many loads in flight and a third
-    // of the chains.
-    if (vec && (int64_t)P.n_rows * units < 148 * 8 * 256) {
-        hc::k_paged_append_vec<T, C, 1><<<dim3((unsigned)P.n_rows, (unsigned)((units + 255) / 256)), 256, 0, s>>>(A);
-    } else if (vec) {
-        hc::k_paged_append_vec<T, C, 3><<<dim3((unsigned)P.n_rows, (unsigned)((units + 767) / 768)), 256, 0, s>>>(A);
+    if (vec) {
+        hc::k_paged_append_vec<T, C><<<dim3((unsigned)P.n_rows, (unsigned)((units + 255) / 256)), 256, 0, s>>>(A);
     } else {
         hc::k_paged_append<T, C><<<dim3((unsigned)P.n_rows, (unsigned)((units + 255) / 256)), 256, 0, s>>>(A);
     }
@@ -483,9 +471,16 @@ struct AttnPlan {
 AttnPlan attn_plan(const hc::PagedAttnArgs& A, const hc_paged_batch* b, int c16) {
     AttnPlan plan = {ATTN_ANY, 0};
     if (!hc::paged_split_ok(A.p, c16)) return plan;
-    if ((int64_t)b->max_q_len * A.G > 64 && hc::paged_tc_ok(A, c16)) {
+    // Few rows: the split kernel, a sequence's rows in tiles of 16.  Many: tcgen05, in
+    // tiles of 256, which take up to twice as long each, so from about twice as
+    // many small tiles on.  (32 sequences of 4,096 keys, 32 heads over 8 of 128, us,
+    // 16-row tiles / 256-row tiles: 4 tokens each, f16 119 / 147, f32 126 / 224; 6
+    // tokens 207 / 147, 227 / 226; 32 tokens 702 / 148, 817 / 234.  One sequence
+    // of 6 tokens: 26 / 19, 25 / 25.)
+    const int64_t few = hc::paged_tiles(A, b->max_q_len, 16), many = hc::paged_tiles(A, b->max_q_len, 256);
+    if (2 * few > 3 * many && hc::paged_tc_ok(A, c16)) {
         plan.kernel = ATTN_TC;
-        plan.bytes = hc::paged_tc_bytes(A, b->max_kv_len);
+        plan.bytes = hc::paged_tc_bytes(A, b->max_q_len, b->max_kv_len);
     } else {
         plan.kernel = ATTN_SPLIT;
         plan.bytes = hc::paged_split_bytes(A, b->max_q_len, b->max_kv_len);
@@ -532,7 +527,7 @@ HC_EXPORT int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch
     // workspace does not know the scale, so another one goes to the kernel without one
     if (plan.kernel == ATTN_TC && !(scale > 0.0f)) plan.kernel = ATTN_ANY;
     if (plan.kernel == ATTN_TC)
-        return hc::launch_paged_tc(A, q16, batch->max_kv_len, workspace, (cudaStream_t)stream);
+        return hc::launch_paged_tc(A, q16, batch->max_q_len, batch->max_kv_len, workspace, (cudaStream_t)stream);
     if (plan.kernel == ATTN_SPLIT) return hc::launch_paged_split(A, q16, c16, batch->max_q_len, batch->max_kv_len, workspace, (cudaStream_t)stream);
     return hc::launch_paged_generic(A, q16, c16, (cudaStream_t)stream);
 }

@@ -164,8 +164,8 @@ __device__ __forceinline__ void store_row4(const PagedAttnArgs& A, int row, int 
 
 // Many rows per sequence (hc_paged_tc.cu): tcgen05 products over 256-row tiles.
 bool paged_tc_ok(const PagedAttnArgs& A, int c16);
-size_t paged_tc_bytes(const PagedAttnArgs& A, int max_kv_len);  // workspace
-int launch_paged_tc(const PagedAttnArgs& A, int q16, int max_kv_len, void* ws, cudaStream_t s);
+size_t paged_tc_bytes(const PagedAttnArgs& A, int max_q_len, int max_kv_len);  // workspace
+int launch_paged_tc(const PagedAttnArgs& A, int q16, int max_q_len, int max_kv_len, void* ws, cudaStream_t s);
 
 // Few rows per sequence (hc_paged_split.cu): the keys split over CTAs.
 bool paged_split_ok(const PagedArgs& P, int c16);
@@ -176,5 +176,57 @@ int launch_paged_split(const PagedAttnArgs& A, int q16, int c16, int max_q_len, 
 
 // Any shape (hc_paged.cu).
 int launch_paged_generic(const PagedAttnArgs& A, int q16, int c16, cudaStream_t s);
+
+// The results of a row's n runs of keys as one: with M = max m_s,
+// l = sum 2^(m_s - M) l_s, o = sum 2^(m_s - M) o_s, four columns from d on, in the
+// runs' order.  Eight runs' results are requested at once (a chain of loads, one
+// after another, took 2 to 4 us longer).
+template <typename RowOf>
+__device__ __forceinline__ void join_runs(int n, RowOf row_of, const float* po, const float2* pml, int hd, int d, float& mx,
+                                          float& l, float4& v) {
+    constexpr int N = 8;
+    mx = -INFINITY;
+    l = 0.0f;
+    v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s = 0; s < n; s += N) {
+        float2 ml[N];
+        float4 y[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int64_t r = row_of(min(s + i, n - 1));
+            ml[i] = pml[r];
+            y[i] = *reinterpret_cast<const float4*>(po + r * hd + d);
+            if (s + i >= n) ml[i] = make_float2(-INFINITY, 0.0f);
+        }
+        float top = mx;
+#pragma unroll
+        for (int i = 0; i < N; i++) top = fmaxf(top, ml[i].x);
+        if (l != 0.0f) {
+            const float f = exp2f(mx - top);
+            l *= f;
+            v.x *= f;
+            v.y *= f;
+            v.z *= f;
+            v.w *= f;
+        }
+        mx = top;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (ml[i].y == 0.0f) continue;  // saw nothing
+            const float f = exp2f(ml[i].x - mx);
+            l = fmaf(f, ml[i].y, l);
+            v.x = fmaf(f, y[i].x, v.x);
+            v.y = fmaf(f, y[i].y, v.y);
+            v.z = fmaf(f, y[i].z, v.z);
+            v.w = fmaf(f, y[i].w, v.w);
+        }
+    }
+}
+
+// Row tiles of all sequences, at most, from what the host knows.
+inline int64_t paged_tiles(const PagedAttnArgs& A, int max_q_len, int rows) {
+    const int64_t each = ((int64_t)max_q_len * A.G + rows - 1) / rows;
+    return std::max<int64_t>(1, std::min(A.p.n_seqs * each, (int64_t)A.p.n_rows * A.G / rows + A.p.n_seqs));
+}
 
 }  // namespace hc

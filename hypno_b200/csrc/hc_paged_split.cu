@@ -625,12 +625,9 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
     }
 }
 
-// Joins the partial results of a pair that was cut: with M = max m_s, o = sum
-// 2^(m_s - M) o_s / sum 2^(m_s - M) l_s, in the order of the CTAs.  Bound by
-// latency (a pair has a few KB of partial results), so what can be worked out
-// from the batch alone is done before the wait, and JOIN CTAs' results are
-// requested at once.
-constexpr int JOIN = 8;
+// Joins the partial results of a pair that was cut, in the order of the CTAs.
+// Bound by latency (a pair has a few KB of them), so what can be worked out from
+// the batch alone is done before the wait.
 template <typename QT>
 __global__ void __launch_bounds__(SP_THREADS) k_paged_join(const __grid_constant__ SplitArgs X) {
     const PagedAttnArgs& A = X.a;
@@ -659,41 +656,9 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_join(const __grid_constant
     auto slot = [&](int c) -> int64_t { return c == c0 ? s0 : 2 * (int64_t)c; };
     for (int x = blockIdx.y * SP_THREADS + threadIdx.x; x < mrows * hq; x += SP_THREADS * gridDim.y) {
         const int m = x / hq, d = (x - m * hq) * 4;
-        float mx = -INFINITY, l = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int cb = c0; cb <= c1; cb += JOIN) {
-            float2 ml[JOIN];
-            float4 y[JOIN];
-#pragma unroll
-            for (int i = 0; i < JOIN; i++) {
-                const int64_t at_row = slot(min(cb + i, c1)) * X.rows + m;
-                ml[i] = X.pml[at_row];
-                y[i] = *reinterpret_cast<const float4*>(X.po + at_row * P.hd + d);
-                if (cb + i > c1) ml[i] = make_float2(-INFINITY, 0.0f);
-            }
-            float top = mx;
-#pragma unroll
-            for (int i = 0; i < JOIN; i++) top = fmaxf(top, ml[i].x);
-            if (l != 0.0f) {
-                const float f = exp2f(mx - top);
-                l *= f;
-                v.x *= f;
-                v.y *= f;
-                v.z *= f;
-                v.w *= f;
-            }
-            mx = top;
-#pragma unroll
-            for (int i = 0; i < JOIN; i++) {
-                if (ml[i].y == 0.0f) continue;  // saw nothing
-                const float f = exp2f(ml[i].x - mx);
-                l = fmaf(f, ml[i].y, l);
-                v.x = fmaf(f, y[i].x, v.x);
-                v.y = fmaf(f, y[i].y, v.y);
-                v.z = fmaf(f, y[i].z, v.z);
-                v.w = fmaf(f, y[i].w, v.w);
-            }
-        }
+        float mx, l;
+        float4 v;
+        join_runs(c1 - c0 + 1, [&](int i) { return slot(c0 + i) * X.rows + m; }, X.po, X.pml, P.hd, d, mx, l, v);
         const int t = token_of(A, m0 + m), row = r0 + t, head = kvh * A.G + (m0 + m) - t * A.G;
         store_row4<QT>(A, row, head, d, l, v);
         if (A.lse && d == 0)
@@ -731,15 +696,19 @@ int launch_split_t(SplitArgs& X, cudaStream_t s) {
 
 template <typename QT, typename CT>
 int launch_split_hd(SplitArgs& X, cudaStream_t s) {
-    if (X.rows == 8) return X.a.p.hd <= 64 ? launch_split_t<QT, CT, 64, 1>(X, s) : launch_split_t<QT, CT, 128, 1>(X, s);
-    return X.a.p.hd <= 64 ? launch_split_t<QT, CT, 64, 2>(X, s) : launch_split_t<QT, CT, 128, 2>(X, s);
+    const int hd = X.a.p.hd;
+    if constexpr (sizeof(CT) == 2) {
+        if (hd > 128) return launch_split_t<QT, CT, 256, 1>(X, s);
+    }
+    if (X.rows == 8) return hd <= 64 ? launch_split_t<QT, CT, 64, 1>(X, s) : launch_split_t<QT, CT, 128, 1>(X, s);
+    return hd <= 64 ? launch_split_t<QT, CT, 64, 2>(X, s) : launch_split_t<QT, CT, 128, 2>(X, s);
 }
 
 }  // namespace
 
 bool paged_split_ok(const PagedArgs& P, int c16) {
     const int64_t e = c16 ? 8 : 4;
-    return P.hd <= 128 && P.hd % e == 0 && ((uintptr_t)P.k | (uintptr_t)P.v) % 16 == 0 &&
+    return P.hd <= (c16 ? 256 : 128) && P.hd % e == 0 && ((uintptr_t)P.k | (uintptr_t)P.v) % 16 == 0 &&
            (P.kps | P.khs | P.kss | P.vps | P.vhs | P.vss) % e == 0;
 }
 
@@ -762,7 +731,8 @@ int launch_paged_split(const PagedAttnArgs& A, int q16, int c16, int max_q_len, 
     SplitArgs X;
     X.a = A;
     X.whole = paged_split_whole(A, max_q_len, max_kv_len);
-    X.rows = (int64_t)max_q_len * A.G <= 8 ? 8 : 16;
+    // 16 rows of more than 128 elements do not fit the registers
+    X.rows = (int64_t)max_q_len * A.G <= 8 || A.p.hd > 128 ? 8 : 16;
     X.po = (float*)ws;
     X.pml = (float2*)((float*)ws + (size_t)2 * SP_CTAS * 16 * A.p.hd);
     if (q16) return c16 ? launch_split_hd<__half, __half>(X, s) : launch_split_hd<__half, float>(X, s);

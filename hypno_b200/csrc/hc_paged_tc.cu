@@ -272,6 +272,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
     int& abort_flag = C.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t q_s = smem_u32(smem_raw) + TC_CTRL, ring = q_s + 2 * Sh::QH;
+    pdl_trigger();  // the join may become resident; it waits for this grid's end
 
     if (warp == 0) {
         int seq = 0, tile = 0;
@@ -1036,9 +1037,10 @@ template <typename QT>
 __global__ void __launch_bounds__(256) k_paged_tc_join(const __grid_constant__ TcArgs X) {
     const PagedAttnArgs& A = X.a;
     const PagedArgs& P = A.p;
-    pdl_wait();
     int seq = 0, tile = 0;
-    if (!find_tile(P, A.G, TC_ROWS, gridDim.x - 1 - blockIdx.x, seq, tile)) return;
+    const bool any = find_tile(P, A.G, TC_ROWS, gridDim.x - 1 - blockIdx.x, seq, tile);
+    pdl_wait();  // (every CTA waits: the next kernel on the stream begins when this grid has ended)
+    if (!any) return;
     const int kvh = blockIdx.y, m0 = tile * TC_ROWS;
     int r0, r1;
     seq_rows(P, seq, r0, r1);
@@ -1047,22 +1049,9 @@ __global__ void __launch_bounds__(256) k_paged_tc_join(const __grid_constant__ T
     const int64_t slot = ((int64_t)blockIdx.x * P.nkv + kvh) * X.nsplit;
     for (int x = blockIdx.z * 256 + threadIdx.x; x < mrows * hq; x += 256 * gridDim.z) {
         const int m = x / hq, d = (x - m * hq) * 4;
-        float mx = -INFINITY;
-        for (int s = 0; s < X.nsplit; s++) mx = fmaxf(mx, X.pml[(slot + s) * TC_ROWS + m].x);
-        float l = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int s = 0; s < X.nsplit; s++) {
-            const float2 ml = X.pml[(slot + s) * TC_ROWS + m];
-            const float4 y = *reinterpret_cast<const float4*>(X.po + ((slot + s) * TC_ROWS + m) * P.hd + d);
-            if (ml.y == 0.0f) continue;  // saw nothing
-            const float f = exp2f(ml.x - mx);
-            l = fmaf(f, ml.y, l);
-            v.x = fmaf(f, y.x, v.x);
-            v.y = fmaf(f, y.y, v.y);
-            v.z = fmaf(f, y.z, v.z);
-            v.w = fmaf(f, y.w, v.w);
-        }
+        float mx, l;
+        float4 v;
+        join_runs(X.nsplit, [&](int s) { return (slot + s) * TC_ROWS + m; }, X.po, X.pml, P.hd, d, mx, l, v);
         const int t = token_of(A, m0 + m), row = r0 + t, head = kvh * A.G + (m0 + m) - t * A.G;
         store_row4<QT>(A, row, head, d, l, v);
         if (A.lse && d == 0)
@@ -1072,10 +1061,12 @@ __global__ void __launch_bounds__(256) k_paged_tc_join(const __grid_constant__ T
 
 int64_t tc_tiles(const PagedAttnArgs& A) { return (int64_t)A.p.n_rows * A.G / TC_ROWS + A.p.n_seqs; }
 
-// Runs per row tile: cut where the row tiles alone leave SMs idle, into runs
-// of four key tiles at least.
-int tc_nsplit(const PagedAttnArgs& A, int max_kv_len) {
-    const int64_t pairs = ((int64_t)A.p.n_rows * A.G + TC_ROWS - 1) / TC_ROWS * A.p.nkv;
+// Runs per row tile: cut where the row tiles alone leave SMs idle, into runs of
+// four key tiles at least and no more runs than SMs (128 rows of 32 heads over
+// 16,384 keys: 64 us in nine runs, 286 in one; 8 sequences of 17 rows over
+// 4,096: 48 in two runs, 74 in one or in six).
+int tc_nsplit(const PagedAttnArgs& A, int max_q_len, int max_kv_len) {
+    const int64_t pairs = paged_tiles(A, max_q_len, TC_ROWS) * A.p.nkv;
     const int64_t len = A.window > 0 ? std::min<int64_t>(max_kv_len, (int64_t)A.window + TC_ROWS) : max_kv_len;
     const int64_t units = (len + TC_KEYS - 1) / TC_KEYS;
     if (pairs * 2 > 148) return 1;
@@ -1092,7 +1083,7 @@ int launch_tc_t(const TcArgs& X, cudaStream_t s) {
     k_paged_tc<QT, HD, TMA><<<dim3((unsigned)(tiles * X.nsplit), P.nkv), TC_THREADS, Sh::SMEM, s>>>(X);
     HC_LAUNCH_CHECK();
     if (X.nsplit > 1) {
-        k_paged_tc_join<QT><<<dim3((unsigned)tiles, P.nkv, 8), 256, 0, s>>>(X);
+        HC_TRY(launch_pdl(k_paged_tc_join<QT>, dim3((unsigned)tiles, P.nkv, 8), dim3(256), 0, s, X));
         HC_LAUNCH_CHECK();
     }
     return HC_OK;
@@ -1129,15 +1120,15 @@ bool paged_tc_ok(const PagedAttnArgs& A, int c16) {
            (P.kps | P.khs | P.kss | P.vps | P.vhs | P.vss) % 8 == 0 && (int64_t)P.n_rows * A.G < (1 << 30);
 }
 
-size_t paged_tc_bytes(const PagedAttnArgs& A, int max_kv_len) {
-    const int n = tc_nsplit(A, max_kv_len);
+size_t paged_tc_bytes(const PagedAttnArgs& A, int max_q_len, int max_kv_len) {
+    const int n = tc_nsplit(A, max_q_len, max_kv_len);
     return n == 1 ? 0 : (size_t)tc_tiles(A) * A.p.nkv * n * TC_ROWS * ((size_t)A.p.hd * 4 + 8);
 }
 
-int launch_paged_tc(const PagedAttnArgs& A, int q16, int max_kv_len, void* ws, cudaStream_t s) {
+int launch_paged_tc(const PagedAttnArgs& A, int q16, int max_q_len, int max_kv_len, void* ws, cudaStream_t s) {
     TcArgs X;
     X.a = A;
-    X.nsplit = tc_nsplit(A, max_kv_len);
+    X.nsplit = tc_nsplit(A, max_q_len, max_kv_len);
     X.po = (float*)ws;
     X.pml = (float2*)((float*)ws + (size_t)tc_tiles(A) * A.p.nkv * X.nsplit * TC_ROWS * A.p.hd);
     if (q16) return A.p.hd <= 64 ? launch_tc_copy<__half, 64>(X, s) : launch_tc_copy<__half, 128>(X, s);

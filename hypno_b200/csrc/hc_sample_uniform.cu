@@ -850,9 +850,11 @@ HC_EXPORT int hc_sample_uniform_dev(const float* logits_dev, size_t ld, int B, i
     if (B == 0) return HC_OK;
     HC_CHECK((uintptr_t)logits_dev % 4 == 0, HC_ERR_INVALID, "hc_sample_uniform_dev: misaligned logits");
     cudaStream_t s = (cudaStream_t)stream;
-    // CTAs a row: slices of 4,096 logits or more, up to eight CTAs (two a row, so
-    // that 256 rows are resident at once, took a third longer: the passes count);
-    // sixteen where the GPU holds them all on SMs of their own.
+    // CTAs a row, of slices of 4,096 logits or more: eight, sixteen where each has
+    // an SM of its own.  128,256 logits, top-k 50 and top-p, us, 4 / 8 / 16 CTAs:
+    // 8 rows 99 / 61 / 43, 32 rows 102 / 64 / 86, 64 rows 108 / 76, 256 rows
+    // 257 / 291 / 435; 256 rows of different settings (greedy, top-k, top-p, min-p,
+    // none) 182 / 128: more CTAs a row even out rows that take unlike times.
     int cs = 1;
     while (cs < 8 && V > cs * 4096) cs *= 2;
     if ((int64_t)B * 16 <= 148 && V > 8 * 4096) cs = 16;
