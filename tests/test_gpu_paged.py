@@ -98,6 +98,16 @@ def test_short_chunks_over_many_runs(cuda_device, types, dim, page, tokens):
     check_attention(ref.Case(tokens, lens, 8, 2, dim, page, 13, *types), cuda_device, window=600)
 
 
+@pytest.mark.parametrize("types", TYPES[:3], ids=IDS[:3])
+def test_many_chunks_of_unlike_lengths(cuda_device, types):
+    """More row tiles than SMs, of sequences whose lengths span every order of magnitude."""
+    new = [1, 70, 0, 33, 5, 129, 64, 2, 90, 200] * 2
+    kv = [n + (37 * i * i) % 900 * (i % 5 > 0) for i, n in enumerate(new)]
+    kv[2], kv[12] = 0, 1200
+    check_attention(ref.Case(new, kv, 16, 8, 64, 16, 14, *types), cuda_device)
+    check_attention(ref.Case(new, kv, 16, 8, 64, 16, 15, *types), cuda_device, window=100)
+
+
 @pytest.mark.parametrize("types", TYPES, ids=IDS)
 def test_rows_that_see_nothing(cuda_device, types):
     """Empty sequences, more rows than positions, and rows over holes only."""
