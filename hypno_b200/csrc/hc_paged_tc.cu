@@ -42,7 +42,7 @@
 // 512 tokens over 16,384 keys, 64 heads over 8 of 128, f16: 301 us on an idle
 // GPU, 899 TFLOP/s (333 us, 812, where it runs hot); bound by the chain from S_h to
 // P_h of a half.  4 prompts of 2,048, 32 heads over 8: f16 222 us, 619 TFLOP/s;
-// f32 361 to 400 us, 344 to 381 TFLOP/s of twice as many products; a CTA's start
+// f32 342 to 383 us, 359 to 402 TFLOP/s of twice as many products; a CTA's start
 // (queries to shared memory) and end, some 19,000 cycles of 55,000, overlap
 // nothing.  Key by key copies in place of boxes: 477, 335 and 434 us.
 //
@@ -1131,8 +1131,8 @@ int64_t tc_tiles(const PagedAttnArgs& A) { return (int64_t)A.p.n_rows * A.G / TC
 
 // Runs per row tile: cut where the row tiles alone leave SMs idle, into runs of
 // four key tiles at least and no more runs than SMs (128 rows of 32 heads over
-// 16,384 keys: 64 us in nine runs, 286 in one; 8 sequences of 17 rows over
-// 4,096: 48 in two runs, 74 in one or in six).
+// 16,384 keys: 64 us in nine runs, 286 in one; 8 sequences of 16 tokens over
+// 4,096: 47 in two runs, 74 in one).
 int tc_nsplit(const PagedAttnArgs& A, int max_q_len, int max_kv_len) {
     const int64_t pairs = paged_tiles(A, max_q_len, TC_ROWS) * A.p.nkv;
     const int64_t len = A.window > 0 ? std::min<int64_t>(max_kv_len, (int64_t)A.window + TC_ROWS) : max_kv_len;
