@@ -491,7 +491,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         const int pos = in ? first + token_of(A, mh + r) : -1;
         const int lo_pos = A.window > 0 ? pos - A.window + 1 : 0;
         const int p_min = first + token_of(A, mh), l_max = A.window > 0 ? first + token_of(A, mh + rows - 1) - A.window + 1 : 0;
-        const bool one_token = rows > 0 && token_of(A, mh) == token_of(A, mh + rows - 1);
         const float cf = A.scale * LOG2E * up;
         float m = -INFINITY, l = 0.0f;  // running maximum (log2 units), sum of weights
         float acc[HILO ? HO : 1];       // f32 queries: the running outputs
@@ -579,14 +578,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             const uint4 b4 = *reinterpret_cast<const uint4*>(bits);
             const bool whole = k0 + TC_KEYS - 1 <= p_min && k0 >= l_max && (b4.x & b4.y & b4.z & b4.w) == 0xffffffffu;
             const int hi_c = pos - k0, lo_c = lo_pos - k0;
-            // A key that some rows of the half see and others do not must not
-            // reach the latter through 0 * v where v is not finite: such a tile
-            // (rare) leaves the products to the row's thread, masked keys left out.
+            // A key that some rows (of either half: the tile is both's) see and others
+            // do not must not reach the latter through 0 * v where v is not finite:
+            // such a tile (rare) leaves the products to the row's thread, masked keys
+            // left out.  Keys without a page are zeros.
+            const bool equal = min(k0 + TC_KEYS, rg.end) - 1 <= p_min && max(k0, rg.seen) >= l_max;  // this half's rows see them all
             bool skip = false;
             uint32_t vt = 0;
             // keys of the tile that no row sees: what their memory holds is nobody's
             const bool strangers = TMA && (k0 < rg.seen || k0 + TC_KEYS > rg.end);
-            if ((!whole && !one_token) || strangers) {
+            if (!equal || strangers) {
                 const int n = 2 * (j - rg.ja) + 1, slot = n % NS;
                 ok = mbar_wait(&B.full[slot], (uint32_t)(n / NS) & 1u, &abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
@@ -603,7 +604,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
                             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vt + (uint32_t)(c * (TC_KEYS * 128) + r * 128 + i * 16)), "r"(0) : "memory");
                 fence_async_shared();
             }
-            if (!whole && !one_token) {
+            if (!equal) {
                 // (the other half may still be writing its zeros: a stranger is not looked at)
                 uint32_t bad = 0;
                 for (int i = r + g * TC_HALF; i < Sh::TILE / 16; i += 2 * TC_HALF) {

@@ -152,6 +152,27 @@ def test_later_tokens_do_not_reach_a_row(cuda_device, types, bad, new):
     assert bool((~torch.isfinite(windowed[~ok])).all())
 
 
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("new,heads,kv_heads,page,window,at", [(65, 4, 2, 16, 30, 50), (65, 4, 2, 20, 30, 50), (65, 4, 2, 16, 30, 94), (2, 128, 1, 16, 0, 61),
+                                                              (3, 128, 1, 20, 0, 62), (3, 128, 1, 20, 0, 61),
+                                                              (2, 128, 1, 16, 5, 56)])
+def test_a_lone_token_does_not_see_its_neighbours_keys(cuda_device, types, bad, new, heads, kv_heads, page, window, at):
+    """128 packed rows of which the last, or all, are one token's: a key or value
+    that is not finite and that only the other rows see does not reach it."""
+    c = ref.Case([new], [new + 60], heads, kv_heads, 64, page, 16, *types)
+    kv, batch, q, _, _ = on_device(c, cuda_device)
+    clean = paged.attention(kv, batch, q, window=window)
+    for t in (kv.k, kv.v):
+        t[int(c.table[0, at // page]), :, at % page] = bad
+    got = paged.attention(kv, batch, q, window=window)
+    sees = torch.tensor([at <= p and (not window or at > p - window) for _, p in c.where()], device=cuda_device)
+    assert 0 < int(sees.sum()) < new
+    tol = 2.0 ** -9 if q.dtype == torch.float16 else 2.0 ** -17      # as above
+    assert bool(((got - clean).abs()[~sees] <= 6 * tol).all())
+    assert bool((~torch.isfinite(got[sees])).all())
+
+
 @pytest.mark.parametrize("types", TYPES[:3], ids=IDS[:3])
 @pytest.mark.parametrize("order", ["head", "page"])
 def test_strides(cuda_device, types, order):
