@@ -396,7 +396,8 @@ __global__ void __launch_bounds__(UT, 4) k_sample_cluster(const float* __restric
     URow R;
     R.l = logits + (size_t)row * ld;
     R.V = V;
-    R.inv = T > 0.0f ? __fdiv_rn(1.0f, T) : 1.0f;
+    // Finite for every T: 1 / T overflows below 2^-128, and the maximum's exponent would be 0 * inf.
+    R.inv = T > 0.0f ? fminf(__fdiv_rn(1.0f, T), FLT_MAX) : 1.0f;
 
     // Places are counted from the 16-byte boundary at or before the row's first
     // logit: place = index + off.  A warp has the run [w0, w1) of places, 128 at

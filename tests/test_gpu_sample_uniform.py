@@ -102,6 +102,22 @@ def test_special_rows(cuda_device):
             assert token[0] == 1 and token[1] == token[2] == -1 and token[3] in (0, 2) and token[4] in (0, 1) and token[5] in (0, 2)
 
 
+@pytest.mark.parametrize("V", [5, 3000, 40001])
+@pytest.mark.parametrize("T", [1e-45, 1e-39, 2.9e-39, 2.0 ** -128, 2.0 ** -126, 1e-30])
+def test_temperatures_whose_reciprocal_overflows(cuda_device, V, T):
+    """Only the maxima have a mass, and they share it."""
+    g = np.random.default_rng(V)
+    l = (g.standard_normal((3, V)) * 3).astype(np.float32)
+    l[1, g.permutation(V)[:V // 3 + 1]] = 20.0
+    l[2] = -7.5
+    s = [(T, k, p, m) for k in (0, 1, 3, V - 1) for p in (1.0, 0.6) for m in (0.0, 0.5, 1.0)]
+    u = g.random(3 * len(s)).astype(np.float32)
+    with np.errstate(over="ignore"):
+        token = draws(cuda_device, l, s, u)
+    top = np.tile(l == l.max(1, keepdims=True), (len(s), 1))
+    assert all(0 <= t < V and top[r, t] for r, t in enumerate(token))
+
+
 def test_frequencies(cuda_device):
     """Evenly spaced u visit every kept token in proportion to its share."""
     n = 4096
