@@ -175,8 +175,53 @@ def call(name, *args):
     return check(getattr(load(), name)(*args))
 
 
+def _torch_calls():
+    """torch's calls for the current device, its change, and a device's current
+    stream, looked up at their first use (this module needs no torch)."""
+    import torch
+    c = torch._C
+    return (getattr(c, "_cuda_getDevice", torch.cuda.current_device), torch.cuda.set_device,
+            getattr(c, "_cuda_getCurrentRawStream", lambda i: torch.cuda.current_stream(i).cuda_stream))
+
+
+_calls = None
+
+
 def raw_stream(index):
     """torch's current stream of a CUDA device, as the integer the C ABI takes."""
-    import torch
-    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return get(index) if get is not None else torch.cuda.current_stream(index).cuda_stream
+    global _calls
+    if _calls is None:
+        _calls = _torch_calls()
+    return _calls[2](index)
+
+
+def current_device():
+    """Index of torch's current CUDA device."""
+    global _calls
+    if _calls is None:
+        _calls = _torch_calls()
+    return _calls[0]()
+
+
+class on_device:
+    """Makes a CUDA device current for a `with` block.  The C entry points launch
+    on and allocate from the current device, whatever the device of the pointers
+    and of the stream they are given (a default stream's handle is 0 on each)."""
+
+    __slots__ = ("index", "was")
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        self.was = current_device()
+        if self.was != self.index:
+            _set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.was != self.index:
+            _set_device(self.was)
+
+
+def _set_device(index):
+    _calls[1](index)

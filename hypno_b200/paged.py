@@ -16,16 +16,18 @@ prompts and single tokens alike) into rows, appends them, and attends:
     q = append(kv, batch, k, v, q=q, rope=rope)
     out = attention(kv, batch, q)
 
-The operators run on torch's current stream of the pool's device and do not
-synchronize; use `with torch.cuda.stream(...)` (or an ExternalStream of
-HypnoModel.stream) for another one.  Errors raise HypnoCudaError, ValueError
-or TypeError.  They call hc_paged_append_dev and hc_paged_attention_dev.
+The operators run on torch's current stream of the pool's device, whichever
+device is current, and do not synchronize; use `with torch.cuda.stream(...)`
+(or an ExternalStream of HypnoModel.stream) for another one.  Errors raise
+HypnoCudaError, ValueError or TypeError.  They call hc_paged_append_dev and
+hc_paged_attention_dev.
 """
 import ctypes
 
 import numpy as np
 import torch
 
+from . import _lib
 from ._lib import (DTYPE_FP16, DTYPE_FP32, HC_PAGED_BATCH, HC_ROWS, KV_FP16, KV_FP32, HcPagedKV, call, check, load, raw_stream)
 
 __all__ = ["PagedKV", "PagedBatch", "append", "attention", "rope_table", "PageTable"]
@@ -137,6 +139,9 @@ def append(kv, batch, k, v, q=None, rope=None, pairs="adjacent", q_out=None):
     through.  Returns the rotated queries (in q_out, which may be q), or None.
     k, v and q have one type, float32 or float16, and any row and head
     strides; no two rows of one call may name the same position."""
+    if _lib.current_device() != kv.index:
+        with _lib.on_device(kv.index):
+            return append(kv, batch, k, v, q, rope, pairs, q_out)
     _same_device(kv, batch)
     dtype = k.dtype
     code = _DTYPE.get(dtype)
@@ -181,6 +186,9 @@ def attention(kv, batch, q, out=None, scale=None, window=0, lse=None):
     float16, out the same; lse, if given, is a contiguous [n_rows, n_heads]
     float32 tensor for the log of the sums.  The softmax is exact (the
     flat-cache forward passes keep the reference's polynomial)."""
+    if _lib.current_device() != kv.index:
+        with _lib.on_device(kv.index):
+            return attention(kv, batch, q, out, scale, window, lse)
     _same_device(kv, batch)
     dtype = q.dtype
     code = _DTYPE.get(dtype)

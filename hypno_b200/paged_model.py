@@ -20,7 +20,7 @@ import torch
 
 from . import hypno_file as hf
 from . import paged, sampling
-from ._lib import call, load, raw_stream
+from ._lib import call, load, on_device, raw_stream
 
 __all__ = ["PagedModel", "PagedGenerator"]
 
@@ -34,7 +34,8 @@ class _Linear:
         self.q4 = self.dense = None
         if dt == hf.DT_Q4_0:
             self.q4 = ctypes.c_void_p()
-            call("hc_q4_matrix_upload", raw.ctypes.data, raw.size, self.n, self.k, ctypes.byref(self.q4))
+            with on_device(device.index):
+                call("hc_q4_matrix_upload", raw.ctypes.data, raw.size, self.n, self.k, ctypes.byref(self.q4))
         elif dt == hf.DT_FP32:
             self.dense = torch.from_numpy(raw.view(np.float32).reshape(self.n, self.k).copy()).to(device)
         else:
@@ -44,7 +45,9 @@ class _Linear:
         if self.dense is not None:
             return x @ self.dense.T
         y = torch.empty((x.shape[0], self.n), dtype=torch.float32, device=x.device)
-        call("hc_q4_matmul_dev", self.q4, x.contiguous().data_ptr(), x.shape[0], y.data_ptr(), raw_stream(x.get_device()))
+        x = x.contiguous()
+        with on_device(x.get_device()):
+            call("hc_q4_matmul_dev", self.q4, x.data_ptr(), x.shape[0], y.data_ptr(), raw_stream(x.get_device()))
         return y
 
     def close(self):
@@ -54,13 +57,13 @@ class _Linear:
 
 
 class PagedModel:
-    """A .hypno image (bytes or a uint8 array) on a CUDA device with one page
-    pool per layer."""
+    """A .hypno image (bytes or a uint8 array) on a CUDA device, current or not,
+    with one page pool per layer."""
 
     def __init__(self, image, n_pages, page_size=16, cache_dtype=torch.float16, device="cuda"):
         man = hf.Manifest(np.frombuffer(image, np.uint8) if isinstance(image, (bytes, bytearray)) else image)
         meta = man.metadata
-        self.device = torch.device(device, torch.cuda.current_device()) if str(device) == "cuda" else torch.device(device)
+        self.device = torch.device("cuda", torch.cuda.current_device()) if str(device) == "cuda" else torch.device(device)
         self.heads, self.kv_heads = int(meta["num_attention_heads"]), int(meta["num_key_value_heads"])
         self.hidden, self.layers = int(meta["hidden_size"]), int(meta["num_hidden_layers"])
         self.dim, self.vocab = self.hidden // self.heads, int(meta["vocab_size"])
@@ -76,7 +79,8 @@ class PagedModel:
         if dt == hf.DT_Q4_0:
             q = torch.from_numpy(np.frombuffer(raw, np.uint8).copy()).to(self.device)
             self.embed = torch.empty((self.vocab, self.hidden), dtype=torch.float32, device=self.device)
-            call("hc_q4_0_dequantize_dev", q.data_ptr(), q.numel(), self.embed.data_ptr(), raw_stream(self.device.index))
+            with on_device(self.device.index):
+                call("hc_q4_0_dequantize_dev", q.data_ptr(), q.numel(), self.embed.data_ptr(), raw_stream(self.device.index))
             torch.cuda.synchronize(self.device)
         else:
             self.embed = vector(name).view(self.vocab, self.hidden)

@@ -6,6 +6,7 @@ its XorShift64 states is engine.DeviceSampler.
 """
 import torch
 
+from . import _lib
 from ._lib import check, load, raw_stream
 
 __all__ = ["sample"]
@@ -37,6 +38,9 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
         raise TypeError("logits must be a 2-dimensional float32 CUDA tensor")
     rows, vocab = logits.shape
     dev = logits.device
+    if _lib.current_device() != dev.index:
+        with _lib.on_device(dev.index):
+            return sample(logits, u, temperature, top_k, top_p, min_p, out, logprob)
     if vocab < 1:
         raise ValueError("logits without a vocabulary")
     if vocab > 1 and logits.stride(1) != 1:

@@ -13,7 +13,8 @@
  *  - Handles are opaque.  Model-level calls are ordered on the model's own
  *    CUDA stream; calls that take or return HOST buffers synchronize before
  *    returning.  The *_dev variants take device pointers and a stream and do
- *    not synchronize.
+ *    not synchronize; they launch on the calling thread's current device,
+ *    which has to be the device of the pointers and of the stream.
  *  - dtype codes are the reference's DType discriminants (dtype.rs:6-15):
  *    0 = FP32, 1 = FP16, 2 = Q8_0, 3 = Q4_0.
  *  - There is no CPU fallback: without a usable CUDA device every compute

@@ -120,3 +120,25 @@ def sample(l, u, T, k, p, least):
     goal = min(int(np.floor(np.float64(np.float32(u)) * np.float64(total))), total - 1)
     t = int(np.argmax(np.cumsum(held) > goal))
     return t, held[t] / total, held, total
+
+
+class Elsewhere:
+    """Stands in for a process whose current CUDA device is another than the
+    tensors': the package's view of the current device, and of every call into
+    the library the device it was made on (the real one stays device 0)."""
+
+    def __init__(self, monkeypatch, *modules):
+        from hypno_b200 import _lib
+        self.device, self.calls, lib = 7, [], _lib.load()
+        monkeypatch.setattr(_lib, "current_device", lambda: self.device)
+        monkeypatch.setattr(_lib, "_set_device", lambda i: setattr(self, "device", i))
+
+        def of(name):
+            def run(*args):
+                self.calls.append((name, self.device))
+                return getattr(lib, name)(*args)
+            return run
+
+        library = type("Library", (), {"__getattr__": lambda _, name: of(name)})()
+        for m in (_lib, *modules):
+            monkeypatch.setattr(m, "load", lambda: library)

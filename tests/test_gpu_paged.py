@@ -276,6 +276,18 @@ def test_graph_capture(cuda_device):
     assert torch.equal(out, want)
 
 
+def test_another_device_than_the_current_one(cuda_device, monkeypatch):
+    c = ref.Case([1, 70], [900, 300], 8, 2, 128, 16, 13)
+    kv, batch, q, kn, vn = on_device(c, cuda_device)
+    want = paged.append(kv, batch, kn, vn, q=q), paged.attention(kv, batch, q)
+    far = ref.Elsewhere(monkeypatch, paged)
+    got = paged.append(kv, batch, kn, vn, q=q), paged.attention(kv, batch, q)
+    assert far.device == 7                                # as it was
+    assert {n for n, d in far.calls if d == 0} >= {"hc_paged_append_dev", "hc_paged_attention_dev"}
+    assert {n for n, d in far.calls if d != 0} <= {"hc_paged_attention_workspace"}  # (host arithmetic)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ---------------------------------------------------------------- append
 
 @pytest.mark.parametrize("types", TYPES, ids=IDS)

@@ -12,6 +12,8 @@ from hypno_b200 import hypno_file as hf
 from hypno_b200 import ops, paged, synth
 from hypno_b200.paged_model import PagedGenerator, PagedModel
 
+from . import _paged as ref
+
 pytestmark = pytest.mark.gpu
 CFG = dict(hidden=256, layers=2, heads=8, kv_heads=2, inter=384, vocab=700, theta=10000.0, max_pos=256)
 
@@ -95,6 +97,21 @@ def test_tokens_do_not_depend_on_the_schedule(cuda_device, image):
         got = tokens(*other)
         # a draw or a greedy pick may turn where two tokens lie within the logits' rounding
         assert sum(got[k] != want[k] for k in want) <= 1
+
+
+def test_another_device_than_the_current_one(cuda_device, image, monkeypatch):
+    from hypno_b200 import paged_model, sampling
+    far = ref.Elsewhere(monkeypatch, paged, sampling, paged_model)
+    m = PagedModel(image, n_pages=4, page_size=16, device="cuda:0")
+    tokens = m.step([3, 4, 5], np.array([[1], [2]]), [0, 2, 3], [2, 1], [(0.3, 0.0, 0, 1.0, 0.0)] * 2)
+    m.close()
+    assert tokens.shape == (2,) and far.device == 7
+    there = {"hc_rope_table_host", "hc_paged_attention_workspace", "hc_q4_matrix_free"}  # host work and a release need no device
+    assert {n for n, d in far.calls if d != 0} <= there
+    assert {n for n, d in far.calls if d == 0} >= {"hc_q4_matrix_upload", "hc_paged_append_dev", "hc_paged_attention_dev", "hc_sample_uniform_dev"}
+    m = PagedModel(image, n_pages=4, device=torch.device("cuda"))
+    assert m.device == torch.device("cuda:0")
+    m.close()
 
 
 def test_example_runs(cuda_device, capsys):

@@ -149,6 +149,16 @@ def test_strided_rows_outputs_and_streams(cuda_device):
     assert torch.equal(out, want[0]) and torch.equal(lp, want[1])
 
 
+def test_another_device_than_the_current_one(cuda_device, monkeypatch):
+    g = torch.Generator(device=cuda_device).manual_seed(2)
+    l, u = torch.randn((3, 500), generator=g, device=cuda_device), torch.rand(3, generator=g, device=cuda_device)
+    want = sampling.sample(l, u, 0.9, 30)
+    far = ref.Elsewhere(monkeypatch, sampling)
+    got = sampling.sample(l, u, 0.9, 30)
+    assert far.device == 7 and far.calls == [("hc_sample_uniform_dev", 0)]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_refusals(cuda_device):
     l, u = torch.zeros((2, 10), device=cuda_device), torch.zeros(2, device=cuda_device)
     with pytest.raises(TypeError):

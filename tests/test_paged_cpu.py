@@ -114,3 +114,19 @@ def test_host_tensors_are_refused():
         paged.PagedBatch(i.view(1, 2), i, i[:1], 1, 1)
     with pytest.raises(TypeError):
         sampling.sample(torch.zeros((1, 8)), torch.zeros(1))
+
+
+def test_a_device_is_current_within_the_block_and_the_former_after_it(monkeypatch):
+    log, state = [], {"device": 3}
+    monkeypatch.setattr(_lib, "current_device", lambda: state["device"])
+    monkeypatch.setattr(_lib, "_set_device", lambda i: (log.append(i), state.update(device=i)))
+    with _lib.on_device(1):
+        assert state["device"] == 1
+    assert state["device"] == 3 and log == [1, 3]
+    with pytest.raises(RuntimeError):
+        with _lib.on_device(0):
+            raise RuntimeError
+    assert state["device"] == 3 and log == [1, 3, 0, 3]
+    with _lib.on_device(3):  # current already: no call
+        pass
+    assert log == [1, 3, 0, 3]
