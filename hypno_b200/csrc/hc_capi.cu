@@ -9,7 +9,9 @@
 #include <cstdio>
 #include <cstring>
 #include <atomic>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 
 // ============================================================ errors
@@ -336,6 +338,16 @@ HC_EXPORT int hc_q4_matrix_free(hc_q4_matrix* m) {
     return HC_OK;
 }
 
+static int q4_matmul_rows(const hc_q4_matrix* w, const float* x, size_t mtok, float* y, cudaStream_t s) {
+    DevWeight dw;
+    dw.dtype = HC_DTYPE_Q4_0;
+    dw.n = w->n;
+    dw.k = w->k;
+    dw.q4 = *w;
+    dw.present = true;
+    return hc::launch_matmul(dw, x, w->k, mtok, y, w->n, hc::EPI_STORE, nullptr, 0, s);
+}
+
 HC_EXPORT int hc_q4_matmul_dev(const hc_q4_matrix* w, const float* x, size_t mtok, float* y, void* stream) {
     HC_CHECK(w && x && y, HC_ERR_INVALID, "hc_q4_matmul_dev: NULL argument");
     cudaStream_t s = (cudaStream_t)stream;
@@ -351,13 +363,46 @@ HC_EXPORT int hc_q4_matmul_dev(const hc_q4_matrix* w, const float* x, size_t mto
         if (cs == cudaStreamCaptureStatusNone && (++calls & 63u) == 0) return hc::gemm_check(ws);
         return HC_OK;
     }
-    DevWeight dw;
-    dw.dtype = HC_DTYPE_Q4_0;
-    dw.n = w->n;
-    dw.k = w->k;
-    dw.q4 = *w;
-    dw.present = true;
-    return hc::launch_matmul(dw, x, w->k, mtok, y, w->n, hc::EPI_STORE, nullptr, 0, s);
+    return q4_matmul_rows(w, x, mtok, y, s);
+}
+
+struct hc_q4_workspace {
+    hc::GemmWorkspace* ws;
+};
+
+HC_EXPORT int hc_q4_workspace_new(hc_q4_workspace** out) {
+    HC_CHECK(out, HC_ERR_INVALID, "hc_q4_workspace_new: NULL out");
+    *out = nullptr;
+    try {
+        std::unique_ptr<hc_q4_workspace> ws(new hc_q4_workspace{nullptr});
+        ws->ws = hc::gemm_workspace_new();
+        *out = ws.release();
+    } catch (const std::bad_alloc&) {
+        hc_set_error("hc_q4_workspace_new: out of host memory");
+        return HC_ERR_OOM;
+    }
+    return HC_OK;
+}
+
+HC_EXPORT int hc_q4_workspace_free(hc_q4_workspace* ws) {
+    if (!ws) return HC_OK;
+    hc::gemm_workspace_free(ws->ws);
+    delete ws;
+    return HC_OK;
+}
+
+HC_EXPORT int hc_q4_matmul_ws_dev(const hc_q4_matrix* w, const float* x, size_t mtok, float* y, hc_q4_workspace* ws,
+                                  void* stream) {
+    HC_CHECK(w && x && y && ws, HC_ERR_INVALID, "hc_q4_matmul_ws_dev: NULL argument");
+    cudaStream_t s = (cudaStream_t)stream;
+    if (hc::gemm_tc_eligible(*w, mtok))
+        return hc::gemm_tc(ws->ws, *w, x, w->k, mtok, y, w->n, hc::EPI_STORE, nullptr, 0, s);
+    return q4_matmul_rows(w, x, mtok, y, s);
+}
+
+HC_EXPORT int hc_q4_workspace_check(hc_q4_workspace* ws, void* stream) {
+    HC_CHECK(ws, HC_ERR_INVALID, "hc_q4_workspace_check: NULL workspace");
+    return hc::gemm_check_on(ws->ws, (cudaStream_t)stream);
 }
 
 // ============================================================ synthetic inputs

@@ -54,6 +54,9 @@ __device__ __forceinline__ void store_x16(__half* row, int k, int e, float v) {
 // Reads and clears the device flag set by a timed-out pipeline wait
 // (synchronizes the device); HC_ERR_TIMEOUT when a kernel aborted.
 int gemm_check(GemmWorkspace* ws);
+// The same for launches on one stream, which is waited for (gemm_check waits
+// for those that order with the default stream).
+int gemm_check_on(GemmWorkspace* ws, cudaStream_t s);
 
 // The workspace's device error flag (allocated on first use; null when that
 // fails): other pipelined kernels report expired waits through it too, so

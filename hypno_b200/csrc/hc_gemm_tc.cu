@@ -1131,7 +1131,7 @@ int gemm_tc_impl(GemmWorkspace* ws, const hc_q4_matrix& w, const float* x, size_
     }
     if (!ws->err) {
         HC_CUDA(cudaMalloc((void**)&ws->err, sizeof(int)));
-        HC_CUDA(cudaMemset(ws->err, 0, sizeof(int)));
+        HC_CUDA(cudaMemsetAsync(ws->err, 0, sizeof(int), s));  // (s need not order with the default stream)
     }
     int nsm = 148;
     HC_CUDA(cudaDeviceGetAttribute(&nsm, cudaDevAttrMultiProcessorCount, dev));
@@ -1143,7 +1143,7 @@ int gemm_tc_impl(GemmWorkspace* ws, const hc_q4_matrix& w, const float* x, size_
         ws->sk_cap = 0;
         HC_CUDA(cudaMalloc((void**)&ws->sk_part, (size_t)nsm * 32 * BM * sizeof(float)));
         HC_CUDA(cudaMalloc((void**)&ws->sk_flag, (size_t)nsm * 4 * sizeof(int)));
-        HC_CUDA(cudaMemset(ws->sk_flag, 0, (size_t)nsm * 4 * sizeof(int)));
+        HC_CUDA(cudaMemsetAsync(ws->sk_flag, 0, (size_t)nsm * 4 * sizeof(int), s));
         ws->sk_cap = nsm;
         ws->generation++;
     }
@@ -1255,6 +1255,12 @@ int* gemm_error_flag(GemmWorkspace* ws) {
     return ws->err;
 }
 
+static int gemm_timed_out() {
+    hc_set_error("a bounded pipeline wait timed out in a tcgen05 GEMM or a TMA attention kernel (the kernel "
+                 "aborted and skipped its stores)");
+    return HC_ERR_TIMEOUT;
+}
+
 int gemm_check(GemmWorkspace* ws) {
     if (!ws || !ws->err) return HC_OK;
     int h = 0;
@@ -1264,9 +1270,26 @@ int gemm_check(GemmWorkspace* ws) {
         // an aborted stream-K launch may leave contributor flags raised;
         // a later owner would then add a stale slot without waiting
         if (ws->sk_flag) HC_CUDA(cudaMemset(ws->sk_flag, 0, (size_t)ws->sk_cap * 4 * sizeof(int)));
-        hc_set_error("a bounded pipeline wait timed out in a tcgen05 GEMM or a TMA attention kernel (the kernel "
-                     "aborted and skipped its stores)");
-        return HC_ERR_TIMEOUT;
+        return gemm_timed_out();
+    }
+    return HC_OK;
+}
+
+int gemm_check_on(GemmWorkspace* ws, cudaStream_t s) {
+    int *err, *flag, cap;
+    {
+        std::lock_guard<std::mutex> lock(ws->mu);
+        err = ws->err, flag = ws->sk_flag, cap = ws->sk_cap;
+    }
+    if (!err) return HC_OK;
+    int h = 0;
+    HC_CUDA(cudaMemcpyAsync(&h, err, sizeof(int), cudaMemcpyDeviceToHost, s));
+    HC_CUDA(cudaStreamSynchronize(s));
+    if (h) {  // as above, in the stream's order
+        HC_CUDA(cudaMemsetAsync(err, 0, sizeof(int), s));
+        if (flag) HC_CUDA(cudaMemsetAsync(flag, 0, (size_t)cap * 4 * sizeof(int), s));
+        HC_CUDA(cudaStreamSynchronize(s));
+        return gemm_timed_out();
     }
     return HC_OK;
 }

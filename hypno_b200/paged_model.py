@@ -13,6 +13,7 @@ The forward pass is transformer.rs:281-528 with the exact softmax instead of the
 reference's polynomial (hypno_b200.engine keeps that one).
 """
 import ctypes
+import threading
 from collections import deque
 
 import numpy as np
@@ -28,7 +29,8 @@ __all__ = ["PagedModel", "PagedGenerator"]
 class _Linear:
     """One weight matrix on the device: Q4_0 in the backend's layout, or FP32."""
 
-    def __init__(self, man, name, device):
+    def __init__(self, man, name, device, workspace):
+        self.workspace = workspace
         (self.n, self.k), dt, _, _ = man.tensors[name]
         raw = np.frombuffer(man.tensor_bytes(name)[0], np.uint8)
         self.q4 = self.dense = None
@@ -47,7 +49,7 @@ class _Linear:
         y = torch.empty((x.shape[0], self.n), dtype=torch.float32, device=x.device)
         x = x.contiguous()
         with on_device(x.get_device()):
-            call("hc_q4_matmul_dev", self.q4, x.data_ptr(), x.shape[0], y.data_ptr(), raw_stream(x.get_device()))
+            call("hc_q4_matmul_ws_dev", self.q4, x.data_ptr(), x.shape[0], y.data_ptr(), self.workspace, raw_stream(x.get_device()))
         return y
 
     def close(self):
@@ -64,6 +66,9 @@ class PagedModel:
         man = hf.Manifest(np.frombuffer(image, np.uint8) if isinstance(image, (bytes, bytearray)) else image)
         meta = man.metadata
         self.device = torch.device("cuda", torch.cuda.current_device()) if str(device) == "cuda" else torch.device(device)
+        self.workspace = ctypes.c_void_p()  # of this model's products
+        with on_device(self.device.index):
+            call("hc_q4_workspace_new", ctypes.byref(self.workspace))
         self.heads, self.kv_heads = int(meta["num_attention_heads"]), int(meta["num_key_value_heads"])
         self.hidden, self.layers = int(meta["hidden_size"]), int(meta["num_hidden_layers"])
         self.dim, self.vocab = self.hidden // self.heads, int(meta["vocab_size"])
@@ -84,17 +89,21 @@ class PagedModel:
             torch.cuda.synchronize(self.device)
         else:
             self.embed = vector(name).view(self.vocab, self.hidden)
-        self.lm_head = _Linear(man, "lm_head.weight" if "lm_head.weight" in man.tensors else name, self.device)
+        self.lm_head = _Linear(man, "lm_head.weight" if "lm_head.weight" in man.tensors else name, self.device, self.workspace)
         self.norm = vector("model.norm.weight")
         self.blocks, self.caches = [], []
         for i in range(self.layers):
             p = f"model.layers.{i}."
-            block = {k: _Linear(man, p + n + ".weight", self.device) for k, n in
+            block = {k: _Linear(man, p + n + ".weight", self.device, self.workspace) for k, n in
                      (("q", "self_attn.q_proj"), ("k", "self_attn.k_proj"), ("v", "self_attn.v_proj"), ("o", "self_attn.o_proj"),
                       ("gate", "mlp.gate_proj"), ("up", "mlp.up_proj"), ("down", "mlp.down_proj"))}
             block["in"], block["post"] = vector(p + "input_layernorm.weight"), vector(p + "post_attention_layernorm.weight")
             self.blocks.append(block)
             self.caches.append(paged.PagedKV.alloc(n_pages, page_size, self.kv_heads, self.dim, cache_dtype, self.device))
+        # the model's passes follow one another, the first one what was made here
+        self.lock, self.done = threading.Lock(), torch.cuda.Event()
+        with on_device(self.device.index):
+            self.done.record(torch.cuda.current_stream())
 
     def _normed(self, x, w):
         return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + self.eps) * w
@@ -102,7 +111,21 @@ class PagedModel:
     def logits(self, ids, batch, last):
         """Runs the packed rows' token ids (int64 on the device) through the
         layers, storing their keys and values, and returns the logits of the
-        rows `last`."""
+        rows `last`.  Passes of one model on different streams, or from different
+        threads, are made to follow one another on the device (they share its
+        workspace and pools); other models run beside them.  A pass captured in a
+        graph is not: its replays must not overlap the model's other passes."""
+        with self.lock, on_device(self.device.index):
+            stream = torch.cuda.current_stream()
+            if torch.cuda.is_current_stream_capturing():
+                return self._layers(ids, batch, last)
+            stream.wait_event(self.done)
+            try:
+                return self._layers(ids, batch, last)
+            finally:
+                self.done.record(stream)
+
+    def _layers(self, ids, batch, last):
         n = ids.shape[0]
         x = self.embed[ids]
         for b, kv in zip(self.blocks, self.caches):
@@ -113,6 +136,12 @@ class PagedModel:
             h = self._normed(x, b["post"])
             x = x + b["down"](torch.nn.functional.silu(b["gate"](h)) * b["up"](h))
         return self.lm_head(self._normed(x[last], self.norm))
+
+    def check(self):
+        """Waits for the current stream; raises HypnoCudaError if a product on it
+        gave up a bounded wait since the last check (its output is not written)."""
+        with on_device(self.device.index):
+            call("hc_q4_workspace_check", self.workspace, raw_stream(self.device.index))
 
     def step(self, ids, table, q_start, kv_len, settings):
         """One step of a serving loop from host arrays: ids of the packed rows,
@@ -125,7 +154,9 @@ class PagedModel:
         batch = paged.PagedBatch(t(table, np.int32), t(start, np.int32), t(length, np.int32), int(np.diff(start).max()), int(length.max()))
         logits = self.logits(t(ids, np.int64), batch, t(start[1:] - 1, np.int64))
         u, temp, k, p, m = (t([s[i] for s in settings], np.int32 if i == 2 else np.float32) for i in range(5))
-        return sampling.sample(logits, u, temp, k, p, m)[0].cpu().numpy()
+        tokens = sampling.sample(logits, u, temp, k, p, m)[0].cpu().numpy()
+        self.check()
+        return tokens
 
     def close(self):
         for b in self.blocks:
@@ -133,6 +164,9 @@ class PagedModel:
                 if isinstance(w, _Linear):
                     w.close()
         self.lm_head.close()
+        with on_device(self.device.index):
+            load().hc_q4_workspace_free(self.workspace)
+        self.workspace = ctypes.c_void_p()
 
 
 class _Request:

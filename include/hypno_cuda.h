@@ -109,6 +109,22 @@ int hc_q4_matrix_free(hc_q4_matrix* mat);
  * kernels::matmul_q4_0 (turbo::batch_matmul for mtok > 1). */
 int hc_q4_matmul_dev(const hc_q4_matrix* w, const float* x, size_t mtok, float* y, void* stream);
 
+/* The device scratch of products of two or more rows (the rows as fp16 parts,
+ * partial sums, flags), which the first one allocates and larger ones grow.
+ * Products that share a workspace must run one after another: on one stream,
+ * or ordered by events.  hc_q4_matmul_dev has a single one for the process, so
+ * that holds for all its calls; a program with several streams gives each its
+ * own and calls hc_q4_matmul_ws_dev, the same product.  Freed when the
+ * products that use it have ended. */
+typedef struct hc_q4_workspace hc_q4_workspace;
+int hc_q4_workspace_new(hc_q4_workspace** out);
+int hc_q4_workspace_free(hc_q4_workspace* ws);
+int hc_q4_matmul_ws_dev(const hc_q4_matrix* w, const float* x, size_t mtok, float* y, hc_q4_workspace* ws,
+                        void* stream);
+/* Waits for `stream`; HC_ERR_TIMEOUT if a product since the last check gave up
+ * a bounded wait and left its output unwritten. */
+int hc_q4_workspace_check(hc_q4_workspace* ws, void* stream);
+
 /* The same product as hc_q4_matmul_dev for callers that cannot allocate
  * device memory while running (a serving process whose device memory is all
  * handed to its own pool at start-up, or code that may not call cudaMalloc,

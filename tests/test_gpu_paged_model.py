@@ -99,6 +99,121 @@ def test_tokens_do_not_depend_on_the_schedule(cuda_device, image):
         assert sum(got[k] != want[k] for k in want) <= 1
 
 
+WIDE = dict(CFG, hidden=1024, heads=8, inter=2816)
+
+
+def passes(device, first_page, n, tokens, steps, seed):
+    """Arguments of `steps` calls of PagedModel.logits: n sequences, `tokens` new ones each a call,
+    in pages of their own from first_page on; and the pages behind the last."""
+    per = -(-tokens * steps // 16)
+    table = torch.arange(first_page, first_page + n * per, dtype=torch.int32, device=device).view(n, per)
+    g = torch.Generator(device=device).manual_seed(seed)
+    out = []
+    for i in range(1, steps + 1):
+        batch = paged.PagedBatch(table, torch.arange(0, tokens * n + 1, tokens, dtype=torch.int32, device=device),
+                                 torch.full((n,), tokens * i, dtype=torch.int32, device=device), tokens, tokens * i)
+        ids = torch.randint(0, CFG["vocab"], (tokens * n,), generator=g, device=device)
+        out.append((ids, batch, torch.arange(tokens * n, device=device)))
+    return out, first_page + n * per
+
+
+SHAPES = [(3, 40, 6), (13, 2, 30), (1, 90, 2), (2, 1, 60)]  # sequences, tokens, calls: products of every tile size, and single rows
+
+
+def alone(m, todo):
+    """The logits of each list of calls, one call at a time."""
+    out = []
+    for calls in todo:
+        out.append([])
+        for c in calls:
+            out[-1].append(m.logits(*c))
+            torch.cuda.synchronize()
+    return out
+
+
+def same(got, want):
+    return all(len(a) == len(b) and all(torch.equal(x, y) for x, y in zip(a, b)) for a, b in zip(got, want))
+
+
+def test_models_on_streams_of_their_own(cuda_device):
+    """Four models, each on its own stream with nothing that waits between them."""
+    image = synth.build_image(WIDE, seed=1, std=0.05)
+    todo = [passes(cuda_device, 0, *shape, seed=i)[0] for i, shape in enumerate(SHAPES)]
+    m = PagedModel(image, n_pages=60, page_size=16)
+    want = [alone(m, [calls])[0] for calls in todo]
+    m.close()
+    models, streams = [PagedModel(image, n_pages=60, page_size=16) for _ in todo], [torch.cuda.Stream() for _ in todo]
+    torch.cuda.synchronize()
+    got = [[] for _ in todo]
+    for i in range(max(map(len, todo))):
+        for k, calls in enumerate(todo):
+            if i < len(calls):
+                with torch.cuda.stream(streams[k]):
+                    got[k].append(models[k].logits(*calls[i]))
+    torch.cuda.synchronize()
+    assert same(got, want)
+    for m in models:
+        m.check()
+        m.close()
+
+
+@pytest.mark.parametrize("threads", [False, True])
+def test_one_model_on_several_streams(cuda_device, threads):
+    """Requests of one model, each on its own stream, in turn from one thread or from a thread each."""
+    import threading
+    todo, at = [], 0
+    for i, shape in enumerate(SHAPES):
+        calls, at = passes(cuda_device, at, *shape, seed=i)
+        todo.append(calls)
+    m = PagedModel(synth.build_image(WIDE, seed=1, std=0.05), n_pages=at, page_size=16)
+    want = alone(m, todo)
+    streams, got, errors = [torch.cuda.Stream() for _ in todo], [[] for _ in todo], []
+    torch.cuda.synchronize()
+
+    def run(k, calls):
+        try:
+            with torch.cuda.stream(streams[k]):
+                for c in calls:
+                    got[k].append(m.logits(*c))
+        except Exception as e:  # (of a thread: for the assertion below)
+            errors.append(e)
+
+    if threads:
+        each = [threading.Thread(target=run, args=(k, calls)) for k, calls in enumerate(todo)]
+        for t in each:
+            t.start()
+        for t in each:
+            t.join()
+    else:
+        for i in range(max(map(len, todo))):
+            for k, calls in enumerate(todo):
+                run(k, calls[i:i + 1])
+    torch.cuda.synchronize()
+    assert not errors and same(got, want)
+    m.check()
+    m.close()
+
+
+def test_an_aborted_product_is_reported(cuda_device, image, monkeypatch):
+    """step() raises what the check of its products says, instead of returning tokens."""
+    from hypno_b200 import paged_model
+    from hypno_b200._lib import HypnoCudaError
+    m = PagedModel(image, n_pages=4, page_size=16)
+    args = [3, 4], np.array([[1]]), [0, 2], [2], [(0.3, 0.0, 0, 1.0, 0.0)]
+    assert m.step(*args).shape == (1,)
+    real = paged_model.call
+
+    def call(name, *a):
+        if name == "hc_q4_workspace_check":
+            raise HypnoCudaError(-7, "a bounded pipeline wait timed out")
+        return real(name, *a)
+
+    monkeypatch.setattr(paged_model, "call", call)
+    with pytest.raises(HypnoCudaError):
+        m.step(*args)
+    m.close()
+
+
 def test_another_device_than_the_current_one(cuda_device, image, monkeypatch):
     from hypno_b200 import paged_model, sampling
     far = ref.Elsewhere(monkeypatch, paged, sampling, paged_model)

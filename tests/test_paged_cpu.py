@@ -130,3 +130,14 @@ def test_a_device_is_current_within_the_block_and_the_former_after_it(monkeypatc
     with _lib.on_device(3):  # current already: no call
         pass
     assert log == [1, 3, 0, 3]
+
+
+def test_product_workspaces_without_a_device(lib):
+    import ctypes
+    a, b = ctypes.c_void_p(), ctypes.c_void_p()
+    assert lib.hc_q4_workspace_new(ctypes.byref(a)) == 0 and lib.hc_q4_workspace_new(ctypes.byref(b)) == 0
+    assert a.value and b.value and a.value != b.value
+    assert lib.hc_q4_workspace_check(a, None) == 0            # no product has run in it
+    assert lib.hc_q4_workspace_new(None) == -1 and lib.hc_q4_workspace_check(None, None) == -1
+    assert lib.hc_q4_matmul_ws_dev(None, None, 2, None, a, None) == -1
+    assert lib.hc_q4_workspace_free(a) == 0 and lib.hc_q4_workspace_free(b) == 0 and lib.hc_q4_workspace_free(None) == 0
