@@ -111,7 +111,9 @@ class PagedModel:
     def logits(self, ids, batch, last):
         """Runs the packed rows' token ids (int64 on the device) through the
         layers, storing their keys and values, and returns the logits of the
-        rows `last`.  Passes of one model on different streams, or from different
+        rows `last`.  An id outside the vocabulary gives NaN for its row and the
+        rows of its sequence that see it (step() and PagedGenerator refuse it).
+        Passes of one model on different streams, or from different
         threads, are made to follow one another on the device (they share its
         workspace and pools); other models run beside them.  A pass captured in a
         graph is not: its replays must not overlap the model's other passes."""
@@ -127,7 +129,8 @@ class PagedModel:
 
     def _layers(self, ids, batch, last):
         n = ids.shape[0]
-        x = self.embed[ids]
+        known = (ids >= 0) & (ids < self.vocab)
+        x = self.embed[torch.where(known, ids, 0)].masked_fill_(~known[:, None], float("nan"))
         for b, kv in zip(self.blocks, self.caches):
             h = self._normed(x, b["in"])
             q, k, v = b["q"](h).view(n, -1, self.dim), b["k"](h).view(n, -1, self.dim), b["v"](h).view(n, -1, self.dim)
@@ -148,6 +151,7 @@ class PagedModel:
         the sequences' pages, row starts and lengths, and per sequence
         (u, temperature, top_k, top_p, min_p); returns the token drawn after
         each sequence's last row."""
+        _check_ids(ids, self.vocab)
         dev = self.device
         start, length = np.asarray(q_start, np.int32), np.asarray(kv_len, np.int32)
         t = lambda a, d: torch.from_numpy(np.ascontiguousarray(a, d)).to(dev)  # noqa: E731
@@ -169,6 +173,15 @@ class PagedModel:
         self.workspace = ctypes.c_void_p()
 
 
+def _check_ids(ids, vocab):
+    """Refuses token ids outside the vocabulary."""
+    a = np.asarray(ids)
+    if a.dtype.kind not in "iu":
+        raise TypeError(f"token ids must be integers, not {a.dtype}")
+    if a.size and not 0 <= int(a.min()) <= int(a.max()) < vocab:
+        raise ValueError(f"token ids from {int(a.min())} to {int(a.max())}, the vocabulary has {vocab}")
+
+
 class _Request:
     def __init__(self, rid, prompt, max_tokens, settings, seed):
         self.id, self.prompt, self.max_tokens, self.settings = rid, [int(t) for t in prompt], max_tokens, settings
@@ -180,7 +193,8 @@ class _Request:
 
 class PagedGenerator:
     """Continuous batching over a model with `step(ids, table, q_start, kv_len,
-    settings)` (PagedModel).  A request is admitted when the pool can hold it to
+    settings)`, `n_pages`, `page_size`, `max_pos` and, where it has one, `vocab`
+    (PagedModel).  A request is admitted when the pool can hold it to
     its last token; a step feeds every running request its next token and fills
     up to `budget` rows with chunks of the prompts still entering."""
 
@@ -200,6 +214,9 @@ class PagedGenerator:
     def submit(self, prompt, max_tokens, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, seed=0):
         """Queues a request; returns its id."""
         r = _Request(self.next_id, prompt, int(max_tokens), (float(temperature), int(top_k), float(top_p), float(min_p)), seed)
+        vocab = getattr(self.model, "vocab", None)
+        if vocab is not None:
+            _check_ids(r.prompt, vocab)
         if not r.prompt or r.max_tokens < 1:
             raise ValueError("a request needs a prompt and at least one token to make")
         if len(r.prompt) + r.max_tokens > self.model.max_pos or self._need(r) > self.model.n_pages:

@@ -194,6 +194,22 @@ def test_one_model_on_several_streams(cuda_device, threads):
     m.close()
 
 
+def test_ids_outside_the_vocabulary_on_the_device(cuda_device, image):
+    """They make their row NaN, and the rows of their sequence that see it; earlier
+    ones stay within the framework's bar for logits, other sequences keep their bits."""
+    m = PagedModel(image, n_pages=6, page_size=16)
+    i32 = dict(dtype=torch.int32, device=cuda_device)
+    batch = paged.PagedBatch(torch.tensor([[1], [4]], **i32), torch.tensor([0, 4, 7], **i32), torch.tensor([4, 3], **i32), 4, 4)
+    last = torch.arange(7, device=cuda_device)
+    want = m.logits(torch.tensor([5, 6, 7, 8, 9, 10, 11], device=cuda_device), batch, last)
+    for bad in (-1, CFG["vocab"], 2 ** 40):
+        got = m.logits(torch.tensor([5, 6, bad, 8, 9, 10, 11], device=cuda_device), batch, last)
+        assert bool(torch.isnan(got[2:4]).all()) and torch.equal(got[4:], want[4:])
+        # (rows of a tile with such a value add its products in another order)
+        assert bool(((got[:2] - want[:2]).abs() <= 1e-3 * want.abs().max().clamp_min(1.0)).all())
+    m.close()
+
+
 def test_an_aborted_product_is_reported(cuda_device, image, monkeypatch):
     """step() raises what the check of its products says, instead of returning tokens."""
     from hypno_b200 import paged_model

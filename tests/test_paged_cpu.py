@@ -141,3 +141,24 @@ def test_product_workspaces_without_a_device(lib):
     assert lib.hc_q4_workspace_new(None) == -1 and lib.hc_q4_workspace_check(None, None) == -1
     assert lib.hc_q4_matmul_ws_dev(None, None, 2, None, a, None) == -1
     assert lib.hc_q4_workspace_free(a) == 0 and lib.hc_q4_workspace_free(b) == 0 and lib.hc_q4_workspace_free(None) == 0
+
+
+@pytest.mark.parametrize("bad", [[-1], [5, 97], [3, -2, 4], [2 ** 40]])
+def test_ids_outside_the_vocabulary_are_refused(bad):
+    m = Plain()
+    m.vocab = 97
+    gen = PagedGenerator(m)
+    first = gen.submit([0, 96], 2)
+    with pytest.raises(ValueError):
+        gen.submit(bad, 2)
+    assert len(gen.waiting) == 1 and gen.submit([1], 1) == first + 1    # nothing of the refused one is left
+    assert sorted(gen.run()) == [first, first + 1]
+
+
+def test_a_step_refuses_ids_before_any_device_work():
+    from hypno_b200.paged_model import PagedModel
+    m = PagedModel.__new__(PagedModel)      # without weights or a device
+    m.vocab = 50
+    for ids, error in (([3, 50], ValueError), ([-1], ValueError), ([1.5], TypeError)):
+        with pytest.raises(error):
+            m.step(ids, np.zeros((1, 1), np.int32), [0, len(ids)], [len(ids)], [(0.0, 0.0, 0, 1.0, 0.0)])
