@@ -3,6 +3,8 @@
 // entry points with their checks of arguments.
 #include "hc_paged.h"
 
+#include <climits>
+
 namespace hc {
 
 namespace {
@@ -87,7 +89,7 @@ __global__ void __launch_bounds__(AP_THREADS) k_paged_append_vec(AppendArgs A) {
     int r0, r1;
     seq_rows(P, seq, r0, r1);
     if (row < r0 || row >= r1) return;
-    const int pos = __ldg(P.kv_len + seq) - (r1 - r0) + (row - r0);
+    const int pos = seq_len(P, seq) - (r1 - r0) + (row - r0);
     if (rotated) {
         const float2* cs = A.rope + (int64_t)min(max(pos, 0), A.rope_rows - 1) * half + (A.halves ? i0 : i0 >> 1);
         const float4 c01 = __ldg(reinterpret_cast<const float4*>(cs)), c23 = __ldg(reinterpret_cast<const float4*>(cs + 2));
@@ -132,7 +134,7 @@ __global__ void __launch_bounds__(256) k_paged_append(AppendArgs A) {
     int r0, r1;
     seq_rows(P, seq, r0, r1);
     if (row < r0 || row >= r1) return;
-    const int pos = __ldg(P.kv_len + seq) - (r1 - r0) + (row - r0);
+    const int pos = seq_len(P, seq) - (r1 - r0) + (row - r0);
     int i0 = 2 * j, i1 = 2 * j + 1;
     const int half = A.rot >> 1;
     const bool rotated = j < half;
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(GT) k_paged_generic(PagedAttnArgs A) {
     int r0, r1;
     seq_rows(P, seq, r0, r1);
     const int T_b = r1 - r0, m0 = s_tile * GM, mrows = min(GM, T_b * A.G - m0);
-    const int first = __ldg(P.kv_len + seq) - T_b;  // position of the sequence's first row
+    const int first = seq_len(P, seq) - T_b;  // position of the sequence's first row
     for (int i = threadIdx.x; i < mrows * hd; i += GT) {
         const int m = i / hd, d = i - m * hd, row = token_of(A, m0 + m), g = (m0 + m) - row * A.G;
         Q[m * ldk + d] = to_f32(((const T*)A.q)[(r0 + row) * A.q_rs + (kvh * A.G + g) * A.q_hs + d]) * A.scale;
@@ -217,19 +219,19 @@ __global__ void __launch_bounds__(GT) k_paged_generic(PagedAttnArgs A) {
     const int m = threadIdx.x >> 3, t = threadIdx.x & 7;
     const int pos = m < mrows ? first + token_of(A, m0 + m) : -1;
     const int lo = A.window > 0 ? max(0, pos - A.window + 1) : 0;
-    const int last = first + token_of(A, m0 + mrows - 1);                      // last position seen by the tile
-    const int p0 = first + token_of(A, m0);
-    const int begin = A.window > 0 ? max(0, p0 - A.window + 1) / GN * GN : 0;
+    int begin, end;  // positions seen by the tile
+    visible(A, first, m0, mrows, begin, end);
+    begin = begin / GN * GN;
     float o[HDMAX / 8];
 #pragma unroll
     for (int i = 0; i < HDMAX / 8; i++) o[i] = 0.0f;
     float mx = -INFINITY, l = 0.0f;
-    for (int j0 = begin; j0 <= last; j0 += GN) {
+    for (int j0 = begin; j0 < end; j0 += GN) {
         __syncthreads();
         if (threadIdx.x < GN) {
             const int j = j0 + threadIdx.x;
             int slot = 0;
-            const int page = j <= last ? lookup(P, seq, j, slot) : -1;
+            const int page = j < end ? lookup(P, seq, j, slot) : -1;
             s_ko[threadIdx.x] = page < 0 ? -1 : page * P.kps + kvh * P.khs + slot * P.kss;
             s_vo[threadIdx.x] = page < 0 ? -1 : page * P.vps + kvh * P.vhs + slot * P.vss;
         }
@@ -361,6 +363,7 @@ int paged_args(const char* who, const hc_paged_kv* kv, const hc_paged_batch* b, 
     P.n_seqs = b->n_seqs;
     P.max_pages = b->max_pages;
     P.n_rows = b->n_rows;
+    P.reach = (int)std::min<int64_t>((int64_t)b->max_pages * kv->page_size, INT_MAX - 1024);  // (tiles are counted past it)
     return HC_OK;
 }
 

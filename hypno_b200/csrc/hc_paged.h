@@ -22,6 +22,7 @@ struct PagedArgs {
     int n_pages, page_size, page_shift;  // page_shift >= 0: page_size = 1 << page_shift
     int nkv, hd;
     int n_seqs, max_pages, n_rows;
+    int reach;  // positions that a row of the table can name: what lies past them are holes, and not visited
 };
 
 struct PagedAttnArgs {
@@ -59,6 +60,9 @@ __device__ __forceinline__ void seq_rows(const PagedArgs& P, int b, int& r0, int
     r0 = min(max(__ldg(P.q_start + b), 0), P.n_rows);
     r1 = min(max(__ldg(P.q_start + b + 1), r0), P.n_rows);
 }
+
+// Positions of sequence b (a negative length counts as none).
+__device__ __forceinline__ int seq_len(const PagedArgs& P, int b) { return max(__ldg(P.kv_len + b), 0); }
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
@@ -133,8 +137,8 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 }
 // Visible positions of packed rows [m0, m0 + n) of a sequence: [begin, end).
 __device__ __forceinline__ void visible(const PagedAttnArgs& A, int first, int m0, int n, int& begin, int& end) {
-    end = max(0, first + token_of(A, m0 + n - 1) + 1);
-    begin = A.window > 0 ? max(0, first + token_of(A, m0) - A.window + 1) : 0;
+    end = min(max(0, first + token_of(A, m0 + n - 1) + 1), A.p.reach);
+    begin = A.window > 0 ? max(0, max(0, first + token_of(A, m0) + 1) - A.window) : 0;
     begin = min(begin, end);
 }
 

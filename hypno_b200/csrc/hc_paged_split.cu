@@ -99,11 +99,11 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& A, int R, int b
     SeqWork w;
     seq_rows(A.p, b, w.r0, w.r1);
     const int T = w.r1 - w.r0;
-    w.first = __ldg(A.p.kv_len + b) - T;
+    w.first = seq_len(A.p, b) - T;
     const int64_t tiles = ((int64_t)T * A.G + R - 1) / R;
     // positions seen by any tile, at most: the last tile's end from the first tile's begin, per tile no
     // more than its window and its own tokens
-    int len = max(0, w.first + T);
+    int len = min(max(0, w.first + T), A.p.reach);
     if (A.window > 0) len = (int)min((int64_t)len, (int64_t)A.window + R);
     w.units = max(1, len / UNIT + (len % UNIT != 0));
     w.pairs = (int)(tiles * A.p.nkv);

@@ -277,7 +277,7 @@ __device__ __forceinline__ bool tile_at(const TcArgs& X, int n, int& seq, int& i
         if (b >= P.n_seqs) return 0;
         int r0, r1;
         seq_rows(P, b, r0, r1);
-        const int len = min(max(__ldg(P.kv_len + b), 1), span);
+        const int len = min(max(seq_len(P, b), 1), span);
         cls = (int)((int64_t)(len - 1) * CLASSES / span);
         return (int)(((int64_t)(r1 - r0) * A.G + TC_ROWS - 1) / TC_ROWS);
     };
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
             // once for all warps: everything that follows from the tile's place
             int a, b;
             seq_rows(P, seq, a, b);
-            const int at = __ldg(P.kv_len + seq) - (b - a), m = tile * TC_ROWS;
+            const int at = seq_len(P, seq) - (b - a), m = tile * TC_ROWS;
             s_tile[1] = seq;
             s_tile[2] = m;
             s_tile[3] = a;

@@ -294,7 +294,7 @@ typedef struct hc_paged_kv {
  * at position kv_len[b] - (q_start[b + 1] - q_start[b]) + i.  Position p of
  * sequence b lives in page block_table[b * table_stride + p / page_size]; an
  * entry outside [0, n_pages) and a position beyond max_pages * page_size is a
- * hole.  All arrays are device memory.  max_q_len and max_kv_len are the
+ * hole, whatever kv_len[b] is (below 0: no positions).  All arrays are device memory.  max_q_len and max_kv_len are the
  * caller's upper bounds on the rows and positions of a sequence; they choose
  * launches and hold off no work (a larger sequence is served all the same,
  * more slowly). */

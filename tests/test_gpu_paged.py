@@ -121,6 +121,38 @@ def test_rows_that_see_nothing(cuda_device, types):
 
 
 @pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("new,dim", [(1, 64), (150, 64), (1, 7), (40, 7), (3, 160)])
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 70, 10 ** 9, -1, -2 ** 31])
+def test_lengths_past_the_table(cuda_device, types, new, dim, length):
+    """Positions past the table are holes however many the length names: such rows
+    see all of the table's, stores go nowhere; a negative length sees nothing."""
+    c = ref.Case([new], [48 + new], 4, 2, dim, 16, 17, *types)
+    c.table = np.ascontiguousarray(c.table[:, :3])
+    want, want_lse, A, M = ref.attention(c)
+    kv, batch, q, kn, vn = on_device(c, cuda_device)
+    batch = paged.PagedBatch(batch.block_table, batch.q_start, torch.tensor([length], dtype=torch.int32, device=cuda_device), new, 48)
+    lse = torch.empty((new, 4), device=cuda_device)
+    before = kv.k.clone(), kv.v.clone()
+    got = paged.attention(kv, batch, q, lse=lse).cpu().numpy().astype(np.float64)
+    turned = paged.append(kv, batch, kn, vn, q=q, rope=paged.rope_table(48, dim // 2 * 2, 1e4, cuda_device))
+    assert bool(torch.isfinite(turned).all()) and torch.equal(kv.k, before[0]) and torch.equal(kv.v, before[1])
+    if length < 0:
+        assert np.all(got == 0) and bool(torch.all(lse == -float("inf")))
+        return
+    assert np.all(np.abs(got - want) <= ref.tolerance(c, A, M, types[0] == np.float16))
+    room = A[..., 0] * 2.0 ** -20 + 2.0 ** -19 + np.abs(want_lse) * 2.0 ** -22
+    assert np.all(np.abs(lse.cpu().numpy() - want_lse) <= room)
+    # a window that reaches back from there leaves nothing, the widest one everything where there is something
+    assert bool((paged.attention(kv, batch, q, window=100) == 0).all())
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("new,dim", [(5, 64), (150, 64), (40, 7)])
+def test_the_widest_window_with_more_rows_than_positions(cuda_device, types, new, dim):
+    check_attention(ref.Case([new], [new - 4], 4, 2, dim, 16, 18, *types), cuda_device, window=2 ** 31 - 1)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
 @pytest.mark.parametrize("stale", [np.nan, np.inf, -65504.0])
 def test_stale_slots_do_not_reach_a_row(cuda_device, types, stale):
     """Unused slots of a page and spare pages hold NaN, infinities or the lowest value."""
