@@ -43,7 +43,7 @@ class PagedKV:
     dimension contiguous; the other strides are free (a [n_pages, page_size,
     n_kv_heads, head_dim] pool is passed as pool.transpose(1, 2))."""
 
-    __slots__ = ("k", "v", "struct", "ref", "device", "index", "n_kv_heads", "head_dim", "page_size", "n_pages")
+    __slots__ = ("_k", "_v", "struct", "ref", "device", "index", "n_kv_heads", "head_dim", "page_size", "n_pages")
 
     def __init__(self, k_pages, v_pages):
         for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
@@ -55,12 +55,16 @@ class PagedKV:
                 raise ValueError(f"the last dimension of {name} must be contiguous")
         if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.device != v_pages.device:
             raise ValueError("k_pages and v_pages must have one shape, type and device")
-        self.k, self.v = k_pages, v_pages
+        self._k, self._v = k_pages, v_pages
         self.device, self.index = k_pages.device, k_pages.device.index
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k_pages.shape
         self.struct = HcPagedKV(k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], *v_pages.stride()[:3],
                                 _KV[k_pages.dtype], self.n_pages, self.page_size, self.n_kv_heads, self.head_dim, 0)
         self.ref = ctypes.addressof(self.struct)
+
+    # (the struct holds their addresses: another pool is another PagedKV)
+    k = property(lambda self: self._k, doc="The keys' pages.")
+    v = property(lambda self: self._v, doc="The values' pages.")
 
     @classmethod
     def alloc(cls, n_pages, page_size, n_kv_heads, head_dim, dtype=torch.float16, device="cuda"):
@@ -83,9 +87,10 @@ class PagedBatch:
     sequence b are q_start[b] .. q_start[b + 1] - 1), kv_len [n_seqs] (its
     positions, the new ones included), all int32 on the pool's device.
     max_q_len and max_kv_len are the host's upper bounds on a sequence's rows
-    and positions: they choose launches, not results."""
+    and positions: they choose launches, not results.  The tensors' contents may
+    change between calls; other tensors or bounds are another batch."""
 
-    __slots__ = ("block_table", "q_start", "kv_len", "max_q_len", "max_kv_len", "index", "n_rows", "blob")
+    __slots__ = ("_tensors", "_bounds", "index", "n_rows", "blob")
 
     def __init__(self, block_table, q_start, kv_len, max_q_len, max_kv_len):
         index = kv_len.get_device()
@@ -97,17 +102,23 @@ class PagedBatch:
             raise ValueError(f"a block_table of {n} rows needs {n} lengths and {n + 1} row starts")
         if max_q_len < 0 or max_kv_len < 0:
             raise ValueError("max_q_len and max_kv_len must not be negative")
-        self.block_table, self.q_start, self.kv_len = block_table, q_start, kv_len
-        self.max_q_len, self.max_kv_len, self.index = max_q_len, max_kv_len, index
+        self._tensors, self._bounds, self.index = (block_table, q_start, kv_len), (max_q_len, max_kv_len), index
         self.n_rows = -1
+
+    # (read only: what pack() made of them is kept)
+    block_table = property(lambda self: self._tensors[0])
+    q_start = property(lambda self: self._tensors[1])
+    kv_len = property(lambda self: self._tensors[2])
+    max_q_len = property(lambda self: self._bounds[0])
+    max_kv_len = property(lambda self: self._bounds[1])
 
     def pack(self, n_rows):
         """The batch with so many rows as the C ABI takes it."""
         if n_rows != self.n_rows:
-            t = self.block_table
+            t, starts, lengths = self._tensors
             n, pages = t.shape
-            self.blob = HC_PAGED_BATCH.pack(t.data_ptr(), self.q_start.data_ptr(), self.kv_len.data_ptr(), t.stride(0), n,
-                                            pages, n_rows, self.max_q_len, self.max_kv_len, 0)
+            self.blob = HC_PAGED_BATCH.pack(t.data_ptr(), starts.data_ptr(), lengths.data_ptr(), t.stride(0), n, pages, n_rows,
+                                            *self._bounds, 0)
             self.n_rows = n_rows
         return self.blob
 

@@ -162,3 +162,12 @@ def test_a_step_refuses_ids_before_any_device_work():
     for ids, error in (([3, 50], ValueError), ([-1], ValueError), ([1.5], TypeError)):
         with pytest.raises(error):
             m.step(ids, np.zeros((1, 1), np.int32), [0, len(ids)], [len(ids)], [(0.0, 0.0, 0, 1.0, 0.0)])
+
+
+def test_what_a_handle_was_made_of_cannot_be_replaced():
+    """The C structures hold the tensors' addresses, so another tensor must not be put in their place."""
+    kv, batch = paged.PagedKV.__new__(paged.PagedKV), paged.PagedBatch.__new__(paged.PagedBatch)
+    for obj, names in ((kv, ("k", "v")), (batch, ("block_table", "q_start", "kv_len", "max_q_len", "max_kv_len"))):
+        for name in names:
+            with pytest.raises(AttributeError):
+                setattr(obj, name, None)
