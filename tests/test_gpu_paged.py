@@ -320,6 +320,31 @@ def test_another_device_than_the_current_one(cuda_device, monkeypatch):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("types", TYPES[:3], ids=IDS[:3])
+@pytest.mark.parametrize("new", [[1, 1], [70, 200, 1], [9, 9, 9]])
+def test_a_captured_step(cuda_device, types, new):
+    """Append and attention in one graph, replayed with other rows, lengths and pages in the same tensors."""
+    c, d = (ref.Case(new, [n + 700 + i for n in new], 8, 2, 64, 16, 14 + i, *types) for i in range(2))
+    kv, batch, q, kn, vn = on_device(c, cuda_device)
+    rope = paged.rope_table(1024, 64, 1e4, cuda_device)
+
+    def step():
+        return paged.attention(kv, batch, paged.append(kv, batch, kn, vn, q=q, rope=rope))
+
+    first = step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for x in (d, c):
+        for t, a in ((kv.k, x.k), (kv.v, x.v), (batch.block_table, x.table), (batch.kv_len, x.kv_len), (q, x.q), (kn, x.kn), (vn, x.vn)):
+            t.copy_(torch.from_numpy(a))
+        g.replay()
+        got = out.clone()
+        assert torch.equal(got, step())
+    assert torch.equal(got, first)
+
+
 # ---------------------------------------------------------------- append
 
 @pytest.mark.parametrize("types", TYPES, ids=IDS)

@@ -79,6 +79,45 @@ def test_logits(cuda_device, image, sizes):
     m.close()
 
 
+@pytest.mark.parametrize("sizes", [(40,), (17, 1, 1, 21)])
+def test_logits_over_an_fp32_cache(cuda_device, image, sizes):
+    ids = synth.prompt_ids(CFG["vocab"], 40, seed=4).astype(np.int64)
+    want = forward(image, ids)
+    m = PagedModel(image, n_pages=8, page_size=16, cache_dtype=torch.float32)
+    t = paged.PageTable(8, 16, 1, 16)
+    i32 = dict(dtype=torch.int32, device=cuda_device)
+    at = 0
+    for n in sizes:
+        length = t.grow(0, n)
+        batch = paged.PagedBatch(torch.from_numpy(t.table[:, :3].copy()).to(cuda_device), torch.tensor([0, n], **i32), torch.tensor([length], **i32), n, length)
+        got = m.logits(torch.from_numpy(ids[at:at + n]).to(cuda_device), batch, torch.arange(n, device=cuda_device)).cpu().numpy()
+        assert np.max(np.abs(got - want[at:at + n])) <= 1e-3 * max(1.0, np.abs(want).max())
+        at += n
+    m.close()
+
+
+def test_a_captured_pass(cuda_device, image):
+    """A pass of the model in a graph, replayed with other tokens in the same pages."""
+    m = PagedModel(image, n_pages=6, page_size=16)
+    i32 = dict(dtype=torch.int32, device=cuda_device)
+    batch = paged.PagedBatch(torch.tensor([[1], [4]], **i32), torch.tensor([0, 4, 7], **i32), torch.tensor([4, 3], **i32), 4, 4)
+    ids, last = torch.tensor([5, 6, 7, 8, 9, 10, 11], device=cuda_device), torch.tensor([3, 6], device=cuda_device)
+    first = m.logits(ids, batch, last)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = m.logits(ids, batch, last)
+    g.replay()
+    assert torch.equal(out, first)
+    ids.copy_(torch.tensor([50, 60, 70, 80, 90, 100, 110]))
+    g.replay()
+    got = out.clone()
+    assert torch.equal(got, m.logits(ids, batch, last)) and not torch.equal(got, first)
+    m.check()
+    del g, out
+    m.close()
+
+
 def test_tokens_do_not_depend_on_the_schedule(cuda_device, image):
     def tokens(max_seqs, budget):
         m = PagedModel(image, n_pages=40, page_size=16)

@@ -149,6 +149,24 @@ def test_strided_rows_outputs_and_streams(cuda_device):
     assert torch.equal(out, want[0]) and torch.equal(lp, want[1])
 
 
+@pytest.mark.parametrize("B,V", [(1, 40001), (12, 5000)])
+def test_graph_capture(cuda_device, B, V):
+    g = torch.Generator(device=cuda_device).manual_seed(B)
+    l, u = torch.randn((B, V), generator=g, device=cuda_device) * 3, torch.rand(B, generator=g, device=cuda_device)
+    args = 0.8, 40, 0.9, 0.01
+    sampling.sample(l, u, *args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = sampling.sample(l, u, *args)
+    for _ in range(3):
+        l.copy_(torch.randn((B, V), generator=g, device=cuda_device) * 3)
+        u.copy_(torch.rand(B, generator=g, device=cuda_device))
+        graph.replay()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, sampling.sample(l, u, *args)))
+
+
 def test_another_device_than_the_current_one(cuda_device, monkeypatch):
     g = torch.Generator(device=cuda_device).manual_seed(2)
     l, u = torch.randn((3, 500), generator=g, device=cuda_device), torch.rand(3, generator=g, device=cuda_device)
