@@ -21,7 +21,7 @@ import torch
 
 from . import hypno_file as hf
 from . import paged, sampling
-from ._lib import call, load, on_device, raw_stream
+from ._lib import call, check, load, on_device, raw_stream
 
 __all__ = ["PagedModel", "PagedGenerator"]
 
@@ -44,12 +44,12 @@ class _Linear:
             raise ValueError(f"{name}: dtype {dt} is not supported here")
 
     def __call__(self, x):
+        """x times the matrix, with the matrix's device current."""
         if self.dense is not None:
             return x @ self.dense.T
-        y = torch.empty((x.shape[0], self.n), dtype=torch.float32, device=x.device)
         x = x.contiguous()
-        with on_device(x.get_device()):
-            call("hc_q4_matmul_ws_dev", self.q4, x.data_ptr(), x.shape[0], y.data_ptr(), self.workspace, raw_stream(x.get_device()))
+        y = torch.empty((x.shape[0], self.n), dtype=torch.float32, device=x.device)
+        check(load().hc_q4_matmul_ws_dev(self.q4, x.data_ptr(), x.shape[0], y.data_ptr(), self.workspace, raw_stream(x.get_device())))
         return y
 
     def close(self):
@@ -117,20 +117,25 @@ class PagedModel:
         threads, are made to follow one another on the device (they share its
         workspace and pools); other models run beside them.  A pass captured in a
         graph is not: its replays must not overlap the model's other passes."""
+        known = (ids >= 0) & (ids < self.vocab)
+        return self._pass(torch.where(known, ids, 0), batch, last, ~known[:, None])
+
+    def _pass(self, ids, batch, last, unknown=None):
         with self.lock, on_device(self.device.index):
             stream = torch.cuda.current_stream()
             if torch.cuda.is_current_stream_capturing():
-                return self._layers(ids, batch, last)
+                return self._layers(ids, batch, last, unknown)
             stream.wait_event(self.done)
             try:
-                return self._layers(ids, batch, last)
+                return self._layers(ids, batch, last, unknown)
             finally:
                 self.done.record(stream)
 
-    def _layers(self, ids, batch, last):
+    def _layers(self, ids, batch, last, unknown):
         n = ids.shape[0]
-        known = (ids >= 0) & (ids < self.vocab)
-        x = self.embed[torch.where(known, ids, 0)].masked_fill_(~known[:, None], float("nan"))
+        x = self.embed[ids]
+        if unknown is not None:
+            x.masked_fill_(unknown, float("nan"))
         for b, kv in zip(self.blocks, self.caches):
             h = self._normed(x, b["in"])
             q, k, v = b["q"](h).view(n, -1, self.dim), b["k"](h).view(n, -1, self.dim), b["v"](h).view(n, -1, self.dim)
@@ -156,7 +161,7 @@ class PagedModel:
         start, length = np.asarray(q_start, np.int32), np.asarray(kv_len, np.int32)
         t = lambda a, d: torch.from_numpy(np.ascontiguousarray(a, d)).to(dev)  # noqa: E731
         batch = paged.PagedBatch(t(table, np.int32), t(start, np.int32), t(length, np.int32), int(np.diff(start).max()), int(length.max()))
-        logits = self.logits(t(ids, np.int64), batch, t(start[1:] - 1, np.int64))
+        logits = self._pass(t(ids, np.int64), batch, t(start[1:] - 1, np.int64))
         u, temp, k, p, m = (t([s[i] for s in settings], np.int32 if i == 2 else np.float32) for i in range(5))
         tokens = sampling.sample(logits, u, temp, k, p, m)[0].cpu().numpy()
         self.check()
