@@ -159,6 +159,10 @@ class PagedModel:
         _check_ids(ids, self.vocab)
         dev = self.device
         start, length = np.asarray(q_start, np.int32), np.asarray(kv_len, np.int32)
+        if start.ndim != 1 or start.size < 2 or start[0] != 0 or start[-1] != len(ids) or np.diff(start).min() < 1:
+            raise ValueError(f"row starts {start.tolist()} of {len(ids)} rows: they begin at 0, each sequence has a row, and the last ends")
+        if length.shape != (start.size - 1,) or len(settings) != start.size - 1:
+            raise ValueError(f"{start.size - 1} sequences with {length.size} lengths and {len(settings)} settings")
         t = lambda a, d: torch.from_numpy(np.ascontiguousarray(a, d)).to(dev)  # noqa: E731
         batch = paged.PagedBatch(t(table, np.int32), t(start, np.int32), t(length, np.int32), int(np.diff(start).max()), int(length.max()))
         logits = self._pass(t(ids, np.int64), batch, t(start[1:] - 1, np.int64))

@@ -171,3 +171,14 @@ def test_what_a_handle_was_made_of_cannot_be_replaced():
         for name in names:
             with pytest.raises(AttributeError):
                 setattr(obj, name, None)
+
+
+@pytest.mark.parametrize("start,kv_len,settings", [([0, 2], [2], 1), ([1, 3], [2], 1), ([0, 2, 2, 3], [2, 1, 1], 3), ([0, 4, 3], [4, 1], 2), ([0], [], 0),
+                                                   ([0, 1, 3], [1], 2), ([0, 1, 3], [1, 2], 1), ([0, 5], [5], 1)])
+def test_a_step_refuses_rows_that_do_not_fit_together(start, kv_len, settings):
+    """Before any device work, where a row past the end would fail an assertion."""
+    from hypno_b200.paged_model import PagedModel
+    m = PagedModel.__new__(PagedModel)
+    m.vocab, m.device = 50, None
+    with pytest.raises(ValueError):
+        m.step([1, 2, 3], np.zeros((len(kv_len), 1), np.int32), start, kv_len, [(0.0, 0.0, 0, 1.0, 0.0)] * settings)
