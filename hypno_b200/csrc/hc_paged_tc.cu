@@ -491,7 +491,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const __grid_constan
         const int pos = in ? first + token_of(A, mh + r) : -1;
         const int lo_pos = A.window > 0 ? pos - A.window + 1 : 0;
         const int p_min = first + token_of(A, mh), l_max = A.window > 0 ? first + token_of(A, mh + rows - 1) - A.window + 1 : 0;
-        const float cf = A.scale * LOG2E * up;
+        // (never 0, which would make -inf, a masked key, NaN: a row of zeros has the least `up`)
+        const float cf = fmaxf(A.scale * LOG2E * up, 1.401298464e-45f);
         float m = -INFINITY, l = 0.0f;  // running maximum (log2 units), sum of weights
         float acc[HILO ? HO : 1];       // f32 queries: the running outputs
         if constexpr (HILO) {

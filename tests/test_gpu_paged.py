@@ -255,6 +255,17 @@ def test_wide_scores(cuda_device, types):
         check_attention(c, cuda_device, scale=1e8)
 
 
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("new", [1, 150])
+@pytest.mark.parametrize("scale", [1e-8, 1e-30, 1e-45])
+def test_tiny_scales_and_queries_of_zero(cuda_device, types, new, scale):
+    """Scores of (nearly) 0 behind a mask: every visible key weighs the same."""
+    c = ref.Case([new], [new + 20], 4, 2, 64, 16, 19, *types)
+    c.q[::2] = 0
+    check_attention(c, cuda_device, scale=scale)
+    check_attention(c, cuda_device, scale=scale, window=9)
+
+
 def test_long_cache_offsets(cuda_device):
     """Pages whose elements lie beyond 2^31 of the pool, and many splits."""
     dim, page, heads = 128, 16, 8
