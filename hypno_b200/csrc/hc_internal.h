@@ -109,7 +109,9 @@ int launch_gemv1_fused(const DevWeight& w, const float* x, float* y, const float
 // Launches kfn as a programmatic dependent of the stream's previous kernel:
 // its CTAs may become resident while that kernel still runs, which hides the
 // launch gap of short dependent kernels (the single-token decode chain).
-// kfn must call pdl_wait() before its first global memory access.
+// kfn must call pdl_wait() before its first access of global memory that the
+// kernel in front writes, or, where that one is itself a programmatic
+// dependent, any kernel before it.
 template <typename... KArgs, typename... Args>
 inline int launch_pdl(void (*kfn)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args... args) {
     cudaLaunchConfig_t cfg = {};

@@ -462,11 +462,11 @@ static int attn_checks(const char* who, const hc_paged_kv* kv, const hc_paged_ba
 }
 
 namespace {
-// Which kernel takes a call.  Up to 64 packed rows a sequence (single tokens,
-// short runs) read the keys once for 8 or 16 rows; more rows pay for the
-// 256-row tiles of the tcgen05 kernel where the cache is FP16, and stay with
-// the 16-row one where it is FP32.  Unaligned or odd heads take the kernel
-// for any shape.
+// Which kernel takes a call, by its row tiles at most.  Few (single tokens; up to
+// 16 packed rows of one sequence): the split kernel, which reads the keys once
+// for 8 or 16 rows.  More, over an FP16 cache: the 256-row tiles of the tcgen05
+// kernel; over an FP32 one: the split kernel still.  Unaligned or odd heads
+// take the kernel for any shape.
 enum AttnKernel { ATTN_ANY, ATTN_SPLIT, ATTN_TC };
 struct AttnPlan {
     AttnKernel kernel;

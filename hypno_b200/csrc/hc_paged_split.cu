@@ -12,10 +12,11 @@
 //
 // Bound by the bytes of K and V: each is read once, and R rows share it.  8
 // sequences of up to 32,768 FP16 keys, 64 heads over 8 of 128: 139 us, 5.8 TB/s;
-// with f32 queries the products in two parts count as well (32 sequences of up
-// to 2,304 keys, 32 heads over 8: 42 us, 4.4 TB/s).  FP32 cache: by the
-// instructions that split the operands (32 full sequences of 2,304 keys: 223 us,
-// 2.7 TB/s; 512 tokens over 4,096 keys: 1.8 ms, 18 TFLOP/s).
+// with f32 queries by latency: twelve warps an SM wait for chains of dependent
+// two-part products (32 sequences of up to 2,304 keys, 32 heads over 8: 41 us,
+// 4.4 TB/s; issue slots 42%, tensor pipe 17%).  FP32 cache: likewise, with three
+// products and the splitting of both operands (32 full sequences of 2,304 keys:
+// 223 us, 2.7 TB/s; 512 tokens over 4,096 keys: 1.8 ms, 18 TFLOP/s).
 // Products: mma.sync on S^T = K Q^T and O^T = V^T P^T, keys and head columns on
 // the 16-row side and the query rows on the 8-column side (8 rows a CTA where a
 // token's group fits them, 57 us, 16 rows 73: 32 full sequences of 2,304 keys, f32
@@ -26,8 +27,11 @@
 // q = 2^e (hi + lo) with hi, lo fp16 and e the row's own (22 bits, any range),
 // their weights as hi + lo too.  FP32 cache: m16n8k8 tf32 products of both
 // operands split in two (hi hi + hi lo + lo hi, 22 bits, the full exponent
-// range).  Weights are held times 2^14 in fp16, so that one of 2^-28 of the
-// largest still has 11 bits.
+// range).  Over an FP16 cache weights are held times 2^14 in fp16, so that one of
+// 2^-28 of the largest still has 11 bits; with 16-bit queries in one part (half
+// the products; the sums take them unrounded), which adds to a result's own
+// rounding less than that itself: relative error against 64 bits 2.2e-4 where f32
+// weights have 2.1e-4 (single tokens over 32,768 keys).
 #include "hc_paged.h"
 
 namespace hc {
@@ -634,7 +638,10 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
 
 // Joins the partial results of a pair that was cut, in the order of the CTAs.
 // Bound by latency (a pair has a few KB of them), so what can be worked out from
-// the batch alone is done before the wait.
+// the batch alone is done before the wait.  The batch may be read there: the
+// kernel in front is not a programmatic dependent, so all that came before it
+// (and may have written the batch) had ended when it began, and it writes only
+// partial results and outputs.
 template <typename QT>
 __global__ void __launch_bounds__(SP_THREADS) k_paged_join(const __grid_constant__ SplitArgs X) {
     const PagedAttnArgs& A = X.a;

@@ -15,7 +15,11 @@
 // independent work.  The products start when each thread has 32 of its 64
 // weights.
 //
-// 16-bit queries: O adds up in tensor memory, so the running maximum m moves
+// 16-bit queries: the weights are fp16 for the product with V (the operand type
+// that runs at the full rate; l adds them up before they are rounded), which
+// adds to a result's own rounding less than that itself: relative error against
+// 64 bits 2.7e-4 where f32 weights have 2.1e-4 (512 tokens over 16,384 keys).
+// O adds up in tensor memory, so the running maximum m moves
 // only when a row's maximum passes it by more than 2^TAU (the weights are held
 // times 2^BIAS and stay below 2^15, so that one of 2^-25 of the largest still
 // has 11 bits); O is rescaled in the first tiles and rarely after them.
@@ -39,12 +43,12 @@
 // four rows an instruction took 78 cycles each, 10,000 a pair.)  Keys without a
 // page are zeros; keys of a box that no row sees are zeroed by the rows' threads.
 //
-// 512 tokens over 16,384 keys, 64 heads over 8 of 128, f16: 301 us on an idle
-// GPU, 899 TFLOP/s (333 us, 812, where it runs hot); bound by the chain from S_h to
-// P_h of a half.  4 prompts of 2,048, 32 heads over 8: f16 222 us, 619 TFLOP/s;
-// f32 342 to 383 us, 359 to 402 TFLOP/s of twice as many products; a CTA's start
+// 512 tokens over 16,384 keys, 64 heads over 8 of 128, f16: 331 us, 816 TFLOP/s
+// (301 us, 899, with the GPU cool); bound by the chain from S_h to P_h of a half.
+// 4 prompts of 2,048, 32 heads over 8: f32 380 us, 362 TFLOP/s of twice as many
+// products (342 us with the GPU cool), f16 222 us, 619 TFLOP/s (cool); a CTA's start
 // (queries to shared memory) and end, some 19,000 cycles of 55,000, overlap
-// nothing.  Key by key copies in place of boxes: 477, 335 and 434 us.
+// nothing.  Key by key copies in place of boxes, cool: 477, 434 and 335 us.
 //
 // The loop of the rows' warps is kept short (values that are not finite have a
 // loop of their own): the instruction fetch of code unrolled for every case cost
@@ -209,9 +213,10 @@ __device__ __forceinline__ f2 mul2(f2 a, f2 b) {
 }
 // 2^x of a pair without the special function unit: x = n + r with n the nearest
 // integer (read from the low bits of x + 1.5 2^23), 2^r by the polynomial of
-// degree 5 with the least relative error on [-1/2, 1/2] (Remez exchange:
-// 7.5e-8; degree 3 would do for fp16 weights but not for the sums), n added
-// to the exponent.  x below -126 counts as -126.
+// degree 5 with the least relative error on [-1/2, 1/2] (Remez exchange, the
+// coefficients then rounded to f32: 1.6e-7 as they stand, 2.1e-7 evaluated in
+// f32; degree 3 would do for fp16 weights but not for the sums), n added to the
+// exponent.  x below -126 counts as -126.
 __device__ __forceinline__ void ex2_poly(f2 x, float& y0, float& y1) {
     float a, b;
     untwo(x, a, b);
@@ -264,7 +269,7 @@ __device__ __forceinline__ TcRange tc_range(const PagedAttnArgs& A, int first, i
 // sixteenth of the longest, and a sequence's later tiles, which see more of
 // them, before its earlier ones (a CTA that begins last should end soon; all
 // heads of a tile are next to one another; 24 ragged sequences of up to 257
-// tokens over up to 4,001 keys: 164 us, 196 in the sequences' order).  Executed
+// tokens over up to 4,001 keys: 164 to 169 us, 196 in the sequences' order).  Executed
 // by a whole warp; false past the last tile.
 __device__ __forceinline__ bool tile_at(const TcArgs& X, int n, int& seq, int& in_seq) {
     constexpr int CLASSES = 16;
@@ -1108,7 +1113,7 @@ __global__ void __launch_bounds__(256) k_paged_tc_join(const __grid_constant__ T
     const PagedAttnArgs& A = X.a;
     const PagedArgs& P = A.p;
     int seq = 0, tile = 0;
-    const bool any = tile_at(X, (int)blockIdx.x, seq, tile);
+    const bool any = tile_at(X, (int)blockIdx.x, seq, tile);  // (reads the batch before the wait, as k_paged_join does)
     pdl_wait();  // (every CTA waits: the next kernel on the stream begins when this grid has ended)
     if (!any) return;
     const int kvh = blockIdx.y, m0 = tile * TC_ROWS;

@@ -21,10 +21,10 @@
 // slow path, a radix search over the logits' keys.  Nothing of a row stays in
 // shared memory but the lists, so that several rows share an SM and one's
 // serial parts (barriers, the first CTA's work) hide behind another's passes.
-// Bound by the latency of the cluster barriers for few rows, by the
-// instructions of the passes (not by the one read of the logits) for many: a
-// weight is some 30 of them.  A row of 49,152 logits: 18 us; 32 rows of 128,256:
-// 36 us; 256 rows: 128 us, 1 TB/s of logits.
+// Bound by latency: a row is a chain of 6 to 10 cluster barriers with the first
+// CTA's work between them, and nothing is full even with 256 rows (43% of the issue
+// slots, 12% of DRAM).  A row of 49,152 logits: 18 us; 32 rows of 128,256: 35 to
+// 48 us; 256 rows: 120 to 146 us, 0.9 to 1.1 TB/s of logits.
 #include "hc_internal.h"
 #include "hc_common.cuh"
 

@@ -196,7 +196,10 @@ def attention(kv, batch, q, out=None, scale=None, window=0, lse=None):
     that sees nothing gives zeros.  q is [n_rows, n_heads, head_dim] float32 or
     float16, out the same; lse, if given, is a contiguous [n_rows, n_heads]
     float32 tensor for the log of the sums.  The softmax is exact (the
-    flat-cache forward passes keep the reference's polynomial)."""
+    flat-cache forward passes keep the reference's polynomial).  Scores and sums
+    are float32; float16 queries over a float16 cache round the weights to 11
+    bits for their product with V (an error like the output's own rounding),
+    float32 ones keep 22 bits."""
     if _lib.current_device() != kv.index:
         with _lib.on_device(kv.index):
             return attention(kv, batch, q, out, scale, window, lse)

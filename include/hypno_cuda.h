@@ -333,7 +333,12 @@ int hc_paged_append_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, cons
  * j > p - window), holes left out; a row that sees nothing gives zeros.  Query
  * head h reads KV head h / (n_heads / n_kv_heads).  The softmax is the exact
  * exponential's (the flat-cache forward passes keep the reference's
- * polynomial).  q and out are `dtype`; lse (may be NULL) receives the natural
+ * polynomial).  Scores and sums are f32.  With FP16 queries over an FP16 cache
+ * the weights are rounded to 11 bits for their product with V, which adds about
+ * as much error as the rounding of an FP16 output does, at most; FP32 queries
+ * or caches keep 22 bits.  What a row does not see cannot reach it, whatever it
+ * holds; a row that sees a key or value that is not finite may be NaN where the
+ * formula is not.  q and out are `dtype`; lse (may be NULL) receives the natural
  * log of each row's sum of exponentials, [n_rows][n_heads], -inf for a row
  * that sees nothing.  The call needs hc_paged_attention_workspace bytes of
  * device memory (16-byte aligned; contents do not matter, and calls on
