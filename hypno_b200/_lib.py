@@ -22,7 +22,7 @@ ERR_NAMES = {
 }
 
 DTYPE_FP32, DTYPE_FP16, DTYPE_Q8_0, DTYPE_Q4_0 = 0, 1, 2, 3
-KV_FP32, KV_FP16 = 0, 1
+KV_FP32, KV_FP16, KV_Q4 = 0, 1, 2
 
 
 class HypnoCudaError(RuntimeError):
@@ -73,9 +73,36 @@ class HcPagedKV(ctypes.Structure):
     ]
 
 
-# hc_paged_batch and hc_rows, in the order of their fields: passed by address as packed bytes
+class HcPagedKV4(ctypes.Structure):
+    _fields_ = [
+        ("base", HcPagedKV),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("ks_page_stride", ctypes.c_int64),
+        ("ks_head_stride", ctypes.c_int64),
+        ("ks_pos_stride", ctypes.c_int64),
+        ("vs_page_stride", ctypes.c_int64),
+        ("vs_head_stride", ctypes.c_int64),
+        ("vs_pos_stride", ctypes.c_int64),
+    ]
+
+
+class HcPageBounds(ctypes.Structure):
+    _fields_ = [
+        ("lo", ctypes.c_void_p),
+        ("hi", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("n_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+    ]
+
+
+# hc_paged_batch, hc_rows and hc_page_lists, in the order of their fields: passed by address as packed bytes
 HC_PAGED_BATCH = struct.Struct("PPPq6i")
 HC_ROWS = struct.Struct("Pqq")
+HC_PAGE_LISTS = struct.Struct("Pqq2i")
 
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
@@ -133,6 +160,13 @@ SIGNATURES = {
     "hc_paged_append_dev": (_I, [_P, _P, _P, _P, _P, _P, _I, _U32, _P, _I, _I, _I, _P]),
     "hc_paged_attention_workspace": (_I, [_P, _P, _I, _U32, _I, ctypes.POINTER(_SZ)]),
     "hc_paged_attention_dev": (_I, [_P, _P, _P, _P, _P, _I, _U32, _F, _I, _P, _SZ, _P]),
+    "hc_paged_list_attention_workspace": (_I, [_P, _P, _P, _I, _U32, _I, ctypes.POINTER(_SZ)]),
+    "hc_paged_list_attention_dev": (_I, [_P, _P, _P, _P, _P, _P, _I, _U32, _F, _I, _P, _SZ, _P]),
+    "hc_paged_values_dev": (_I, [_P, _P, _P, _P]),
+    "hc_page_bounds_update_dev": (_I, [_P, _P, _P, _P]),
+    "hc_page_bounds_values_dev": (_I, [_P, _P, _P, _P]),
+    "hc_page_select_workspace": (_I, [_P, _P, ctypes.POINTER(_SZ)]),
+    "hc_page_select_dev": (_I, [_P, _P, _P, _I, _U32, _I, _I, _I, _P, _P, _SZ, _P]),
     "hc_rope_table_host": (_I, [_SZ, _SZ, _F, _P]),
     "hc_phase_name": (ctypes.c_char_p, [_I]),
     "hc_comm_unique_id": (_I, [_P]),

@@ -1,0 +1,461 @@
+// Bounds of the keys of a paged cache's pages, and the pages that a row's queries
+// are to read by them.
+#include "hc_paged.h"
+
+#include <type_traits>
+
+namespace hc {
+
+namespace {
+
+struct Bounds {
+    int8_t* lo;
+    int8_t* hi;
+    float* scale;
+};
+
+// Biased exponent of the least power of two, from 2^-120 on, of which the
+// magnitude with these bits (finite) is at most 127: 127 = 1.984375 x 64.
+__device__ __forceinline__ int unit_exponent(uint32_t top) {
+    return max((int)(top >> 23) - 6 + ((top & 0x7FFFFFu) > 0x7E0000u), 7);
+}
+__device__ __forceinline__ float power(int biased) { return __uint_as_float((uint32_t)biased << 23); }
+
+// Four elements of a key as floats.
+template <typename CT, bool VEC>
+__device__ __forceinline__ void key4(const PagedArgs& P, const PagedScales& C, int page, int head, int slot, int d, float* x) {
+    const int64_t at = page * P.kps + head * P.khs + slot * P.kss;
+    if constexpr (std::is_same<CT, q4x>::value) {
+        const uint32_t w = __ldg(reinterpret_cast<const unsigned short*>((const uint8_t*)P.k + at + (d >> 1)));
+        const float s = __half2float(C.k[page * C.kps + head * C.khs + slot * C.kss + (d >> 5)]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = (float)((int)(w >> (4 * i) & 15) - 8) * s;
+    } else {
+        const CT* p = (const CT*)P.k + at + d;
+        if constexpr (VEC && sizeof(CT) == 4) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+        } else if constexpr (VEC) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+            x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = to_f32(p[i]);
+        }
+    }
+}
+
+// A CTA takes one page and KV head at a time: a thread four elements of every
+// (threads / quads)-th slot, the slots' results joined in shared memory.
+constexpr int BD_THREADS = 128;
+
+template <typename CT, bool VEC>
+__global__ void __launch_bounds__(BD_THREADS) k_page_bounds(PagedArgs P, PagedScales C, Bounds B) {
+    __shared__ float s_lo[BD_THREADS * 4], s_hi[BD_THREADS * 4];
+    __shared__ uint32_t s_top[BD_THREADS / 32];
+    const int head = blockIdx.y, b = blockIdx.z;
+    int r0, r1;
+    seq_rows(P, b, r0, r1);
+    const int n = min(seq_len(P, b), P.reach);
+    const int begin = max(seq_len(P, b) - (r1 - r0), 0);
+    if (r1 == r0 || begin >= n) return;
+    const int i0 = page_of(P, begin), i1 = page_of(P, n - 1);
+    const int hq = P.hd >> 2, rows = BD_THREADS / hq, q = threadIdx.x % hq, r = threadIdx.x / hq;
+    for (int i = i0 + blockIdx.x; i <= i1; i += gridDim.x) {
+        int slot;
+        const int page = lookup(P, b, i * P.page_size, slot);
+        if (page < 0) continue;
+        const int filled = min(P.page_size, n - i * P.page_size);
+        float lo[4], hi[4];
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) lo[k] = INFINITY, hi[k] = -INFINITY;
+        if (r < rows) {
+#pragma unroll 4
+            for (int s = r; s < filled; s += rows) {
+                float x[4];
+                key4<CT, VEC>(P, C, page, head, s, 4 * q, x);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    lo[k] = fminf(lo[k], x[k]);
+                    hi[k] = fmaxf(hi[k], x[k]);
+                    top = max(top, __float_as_uint(x[k]) & 0x7FFFFFFFu);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                s_lo[r * P.hd + 4 * q + k] = lo[k];
+                s_hi[r * P.hd + 4 * q + k] = hi[k];
+            }
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < BD_THREADS / 32; w++) top = max(top, s_top[w]);
+        const bool fine = top < 0x7F800000u;
+        const int e = fine ? unit_exponent(top) : 255;
+        const float inv = fine ? power(254 - e) : 0.0f;
+        const int64_t at = (int64_t)page * P.nkv + head;
+        if (threadIdx.x == 0) B.scale[at] = power(e);  // 255: infinity
+        if (threadIdx.x < hq) {
+            uint32_t lw = 0, hw = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float l = s_lo[4 * q + k], h = s_hi[4 * q + k];
+                for (int x = 1; x < rows; x++) {
+                    l = fminf(l, s_lo[x * P.hd + 4 * q + k]);
+                    h = fmaxf(h, s_hi[x * P.hd + 4 * q + k]);
+                }
+                if (fine) {
+                    lw |= (uint32_t)((int)floorf(l * inv) & 255) << (8 * k);
+                    hw |= (uint32_t)((int)ceilf(h * inv) & 255) << (8 * k);
+                }
+            }
+            reinterpret_cast<uint32_t*>(B.lo + at * P.hd)[q] = lw;
+            reinterpret_cast<uint32_t*>(B.hi + at * P.hd)[q] = hw;
+        }
+        __syncthreads();
+    }
+}
+
+__global__ void __launch_bounds__(256) k_bounds_values(Bounds B, int hd, int64_t quads, float* lo, float* hi) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= quads) return;
+    const float s = B.scale[i * 4 / hd];
+    const uint32_t l = reinterpret_cast<const uint32_t*>(B.lo)[i], h = reinterpret_cast<const uint32_t*>(B.hi)[i];
+    float4 a, b;
+    a.x = (float)(int8_t)l * s, a.y = (float)(int8_t)(l >> 8) * s, a.z = (float)(int8_t)(l >> 16) * s, a.w = (float)(int8_t)(l >> 24) * s;
+    b.x = (float)(int8_t)h * s, b.y = (float)(int8_t)(h >> 8) * s, b.z = (float)(int8_t)(h >> 16) * s, b.w = (float)(int8_t)(h >> 24) * s;
+    reinterpret_cast<float4*>(lo)[i] = a;
+    reinterpret_cast<float4*>(hi)[i] = b;
+}
+
+// ============================================================ selection
+
+struct SelectArgs {
+    PagedArgs p;  // the batch, page size and heads; no pool
+    Bounds b;
+    const void* q;
+    int64_t q_rs, q_hs;
+    int G;
+    int budget, first, recent;
+    int32_t* out;
+    uint32_t* keys;  // [row][KV head][max_pages], score_key()
+};
+
+// Position of packed row `row` and its sequence (false: it belongs to none).
+__device__ __forceinline__ bool place_of(const PagedArgs& P, int row, int& seq, int& pos) {
+    int lo = 0, hi = P.n_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (__ldg(P.q_start + mid) <= row) lo = mid;
+        else hi = mid - 1;
+    }
+    int r0, r1;
+    seq_rows(P, lo, r0, r1);
+    seq = lo;
+    pos = seq_len(P, lo) - (r1 - r0) + (row - r0);
+    return row >= r0 && row < r1;
+}
+
+// Scores: four lanes a page, 16 bytes of its bounds each in turn; eight query heads
+// at a time, their codes in shared memory as two vectors, what is above zero (it
+// meets hi) and what is below (it meets lo).  A sum of products of bytes is
+// exact (below 2^22), and is held with the two powers of two as a whole number of
+// the scores' order: 9 bits of exponent, 21 below the leading one, so that no score
+// overflows, underflows or is rounded.
+constexpr uint32_t KEY_ZERO = 0x80000000u, KEY_HOLE = 1u, KEY_INF = 0xfffffffeu, KEY_KEPT = 0xffffffffu;
+
+// sum 2^(et - 127) 2^(es - 127), et and es from 7 to 249, et = 0: zero.
+__device__ __forceinline__ uint32_t score_key(int sum, int et, int es) {
+    if (sum == 0 || et == 0) return KEY_ZERO;
+    const uint32_t b = __float_as_uint((float)abs(sum));
+    const uint32_t m = ((b >> 23) - 127 + et + es - 13) << 21 | (b & 0x7FFFFFu) >> 2;
+    return sum < 0 ? KEY_ZERO - m : KEY_ZERO + m;
+}
+
+constexpr int SC_THREADS = 128, SC_PAGES = SC_THREADS / 4, SC_HEADS = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(SC_THREADS) k_page_scores(const __grid_constant__ SelectArgs A) {
+    const PagedArgs& P = A.p;
+    extern __shared__ __align__(16) uint8_t sm[];
+    const int hd = P.hd, G = A.G, stride = (hd + 15) / 16 * 16;
+    uint8_t* qp = sm;                       // [G][stride]
+    uint8_t* qn = sm + (size_t)G * stride;  // [G][stride]
+    int* unit = reinterpret_cast<int*>(sm + 2 * (size_t)G * stride);  // exponents of t, 0: not finite
+    const int kvh = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_trigger();
+    for (int row = blockIdx.z; row < P.n_rows; row += gridDim.z) {
+        int seq, pos;
+        if (!place_of(P, row, seq, pos)) continue;
+        const int n = pages_seen(P, pos);
+        if (n <= A.budget || blockIdx.x * SC_PAGES >= n) continue;  // all of them, or none here
+        __syncthreads();
+        for (int g = warp; g < G; g += SC_THREADS / 32) {
+            const T* q = (const T*)A.q + row * A.q_rs + (kvh * G + g) * A.q_hs;
+            uint32_t top = 0;
+            for (int d = lane; d < hd; d += 32) top = max(top, __float_as_uint(to_f32(q[d])) & 0x7FFFFFFFu);
+            top = __reduce_max_sync(0xffffffffu, top);
+            const bool fine = top < 0x7F800000u;
+            const int e = fine ? unit_exponent(top) : 0;
+            const float inv = fine ? power(254 - e) : 0.0f;
+            for (int d = lane; d < stride; d += 32) {
+                const int c = fine && d < hd ? __float2int_rn(to_f32(q[d]) * inv) : 0;
+                qp[g * stride + d] = (uint8_t)max(c, 0);
+                qn[g * stride + d] = (uint8_t)min(c, 0);
+            }
+            if (lane == 0) unit[g] = e;
+        }
+        __syncthreads();
+        uint32_t* keys = A.keys + ((int64_t)row * P.nkv + kvh) * P.max_pages;
+        const int sub = threadIdx.x & 3;
+        for (int i0 = blockIdx.x * SC_PAGES; i0 < n; i0 += gridDim.x * SC_PAGES) {
+            const int i = i0 + (threadIdx.x >> 2);
+            int slot, page = -1;
+            if (i < n) page = lookup(P, seq, i * P.page_size, slot);
+            const int64_t at = ((int64_t)max(page, 0) * P.nkv + kvh) * hd;
+            uint32_t best = 0;
+            const uint32_t scale = page < 0 ? 0 : __float_as_uint(__ldg(A.b.scale + (int64_t)page * P.nkv + kvh)) >> 23;
+            const int es = min(max((int)scale, 7), 249);
+            for (int g0 = 0; g0 < G; g0 += SC_HEADS) {
+                int acc[SC_HEADS];
+#pragma unroll
+                for (int g = 0; g < SC_HEADS; g++) acc[g] = 0;
+                if (page >= 0) {
+                    if (hd % 16 == 0) {
+                        for (int x = sub; x < hd / 16; x += 4) {
+                            const int4 h = __ldg(reinterpret_cast<const int4*>(A.b.hi + at) + x), l = __ldg(reinterpret_cast<const int4*>(A.b.lo + at) + x);
+#pragma unroll
+                            for (int g = 0; g < SC_HEADS; g++) {
+                                if (g0 + g >= G) break;
+                                const int4 p = reinterpret_cast<const int4*>(qp + (g0 + g) * stride)[x], m = reinterpret_cast<const int4*>(qn + (g0 + g) * stride)[x];
+                                acc[g] = __dp4a(h.x, p.x, __dp4a(h.y, p.y, __dp4a(h.z, p.z, __dp4a(h.w, p.w, acc[g]))));
+                                acc[g] = __dp4a(l.x, m.x, __dp4a(l.y, m.y, __dp4a(l.z, m.z, __dp4a(l.w, m.w, acc[g]))));
+                            }
+                        }
+                    } else {
+                        for (int x = sub; x < hd / 4; x += 4) {
+                            const int h = __ldg(reinterpret_cast<const int*>(A.b.hi + at) + x), l = __ldg(reinterpret_cast<const int*>(A.b.lo + at) + x);
+#pragma unroll
+                            for (int g = 0; g < SC_HEADS; g++) {
+                                if (g0 + g >= G) break;
+                                acc[g] = __dp4a(h, reinterpret_cast<const int*>(qp + (g0 + g) * stride)[x], acc[g]);
+                                acc[g] = __dp4a(l, reinterpret_cast<const int*>(qn + (g0 + g) * stride)[x], acc[g]);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < SC_HEADS; g++) {
+                    acc[g] += __shfl_xor_sync(0xffffffffu, acc[g], 1);
+                    acc[g] += __shfl_xor_sync(0xffffffffu, acc[g], 2);
+                    if (g0 + g < G) best = max(best, score_key(acc[g], unit[g0 + g], es));
+                }
+            }
+            if (sub == 0 && i < n) {
+                uint32_t key = KEY_KEPT;  // whatever it scores
+                if (i >= A.first && i < n - A.recent) key = page < 0 ? KEY_HOLE : scale == 255 ? KEY_INF : best;
+                keys[i] = key;
+            }
+        }
+    }
+}
+
+// One CTA per (row, KV head): the budget-th largest key by four passes of eight
+// bits, then what is above it and, of what equals it, the first by index.  A
+// thread's keys are a run, so that one scan over the threads places them all.
+constexpr int PK_THREADS = 256;
+
+__global__ void __launch_bounds__(PK_THREADS) k_page_pick(const __grid_constant__ SelectArgs A) {
+    const PagedArgs& P = A.p;
+    __shared__ int s_hist[256], s_sum[2][PK_THREADS / 32];
+    __shared__ uint32_t s_digit;
+    __shared__ int s_left;
+    const int row = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int seq, pos;
+    const bool any = place_of(P, row, seq, pos);
+    const int n = any ? pages_seen(P, pos) : 0;
+    pdl_wait();
+    if (!any) return;
+    int32_t* out = A.out + ((int64_t)row * P.nkv + kvh) * A.budget;
+    if (n <= A.budget) {
+        for (int i = tid; i < A.budget; i += PK_THREADS) out[i] = i < n ? i : -1;
+        return;
+    }
+    const uint32_t* keys = A.keys + ((int64_t)row * P.nkv + kvh) * P.max_pages;
+    uint32_t prefix = 0, mask = 0;
+    int left = A.budget;  // of the keys that share the prefix, so many are to be taken
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        s_hist[tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += PK_THREADS) {
+            const uint32_t k = keys[i];
+            if ((k & mask) == prefix) atomicAdd(&s_hist[k >> shift & 255], 1);
+        }
+        __syncthreads();
+        // keys above digit tid: a scan from the top
+        const int c = s_hist[255 - tid];
+        int incl = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += t;
+        }
+        if (lane == 31) s_sum[0][warp] = incl;
+        __syncthreads();
+        for (int w = 0; w < warp; w++) incl += s_sum[0][w];
+        if (incl >= left && incl - c < left) {
+            s_digit = 255 - tid;
+            s_left = left - (incl - c);
+        }
+        __syncthreads();
+        prefix |= s_digit << shift;
+        mask |= 255u << shift;
+        left = s_left;
+        __syncthreads();
+    }
+    const int run = (n + PK_THREADS - 1) / PK_THREADS, i0 = min(tid * run, n), i1 = min(i0 + run, n);
+    int above = 0, equal = 0;
+    for (int i = i0; i < i1; i++) {
+        const uint32_t k = keys[i];
+        above += k > prefix;
+        equal += k == prefix;
+    }
+    int a = above, e = equal;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, e, o);
+        if (lane >= o) a += x, e += y;
+    }
+    if (lane == 31) s_sum[0][warp] = a, s_sum[1][warp] = e;
+    __syncthreads();
+    for (int w = 0; w < warp; w++) a += s_sum[0][w], e += s_sum[1][w];
+    a -= above;
+    e -= equal;
+    int at = a + min(e, left);
+    for (int i = i0; i < i1; i++) {
+        const uint32_t k = keys[i];
+        if (k > prefix || (k == prefix && e++ < left)) out[at++] = i;
+    }
+}
+
+template <typename CT>
+int launch_bounds_t(const PagedArgs& P, const PagedScales& C, const Bounds& B, bool vec, int touched, cudaStream_t s) {
+    const dim3 grid((unsigned)touched, (unsigned)P.nkv, (unsigned)P.n_seqs);
+    if (vec) k_page_bounds<CT, true><<<grid, BD_THREADS, 0, s>>>(P, C, B);
+    else k_page_bounds<CT, false><<<grid, BD_THREADS, 0, s>>>(P, C, B);
+    HC_LAUNCH_CHECK();
+    return HC_OK;
+}
+
+int bounds_ok(const char* who, const hc_page_bounds* b) {
+    HC_CHECK(b, HC_ERR_INVALID, "%s: NULL bounds", who);
+    HC_CHECK(b->n_pages >= 1 && b->page_size >= 1 && b->n_kv_heads >= 1 && b->n_kv_heads <= 65535, HC_ERR_INVALID,
+             "%s: bounds of %d pages of %d positions, %d heads", who, b->n_pages, b->page_size, b->n_kv_heads);
+    HC_CHECK(b->head_dim >= 4 && b->head_dim % 4 == 0 && b->head_dim <= 256, HC_ERR_UNSUPPORTED,
+             "%s: head_dim %d (a multiple of 4, at most 256)", who, b->head_dim);
+    HC_CHECK(b->lo && b->hi && b->scale && ((uintptr_t)b->lo | (uintptr_t)b->hi) % 16 == 0 && (uintptr_t)b->scale % 4 == 0, HC_ERR_INVALID,
+             "%s: NULL or misaligned bounds", who);
+    return HC_OK;
+}
+
+size_t key_bytes(const hc_page_bounds* b, const hc_paged_batch* batch) {
+    return (size_t)std::max(batch->n_rows, 0) * b->n_kv_heads * std::max(batch->max_pages, 0) * 4;
+}
+
+}  // namespace
+
+}  // namespace hc
+
+HC_EXPORT int hc_page_bounds_update_dev(const hc_page_bounds* b, const hc_paged_kv* kv, const hc_paged_batch* batch, void* stream) {
+    const char* who = "hc_page_bounds_update_dev";
+    hc::PagedArgs P;
+    hc::PagedScales C;
+    HC_TRY(hc::bounds_ok(who, b));
+    HC_TRY(hc::page_args(who, kv, batch, P, C));
+    HC_CHECK(b->n_pages == P.n_pages && b->page_size == P.page_size && b->n_kv_heads == P.nkv && b->head_dim == P.hd, HC_ERR_INVALID,
+             "%s: bounds of %d pages of %d positions, %d heads of %d, for a cache of %d, %d, %d, %d", who, b->n_pages, b->page_size,
+             b->n_kv_heads, b->head_dim, P.n_pages, P.page_size, P.nkv, P.hd);
+    HC_CHECK(P.n_seqs <= 65535, HC_ERR_INVALID, "%s: %d sequences", who, P.n_seqs);
+    if (P.n_rows == 0 || P.max_pages == 0) return HC_OK;
+    const hc::Bounds B = {b->lo, b->hi, b->scale};
+    cudaStream_t s = (cudaStream_t)stream;
+    // (more pages than the host's bound of the rows are walked by the same CTAs)
+    const int64_t rows = std::max(std::min(batch->max_q_len, P.n_rows), 1);
+    const int touched = (int)std::min<int64_t>((rows + P.page_size - 2) / P.page_size + 1, P.max_pages);
+    const bool vec = kv->kv_dtype == HC_KV_Q4 || ((uintptr_t)P.k % 16 == 0 && (P.kps | P.khs | P.kss) % 4 == 0);
+    if (kv->kv_dtype == HC_KV_Q4) return hc::launch_bounds_t<hc::q4x>(P, C, B, true, touched, s);
+    if (kv->kv_dtype == HC_KV_FP16) return hc::launch_bounds_t<__half>(P, C, B, vec, touched, s);
+    return hc::launch_bounds_t<float>(P, C, B, vec, touched, s);
+}
+
+HC_EXPORT int hc_page_bounds_values_dev(const hc_page_bounds* b, float* lo_out, float* hi_out, void* stream) {
+    const char* who = "hc_page_bounds_values_dev";
+    HC_TRY(hc::bounds_ok(who, b));
+    HC_CHECK(lo_out && hi_out && ((uintptr_t)lo_out | (uintptr_t)hi_out) % 16 == 0, HC_ERR_INVALID, "%s: NULL or misaligned output", who);
+    const int64_t quads = (int64_t)b->n_pages * b->n_kv_heads * b->head_dim / 4, blocks = (quads + 255) / 256;
+    HC_CHECK(blocks <= 0x7fffffff, HC_ERR_INVALID, "%s: %d pages", who, b->n_pages);
+    const hc::Bounds B = {b->lo, b->hi, b->scale};
+    hc::k_bounds_values<<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(B, b->head_dim, quads, lo_out, hi_out);
+    HC_LAUNCH_CHECK();
+    return HC_OK;
+}
+
+HC_EXPORT int hc_page_select_workspace(const hc_page_bounds* b, const hc_paged_batch* batch, size_t* bytes) {
+    const char* who = "hc_page_select_workspace";
+    HC_TRY(hc::bounds_ok(who, b));
+    HC_CHECK(batch && bytes, HC_ERR_INVALID, "%s: NULL batch or bytes", who);
+    *bytes = hc::key_bytes(b, batch);
+    return HC_OK;
+}
+
+HC_EXPORT int hc_page_select_dev(const hc_page_bounds* b, const hc_paged_batch* batch, const hc_rows* q, int n_heads, uint32_t dtype,
+                                 int budget, int first, int recent, int32_t* out, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "hc_page_select_dev";
+    hc::SelectArgs A;
+    hc::PagedScales C;
+    HC_TRY(hc::bounds_ok(who, b));
+    // (a pool that stands for its sizes: no key is read)
+    const hc_paged_kv kv = {b->lo, b->hi, 0, 0, 0, 0, 0, 0, HC_KV_FP16, b->n_pages, b->page_size, b->n_kv_heads, b->head_dim, 0};
+    HC_TRY(hc::page_args(who, &kv, batch, A.p, C));
+    HC_CHECK(dtype == HC_DTYPE_FP32 || dtype == HC_DTYPE_FP16, HC_ERR_UNSUPPORTED, "%s: dtype %u", who, dtype);
+    HC_CHECK(n_heads >= 1 && n_heads % A.p.nkv == 0, HC_ERR_INVALID, "%s: %d query heads over %d KV heads", who, n_heads, A.p.nkv);
+    HC_CHECK(first >= 0 && recent >= 0 && budget >= 1 && (int64_t)first + recent <= budget, HC_ERR_INVALID,
+             "%s: a budget of %d pages with the first %d and the last %d", who, budget, first, recent);
+    A.G = n_heads / A.p.nkv;
+    const size_t smem = 2 * (size_t)A.G * ((A.p.hd + 15) / 16 * 16) + 4 * (size_t)A.G;
+    HC_CHECK(smem <= 48 * 1024, HC_ERR_UNSUPPORTED, "%s: %d query heads of %d a KV head", who, A.G, A.p.hd);
+    if (batch->n_rows == 0) return HC_OK;
+    HC_TRY(hc::page_rows_ok(who, "q", q, dtype));
+    HC_CHECK(out && (uintptr_t)out % 4 == 0, HC_ERR_INVALID, "%s: NULL or misaligned out", who);
+    const size_t need = hc::key_bytes(b, batch);
+    HC_CHECK(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 16 == 0)), HC_ERR_INVALID,
+             "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, need, workspace_bytes);
+    A.b = {b->lo, b->hi, b->scale};
+    A.q = q->data;
+    A.q_rs = q->row_stride;
+    A.q_hs = q->head_stride;
+    A.budget = budget;
+    A.first = first;
+    A.recent = recent;
+    A.out = out;
+    A.keys = (uint32_t*)workspace;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (A.p.max_pages > budget) {
+        const int64_t pairs = (int64_t)A.p.n_rows * A.p.nkv, chunks = (A.p.max_pages + hc::SC_PAGES - 1) / hc::SC_PAGES;
+        const dim3 grid((unsigned)std::max<int64_t>(1, std::min(chunks, (148 * 16 + pairs - 1) / pairs)), (unsigned)A.p.nkv,
+                        (unsigned)std::min(A.p.n_rows, 65535));
+        if (dtype == HC_DTYPE_FP16) hc::k_page_scores<__half><<<grid, hc::SC_THREADS, smem, s>>>(A);
+        else hc::k_page_scores<float><<<grid, hc::SC_THREADS, smem, s>>>(A);
+        HC_LAUNCH_CHECK();
+        HC_TRY(hc::launch_pdl(hc::k_page_pick, dim3((unsigned)A.p.n_rows, (unsigned)A.p.nkv), dim3(hc::PK_THREADS), 0, s, A));
+        HC_LAUNCH_CHECK();
+    } else {
+        hc::k_page_pick<<<dim3((unsigned)A.p.n_rows, (unsigned)A.p.nkv), hc::PK_THREADS, 0, s>>>(A);
+        HC_LAUNCH_CHECK();
+    }
+    return HC_OK;
+}

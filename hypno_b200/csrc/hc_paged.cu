@@ -11,16 +11,6 @@ namespace {
 
 // ============================================================ append
 
-struct AppendArgs {
-    PagedArgs p;
-    const void *k, *v, *q;
-    void* qo;
-    int64_t k_rs, k_hs, v_rs, v_hs, q_rs, q_hs, o_rs, o_hs;
-    const float2* rope;
-    int rope_rows, rot, halves;
-    int nh;  // 0: no queries
-};
-
 __device__ __forceinline__ int seq_of_row(const PagedArgs& P, int r) {
     int lo = 0, hi = P.n_seqs - 1;  // the last sequence whose first row is <= r
     while (lo < hi) {
@@ -184,8 +174,10 @@ __global__ void __launch_bounds__(256) k_paged_append(AppendArgs A) {
 // positions, 16 heads over 8 of 256, took 6.7 ms here and take 72 us there).
 constexpr int GM = 32, GN = 32, GT = 256;
 
-template <typename T, typename C, int HDMAX>
-__global__ void __launch_bounds__(GT) k_paged_generic(PagedAttnArgs A) {
+// LIST: a tile holds query heads of one token, whose keys are the positions of
+// its listed pages one after another.
+template <typename T, typename C, int HDMAX, bool LIST>
+__global__ void __launch_bounds__(GT) k_paged_generic(PagedAttnArgs A, PagedList L) {
     const PagedArgs& P = A.p;
     extern __shared__ float sm[];
     const int hd = P.hd, ldk = hd + 1;
@@ -198,7 +190,13 @@ __global__ void __launch_bounds__(GT) k_paged_generic(PagedAttnArgs A) {
     const int kvh = blockIdx.y;
     if (threadIdx.x < 32) {
         int a = 0, b = 0;
-        const bool ok = find_tile(P, A.G, GM, blockIdx.x, a, b);
+        bool ok;
+        if constexpr (LIST) {
+            const int tg = (A.G + GM - 1) / GM;
+            ok = find_tile(P, tg, 1, blockIdx.x, a, b);
+        } else {
+            ok = find_tile(P, A.G, GM, blockIdx.x, a, b);
+        }
         if (threadIdx.x == 0) {
             s_ok = ok;
             s_seq = a;
@@ -210,7 +208,13 @@ __global__ void __launch_bounds__(GT) k_paged_generic(PagedAttnArgs A) {
     const int seq = s_seq;
     int r0, r1;
     seq_rows(P, seq, r0, r1);
-    const int T_b = r1 - r0, m0 = s_tile * GM, mrows = min(GM, T_b * A.G - m0);
+    const int T_b = r1 - r0;
+    int m0 = s_tile * GM, mrows = min(GM, T_b * A.G - m0);
+    if constexpr (LIST) {
+        const int tg = (A.G + GM - 1) / GM, g0 = (s_tile % tg) * GM;
+        m0 = s_tile / tg * A.G + g0;
+        mrows = min(GM, A.G - g0);
+    }
     const int first = seq_len(P, seq) - T_b;  // position of the sequence's first row
     for (int i = threadIdx.x; i < mrows * hd; i += GT) {
         const int m = i / hd, d = i - m * hd, row = token_of(A, m0 + m), g = (m0 + m) - row * A.G;
@@ -220,8 +224,17 @@ __global__ void __launch_bounds__(GT) k_paged_generic(PagedAttnArgs A) {
     const int pos = m < mrows ? first + token_of(A, m0 + m) : -1;
     const int lo = A.window > 0 ? max(0, pos - A.window + 1) : 0;
     int begin, end;  // positions seen by the tile
-    visible(A, first, m0, mrows, begin, end);
-    begin = begin / GN * GN;
+    const int p_own = first + token_of(A, m0);
+    const int32_t* list = nullptr;
+    if constexpr (LIST) {
+        const int lrow = r0 + token_of(A, m0);
+        list = L.pages + lrow * L.row_stride + kvh * L.head_stride;
+        begin = 0;
+        end = (int)min((int64_t)min(list_count(L, lrow, kvh), pages_seen(P, p_own)) * P.page_size, (int64_t)0x7fffff00);
+    } else {
+        visible(A, first, m0, mrows, begin, end);
+        begin = begin / GN * GN;
+    }
     float o[HDMAX / 8];
 #pragma unroll
     for (int i = 0; i < HDMAX / 8; i++) o[i] = 0.0f;
@@ -231,7 +244,11 @@ __global__ void __launch_bounds__(GT) k_paged_generic(PagedAttnArgs A) {
         if (threadIdx.x < GN) {
             const int j = j0 + threadIdx.x;
             int slot = 0;
-            const int page = j < end ? lookup(P, seq, j, slot) : -1;
+            int page = -1;
+            if (j < end) {
+                if constexpr (LIST) page = lookup_listed(A, list, seq, j, p_own, slot);
+                else page = lookup(P, seq, j, slot);
+            }
             s_ko[threadIdx.x] = page < 0 ? -1 : page * P.kps + kvh * P.khs + slot * P.kss;
             s_vo[threadIdx.x] = page < 0 ? -1 : page * P.vps + kvh * P.vhs + slot * P.vss;
         }
@@ -255,7 +272,7 @@ __global__ void __launch_bounds__(GT) k_paged_generic(PagedAttnArgs A) {
 #pragma unroll
         for (int i = 0; i < GN / 8; i++) {
             const int j = j0 + t + 8 * i;
-            if (j > pos || j < lo || s_ko[t + 8 * i] < 0) s[i] = -INFINITY;
+            if ((!LIST && (j > pos || j < lo)) || s_ko[t + 8 * i] < 0) s[i] = -INFINITY;
             tm = fmaxf(tm, s[i]);
         }
 #pragma unroll
@@ -295,23 +312,28 @@ __global__ void __launch_bounds__(GT) k_paged_generic(PagedAttnArgs A) {
     if (A.lse && t == 0) A.lse[(int64_t)row * A.nh + head] = l == 0.0f ? -INFINITY : mx + logf(l);
 }
 
-template <typename T, typename C>
-int launch_generic_t(const PagedAttnArgs& A, cudaStream_t s) {
-    const int64_t tiles = ((int64_t)A.p.n_rows * A.G) / GM + A.p.n_seqs;
+template <typename T, typename C, bool LIST>
+int launch_generic_t(const PagedAttnArgs& A, const PagedList& L, cudaStream_t s) {
+    const int64_t tiles = LIST ? (int64_t)A.p.n_rows * ((A.G + GM - 1) / GM) : ((int64_t)A.p.n_rows * A.G) / GM + A.p.n_seqs;
     HC_CHECK(tiles <= 0x7fffffff, HC_ERR_INVALID, "paged attention: too many rows");
     const size_t smem = (size_t)((GM + 2 * GN) * (A.p.hd + 1) + GM * (GN + 1)) * sizeof(float);
-    auto kfn = A.p.hd <= 128 ? k_paged_generic<T, C, 128> : k_paged_generic<T, C, 256>;
+    auto kfn = A.p.hd <= 128 ? k_paged_generic<T, C, 128, LIST> : k_paged_generic<T, C, 256, LIST>;
     HC_CUDA(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kfn<<<dim3((unsigned)tiles, (unsigned)A.p.nkv), GT, smem, s>>>(A);
+    kfn<<<dim3((unsigned)tiles, (unsigned)A.p.nkv), GT, smem, s>>>(A, L);
     HC_LAUNCH_CHECK();
     return HC_OK;
 }
 
+template <bool LIST>
+int launch_generic_list(const PagedAttnArgs& A, const PagedList& L, int q16, int c16, cudaStream_t s) {
+    if (q16) return c16 ? launch_generic_t<__half, __half, LIST>(A, L, s) : launch_generic_t<__half, float, LIST>(A, L, s);
+    return c16 ? launch_generic_t<float, __half, LIST>(A, L, s) : launch_generic_t<float, float, LIST>(A, L, s);
+}
+
 }  // namespace
 
-int launch_paged_generic(const PagedAttnArgs& A, int q16, int c16, cudaStream_t s) {
-    if (q16) return c16 ? launch_generic_t<__half, __half>(A, s) : launch_generic_t<__half, float>(A, s);
-    return c16 ? launch_generic_t<float, __half>(A, s) : launch_generic_t<float, float>(A, s);
+int launch_paged_generic(const PagedAttnArgs& A, const PagedList& L, int q16, int c16, cudaStream_t s) {
+    return L.width ? launch_generic_list<true>(A, L, q16, c16, s) : launch_generic_list<false>(A, L, q16, c16, s);
 }
 
 }  // namespace hc
@@ -320,10 +342,12 @@ int launch_paged_generic(const PagedAttnArgs& A, int q16, int c16, cudaStream_t 
 
 namespace {
 
-int paged_args(const char* who, const hc_paged_kv* kv, const hc_paged_batch* b, hc::PagedArgs& P) {
-    HC_CHECK(kv && b, HC_ERR_INVALID, "%s: NULL cache or batch", who);
-    HC_CHECK(kv->kv_dtype == HC_KV_FP32 || kv->kv_dtype == HC_KV_FP16, HC_ERR_UNSUPPORTED, "%s: kv_dtype %d", who,
-             kv->kv_dtype);
+// A pool's own part of the arguments.
+int pool_args(const char* who, const hc_paged_kv* kv, hc::PagedArgs& P, hc::PagedScales& C) {
+    C = {};
+    HC_CHECK(kv, HC_ERR_INVALID, "%s: NULL cache or batch", who);
+    HC_CHECK(kv->kv_dtype == HC_KV_FP32 || kv->kv_dtype == HC_KV_FP16 || kv->kv_dtype == HC_KV_Q4, HC_ERR_UNSUPPORTED,
+             "%s: kv_dtype %d", who, kv->kv_dtype);
     HC_CHECK(kv->n_pages >= 1 && kv->page_size >= 1 && kv->n_kv_heads >= 1 && kv->head_dim >= 1, HC_ERR_INVALID,
              "%s: empty cache (%d pages of %d positions, %d heads of %d)", who, kv->n_pages, kv->page_size,
              kv->n_kv_heads, kv->head_dim);
@@ -332,15 +356,22 @@ int paged_args(const char* who, const hc_paged_kv* kv, const hc_paged_batch* b, 
     HC_CHECK(kv->k_page_stride >= 0 && kv->k_head_stride >= 0 && kv->k_pos_stride >= 0 && kv->v_page_stride >= 0 &&
                  kv->v_head_stride >= 0 && kv->v_pos_stride >= 0,
              HC_ERR_INVALID, "%s: negative pool stride", who);
-    const uintptr_t es = kv->kv_dtype == HC_KV_FP16 ? 2 : 4;
+    const uintptr_t es = kv->kv_dtype == HC_KV_FP16 ? 2 : kv->kv_dtype == HC_KV_Q4 ? 16 : 4;
     HC_CHECK(((uintptr_t)kv->k | (uintptr_t)kv->v) % es == 0, HC_ERR_INVALID, "%s: misaligned pool", who);
-    HC_CHECK(b->n_seqs >= 0 && b->n_rows >= 0 && b->max_pages >= 0 && b->max_q_len >= 0 && b->max_kv_len >= 0,
-             HC_ERR_INVALID, "%s: negative size in the batch", who);
-    HC_CHECK(b->n_seqs > 0 || b->n_rows == 0, HC_ERR_INVALID, "%s: %d rows of no sequence", who, b->n_rows);
-    HC_CHECK(b->n_seqs == 0 || (b->q_start && b->kv_len && (b->block_table || b->max_pages == 0)), HC_ERR_INVALID,
-             "%s: NULL batch array", who);
-    HC_CHECK(b->table_stride >= b->max_pages || b->n_seqs <= 1, HC_ERR_INVALID,
-             "%s: table rows of %d pages at stride %lld", who, b->max_pages, (long long)b->table_stride);
+    if (kv->kv_dtype == HC_KV_Q4) {
+        const hc_paged_kv_q4* q = (const hc_paged_kv_q4*)kv;
+        HC_CHECK(kv->head_dim % 32 == 0 && kv->head_dim <= 256, HC_ERR_UNSUPPORTED,
+                 "%s: head_dim %d of a cache in 4 bits (a multiple of 32, at most 256)", who, kv->head_dim);
+        HC_CHECK((kv->k_page_stride | kv->k_head_stride | kv->k_pos_stride | kv->v_page_stride | kv->v_head_stride | kv->v_pos_stride) % 16 == 0,
+                 HC_ERR_INVALID, "%s: strides of codes in 4 bits that are not multiples of 16 bytes", who);
+        const int64_t sl = hc::q4_slots(kv->head_dim);
+        HC_CHECK(q->k_scale && q->v_scale && ((uintptr_t)q->k_scale | (uintptr_t)q->v_scale) % (2 * sl) == 0, HC_ERR_INVALID,
+                 "%s: NULL or misaligned scales", who);
+        const int64_t st[6] = {q->ks_page_stride, q->ks_head_stride, q->ks_pos_stride, q->vs_page_stride, q->vs_head_stride, q->vs_pos_stride};
+        for (int64_t x : st)
+            HC_CHECK(x >= 0 && x % sl == 0, HC_ERR_INVALID, "%s: a stride of %lld scales (a multiple of %lld)", who, (long long)x, (long long)sl);
+        C = {(__half*)q->k_scale, (__half*)q->v_scale, st[0], st[1], st[2], st[3], st[4], st[5]};
+    }
     P.k = kv->k;
     P.v = kv->v;
     P.kps = kv->k_page_stride;
@@ -349,10 +380,6 @@ int paged_args(const char* who, const hc_paged_kv* kv, const hc_paged_batch* b, 
     P.vps = kv->v_page_stride;
     P.vhs = kv->v_head_stride;
     P.vss = kv->v_pos_stride;
-    P.table = b->block_table;
-    P.q_start = b->q_start;
-    P.kv_len = b->kv_len;
-    P.table_stride = b->table_stride;
     P.n_pages = kv->n_pages;
     P.page_size = kv->page_size;
     P.page_shift = -1;
@@ -360,6 +387,23 @@ int paged_args(const char* who, const hc_paged_kv* kv, const hc_paged_batch* b, 
         if (kv->page_size == (1 << i)) P.page_shift = i;
     P.nkv = kv->n_kv_heads;
     P.hd = kv->head_dim;
+    return HC_OK;
+}
+
+int paged_args(const char* who, const hc_paged_kv* kv, const hc_paged_batch* b, hc::PagedArgs& P, hc::PagedScales& C) {
+    HC_CHECK(kv && b, HC_ERR_INVALID, "%s: NULL cache or batch", who);
+    HC_TRY(pool_args(who, kv, P, C));
+    HC_CHECK(b->n_seqs >= 0 && b->n_rows >= 0 && b->max_pages >= 0 && b->max_q_len >= 0 && b->max_kv_len >= 0,
+             HC_ERR_INVALID, "%s: negative size in the batch", who);
+    HC_CHECK(b->n_seqs > 0 || b->n_rows == 0, HC_ERR_INVALID, "%s: %d rows of no sequence", who, b->n_rows);
+    HC_CHECK(b->n_seqs == 0 || (b->q_start && b->kv_len && (b->block_table || b->max_pages == 0)), HC_ERR_INVALID,
+             "%s: NULL batch array", who);
+    HC_CHECK(b->table_stride >= b->max_pages || b->n_seqs <= 1, HC_ERR_INVALID,
+             "%s: table rows of %d pages at stride %lld", who, b->max_pages, (long long)b->table_stride);
+    P.table = b->block_table;
+    P.q_start = b->q_start;
+    P.kv_len = b->kv_len;
+    P.table_stride = b->table_stride;
     P.n_seqs = b->n_seqs;
     P.max_pages = b->max_pages;
     P.n_rows = b->n_rows;
@@ -400,7 +444,8 @@ HC_EXPORT int hc_paged_append_dev(const hc_paged_kv* kv, const hc_paged_batch* b
                                   int rot_dim, int half_pairs, void* stream) {
     const char* who = "hc_paged_append_dev";
     hc::AppendArgs A;
-    HC_TRY(paged_args(who, kv, batch, A.p));
+    hc::PagedScales C;
+    HC_TRY(paged_args(who, kv, batch, A.p, C));
     HC_CHECK(dtype == HC_DTYPE_FP32 || dtype == HC_DTYPE_FP16, HC_ERR_UNSUPPORTED, "%s: dtype %u", who, dtype);
     HC_CHECK(n_heads >= 0, HC_ERR_INVALID, "%s: n_heads %d", who, n_heads);
     HC_CHECK(half_pairs == 0 || half_pairs == 1, HC_ERR_INVALID, "%s: half_pairs %d", who, half_pairs);
@@ -439,14 +484,24 @@ HC_EXPORT int hc_paged_append_dev(const hc_paged_kv* kv, const hc_paged_batch* b
     A.halves = half_pairs;
     A.nh = q->data ? n_heads : 0;
     cudaStream_t s = (cudaStream_t)stream;
+    if (kv->kv_dtype == HC_KV_Q4) return hc::launch_append_q4(A, C, dtype == HC_DTYPE_FP16, s);
     if (dtype == HC_DTYPE_FP16)
         return kv->kv_dtype == HC_KV_FP16 ? launch_append<__half, __half>(A, s) : launch_append<__half, float>(A, s);
     return kv->kv_dtype == HC_KV_FP16 ? launch_append<float, __half>(A, s) : launch_append<float, float>(A, s);
 }
 
-static int attn_checks(const char* who, const hc_paged_kv* kv, const hc_paged_batch* batch, int n_heads, uint32_t dtype,
-                       int window, hc::PagedAttnArgs& A) {
-    HC_TRY(paged_args(who, kv, batch, A.p));
+namespace {
+
+struct AttnCall {
+    hc::PagedAttnArgs a;
+    hc::PagedScales c;
+    hc::PagedList l;
+};
+
+int attn_checks(const char* who, const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_page_lists* lists, int n_heads,
+                uint32_t dtype, int window, AttnCall& X) {
+    hc::PagedAttnArgs& A = X.a;
+    HC_TRY(paged_args(who, kv, batch, A.p, X.c));
     HC_CHECK(dtype == HC_DTYPE_FP32 || dtype == HC_DTYPE_FP16, HC_ERR_UNSUPPORTED, "%s: dtype %u", who, dtype);
     HC_CHECK(A.p.hd <= 256, HC_ERR_UNSUPPORTED, "%s: head_dim %d (at most 256)", who, A.p.hd);
     HC_CHECK(n_heads >= 1 && n_heads % A.p.nkv == 0, HC_ERR_INVALID, "%s: %d query heads over %d KV heads", who, n_heads,
@@ -458,23 +513,56 @@ static int attn_checks(const char* who, const hc_paged_kv* kv, const hc_paged_ba
     for (int i = 0; i < 31; i++)
         if (A.G == (1 << i)) A.g_shift = i;
     A.window = window;
+    X.l = {};
+    if (lists) {
+        HC_CHECK(lists->width >= 1 && (lists->pages || batch->n_rows == 0), HC_ERR_INVALID, "%s: NULL or empty lists of pages", who);
+        HC_CHECK(lists->row_stride >= 0 && lists->head_stride >= 0 && (uintptr_t)lists->pages % 4 == 0, HC_ERR_INVALID,
+                 "%s: negative stride of, or misaligned lists of pages", who);
+        X.l = {lists->pages, lists->row_stride, lists->head_stride, lists->width};
+    }
     return HC_OK;
 }
 
-namespace {
 // Which kernel takes a call, by its row tiles at most.  Few (single tokens; up to
-// 16 packed rows of one sequence): the split kernel, which reads the keys once
-// for 8 or 16 rows.  More, over an FP16 cache: the 256-row tiles of the tcgen05
-// kernel; over an FP32 one: the split kernel still.  Unaligned or odd heads
-// take the kernel for any shape.
+// 16 packed rows of one sequence), or rows with lists of pages: the split kernel,
+// which reads the keys once for 8 or 16 rows.  More, over an FP16 cache: the
+// 256-row tiles of the tcgen05 kernel; over an FP32 one: the split kernel still;
+// over one in 4 bits: the pages' values as float16 (exactly) in the workspace, and
+// the tcgen05 kernel over those.  Unaligned or odd heads take the kernel for
+// any shape.
 enum AttnKernel { ATTN_ANY, ATTN_SPLIT, ATTN_TC };
 struct AttnPlan {
     AttnKernel kernel;
-    size_t bytes;
+    size_t bytes;      // of the workspace
+    int at_once;       // 4 bits, ATTN_TC: sequences whose values the workspace holds
+    size_t values, of_k;  // bytes of their values and page numbers, of the keys'
 };
-AttnPlan attn_plan(const hc::PagedAttnArgs& A, const hc_paged_batch* b, int c16) {
-    AttnPlan plan = {ATTN_ANY, 0};
-    if (!hc::paged_split_ok(A.p, c16)) return plan;
+
+// The batch of up to n of its sequences from b on, over the values of their pages.
+hc::PagedAttnArgs over_values(const hc::PagedAttnArgs& A, int b, int n, void* ws, const AttnPlan& plan) {
+    hc::PagedAttnArgs B = A;
+    hc::PagedArgs& P = B.p;
+    P.n_seqs = std::min(n, A.p.n_seqs - b);
+    P.q_start = A.p.q_start ? A.p.q_start + b : nullptr;
+    P.kv_len = A.p.kv_len ? A.p.kv_len + b : nullptr;
+    P.k = ws;
+    P.v = (uint8_t*)ws + plan.of_k;
+    P.n_pages = P.n_seqs * P.max_pages;
+    P.kss = P.vss = P.hd;
+    P.khs = P.vhs = (int64_t)P.hd * P.page_size;
+    P.kps = P.vps = P.khs * P.nkv;
+    P.table = (const int32_t*)((uint8_t*)ws + 2 * plan.of_k);
+    P.table_stride = P.max_pages;
+    return B;
+}
+constexpr size_t VALUES_AT_ONCE = (size_t)1 << 30;
+
+size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
+
+AttnPlan attn_plan(const AttnCall& X, const hc_paged_batch* b, int kv) {
+    const hc::PagedAttnArgs& A = X.a;
+    AttnPlan plan = {ATTN_ANY, 0, 0, 0, 0};
+    if (!hc::paged_split_ok(A.p, kv)) return plan;
     // Few rows: the split kernel, a sequence's rows in tiles of 16.  Many: tcgen05, in
     // tiles of 256, which take up to twice as long each, so from about twice as
     // many small tiles on.  (32 sequences of 4,096 keys, 32 heads over 8 of 128, us,
@@ -482,32 +570,36 @@ AttnPlan attn_plan(const hc::PagedAttnArgs& A, const hc_paged_batch* b, int c16)
     // tokens 207 / 147, 227 / 226; 32 tokens 702 / 148, 817 / 234.  One sequence
     // of 6 tokens: 26 / 19, 25 / 25.)
     const int64_t few = hc::paged_tiles(A, b->max_q_len, 16), many = hc::paged_tiles(A, b->max_q_len, 256);
-    if (2 * few > 3 * many && hc::paged_tc_ok(A, c16)) {
-        plan.kernel = ATTN_TC;
-        plan.bytes = hc::paged_tc_bytes(A, b->max_q_len, b->max_kv_len);
-    } else {
-        plan.kernel = ATTN_SPLIT;
-        plan.bytes = hc::paged_split_bytes(A, b->max_q_len, b->max_kv_len);
+    if (!X.l.width && 2 * few > 3 * many) {
+        if (kv == HC_KV_Q4 && A.p.max_pages > 0) {
+            // (sized by the table, not by the host's bound of the lengths, which chooses no results)
+            const size_t page = (size_t)A.p.page_size * A.p.nkv * A.p.hd * 2, each = page * A.p.max_pages;
+            plan.at_once = (int)std::min<size_t>(A.p.n_seqs, std::max<size_t>(1, VALUES_AT_ONCE / (2 * each)));
+            plan.of_k = aligned(each * plan.at_once);
+            plan.values = 2 * plan.of_k + aligned((size_t)4 * plan.at_once * A.p.max_pages);
+            const hc::PagedAttnArgs B = over_values(A, 0, plan.at_once, nullptr, plan);
+            if ((int64_t)plan.at_once * A.p.max_pages <= INT_MAX && hc::paged_tc_ok(B, 1)) {
+                plan.kernel = ATTN_TC;
+                plan.bytes = plan.values + hc::paged_tc_bytes(B, b->max_q_len, b->max_kv_len);
+                return plan;
+            }
+        } else if (hc::paged_tc_ok(A, kv == HC_KV_FP16)) {
+            plan.kernel = ATTN_TC;
+            plan.bytes = hc::paged_tc_bytes(A, b->max_q_len, b->max_kv_len);
+            return plan;
+        }
     }
+    plan.kernel = ATTN_SPLIT;
+    plan.bytes = hc::paged_split_bytes(A, X.l, b->max_q_len, b->max_kv_len);
     return plan;
 }
-}  // namespace
 
-HC_EXPORT int hc_paged_attention_workspace(const hc_paged_kv* kv, const hc_paged_batch* batch, int n_heads,
-                                           uint32_t dtype, int window, size_t* bytes) {
-    hc::PagedAttnArgs A;
-    HC_CHECK(bytes, HC_ERR_INVALID, "hc_paged_attention_workspace: NULL bytes");
-    HC_TRY(attn_checks("hc_paged_attention_workspace", kv, batch, n_heads, dtype, window, A));
-    *bytes = batch->n_rows == 0 ? 0 : attn_plan(A, batch, kv->kv_dtype == HC_KV_FP16).bytes;
-    return HC_OK;
-}
-
-HC_EXPORT int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_rows* q,
-                                     const hc_rows* out, float* lse, int n_heads, uint32_t dtype, float scale, int window, void* workspace,
-                                     size_t workspace_bytes, void* stream) {
-    const char* who = "hc_paged_attention_dev";
-    hc::PagedAttnArgs A;
-    HC_TRY(attn_checks(who, kv, batch, n_heads, dtype, window, A));
+int attention(const char* who, const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_page_lists* lists, const hc_rows* q,
+              const hc_rows* out, float* lse, int n_heads, uint32_t dtype, float scale, int window, void* workspace,
+              size_t workspace_bytes, cudaStream_t stream) {
+    AttnCall X;
+    hc::PagedAttnArgs& A = X.a;
+    HC_TRY(attn_checks(who, kv, batch, lists, n_heads, dtype, window, X));
     if (batch->n_rows == 0) return HC_OK;
     HC_TRY(rows_ok(who, "q", q, dtype));
     HC_TRY(rows_ok(who, "out", out, dtype));
@@ -519,22 +611,92 @@ HC_EXPORT int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch
     A.o_hs = out->head_stride;
     A.lse = lse;
     A.scale = scale;
-    const int q16 = dtype == HC_DTYPE_FP16, c16 = kv->kv_dtype == HC_KV_FP16;
+    const int q16 = dtype == HC_DTYPE_FP16, type = kv->kv_dtype;
     const int64_t e = q16 ? 8 : 4;
     A.qvec = (uintptr_t)q->data % 16 == 0 && (q->row_stride | q->head_stride) % e == 0;
     A.ovec = (uintptr_t)out->data % 16 == 0 && (out->row_stride | out->head_stride) % e == 0;
-    AttnPlan plan = attn_plan(A, batch, c16);
+    AttnPlan plan = attn_plan(X, batch, type);
     HC_CHECK(workspace_bytes >= plan.bytes && (plan.bytes == 0 || (workspace && (uintptr_t)workspace % 16 == 0)),
              HC_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, plan.bytes,
              workspace_bytes);
     // the tcgen05 kernel takes row maxima before it applies the scale; the
-    // workspace does not know the scale, so another one goes to the kernel without one
-    if (plan.kernel == ATTN_TC && !(scale > 0.0f)) plan.kernel = ATTN_ANY;
-    if (plan.kernel == ATTN_TC)
-        return hc::launch_paged_tc(A, q16, batch->max_q_len, batch->max_kv_len, workspace, (cudaStream_t)stream);
-    if (plan.kernel == ATTN_SPLIT) return hc::launch_paged_split(A, q16, c16, batch->max_q_len, batch->max_kv_len, workspace, (cudaStream_t)stream);
-    return hc::launch_paged_generic(A, q16, c16, (cudaStream_t)stream);
+    // workspace does not know the scale, so another one goes to a kernel without one
+    // (over 4 bits: one CTA of the split kernel per pair, which needs none)
+    if (plan.kernel == ATTN_TC && !(scale > 0.0f)) {
+        if (type == HC_KV_Q4) return hc::launch_paged_split(A, X.c, X.l, q16, type, batch->max_q_len, 0, nullptr, stream);
+        plan.kernel = ATTN_ANY;
+    }
+    if (plan.kernel == ATTN_TC && type == HC_KV_Q4) {
+        for (int b = 0; b < A.p.n_seqs; b += plan.at_once) {
+            const hc::PagedAttnArgs B = over_values(A, b, plan.at_once, workspace, plan);
+            hc::PagedArgs from = A.p;
+            from.n_seqs = B.p.n_seqs;
+            from.kv_len = B.p.kv_len;
+            from.table = A.p.table + b * A.p.table_stride;
+            HC_TRY(hc::launch_q4_values(from, X.c, true, (__half*)B.p.k, (__half*)B.p.v, (int32_t*)B.p.table, stream));
+            HC_TRY(hc::launch_paged_tc(B, q16, batch->max_q_len, batch->max_kv_len, (uint8_t*)workspace + plan.values, stream));
+        }
+        return HC_OK;
+    }
+    if (plan.kernel == ATTN_TC) return hc::launch_paged_tc(A, q16, batch->max_q_len, batch->max_kv_len, workspace, stream);
+    if (plan.kernel == ATTN_SPLIT)
+        return hc::launch_paged_split(A, X.c, X.l, q16, type, batch->max_q_len, batch->max_kv_len, workspace, stream);
+    return hc::launch_paged_generic(A, X.l, q16, type == HC_KV_FP16, stream);
 }
+
+int attention_workspace(const char* who, const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_page_lists* lists, int n_heads,
+                        uint32_t dtype, int window, size_t* bytes) {
+    AttnCall X;
+    HC_CHECK(bytes, HC_ERR_INVALID, "%s: NULL bytes", who);
+    HC_TRY(attn_checks(who, kv, batch, lists, n_heads, dtype, window, X));
+    *bytes = batch->n_rows == 0 ? 0 : attn_plan(X, batch, kv->kv_dtype).bytes;
+    return HC_OK;
+}
+
+}  // namespace
+
+HC_EXPORT int hc_paged_attention_workspace(const hc_paged_kv* kv, const hc_paged_batch* batch, int n_heads,
+                                           uint32_t dtype, int window, size_t* bytes) {
+    return attention_workspace("hc_paged_attention_workspace", kv, batch, nullptr, n_heads, dtype, window, bytes);
+}
+
+HC_EXPORT int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_rows* q,
+                                     const hc_rows* out, float* lse, int n_heads, uint32_t dtype, float scale, int window, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+    return attention("hc_paged_attention_dev", kv, batch, nullptr, q, out, lse, n_heads, dtype, scale, window, workspace, workspace_bytes,
+                     (cudaStream_t)stream);
+}
+
+HC_EXPORT int hc_paged_list_attention_workspace(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_page_lists* lists,
+                                                int n_heads, uint32_t dtype, int window, size_t* bytes) {
+    const char* who = "hc_paged_list_attention_workspace";
+    HC_CHECK(lists, HC_ERR_INVALID, "%s: NULL or empty lists of pages", who);
+    return attention_workspace(who, kv, batch, lists, n_heads, dtype, window, bytes);
+}
+
+HC_EXPORT int hc_paged_list_attention_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_page_lists* lists,
+                                          const hc_rows* q, const hc_rows* out, float* lse, int n_heads, uint32_t dtype, float scale,
+                                          int window, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "hc_paged_list_attention_dev";
+    HC_CHECK(lists, HC_ERR_INVALID, "%s: NULL or empty lists of pages", who);
+    return attention(who, kv, batch, lists, q, out, lse, n_heads, dtype, scale, window, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+HC_EXPORT int hc_paged_values_dev(const hc_paged_kv* kv, void* k_out, void* v_out, void* stream) {
+    const char* who = "hc_paged_values_dev";
+    hc::PagedArgs P = {};
+    hc::PagedScales C;
+    HC_TRY(pool_args(who, kv, P, C));
+    HC_CHECK(kv->kv_dtype == HC_KV_Q4, HC_ERR_UNSUPPORTED, "%s: kv_dtype %d", who, kv->kv_dtype);
+    HC_CHECK(k_out && v_out && ((uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0, HC_ERR_INVALID, "%s: NULL or misaligned output", who);
+    return hc::launch_q4_values(P, C, false, (__half*)k_out, (__half*)v_out, nullptr, (cudaStream_t)stream);
+}
+
+// What hc_page_select.cu's entry points take of these checks.
+int hc::page_args(const char* who, const hc_paged_kv* kv, const hc_paged_batch* batch, hc::PagedArgs& P, hc::PagedScales& C) {
+    return paged_args(who, kv, batch, P, C);
+}
+int hc::page_rows_ok(const char* who, const char* what, const hc_rows* r, uint32_t dtype) { return rows_ok(who, what, r, dtype); }
 
 HC_EXPORT int hc_rope_table_host(size_t rows, size_t head_dim, float theta, float* out) {
     HC_CHECK(out || rows == 0 || head_dim == 0, HC_ERR_INVALID, "hc_rope_table_host: NULL out");

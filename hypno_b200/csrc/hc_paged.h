@@ -25,6 +25,24 @@ struct PagedArgs {
     int reach;  // positions that a row of the table can name: what lies past them are holes, and not visited
 };
 
+// The scales of a pool in 4 bits (its k and v are bytes of two codes, their
+// strides too); strides in scales.
+struct PagedScales {
+    __half* k;
+    __half* v;
+    int64_t kps, khs, kss;
+    int64_t vps, vhs, vss;
+};
+
+// The pages that each row reads, per KV head: indexes into its sequence's row of
+// the block table, in ascending order.  A list ends before the first entry that
+// is not above the one in front of it (so -1 ends it).
+struct PagedList {
+    const int32_t* pages;
+    int64_t row_stride, head_stride;
+    int width;  // entries of a list, at most; 0: no lists, a row reads all that it sees
+};
+
 struct PagedAttnArgs {
     PagedArgs p;
     const void* q;
@@ -63,6 +81,70 @@ __device__ __forceinline__ void seq_rows(const PagedArgs& P, int b, int& r0, int
 
 // Positions of sequence b (a negative length counts as none).
 __device__ __forceinline__ int seq_len(const PagedArgs& P, int b) { return max(__ldg(P.kv_len + b), 0); }
+
+// Entries of the list of (row, KV head); a whole warp.
+__device__ __forceinline__ int list_count(const PagedList& L, int row, int kvh) {
+    const int lane = threadIdx.x & 31;
+    const int32_t* e = L.pages + row * L.row_stride + kvh * L.head_stride;
+    for (int i0 = 0; i0 < L.width; i0 += 32) {
+        const int i = i0 + lane;
+        const int here = i < L.width ? __ldg(e + i) : -1, before = i > 0 && i < L.width ? __ldg(e + i - 1) : -1;
+        const unsigned end = __ballot_sync(0xffffffffu, here <= before);
+        if (end) return i0 + __ffs(end) - 1;
+    }
+    return L.width;
+}
+
+// Pages of its block table that a row at position p sees.
+__device__ __forceinline__ int pages_seen(const PagedArgs& P, int p) {
+    return p < 0 ? 0 : min(page_of(P, p) + 1, P.max_pages);
+}
+
+// Page and slot of place v of a list, -1 where the row does not see it.
+__device__ __forceinline__ int lookup_listed(const PagedAttnArgs& A, const int32_t* list, int seq, int v, int p, int& slot) {
+    const PagedArgs& P = A.p;
+    const int i = page_of(P, v);
+    slot = v - i * P.page_size;
+    const int e = __ldg(list + i);
+    if (e >= P.max_pages) return -1;
+    const int64_t pos = (int64_t)e * P.page_size + slot;
+    if (pos > p || (A.window > 0 && pos <= (int64_t)p - A.window)) return -1;
+    const int g = __ldg(P.table + (int64_t)seq * P.table_stride + e);
+    return (unsigned)g < (unsigned)P.n_pages ? g : -1;
+}
+
+// ---- 4 bits: 32 elements of a head share a scale s, a float16 of seven
+// significant bits at most (so that c s, |c| <= 8, and 72 s are float16 values
+// too), an element is the nibble c + 8, element 2 i in the low half of byte i.
+constexpr float Q4_TOP = 896.0f;  // the largest scale: 72 s stays below 65,504
+
+// The scale of 32 elements from the bits of their largest magnitude.
+__device__ __forceinline__ float q4_scale(uint32_t top) {
+    if (top >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
+    const float t = __fdiv_rn(__uint_as_float(top), 7.0f);
+    const float s = __uint_as_float((__float_as_uint(t) + 0x1FFFFu) & ~0x1FFFFu);
+    return fminf(ceilf(s * 16777216.0f) * 0x1p-24f, Q4_TOP);
+}
+__device__ __forceinline__ uint32_t q4_code(float x, float s) {
+    if (!(s > 0.0f)) return 8;  // zeros, and a block that holds a value that is not finite
+    return (uint32_t)((int)fminf(fmaxf(rintf(__fdiv_rn(x, s)), -7.0f), 7.0f) + 8);
+}
+// A scale's slots of a position: a power of two, so that they are copied at once.
+__host__ __device__ constexpr int q4_slots(int hd) { return hd <= 64 ? 2 : hd <= 128 ? 4 : 8; }
+
+// Nibbles j = 0..3 of each half of x as pairs of float16 values: 0x5400 | nibble
+// << 4 is 64 + c + 8, so (64 + c + 8) s - 72 s is c s, exactly.
+__device__ __forceinline__ void q4_pairs(uint32_t x, __half2 s, __half2 s72, uint32_t* out) {
+    const uint32_t n[4] = {x << 4, x, x >> 4, x >> 8};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t b = (n[j] & 0x00F000F0u) | 0x54005400u;
+        const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&b), s, s72);
+        out[j] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+
+struct q4x {};  // the element type of a pool in 4 bits, for the kernels' templates
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
@@ -171,15 +253,36 @@ bool paged_tc_ok(const PagedAttnArgs& A, int c16);
 size_t paged_tc_bytes(const PagedAttnArgs& A, int max_q_len, int max_kv_len);  // workspace
 int launch_paged_tc(const PagedAttnArgs& A, int q16, int max_q_len, int max_kv_len, void* ws, cudaStream_t s);
 
-// Few rows per sequence (hc_paged_split.cu): the keys split over CTAs.
-bool paged_split_ok(const PagedArgs& P, int c16);
-bool paged_split_whole(const PagedAttnArgs& A, int max_q_len, int max_kv_len);
-size_t paged_split_bytes(const PagedAttnArgs& A, int max_q_len, int max_kv_len);  // workspace
-int launch_paged_split(const PagedAttnArgs& A, int q16, int c16, int max_q_len, int max_kv_len, void* ws,
-                       cudaStream_t s);
+// Few rows per sequence, or rows with lists of pages (hc_paged_split.cuh): the keys
+// split over CTAs.  kv: HC_KV_FP32, HC_KV_FP16 or HC_KV_Q4 (with its scales).
+bool paged_split_ok(const PagedArgs& P, int kv);
+bool paged_split_whole(const PagedAttnArgs& A, const PagedList& L, int max_q_len, int max_kv_len);
+size_t paged_split_bytes(const PagedAttnArgs& A, const PagedList& L, int max_q_len, int max_kv_len);  // workspace
+int launch_paged_split(const PagedAttnArgs& A, const PagedScales& C, const PagedList& L, int q16, int kv, int max_q_len,
+                       int max_kv_len, void* ws, cudaStream_t s);
 
 // Any shape (hc_paged.cu).
-int launch_paged_generic(const PagedAttnArgs& A, int q16, int c16, cudaStream_t s);
+int launch_paged_generic(const PagedAttnArgs& A, const PagedList& L, int q16, int c16, cudaStream_t s);
+
+// A pool in 4 bits (hc_paged_q4.cu): append, and the float16 values of pages.
+struct AppendArgs {
+    PagedArgs p;
+    const void *k, *v, *q;
+    void* qo;
+    int64_t k_rs, k_hs, v_rs, v_hs, q_rs, q_hs, o_rs, o_hs;
+    const float2* rope;
+    int rope_rows, rot, halves;
+    int nh;  // 0: no queries
+};
+int launch_append_q4(const AppendArgs& A, const PagedScales& C, int x16, cudaStream_t s);
+
+// The C entry points' checks of a pool and a batch, and of rows.
+int page_args(const char* who, const hc_paged_kv* kv, const hc_paged_batch* batch, PagedArgs& P, PagedScales& C);
+int page_rows_ok(const char* who, const char* what, const hc_rows* r, uint32_t dtype);
+// Every page of the pool, or (a table) page i of the batch's sequence b to page
+// b max_pages + i, its number to `numbers`.
+int launch_q4_values(const PagedArgs& P, const PagedScales& C, bool of_batch, __half* k, __half* v, int32_t* numbers,
+                     cudaStream_t s);
 
 // The results of a row's n runs of keys as one: with M = max m_s,
 // l = sum 2^(m_s - M) l_s, o = sum 2^(m_s - M) o_s, four columns from d on, in the

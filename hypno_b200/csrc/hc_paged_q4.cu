@@ -1,0 +1,265 @@
+// A paged cache in 4 bits: append with rotation, and the values of its pages.
+#include "hc_paged.h"
+
+namespace hc {
+
+namespace {
+
+constexpr int Q4_THREADS = 256;
+
+__device__ __forceinline__ int seq_of_row(const PagedArgs& P, int r) {
+    int lo = 0, hi = P.n_seqs - 1;  // the last sequence whose first row is <= r
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (__ldg(P.q_start + mid) <= r) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool vec, float* x) {
+    if (!vec) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = to_f32(p[i]);
+        return;
+    }
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool vec, const float* x) {
+    if (!vec) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[i] = from_f32<T>(x[i]);
+        return;
+    }
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack(x[0], x[1]), pack(x[2], x[3]), pack(x[4], x[5]), pack(x[6], x[7]));
+    }
+}
+
+// Eight elements of a head a thread; the four threads of 32 elements find their
+// largest magnitude together.  The turned pairs are separately rounded products
+// (a c - b s, not contracted), so that a value at the border of two codes falls
+// the same way whatever kernel or host code computes it; q and k by the same
+// code.  A head's elements are read by the threads that need them: with half
+// pairs twice, from L1.
+//
+// q may be turned in place: the eight elements of a pair's other run are read by
+// another thread too, so in-place queries with half pairs take one thread for
+// both runs (`both`).
+template <typename T, bool HALVES>
+__device__ __forceinline__ void turned(const T* src, int i0, int rot, bool vec, const float2* cs, float* x) {
+    load8(src + i0, vec, x);
+    if (i0 >= rot) return;
+    if constexpr (HALVES) {
+        const int half = rot >> 1;
+        float y[8];
+        if (half % 8 == 0) {
+            load8(src + (i0 < half ? i0 + half : i0 - half), vec, y);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int d = i0 + i;
+                y[i] = d < rot ? to_f32(src[d < half ? d + half : d - half]) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int d = i0 + i;
+            if (d >= rot) break;
+            const float2 t = __ldg(cs + (d < half ? d : d - half));
+            x[i] = d < half ? __fsub_rn(__fmul_rn(x[i], t.x), __fmul_rn(y[i], t.y))
+                            : __fadd_rn(__fmul_rn(y[i], t.y), __fmul_rn(x[i], t.x));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (i0 + 2 * i >= rot) break;
+            const float2 t = __ldg(cs + (i0 >> 1) + i);
+            const float a = x[2 * i], b = x[2 * i + 1];
+            x[2 * i] = __fsub_rn(__fmul_rn(a, t.x), __fmul_rn(b, t.y));
+            x[2 * i + 1] = __fadd_rn(__fmul_rn(a, t.y), __fmul_rn(b, t.x));
+        }
+    }
+}
+
+template <typename T, bool HALVES>
+__global__ void __launch_bounds__(Q4_THREADS) k_q4_append(AppendArgs A, PagedScales C, int vec) {
+    const PagedArgs& P = A.p;
+    const int row = blockIdx.x, hu = P.hd >> 3;
+    const int unit = blockIdx.y * Q4_THREADS + threadIdx.x;
+    if (unit >= (A.nh + 2 * P.nkv) * hu) return;  // (the four threads of a block of 32 leave together)
+    int head = unit / hu;
+    const int i0 = 8 * (unit - head * hu);
+    const int seq = seq_of_row(P, row);
+    int r0, r1;
+    seq_rows(P, seq, r0, r1);
+    if (row < r0 || row >= r1) return;
+    const int pos = seq_len(P, seq) - (r1 - r0) + (row - r0);
+    const float2* cs = A.rot ? A.rope + (int64_t)min(max(pos, 0), A.rope_rows - 1) * (A.rot >> 1) : nullptr;
+    float x[8];
+    if (head < A.nh) {
+        const T* src = (const T*)A.q + row * A.q_rs + head * A.q_hs;
+        T* dst = (T*)A.qo + row * A.o_rs + head * A.o_hs;
+        if constexpr (HALVES) {
+            // the thread of a pair's first element turns both: q_out may be q
+            const int half = A.rot >> 1;
+            if (i0 >= half) {
+                // elements past the pairs pass through; the second runs are the others' work
+                if (i0 + 8 <= A.rot) return;
+                load8(src + i0, vec, x);
+                if (i0 >= A.rot) {
+                    store8(dst + i0, vec, x);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        if (i0 + i >= A.rot) dst[i0 + i] = from_f32<T>(x[i]);
+                }
+                return;
+            }
+            float y[8];
+            const bool even = half % 8 == 0;
+            load8(src + i0, vec, x);
+            if (even) {
+                load8(src + i0 + half, vec, y);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) y[i] = i0 + i < half ? to_f32(src[i0 + i + half]) : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if (i0 + i >= half) break;
+                const float2 t = __ldg(cs + i0 + i);
+                const float a = x[i], b = y[i];
+                x[i] = __fsub_rn(__fmul_rn(a, t.x), __fmul_rn(b, t.y));
+                y[i] = __fadd_rn(__fmul_rn(a, t.y), __fmul_rn(b, t.x));
+            }
+            if (even) {
+                store8(dst + i0, vec, x);
+                store8(dst + i0 + half, vec, y);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (i0 + i < half) {
+                        dst[i0 + i] = from_f32<T>(x[i]);
+                        dst[i0 + i + half] = from_f32<T>(y[i]);
+                    } else if (i0 + i >= A.rot) {
+                        dst[i0 + i] = from_f32<T>(x[i]);  // (a run of eight may hold all pairs and more)
+                    }
+                }
+            }
+        } else {
+            turned<T, false>(src, i0, A.rot, vec, cs, x);
+            store8(dst + i0, vec, x);
+        }
+        return;
+    }
+    const bool is_v = head >= A.nh + P.nkv;
+    head -= is_v ? A.nh + P.nkv : A.nh;
+    if (is_v) load8((const T*)A.v + row * A.v_rs + head * A.v_hs + i0, vec, x);
+    else turned<T, HALVES>((const T*)A.k + row * A.k_rs + head * A.k_hs, i0, A.rot, vec, cs, x);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    const uint32_t four = 0xFu << (threadIdx.x & 28);
+    top = max(top, __shfl_xor_sync(four, top, 1));
+    top = max(top, __shfl_xor_sync(four, top, 2));
+    if (pos < 0) return;
+    int slot;
+    const int page = lookup(P, seq, pos, slot);
+    if (page < 0) return;
+    const float s = q4_scale(top);
+    uint32_t code = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) code |= q4_code(x[i], s) << (4 * i);
+    uint8_t* dst = is_v ? (uint8_t*)P.v + page * P.vps + head * P.vhs + slot * P.vss : (uint8_t*)P.k + page * P.kps + head * P.khs + slot * P.kss;
+    *reinterpret_cast<uint32_t*>(dst + (i0 >> 1)) = code;
+    if ((i0 & 31) == 0) {
+        __half* sc = is_v ? C.v + page * C.vps + head * C.vhs + slot * C.vss : C.k + page * C.kps + head * C.khs + slot * C.kss;
+        sc[i0 >> 5] = __float2half_rn(s);  // exact
+    }
+}
+
+// Values as float16, exactly: eight elements of K and of V a thread, positions of
+// a page side by side in both layouts.  Bound by its writes.
+__global__ void __launch_bounds__(Q4_THREADS) k_q4_values(PagedArgs P, PagedScales C, int of_batch, __half* k, __half* v,
+                                                          int32_t* numbers) {
+    const int hu = P.hd >> 3;
+    int64_t page = blockIdx.x;
+    int src = blockIdx.x;
+    if (of_batch) {
+        const int b = blockIdx.z;
+        page += (int64_t)b * P.max_pages;
+        src = __ldg(P.table + (int64_t)b * P.table_stride + blockIdx.x);
+        const int64_t begin = (int64_t)blockIdx.x * P.page_size;
+        if ((unsigned)src >= (unsigned)P.n_pages || begin >= seq_len(P, b)) src = -1;
+        if (blockIdx.y == 0 && threadIdx.x == 0) numbers[page] = src < 0 ? -1 : (int32_t)page;
+        if (src < 0) return;
+    }
+    const int units = P.nkv * P.page_size * hu;
+    const int unit = blockIdx.y * Q4_THREADS + threadIdx.x;
+    if (unit >= units) return;
+    const int u = unit % hu, at = unit / hu, slot = at % P.page_size, head = at / P.page_size;
+    const int64_t kb = src * P.kps + head * P.khs + slot * P.kss + 4 * u, vb = src * P.vps + head * P.vhs + slot * P.vss + 4 * u;
+    const uint32_t kw = __ldg(reinterpret_cast<const uint32_t*>((const uint8_t*)P.k + kb));
+    const uint32_t vw = __ldg(reinterpret_cast<const uint32_t*>((const uint8_t*)P.v + vb));
+    const __half ks = C.k[src * C.kps + head * C.khs + slot * C.kss + (u >> 2)];
+    const __half vs = C.v[src * C.vps + head * C.vhs + slot * C.vss + (u >> 2)];
+    const int64_t to = (page * P.nkv * P.page_size + at) * P.hd + 8 * u;
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const __half2 s = __half2half2(x ? vs : ks), z = __hmul2(s, __half2half2(__float2half_rn(-72.0f)));
+        uint32_t e[4];
+        q4_pairs(x ? vw : kw, s, z, e);  // (0, 4), (1, 5), (2, 6), (3, 7)
+        *reinterpret_cast<uint4*>((x ? v : k) + to) = make_uint4(__byte_perm(e[0], e[1], 0x5410), __byte_perm(e[2], e[3], 0x5410),
+                                                                __byte_perm(e[0], e[1], 0x7632), __byte_perm(e[2], e[3], 0x7632));
+    }
+}
+
+template <typename T>
+int launch_append_t(const AppendArgs& A, const PagedScales& C, cudaStream_t s) {
+    const PagedArgs& P = A.p;
+    const int64_t et = 16 / (int64_t)sizeof(T);
+    const int vec = ((uintptr_t)A.k | (uintptr_t)A.v | (uintptr_t)A.q | (uintptr_t)A.qo) % 16 == 0 &&
+                    (A.k_rs | A.k_hs | A.v_rs | A.v_hs | (A.nh ? A.q_rs | A.q_hs | A.o_rs | A.o_hs : 0)) % et == 0;
+    const int64_t units = (int64_t)(A.nh + 2 * P.nkv) * (P.hd / 8);
+    HC_CHECK(units <= 65535ll * Q4_THREADS, HC_ERR_INVALID, "hc_paged_append_dev: %d + %d heads of %d", A.nh, P.nkv, P.hd);
+    const dim3 grid((unsigned)P.n_rows, (unsigned)((units + Q4_THREADS - 1) / Q4_THREADS));
+    if (A.halves) k_q4_append<T, true><<<grid, Q4_THREADS, 0, s>>>(A, C, vec);
+    else k_q4_append<T, false><<<grid, Q4_THREADS, 0, s>>>(A, C, vec);
+    HC_LAUNCH_CHECK();
+    return HC_OK;
+}
+
+}  // namespace
+
+int launch_append_q4(const AppendArgs& A, const PagedScales& C, int x16, cudaStream_t s) {
+    return x16 ? launch_append_t<__half>(A, C, s) : launch_append_t<float>(A, C, s);
+}
+
+int launch_q4_values(const PagedArgs& P, const PagedScales& C, bool of_batch, __half* k, __half* v, int32_t* numbers, cudaStream_t s) {
+    const int64_t units = (int64_t)P.nkv * P.page_size * (P.hd / 8), y = (units + Q4_THREADS - 1) / Q4_THREADS;
+    HC_CHECK(y <= 65535 && (!of_batch || P.n_seqs <= 65535), HC_ERR_INVALID, "pages of %d positions of %d heads, %d sequences", P.page_size, P.nkv, P.n_seqs);
+    const dim3 grid((unsigned)(of_batch ? P.max_pages : P.n_pages), (unsigned)y, of_batch ? (unsigned)P.n_seqs : 1u);
+    if (grid.x == 0) return HC_OK;
+    k_q4_values<<<grid, Q4_THREADS, 0, s>>>(P, C, of_batch, k, v, numbers);
+    HC_LAUNCH_CHECK();
+    return HC_OK;
+}
+
+}  // namespace hc

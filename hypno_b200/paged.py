@@ -3,9 +3,14 @@ tokens over the pages.
 
     PagedKV             one layer's pool of pages (any strides), the handle a
                         program keeps with it
+    PagedKV4            the same in 4 bits: codes and a scale for each 32 elements
     PagedBatch          one step's packed rows: block table, row starts, lengths
     append              rotated keys (and queries), values -> pages
-    attention           softmax attention of the rows over their pages
+    attention           softmax attention of the rows over their pages, or over the
+                        pages that each row's list names
+    PageBounds          bounds of each page's keys, kept beside a pool
+    update_bounds       makes them anew for the pages that a step wrote to
+    select_pages        the pages that each row is to read, by a score from the bounds
     rope_table          the model's cos/sin table on the device
     PageTable           host-side owner of pages: sequences grow and are released
 
@@ -16,11 +21,18 @@ prompts and single tokens alike) into rows, appends them, and attends:
     q = append(kv, batch, k, v, q=q, rope=rope)
     out = attention(kv, batch, q)
 
+Long contexts are bound by the bytes of their keys and values: a PagedKV4 holds
+them in 4.5 bits an element, and a step's single tokens need not read them all:
+
+    update_bounds(bounds, kv, batch)
+    out = attention(kv, batch, q, pages=select_pages(bounds, batch, q, budget=64))
+
 The operators run on torch's current stream of the pool's device, whichever
 device is current, and do not synchronize; use `with torch.cuda.stream(...)`
 (or an ExternalStream of HypnoModel.stream) for another one.  Errors raise
-HypnoCudaError, ValueError or TypeError.  They call hc_paged_append_dev and
-hc_paged_attention_dev.
+HypnoCudaError, ValueError or TypeError.  They call hc_paged_append_dev,
+hc_paged_attention_dev, hc_paged_list_attention_dev, hc_page_bounds_update_dev and
+hc_page_select_dev.
 """
 import ctypes
 
@@ -28,9 +40,11 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import (DTYPE_FP16, DTYPE_FP32, HC_PAGED_BATCH, HC_ROWS, KV_FP16, KV_FP32, HcPagedKV, call, check, load, raw_stream)
+from ._lib import (DTYPE_FP16, DTYPE_FP32, HC_PAGE_LISTS, HC_PAGED_BATCH, HC_ROWS, KV_FP16, KV_FP32, KV_Q4, HcPageBounds, HcPagedKV,
+                   HcPagedKV4, call, check, load, raw_stream)
 
-__all__ = ["PagedKV", "PagedBatch", "append", "attention", "rope_table", "PageTable"]
+__all__ = ["PagedKV", "PagedKV4", "PagedBatch", "append", "attention", "PageBounds", "update_bounds", "select_pages", "rope_table",
+           "PageTable"]
 
 _DTYPE = {torch.float32: DTYPE_FP32, torch.float16: DTYPE_FP16}
 _KV = {torch.float32: KV_FP32, torch.float16: KV_FP16}
@@ -71,6 +85,71 @@ class PagedKV:
         """A pool of its own, zeroed."""
         shape = (n_pages, n_kv_heads, page_size, head_dim)
         return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+
+
+def _slots(head_dim):
+    """Scales of a position that are laid out, of which head_dim / 32 are in use."""
+    return 2 if head_dim <= 64 else 4 if head_dim <= 128 else 8
+
+
+class PagedKV4:
+    """One layer's pages in 4 bits.  32 elements of a head share a scale s, a
+    float16 of at most seven significant bits: the least that is not below a
+    seventh of their largest magnitude, 896 at most (values past 6,272 are held
+    as that).  An element is the code c = round(x / s), from -7 to 7, held as
+    c + 8, and stands for c s; 32 elements of which one is not finite are NaN.
+
+    k_codes and v_codes are [n_pages, n_kv_heads, page_size, head_dim / 2] uint8
+    (element 2 i of a head in the low half of byte i, 2 i + 1 in the high half),
+    k_scales and v_scales [n_pages, n_kv_heads, page_size, slots] float16 with 2, 4
+    or 8 slots for heads of up to 64, 128 or 256 elements, the first head_dim / 32 in
+    use.  The last dimensions are contiguous and begin on multiples of 16 bytes
+    (codes) and of their slots (scales); head_dim is a multiple of 32."""
+
+    __slots__ = ("_pools", "struct", "ref", "device", "index", "n_kv_heads", "head_dim", "page_size", "n_pages")
+
+    def __init__(self, k_codes, k_scales, v_codes, v_scales):
+        pools = (k_codes, k_scales, v_codes, v_scales)
+        for t, name in zip(pools, ("k_codes", "k_scales", "v_codes", "v_scales")):
+            want = torch.float16 if "scales" in name else torch.uint8
+            if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.dtype != want or not t.is_cuda:
+                raise TypeError(f"{name} must be a 4-dimensional {want} CUDA tensor")
+            if t.device != k_codes.device:
+                raise ValueError("codes and scales must be on one device")
+            if t.shape[3] > 1 and t.stride(3) != 1:
+                raise ValueError(f"the last dimension of {name} must be contiguous")
+        dim = 2 * k_codes.shape[3]
+        if dim == 0 or dim % 32 or dim > 256:
+            raise ValueError(f"heads of {dim} elements in 4 bits: a multiple of 32, at most 256")
+        scales = (*k_codes.shape[:3], _slots(dim))
+        if v_codes.shape != k_codes.shape or k_scales.shape != scales or v_scales.shape != scales:
+            raise ValueError(f"codes of shape {tuple(k_codes.shape)} need others alike and scales of shape {scales}")
+        self._pools, self.device, self.index, self.head_dim = pools, k_codes.device, k_codes.device.index, dim
+        self.n_pages, self.n_kv_heads, self.page_size = k_codes.shape[:3]
+        base = HcPagedKV(k_codes.data_ptr(), v_codes.data_ptr(), *k_codes.stride()[:3], *v_codes.stride()[:3], KV_Q4, self.n_pages,
+                         self.page_size, self.n_kv_heads, dim, 0)
+        self.struct = HcPagedKV4(base, k_scales.data_ptr(), v_scales.data_ptr(), *k_scales.stride()[:3], *v_scales.stride()[:3])
+        self.ref = ctypes.addressof(self.struct)
+
+    pools = property(lambda self: self._pools, doc="k_codes, k_scales, v_codes, v_scales.")
+
+    @classmethod
+    def alloc(cls, n_pages, page_size, n_kv_heads, head_dim, device="cuda"):
+        """A pool of its own; its values are zeros."""
+        shape = (n_pages, n_kv_heads, page_size)
+        return cls(*(torch.zeros((*shape, n), dtype=t, device=device)
+                     for n, t in ((head_dim // 2, torch.uint8), (_slots(head_dim), torch.float16)) * 2))
+
+    def values(self):
+        """The keys and values of every page as float16, exactly: two contiguous
+        [n_pages, n_kv_heads, page_size, head_dim] tensors."""
+        if _lib.current_device() != self.index:
+            with _lib.on_device(self.index):
+                return self.values()
+        shape = (self.n_pages, self.n_kv_heads, self.page_size, self.head_dim)
+        k, v = (torch.empty(shape, dtype=torch.float16, device=self.device) for _ in range(2))
+        check(load().hc_paged_values_dev(self.ref, k.data_ptr(), v.data_ptr(), raw_stream(self.index)))
+        return k, v
 
 
 def _int32(t, name, dim, index):
@@ -189,7 +268,7 @@ def append(kv, batch, k, v, q=None, rope=None, pairs="adjacent", q_out=None):
     return q_out
 
 
-def attention(kv, batch, q, out=None, scale=None, window=0, lse=None):
+def attention(kv, batch, q, out=None, scale=None, window=0, lse=None, pages=None):
     """out[r, h] = softmax(scale * q[r, h] . K) V over the positions up to the
     row's own (window > 0: the last `window` of them), scale = head_dim ** -0.5
     by default; query head h reads KV head h // (n_heads // n_kv_heads).  A row
@@ -197,12 +276,19 @@ def attention(kv, batch, q, out=None, scale=None, window=0, lse=None):
     float16, out the same; lse, if given, is a contiguous [n_rows, n_heads]
     float32 tensor for the log of the sums.  The softmax is exact (the
     flat-cache forward passes keep the reference's polynomial).  Scores and sums
-    are float32; float16 queries over a float16 cache round the weights to 11
-    bits for their product with V (an error like the output's own rounding),
-    float32 ones keep 22 bits."""
+    are float32; float16 queries over a float16 or 4-bit cache round the weights
+    to 11 bits for their product with V (an error like the output's own rounding),
+    float32 ones keep 22 bits.
+
+    pages, if given, is an [n_rows, n_kv_heads, width] int32 tensor (select_pages()
+    makes them) of the pages that each row reads: indexes into its sequence's row of
+    the block table, ascending; a list ends before the first entry that is not above
+    the one in front of it, so with -1.  Each row then reads its pages by itself, so
+    this is for single tokens and a few rows a sequence; chunks share what they
+    read better without."""
     if _lib.current_device() != kv.index:
         with _lib.on_device(kv.index):
-            return attention(kv, batch, q, out, scale, window, lse)
+            return attention(kv, batch, q, out, scale, window, lse, pages)
     _same_device(kv, batch)
     dtype = q.dtype
     code = _DTYPE.get(dtype)
@@ -222,11 +308,119 @@ def attention(kv, batch, q, out=None, scale=None, window=0, lse=None):
         lse_ptr = lse.data_ptr()
     lib, ref = load(), batch.pack(n)
     need = ctypes.c_size_t()
+    if pages is not None:
+        if not isinstance(pages, torch.Tensor) or pages.dtype is not torch.int32 or pages.dim() != 3 or pages.get_device() != kv.index:
+            raise TypeError(f"pages must be a 3-dimensional int32 tensor on {kv.device}")
+        if pages.shape[0] != n or pages.shape[1] != kv.n_kv_heads or pages.shape[2] < 1:
+            raise ValueError(f"pages of shape {tuple(pages.shape)} for {n} rows and {kv.n_kv_heads} KV heads")
+        if pages.stride(2) != 1 and pages.shape[2] > 1:
+            raise ValueError("pages must be contiguous along its last dimension")
+        lists = HC_PAGE_LISTS.pack(pages.data_ptr(), pages.stride(0), pages.stride(1), pages.shape[2], 0)
+        check(lib.hc_paged_list_attention_workspace(kv.ref, ref, lists, heads, code, window, ctypes.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=kv.device) if need.value else None
+        check(lib.hc_paged_list_attention_dev(kv.ref, ref, lists, qs, os_, lse_ptr, heads, code, dim ** -0.5 if scale is None else scale,
+                                              window, ws.data_ptr() if ws is not None else None, need.value, raw_stream(kv.index)))
+        return out
     check(lib.hc_paged_attention_workspace(kv.ref, ref, heads, code, window, ctypes.byref(need)))
     # the workspace lives until the stream's later allocations reuse it: torch orders them after this call
     ws = torch.empty(need.value, dtype=torch.uint8, device=kv.device) if need.value else None
     check(lib.hc_paged_attention_dev(kv.ref, ref, qs, os_, lse_ptr, heads, code, dim ** -0.5 if scale is None else scale,
                                      window, ws.data_ptr() if ws is not None else None, need.value, raw_stream(kv.index)))
+    return out
+
+
+class PageBounds:
+    """Bounds of the keys of a pool's pages: the smallest and largest key of each
+    element over a page's filled slots are at least lo s and at most hi s.  lo and hi
+    are contiguous [n_pages, n_kv_heads, head_dim] int8 tensors, scale (s) a
+    contiguous [n_pages, n_kv_heads] float32 one: the least power of two of which
+    the page's largest magnitude is at most 127 (infinite, with lo = hi = 0, for a
+    page that holds a key that is not finite).  head_dim is a multiple of 4."""
+
+    __slots__ = ("_tensors", "struct", "ref", "device", "index", "n_pages", "page_size", "n_kv_heads", "head_dim")
+
+    def __init__(self, lo, hi, scale, page_size):
+        for t, name, dim, want in ((lo, "lo", 3, torch.int8), (hi, "hi", 3, torch.int8), (scale, "scale", 2, torch.float32)):
+            if not isinstance(t, torch.Tensor) or t.dim() != dim or t.dtype != want or not t.is_cuda or t.device != lo.device:
+                raise TypeError(f"{name} must be a {dim}-dimensional {want} CUDA tensor on the device of lo")
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+        if hi.shape != lo.shape or scale.shape != lo.shape[:2]:
+            raise ValueError("lo and hi must have one shape, scale that of their first two dimensions")
+        self._tensors, self.device, self.index, self.page_size = (lo, hi, scale), lo.device, lo.device.index, page_size
+        self.n_pages, self.n_kv_heads, self.head_dim = lo.shape
+        self.struct = HcPageBounds(lo.data_ptr(), hi.data_ptr(), scale.data_ptr(), self.n_pages, page_size, self.n_kv_heads, self.head_dim)
+        self.ref = ctypes.addressof(self.struct)
+
+    lo = property(lambda self: self._tensors[0])
+    hi = property(lambda self: self._tensors[1])
+    scale = property(lambda self: self._tensors[2])
+
+    @classmethod
+    def alloc(cls, kv):
+        """Bounds for a pool (PagedKV or PagedKV4), of pages that hold nothing."""
+        shape = (kv.n_pages, kv.n_kv_heads, kv.head_dim)
+        return cls(torch.zeros(shape, dtype=torch.int8, device=kv.device), torch.zeros(shape, dtype=torch.int8, device=kv.device),
+                   torch.zeros(shape[:2], dtype=torch.float32, device=kv.device), kv.page_size)
+
+    def values(self):
+        """lo s and hi s, two [n_pages, n_kv_heads, head_dim] float32 tensors."""
+        if _lib.current_device() != self.index:
+            with _lib.on_device(self.index):
+                return self.values()
+        lo, hi = (torch.empty(self.lo.shape, dtype=torch.float32, device=self.device) for _ in range(2))
+        check(load().hc_page_bounds_values_dev(self.ref, lo.data_ptr(), hi.data_ptr(), raw_stream(self.index)))
+        return lo, hi
+
+
+def update_bounds(bounds, kv, batch):
+    """Makes the bounds of the pages that hold the batch's new rows anew from
+    their keys, up to each sequence's last (call it after append())."""
+    if _lib.current_device() != kv.index:
+        with _lib.on_device(kv.index):
+            return update_bounds(bounds, kv, batch)
+    _same_device(kv, batch)
+    if bounds.index != kv.index:
+        raise ValueError(f"the bounds are on {bounds.device}, the pool on {kv.device}")
+    # no row is read, so their number may stay open where no call has named it yet
+    rows = batch.n_rows if batch.n_rows >= 0 else 2 ** 31 - 1 if batch.block_table.shape[0] else 0
+    check(load().hc_page_bounds_update_dev(bounds.ref, kv.ref, batch.pack(rows), raw_stream(kv.index)))
+
+
+def select_pages(bounds, batch, q, budget, first=1, recent=2, out=None):
+    """The pages that each row is to read, per KV head, as attention() takes them:
+    an [n_rows, n_kv_heads, budget] int32 tensor (out, if given).  Of the pages that
+    hold positions up to the row's own, all if they are `budget` or fewer; else the
+    first `first`, the last `recent`, and of the others those with the largest
+    scores, the lower index first among equals; by index, -1 behind the last.  A
+    page's score is the largest, over the group's query heads, of
+    t sum_d max(c_d lo_d, c_d hi_d) s, with c = round(q / t) and t the least power of
+    two of which the head's largest |q| is at most 127: a bound of the scores of the
+    page's keys, but for the rounding of q.  Scores are exact, so the choice depends
+    on no order of additions.  q is as attention() takes it."""
+    if _lib.current_device() != bounds.index:
+        with _lib.on_device(bounds.index):
+            return select_pages(bounds, batch, q, budget, first, recent, out)
+    _same_device(bounds, batch)
+    code = _DTYPE.get(q.dtype)
+    if code is None:
+        raise TypeError(f"q must be float32 or float16, not {q.dtype}")
+    n, heads, _ = q.shape
+    qs = _rows(q, "q", bounds, q.dtype, n)
+    shape = (n, bounds.n_kv_heads, budget)
+    if out is None:
+        if budget < 1:
+            raise ValueError("budget must be positive")
+        out = torch.empty(shape, dtype=torch.int32, device=bounds.device)
+    elif not isinstance(out, torch.Tensor) or out.dtype is not torch.int32 or out.shape != shape or out.get_device() != bounds.index \
+            or not out.is_contiguous():
+        raise TypeError(f"out must be a contiguous {shape} int32 tensor on {bounds.device}")
+    lib, ref = load(), batch.pack(n)
+    need = ctypes.c_size_t()
+    check(lib.hc_page_select_workspace(bounds.ref, ref, ctypes.byref(need)))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=bounds.device) if need.value else None
+    check(lib.hc_page_select_dev(bounds.ref, ref, qs, heads, code, budget, first, recent, out.data_ptr(),
+                                 ws.data_ptr() if ws is not None else None, need.value, raw_stream(bounds.index)))
     return out
 
 

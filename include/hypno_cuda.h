@@ -46,6 +46,7 @@ extern "C" {
 
 #define HC_KV_FP32 0
 #define HC_KV_FP16 1
+#define HC_KV_Q4 2 /* paged caches only: hc_paged_kv_q4 */
 
 /* ---- library ---------------------------------------------------------- */
 
@@ -283,10 +284,28 @@ typedef struct hc_paged_kv {
     void* v;
     int64_t k_page_stride, k_head_stride, k_pos_stride;
     int64_t v_page_stride, v_head_stride, v_pos_stride;
-    int32_t kv_dtype; /* HC_KV_FP32 or HC_KV_FP16 */
+    int32_t kv_dtype; /* HC_KV_FP32, HC_KV_FP16, or HC_KV_Q4 (then an hc_paged_kv_q4) */
     int32_t n_pages, page_size, n_kv_heads, head_dim;
     int32_t reserved;
 } hc_paged_kv;
+
+/* A pool in 4 bits, passed by its first member, whose kv_dtype is HC_KV_Q4 and
+ * whose k, v and strides are those of the codes, in bytes: head_dim / 2 bytes a
+ * position, element 2 i of a head in the low half of byte i, 2 i + 1 in the high
+ * half, each the nibble c + 8 of a code c in [-7, 7] that stands for c s.  32
+ * elements share the float16 scale s: the scales of a position lie at k_scale +
+ * g * ks_page_stride + h * ks_head_stride + s * ks_pos_stride (in scales), 2, 4 or
+ * 8 slots of which the first head_dim / 32 are in use (head_dim up to 64, 128,
+ * 256).  s has seven significant bits at most and is at most 896.  Strides of
+ * codes are multiples of 16, of scales of their slots, and the pointers aligned to
+ * these; head_dim is a multiple of 32, at most 256. */
+typedef struct hc_paged_kv_q4 {
+    hc_paged_kv base;
+    void* k_scale;
+    void* v_scale;
+    int64_t ks_page_stride, ks_head_stride, ks_pos_stride;
+    int64_t vs_page_stride, vs_head_stride, vs_pos_stride;
+} hc_paged_kv_q4;
 
 /* The new tokens of a step, packed: sequence b owns the rows q_start[b] ..
  * q_start[b + 1] - 1 (q_start[0] = 0, non-decreasing, q_start[n_seqs] =
@@ -323,7 +342,11 @@ typedef struct hc_rows {
  * q_out, which may be q itself.  q, k, v and q_out are `dtype`
  * (HC_DTYPE_FP32 or HC_DTYPE_FP16); arithmetic is f32, rounded once.  A row at
  * a hole stores nothing.  A position at or past rope_rows is refused on the
- * host where max_kv_len shows it; the kernel takes the last row otherwise. */
+ * host where max_kv_len shows it; the kernel takes the last row otherwise.
+ * Into a pool in 4 bits: s is the least scale that is not below a seventh of the
+ * largest magnitude of its 32 elements (values past 6,272 are held as that), c the
+ * nearest whole number to x / s, ties to even; 32 elements of which one is not
+ * finite are all held as NaN. */
 int hc_paged_append_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_rows* k, const hc_rows* v,
                         const hc_rows* q, const hc_rows* q_out, int n_heads, uint32_t dtype, const float* rope, int rope_rows, int rot_dim,
                         int half_pairs, void* stream);
@@ -350,6 +373,64 @@ int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, c
                            float* lse,
                            int n_heads, uint32_t dtype, float scale, int window, void* workspace, size_t workspace_bytes,
                            void* stream);
+
+/* The values of every page of a pool in 4 bits as float16, exactly:
+ * k_out and v_out are [n_pages][n_kv_heads][page_size][head_dim]. */
+int hc_paged_values_dev(const hc_paged_kv* kv, void* k_out, void* v_out, void* stream);
+
+/* Pages that a row reads, per KV head: the i-th of row r and KV head h is
+ * pages[r * row_stride + h * head_stride + i], an index into the sequence's row of
+ * the block table (page j holds the positions j * page_size on).  A list
+ * ascends, and ends before the first entry that is not above the one in front of
+ * it, so with -1, and after `width` entries.  Device memory. */
+typedef struct hc_page_lists {
+    const int32_t* pages;
+    int64_t row_stride, head_stride;
+    int32_t width;
+    int32_t reserved;
+} hc_page_lists;
+
+/* hc_paged_attention_dev over the positions of the listed pages alone. */
+int hc_paged_list_attention_workspace(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_page_lists* lists,
+                                      int n_heads, uint32_t dtype, int window, size_t* bytes);
+int hc_paged_list_attention_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_page_lists* lists,
+                                const hc_rows* q, const hc_rows* out, float* lse, int n_heads, uint32_t dtype, float scale,
+                                int window, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bounds of the keys of each page, in 8 bits: the smallest and largest key of
+ * each element over the page's filled slots are at least lo s and at most hi s,
+ * s the least power of two (from 2^-120 on) of which the page's largest magnitude
+ * is at most 127; infinite, with lo = hi = 0, where a key is not finite. lo and hi
+ * are [n_pages][n_kv_heads][head_dim], scale [n_pages][n_kv_heads]; head_dim is a
+ * multiple of 4, at most 256, and lo and hi are 16-byte aligned. */
+typedef struct hc_page_bounds {
+    int8_t* lo;
+    int8_t* hi;
+    float* scale;
+    int32_t n_pages, page_size, n_kv_heads, head_dim;
+} hc_page_bounds;
+
+/* Makes the bounds of every page that holds a new row of the batch anew from
+ * its keys up to the sequence's last (call it after hc_paged_append_dev). */
+int hc_page_bounds_update_dev(const hc_page_bounds* bounds, const hc_paged_kv* kv, const hc_paged_batch* batch, void* stream);
+/* lo s and hi s as float32. */
+int hc_page_bounds_values_dev(const hc_page_bounds* bounds, float* lo_out, float* hi_out, void* stream);
+
+/* The pages that each row is to read, per KV head: of the n pages that hold
+ * the positions up to the row's own, all if they are `budget` or fewer; else the
+ * first `first`, the last `recent` (together at most budget), and of the others
+ * the ones with the largest scores, the lower index first among equals.  The
+ * score of a page is the largest, over the group's query heads, of
+ * t sum_d max(c_d lo_d, c_d hi_d), times the page's s: c = q / t rounded to a
+ * whole number (ties to even), t the least power of two of which the head's
+ * largest |q| is at most 127, as above (a head that is not finite scores 0).
+ * Scores are exact, so the choice depends on no order of additions.  A page with
+ * infinite s scores +inf, a hole -inf.  out is [n_rows][n_kv_heads][budget], by
+ * index, -1 behind the last; rows that belong to no sequence keep what they had.
+ * workspace: hc_page_select_workspace bytes, 16-byte aligned. */
+int hc_page_select_workspace(const hc_page_bounds* bounds, const hc_paged_batch* batch, size_t* bytes);
+int hc_page_select_dev(const hc_page_bounds* bounds, const hc_paged_batch* batch, const hc_rows* q, int n_heads, uint32_t dtype,
+                       int budget, int first, int recent, int32_t* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The cos/sin table of the model's rotation (transformer.rs:317-343):
  * out[p][j] = (cos, sin)(p * theta^(-2j / head_dim)) for p < rows, j <
