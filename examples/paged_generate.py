@@ -2,10 +2,13 @@
 rotation, attention of chunks and single tokens, and sampling from given
 uniforms, on one GPU.
 
-    python examples/paged_generate.py [model.hypno]
+    python examples/paged_generate.py [model.hypno] [--cache f16|f32|q4] [--keep-pages N]
 
-Without a file it makes a small synthetic model.
+Without a file it makes a small synthetic model.  --cache q4 holds keys and values
+in 4 bits; --keep-pages lets a generated token read N pages of its sequence alone,
+those that score highest for it.
 """
+import argparse
 import os
 import sys
 import time
@@ -13,6 +16,7 @@ import time
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 import numpy as np  # noqa: E402
+import torch  # noqa: E402
 
 from hypno_b200 import synth  # noqa: E402
 from hypno_b200.paged_model import PagedGenerator, PagedModel  # noqa: E402
@@ -21,11 +25,17 @@ SMALL = dict(hidden=512, layers=4, heads=8, kv_heads=2, inter=1408, vocab=8000, 
 
 
 def main(argv):
-    if len(argv) > 1:
-        image = np.memmap(argv[1], dtype=np.uint8, mode="r")
+    ap = argparse.ArgumentParser()
+    ap.add_argument("model", nargs="?")
+    ap.add_argument("--cache", choices=("f16", "f32", "q4"), default="f16")
+    ap.add_argument("--keep-pages", type=int)
+    args = ap.parse_args(argv[1:])
+    if args.model:
+        image = np.memmap(args.model, dtype=np.uint8, mode="r")
     else:
         image = synth.build_image(SMALL, seed=1)
-    model = PagedModel(image, n_pages=256, page_size=16)
+    cache = {"f16": torch.float16, "f32": torch.float32, "q4": "q4"}[args.cache]
+    model = PagedModel(image, n_pages=256, page_size=16, cache_dtype=cache, keep_pages=args.keep_pages)
     gen = PagedGenerator(model, max_seqs=8, budget=128)
     g = np.random.default_rng(0)
     for i in range(12):  # prompts of different lengths, greedy and sampled

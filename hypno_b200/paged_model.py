@@ -60,9 +60,19 @@ class _Linear:
 
 class PagedModel:
     """A .hypno image (bytes or a uint8 array) on a CUDA device, current or not,
-    with one page pool per layer."""
+    with one page pool per layer: of cache_dtype torch.float16 or torch.float32, or
+    "q4" for 4 bits (paged.PagedKV4; heads of a multiple of 32 elements).
 
-    def __init__(self, image, n_pages, page_size=16, cache_dtype=torch.float16, device="cuda"):
+    keep_pages: the pages that a generated token reads per KV head, the first, the
+    last two and those with the largest scores (paged.select_pages), at least 3;
+    None: all.  Prompts read all of theirs."""
+
+    def __init__(self, image, n_pages, page_size=16, cache_dtype=torch.float16, device="cuda", keep_pages=None):
+        if cache_dtype not in (torch.float16, torch.float32, "q4"):
+            raise ValueError(f"cache_dtype must be torch.float16, torch.float32 or 'q4', not {cache_dtype!r}")
+        if keep_pages is not None and keep_pages < 3:
+            raise ValueError(f"keep_pages must be at least 3, not {keep_pages}")
+        self.keep_pages = keep_pages
         man = hf.Manifest(np.frombuffer(image, np.uint8) if isinstance(image, (bytes, bytearray)) else image)
         meta = man.metadata
         self.device = torch.device("cuda", torch.cuda.current_device()) if str(device) == "cuda" else torch.device(device)
@@ -99,7 +109,11 @@ class PagedModel:
                       ("gate", "mlp.gate_proj"), ("up", "mlp.up_proj"), ("down", "mlp.down_proj"))}
             block["in"], block["post"] = vector(p + "input_layernorm.weight"), vector(p + "post_attention_layernorm.weight")
             self.blocks.append(block)
-            self.caches.append(paged.PagedKV.alloc(n_pages, page_size, self.kv_heads, self.dim, cache_dtype, self.device))
+            if cache_dtype == "q4":
+                self.caches.append(paged.PagedKV4.alloc(n_pages, page_size, self.kv_heads, self.dim, self.device))
+            else:
+                self.caches.append(paged.PagedKV.alloc(n_pages, page_size, self.kv_heads, self.dim, cache_dtype, self.device))
+        self.bounds = [None if keep_pages is None else paged.PageBounds.alloc(kv) for kv in self.caches]
         # the model's passes follow one another, the first one what was made here
         self.lock, self.done = threading.Lock(), torch.cuda.Event()
         with on_device(self.device.index):
@@ -108,39 +122,62 @@ class PagedModel:
     def _normed(self, x, w):
         return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + self.eps) * w
 
-    def logits(self, ids, batch, last):
+    def logits(self, ids, batch, last, lone=0):
         """Runs the packed rows' token ids (int64 on the device) through the
         layers, storing their keys and values, and returns the logits of the
-        rows `last`.  An id outside the vocabulary gives NaN for its row and the
-        rows of its sequence that see it (step() and PagedGenerator refuse it).
+        rows `last`.  The first `lone` sequences have one row each, which reads
+        the pages that keep_pages leaves it.  An id outside the vocabulary gives NaN
+        for its row and the rows of its sequence that see it (step() and
+        PagedGenerator refuse it).
         Passes of one model on different streams, or from different
         threads, are made to follow one another on the device (they share its
         workspace and pools); other models run beside them.  A pass captured in a
         graph is not: its replays must not overlap the model's other passes."""
         known = (ids >= 0) & (ids < self.vocab)
-        return self._pass(torch.where(known, ids, 0), batch, last, ~known[:, None])
+        if not 0 <= lone <= batch.block_table.shape[0]:
+            raise ValueError(f"{lone} sequences of one row among {batch.block_table.shape[0]}")
+        return self._pass(torch.where(known, ids, 0), batch, last, lone, ~known[:, None])
 
-    def _pass(self, ids, batch, last, unknown=None):
+    def _pass(self, ids, batch, last, lone=0, unknown=None):
         with self.lock, on_device(self.device.index):
             stream = torch.cuda.current_stream()
             if torch.cuda.is_current_stream_capturing():
-                return self._layers(ids, batch, last, unknown)
+                return self._layers(ids, batch, last, lone, unknown)
             stream.wait_event(self.done)
             try:
-                return self._layers(ids, batch, last, unknown)
+                return self._layers(ids, batch, last, lone, unknown)
             finally:
                 self.done.record(stream)
 
-    def _layers(self, ids, batch, last, unknown):
+    def _attend(self, kv, bounds, batch, parts, q):
+        if bounds is not None:
+            paged.update_bounds(bounds, kv, batch)
+        if parts is None:
+            return paged.attention(kv, batch, q)
+        lone, few, rest = parts
+        out = torch.empty_like(q)
+        pages = paged.select_pages(bounds, few, q[:lone], self.keep_pages)
+        paged.attention(kv, few, q[:lone], out=out[:lone], pages=pages)
+        if rest is not None:
+            paged.attention(kv, rest, q, out=out)
+        return out
+
+    def _layers(self, ids, batch, last, lone, unknown):
         n = ids.shape[0]
+        parts = None
+        if self.keep_pages is not None and lone and batch.block_table.shape[1] > self.keep_pages:
+            table, starts, lengths = batch.block_table, batch.q_start, batch.kv_len
+            few = paged.PagedBatch(table[:lone], starts[:lone + 1], lengths[:lone], 1, batch.max_kv_len)
+            rest = None if lone == table.shape[0] else paged.PagedBatch(table[lone:], starts[lone:], lengths[lone:], batch.max_q_len, batch.max_kv_len)
+            parts = lone, few, rest
         x = self.embed[ids]
         if unknown is not None:
             x.masked_fill_(unknown, float("nan"))
-        for b, kv in zip(self.blocks, self.caches):
+        for b, kv, bounds in zip(self.blocks, self.caches, self.bounds):
             h = self._normed(x, b["in"])
             q, k, v = b["q"](h).view(n, -1, self.dim), b["k"](h).view(n, -1, self.dim), b["v"](h).view(n, -1, self.dim)
             q = paged.append(kv, batch, k, v, q=q, rope=self.rope)
-            x = x + b["o"](paged.attention(kv, batch, q).view(n, -1))
+            x = x + b["o"](self._attend(kv, bounds, batch, parts, q).view(n, -1))
             h = self._normed(x, b["post"])
             x = x + b["down"](torch.nn.functional.silu(b["gate"](h)) * b["up"](h))
         return self.lm_head(self._normed(x[last], self.norm))
@@ -151,11 +188,13 @@ class PagedModel:
         with on_device(self.device.index):
             call("hc_q4_workspace_check", self.workspace, raw_stream(self.device.index))
 
-    def step(self, ids, table, q_start, kv_len, settings):
+    def step(self, ids, table, q_start, kv_len, settings, lone=None):
         """One step of a serving loop from host arrays: ids of the packed rows,
         the sequences' pages, row starts and lengths, and per sequence
         (u, temperature, top_k, top_p, min_p); returns the token drawn after
-        each sequence's last row."""
+        each sequence's last row.  lone: how many of the first sequences have a
+        single row that reads the pages keep_pages leaves it (None: all with one
+        row, up to the first with more)."""
         _check_ids(ids, self.vocab)
         dev = self.device
         start, length = np.asarray(q_start, np.int32), np.asarray(kv_len, np.int32)
@@ -163,9 +202,14 @@ class PagedModel:
             raise ValueError(f"row starts {start.tolist()} of {len(ids)} rows: they begin at 0, each sequence has a row, and the last ends")
         if length.shape != (start.size - 1,) or len(settings) != start.size - 1:
             raise ValueError(f"{start.size - 1} sequences with {length.size} lengths and {len(settings)} settings")
+        single = int(np.argmin(np.append(np.diff(start) == 1, False)))  # leading sequences of one row
+        if lone is None:
+            lone = single
+        elif not 0 <= lone <= single:
+            raise ValueError(f"{lone} sequences of one row, the first {single} have one")
         t = lambda a, d: torch.from_numpy(np.ascontiguousarray(a, d)).to(dev)  # noqa: E731
         batch = paged.PagedBatch(t(table, np.int32), t(start, np.int32), t(length, np.int32), int(np.diff(start).max()), int(length.max()))
-        logits = self._pass(t(ids, np.int64), batch, t(start[1:] - 1, np.int64))
+        logits = self._pass(t(ids, np.int64), batch, t(start[1:] - 1, np.int64), lone)
         u, temp, k, p, m = (t([s[i] for s in settings], np.int32 if i == 2 else np.float32) for i in range(5))
         tokens = sampling.sample(logits, u, temp, k, p, m)[0].cpu().numpy()
         self.check()
@@ -264,7 +308,9 @@ class PagedGenerator:
         table = self.pages.table[[r.seq for r, _ in rows], :width]
         drawn = [r.fed + take >= len(r.prompt) for r, take in rows]  # the others are still inside their prompt
         settings = [((r.rng.random(dtype=np.float32) if d else 0.0), *r.settings) for (r, _), d in zip(rows, drawn)]
-        picked = self.model.step(ids, table, start, length, settings)
+        # (prompts read all their pages, however they are cut into chunks)
+        more = {} if getattr(self.model, "keep_pages", None) is None else {"lone": sum(r.fed >= len(r.prompt) for r, _ in rows)}
+        picked = self.model.step(ids, table, start, length, settings, **more)
         made = []
         for (r, take), d, tok in zip(rows, drawn, picked):
             r.fed += take
