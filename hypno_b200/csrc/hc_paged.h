@@ -132,16 +132,28 @@ __device__ __forceinline__ uint32_t q4_code(float x, float s) {
 // A scale's slots of a position: a power of two, so that they are copied at once.
 __host__ __device__ constexpr int q4_slots(int hd) { return hd <= 64 ? 2 : hd <= 128 ? 4 : 8; }
 
-// Nibbles j = 0..3 of each half of x as pairs of float16 values: 0x5400 | nibble
-// << 4 is 64 + c + 8, so (64 + c + 8) s - 72 s is c s, exactly.
+// Nibbles j = 0..3 of each half of x as pairs of float16 values, exactly, s72 = -72 s:
+// 0x5400 | nibble << 4 is 64 + c + 8, and (64 + c + 8) s - 72 s is c s; 0x6400 | nibble
+// is 1024 + c + 8.  The first takes the nibbles that lie there after no shift, or one
+// of the whole word by 8, the second the others: shifts and logic run at half the
+// rate of the multiply-add units (one shift a word in place of three).
 __device__ __forceinline__ void q4_pairs(uint32_t x, __half2 s, __half2 s72, uint32_t* out) {
-    const uint32_t n[4] = {x << 4, x, x >> 4, x >> 8};
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const uint32_t b = (n[j] & 0x00F000F0u) | 0x54005400u;
+    const __half2 back = __half2half2(__ushort_as_half(0xE408));  // -1032
+    auto odd = [&](uint32_t y) {
+        const uint32_t b = (y & 0x00F000F0u) | 0x54005400u;
         const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&b), s, s72);
-        out[j] = *reinterpret_cast<const uint32_t*>(&v);
-    }
+        return *reinterpret_cast<const uint32_t*>(&v);
+    };
+    auto even = [&](uint32_t y) {
+        const uint32_t b = (y & 0x000F000Fu) | 0x64006400u;
+        const __half2 v = __hmul2(__hadd2(*reinterpret_cast<const __half2*>(&b), back), s);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    };
+    const uint32_t y = x >> 8;
+    out[0] = even(x);
+    out[1] = odd(x);
+    out[2] = even(y);
+    out[3] = odd(y);
 }
 
 struct q4x {};  // the element type of a pool in 4 bits, for the kernels' templates

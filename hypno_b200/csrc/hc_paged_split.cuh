@@ -62,6 +62,8 @@ struct SplitArgs {
     PagedScales c;  // 4 bits only
     PagedList l;    // LIST only
     int tg;         // LIST: tiles of a token
+    int uni;        // 4 bits, LIST: a tile of 16 keys lies in one page
+    int bulk;       // 4 bits: and its codes, and its scales, are one run of memory each
     int whole;
     int ctas;     // CTAs of the line (cut)
     int rows;     // R, rows of a tile
@@ -135,7 +137,7 @@ __device__ __forceinline__ SeqWork seq_work(const SplitArgs& X, int b) {
     // positions seen by any tile, at most: the last tile's end from the first tile's begin, per tile no
     // more than its window and its own tokens
     int len = min(max(0, w.first + T), A.p.reach);
-    if (A.window > 0) len = (int)min((int64_t)len, (int64_t)A.window + R);
+    if (A.window > 0) len = (int)min((int64_t)len, (int64_t)A.window + R + (X.uni ? SP_TK - 1 : 0));  // (uni: from a tile's first key on)
     w.units = max(1, len / UNIT + (len % UNIT != 0));
     w.pairs = (int)(tiles * A.p.nkv);
     return w;
@@ -222,19 +224,15 @@ struct SplitShape {
     static_assert(WARPB >= 16 * LDO * 4, "a warp's outputs fit its ring");
 };
 
-// ---- 4 bits.  A key's bytes as lane c = lane % 4 of its four lanes has them: a
-// quarter of them (two groups of 32 elements, 128 elements apart, for heads above
-// 128), eight elements a word; the keys of a tile in their order.  Values: the
-// eight lanes r = lane / 4 have an eighth of a key's bytes each, of keys 2 c,
-// 2 c + 1, 2 c + 8 and 2 c + 9, which lie in rows c, c + 4, c + 8 and c + 12.  The
-// 16-byte chunks are permuted so that neither reading has bank conflicts.
-__device__ __forceinline__ int q4_row_of(int key) { return (key >> 1 & 3) + (key & 1) * 4 + (key & 8); }
-template <int HD>
-__device__ __forceinline__ int q4_key_chunk(int row, int chunk) { return HD > 128 ? chunk ^ ((row & 1) << 2) : chunk; }
-template <int HD>
-__device__ __forceinline__ int q4_value_chunk(int row, int chunk) {
-    return HD > 128 ? chunk ^ ((row & 3) << 1) : HD > 64 ? chunk ^ (row & 2) : chunk;
-}
+// ---- 4 bits.  Tiles lie in shared memory as in a page: a key's bytes after one
+// another, the scales of all keys behind the codes.  Lane c = lane % 4 of a key's
+// four lanes has a quarter of its bytes (two groups of 32 elements, 128 elements apart,
+// for heads above 128), eight elements a word.  Of the values, lanes r = lane / 4
+// have an eighth of a key's bytes each, of the four keys that their operands take.
+// Key m of the products is key q4_key(m) of the tile: the keys 0, 3, 4, 7 that the
+// four lanes c read at once lie on different banks by pairs (0, 2, 4, 6 would not),
+// and so do the two keys that eight lanes read at once.
+__device__ __forceinline__ int q4_key(int m) { return m ^ (m >> 1 & 1); }  // its own inverse
 // First element of word w of lane c's part of a key.
 template <int HD>
 __device__ __forceinline__ int q4_part(int c, int w) {
@@ -267,10 +265,9 @@ __device__ __forceinline__ void copy_q4(const SplitArgs& X, int kvh, int page0, 
     auto chunk = [&](int key, int page, int slot, int x) {
         const bool in = page >= 0 && x * 32 < P.hd;  // chunks past head_dim are zeros, not read
         const int64_t g = max(page, 0);
-        const int row = q4_row_of(key);
-        cp16(stage + key * ROWB + (q4_key_chunk<HD>(key, x) << 4), in ? kb + g * P.kps + kvh * P.khs + slot * P.kss + x * 16 : kb, in);
-        cp16(stage + SP_TK * ROWB + row * ROWB + (q4_value_chunk<HD>(row, x) << 4),
-             in ? vb + g * P.vps + kvh * P.vhs + slot * P.vss + x * 16 : vb, in);
+        const uint32_t to = stage + key * ROWB + (x << 4);
+        cp16(to, in ? kb + g * P.kps + kvh * P.khs + slot * P.kss + x * 16 : kb, in);
+        cp16(to + SP_TK * ROWB, in ? vb + g * P.vps + kvh * P.vhs + slot * P.vss + x * 16 : vb, in);
     };
     if constexpr (HD <= 64) {
         chunk(r + (c >> 1) * 8, c >> 1 ? page1 : page0, c >> 1 ? slot1 : slot0, c & 1);
@@ -286,7 +283,7 @@ __device__ __forceinline__ void copy_q4(const SplitArgs& X, int kvh, int page0, 
     const bool in = page >= 0;
     const int64_t g = max(page, 0);
     const __half* src = c >> 1 ? X.c.v + g * X.c.vps + kvh * X.c.vhs + slot * X.c.vss : X.c.k + g * X.c.kps + kvh * X.c.khs + slot * X.c.kss;
-    cp_small<SCB>(stage + SC + (c >> 1 ? SP_TK + q4_row_of(key) : key) * SCB, in ? src : X.c.k, in);
+    cp_small<SCB>(stage + SC + ((c >> 1) * SP_TK + key) * SCB, in ? src : X.c.k, in);
 }
 // Lane c's words of a key and their scales s, with z = -72 s.
 template <int HD>
@@ -296,25 +293,31 @@ __device__ __forceinline__ void q4_key_words(uint32_t tile, uint32_t scales, int
 #pragma unroll
     for (int x = 0; x < (HD > 128 ? 2 : 1); x++) {
         if constexpr (HD <= 64) lds_words<2>(tile + row * ROWB + c * 8, w);
-        else lds_words<4>(tile + row * ROWB + (q4_key_chunk<HD>(row, c + 4 * x) << 4), w + 4 * x);
+        else lds_words<4>(tile + row * ROWB + ((c + 4 * x) << 4), w + 4 * x);
         const int g = HD <= 64 ? c >> 1 : c + 4 * x;
         // (the slots past head_dim may hold anything)
         s[x] = g * 32 < hd ? __half2half2(lds_f16(scales + row * SCB + 2 * g)) : __half2half2(__ushort_as_half(0));
         z[x] = __hmul2(s[x], __half2half2(__float2half_rn(-72.0f)));
     }
 }
-// This lane's words of its four keys' values, the scales of each pair of keys.
+// This lane's words of its four keys' values, the scales of each pair of keys: zero
+// for the ones that are not in, whatever their slots hold.
 template <int HD>
-__device__ __forceinline__ void q4_value_words(uint32_t tile, uint32_t scales, uint32_t (*w)[HD / 64], __half2* s, __half2* z) {
+__device__ __forceinline__ void q4_value_words(uint32_t tile, uint32_t scales, uint32_t in, uint32_t (*w)[HD / 64], __half2* s, __half2* z) {
     constexpr int ROWB = HD / 2, SCB = 2 * q4_slots(HD);
     const int r = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3;
+    const int key = q4_key(2 * c);  // then key ^ 1, and both + 8
     __half h[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int row = c + 4 * i;
-        const int at = HD <= 64 ? r * 4 : HD <= 128 ? (q4_value_chunk<HD>(row, r >> 1) << 4) + (r & 1) * 8 : q4_value_chunk<HD>(row, r) << 4;
-        lds_words<HD / 64>(tile + row * ROWB + at, w[i]);
+        const int row = (key ^ (i & 1)) + (i >> 1) * 8;
+        lds_words<HD / 64>(tile + row * ROWB + r * (HD / 16), w[i]);
         h[i] = lds_f16(scales + row * SCB + 2 * (HD <= 64 ? r >> 2 : HD <= 128 ? r >> 1 : r));
+    }
+    if (in != 0xffffu) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (!(in >> ((key ^ (i & 1)) + (i >> 1) * 8) & 1u)) h[i] = __ushort_as_half(0);
     }
 #pragma unroll
     for (int i = 0; i < 2; i++) {
@@ -326,9 +329,32 @@ __device__ __forceinline__ void q4_value_words(uint32_t tile, uint32_t scales, u
 template <int HD>
 __device__ __forceinline__ float q4_value(uint32_t tile, uint32_t scales, int key, int d) {
     constexpr int ROWB = HD / 2, SCB = 2 * q4_slots(HD);
-    const int row = q4_row_of(key);
-    const uint32_t word = lds_u32(tile + row * ROWB + (q4_value_chunk<HD>(row, d >> 5) << 4) + ((d & 31) >> 3) * 4);
-    return (float)((int)(word >> (4 * (d & 7)) & 15) - 8) * __half2float(lds_f16(scales + row * SCB + 2 * (d >> 5)));
+    const uint32_t word = lds_u32(tile + key * ROWB + (d >> 3) * 4);
+    return (float)((int)(word >> (4 * (d & 7)) & 15) - 8) * __half2float(lds_f16(scales + key * SCB + 2 * (d >> 5)));
+}
+// A copy of one run of memory, counted by an mbarrier.
+__device__ __forceinline__ void cp_run(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+// Waits for a stage's copies, a bounded time; the whole warp.
+__device__ __forceinline__ bool run_there(uint64_t* bar, uint32_t parity) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    const long long start = clock64();
+    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+        if (__any_sync(0xffffffffu, clock64() - start > WAIT_CYCLES)) return false;
+    return true;
+}
+// 2^x; results below 2^-126 are zeros.
+template <bool FAST>
+__device__ __forceinline__ float pow2(float x) {
+    if constexpr (FAST) {
+        float y;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+        return y;
+    } else {
+        return exp2f(x);
+    }
 }
 // Eight elements of a query row.
 template <typename QT>
@@ -352,8 +378,13 @@ __device__ __forceinline__ void load_q8(const QT* q, bool in, int vec, int d, fl
     for (int i = 0; i < 8; i++) x[i] = in ? to_f32(q[d + i]) : 0.0f;
 }
 
+// CTAs an SM is to hold at least, for the forms whose copies are planned ahead (their
+// state would take the registers of the third).
+template <typename CT, int HD, int NQ, bool LIST>
+constexpr int split_ctas() { return (LIST || std::is_same<CT, q4x>::value) && NQ == 1 && HD <= 128 ? 3 : 1; }
+
 template <typename QT, typename CT, int HD, int NQ, bool LIST>
-__global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constant__ SplitArgs X) {
+__global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_paged_split(const __grid_constant__ SplitArgs X) {
     using Sh = SplitShape<CT, HD>;
     constexpr bool Q4 = Sh::Q4;
     constexpr bool C16 = Q4 || sizeof(CT) == 2;  // products of float16
@@ -374,7 +405,18 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
     uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 511u);
     __shared__ float s_m[SP_WARPS][R], s_l[SP_WARPS][R];
     __shared__ uint32_t s_in[SP_WARPS][S];
+    __shared__ uint64_t s_full[Q4 ? SP_WARPS : 1][S];  // bulk: the copies of a warp's stages
+    constexpr bool PLAN = Q4 || LIST;  // forms with one page a tile
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    [[maybe_unused]] uint32_t copied = 0;  // bulk: tiles of this warp so far
+    [[maybe_unused]] bool lost = false;    // bulk: a wait ran out
+    if constexpr (Q4) {
+        if (X.bulk) {
+            if (lane < S) mbar_init(&s_full[warp][lane], 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            __syncwarp();
+        }
+    }
     pdl_trigger();  // the join may become resident; it waits for this grid's end
 
     int64_t u, u_end;
@@ -410,6 +452,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
             end = (int)min((int64_t)min(list_count(X.l, row, kvh), pages_seen(P, p_own)) * P.page_size, (int64_t)0x7fffff00);
         } else {
             visible(A, first, m0, mrows, begin, end);
+            if (Q4 && X.uni) begin &= ~(SP_TK - 1);
         }
         const int c0 = (int)min((int64_t)end, begin + (int64_t)unit * UNIT);
         const int c1 = (int)min((int64_t)end, c0 + (int64_t)nunits * UNIT);
@@ -435,9 +478,92 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
                 }
             }
         };
-        look(0);
+        // One page a tile: lane l works out the places of this warp's tiles 32 n + l
+        // ahead of their copies, page, slot << 16 and the keys that are there.
+        [[maybe_unused]] int now_page = -1, then_page = -1, then_entry = -1;
+        [[maybe_unused]] uint32_t now_place = 0, then_place = 0;
+        auto find_entry = [&](int i0) {  // LIST: the index that the list has there
+            const int i = i0 + lane;
+            then_entry = LIST && i < mine ? __ldg(list + page_of(P, c0 + (warp + i * SP_WARPS) * SP_TK)) : 0;
+        };
+        auto find_page = [&](int i0) {
+            const int i = i0 + lane;
+            then_page = -1;
+            then_place = 0;
+            if (i >= mine) return;
+            const int v = c0 + (warp + i * SP_WARPS) * SP_TK;
+            int x = page_of(P, v), n = min(SP_TK, c1 - v), low = 0;
+            const int place = v - x * P.page_size;
+            if constexpr (LIST) {
+                x = then_entry;
+                if (x >= P.max_pages) return;
+                const int64_t pos = (int64_t)x * P.page_size + place;
+                n = (int)min((int64_t)n, p_own - pos + 1);
+                if (A.window > 0) low = (int)min(max(p_own - A.window + 1 - pos, (int64_t)0), (int64_t)SP_TK);
+                if (n <= low) return;
+            }
+            const int g = __ldg(P.table + (int64_t)seq * P.table_stride + x);
+            if ((unsigned)g >= (unsigned)P.n_pages) return;
+            then_page = g;
+            then_place = (uint32_t)place << 16 | (((1u << n) - 1) & ~((1u << low) - 1));
+        };
+        const bool plan = PLAN && X.uni;
+        if (plan) {
+            find_entry(0);
+            find_page(0);
+        } else {
+            look(0);
+        }
+        // bulk: lanes 0 to 3 copy the codes of K and V and their scales
+        [[maybe_unused]] const uint8_t* run_from = nullptr;
+        [[maybe_unused]] int64_t run_page = 0, run_pos = 0;
+        [[maybe_unused]] uint32_t run_bytes = 0, run_to = 0;
+        if constexpr (Q4) {
+            if (X.bulk) {
+                const bool is_v = lane & 1, is_s = lane & 2;
+                const int64_t ps = is_s ? 2 * (is_v ? X.c.vps : X.c.kps) : is_v ? P.vps : P.kps;
+                const int64_t hs = is_s ? 2 * (is_v ? X.c.vhs : X.c.khs) : is_v ? P.vhs : P.khs;
+                run_from = (const uint8_t*)(is_s ? (is_v ? (const void*)X.c.v : (const void*)X.c.k) : is_v ? P.v : P.k) + kvh * hs;
+                run_page = ps;
+                run_pos = is_s ? SCB : ROWB;
+                run_bytes = SP_TK * (is_s ? SCB : ROWB);
+                run_to = ring + (is_s ? SC : 0) + (is_v ? run_bytes : 0);
+            }
+        }
         auto issue = [&](int i) {
-            if (i < mine) {
+            if (plan) {
+                if (i < mine) {
+                    if ((i & 31) == 0) {
+                        now_page = then_page;
+                        now_place = then_place;
+                        find_entry(i + 32);
+                    } else if ((i & 31) == 16) {
+                        find_page(i + 16);
+                    }
+                    const int page = __shfl_sync(0xffffffffu, now_page, i & 31);
+                    const uint32_t at = __shfl_sync(0xffffffffu, now_place, i & 31), in = at & 0xffffu;
+                    if constexpr (Q4) {
+                        if (X.bulk) {
+                            if (lost) return;
+                            const uint32_t st = (copied + i) % S;
+                            if (lane == 0) {
+                                s_in[warp][st] = in;
+                                if (page < 0) mbar_arrive(&s_full[warp][st]);
+                                else mbar_expect_tx(&s_full[warp][st], Sh::STAGE);
+                            }
+                            if (lane < 4 && page >= 0)
+                                cp_run(run_to + st * Sh::STAGE, run_from + page * run_page + (int64_t)(at >> 16) * run_pos, run_bytes, &s_full[warp][st]);
+                            return;
+                        }
+                    }
+                    page0 = in >> kr & 1u ? page : -1;  // (a key that no row sees is zeros)
+                    page1 = in >> (kr + 8) & 1u ? page : -1;
+                    slot0 = (int)(at >> 16) + kr;
+                    slot1 = slot0 + 8;
+                    if (lane == 0) s_in[warp][i % S] = in;
+                }
+            }
+            if (i < mine && !plan) {
                 const uint32_t b0 = __ballot_sync(0xffffffffu, page0 >= 0), b1 = __ballot_sync(0xffffffffu, page1 >= 0);
                 if (lane == 0) {  // one bit per key: the lanes of a row agree
                     uint32_t in = 0;
@@ -445,6 +571,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
                     for (int r = 0; r < 8; r++) in |= ((b0 >> (4 * r)) & 1u) << r | ((b1 >> (4 * r)) & 1u) << (8 + r);
                     s_in[warp][i % S] = in;
                 }
+            }
+            if (i < mine) {
                 if constexpr (Q4) {
                     copy_q4<HD>(X, kvh, page0, slot0, page1, slot1, ring + (i % S) * Sh::STAGE);
                 } else {
@@ -465,7 +593,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
                     cp16(o + (SP_TK + 8) * ROWB, in1 ? v1 + 4 * x * EPC : (const CT*)P.v, in1);
                 }
                 }
-                look(i + 1);
+                if (!plan) look(i + 1);
             }
             cp_commit();
         };
@@ -576,11 +704,20 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
         const uint32_t vget = (uint32_t)(vrow * ROWB + (((mi & 1) ^ (vrow & 7)) << 4));
 
         for (int i = 0; i < mine; i++) {
-            cp_wait<S - 2>();
+            uint32_t st = i % S;
+            if (Q4 && X.bulk) {
+                st = (copied + i) % S;
+                if (!lost && !run_there(&s_full[warp][st], (copied + i) / S & 1)) {
+                    lost = true;  // nothing is issued from here on; what is under way gets its time
+                    for (int k = 1; k < S - 1 && i + k < mine; k++) run_there(&s_full[warp][(copied + i + k) % S], (copied + i + k) / S & 1);
+                }
+            } else {
+                cp_wait<S - 2>();
+            }
             __syncwarp();
             issue(i + S - 1);
-            const uint32_t kt = ring + (i % S) * Sh::STAGE, vt = kt + SP_TK * ROWB;
-            const uint32_t in = s_in[warp][i % S];
+            const uint32_t kt = ring + st * Sh::STAGE, vt = kt + SP_TK * ROWB;
+            const uint32_t in = s_in[warp][st];
             const int j0 = c0 + (warp + i * SP_WARPS) * SP_TK;
             // S^T: [0], [1] = key lane / 4 and this thread's two columns, [2], [3] = key lane / 4 + 8
             float s[NQ][4], sl[HILO ? NQ : 1][4];
@@ -594,8 +731,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
             if constexpr (Q4) {
                 uint32_t w0[LE / 8], w1[LE / 8];  // this lane's part of keys lane / 4 and lane / 4 + 8
                 __half2 s0[HD > 128 ? 2 : 1], s1[HD > 128 ? 2 : 1], z0[HD > 128 ? 2 : 1], z1[HD > 128 ? 2 : 1];
-                q4_key_words<HD>(kt, kt + SC, lane >> 2, P.hd, w0, s0, z0);
-                q4_key_words<HD>(kt, kt + SC, (lane >> 2) + 8, P.hd, w1, s1, z1);
+                q4_key_words<HD>(kt, kt + SC, q4_key(lane >> 2), P.hd, w0, s0, z0);
+                q4_key_words<HD>(kt, kt + SC, q4_key(lane >> 2) + 8, P.hd, w1, s1, z1);
 #pragma unroll
                 for (int w = 0; w < LE / 8; w++) {
                     uint32_t e[4], f[4];
@@ -661,7 +798,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
                     s[n][x] *= cf[n][x];
                     s[n][2 + x] *= cf[n][x];
                     if (!whole) {
-                        const int jj = lane >> 2, j = j0 + jj;
+                        const int jj = Q4 ? q4_key(lane >> 2) : lane >> 2, j = j0 + jj;
                         if (!((in >> jj) & 1u) || (!LIST && (j > ps[n][x] || j < lo[n][x]))) s[n][x] = -INFINITY;
                         if (!((in >> (jj + 8)) & 1u) || (!LIST && (j + 8 > ps[n][x] || j + 8 < lo[n][x]))) s[n][2 + x] = -INFINITY;
                     }
@@ -676,7 +813,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
                         const float m = fmaxf(nm[x], mx[n][x]);
-                        const float f = m == mx[n][x] ? 1.0f : exp2f(mx[n][x] - m);
+                        const float f = m == mx[n][x] ? 1.0f : pow2<PLAN>(mx[n][x] - m);
                         mx[n][x] = m;
                         sum[n][x] *= f;
 #pragma unroll
@@ -689,8 +826,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
                     const float b = mx[n][x] == -INFINITY ? 0.0f : mx[n][x] - BIAS;
-                    s[n][x] = exp2f(s[n][x] - b);
-                    s[n][2 + x] = exp2f(s[n][2 + x] - b);
+                    s[n][x] = pow2<PLAN>(s[n][x] - b);
+                    s[n][2 + x] = pow2<PLAN>(s[n][2 + x] - b);
                     sum[n][x] += s[n][x] + s[n][2 + x];
                 }
             }
@@ -717,7 +854,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
             }
             if (!LIST && careful) {
                 for (int jj = 0; jj < SP_TK; jj++) {
-                    const int src = (jj & 7) * 4 + (lane & 3), j = j0 + jj;
+                    const int src = (Q4 ? q4_key(jj & 7) : jj & 7) * 4 + (lane & 3), j = j0 + jj;
                     const bool key_in = (in >> jj) & 1u;
 #pragma unroll
                     for (int n = 0; n < NQ; n++)
@@ -774,7 +911,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
                 if constexpr (Q4) {
                     uint32_t w[4][LE / 16];  // this lane's run of columns, of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
                     __half2 sv[2], sz[2];
-                    q4_value_words<HD>(vt, kt + SC + SP_TK * SCB, w, sv, sz);
+                    q4_value_words<HD>(vt, kt + SC + SP_TK * SCB, in, w, sv, sz);
 #pragma unroll
                     for (int h = 0; h < HD / 32; h++) {  // four columns
                         uint32_t e[4], f[4];
@@ -838,7 +975,15 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
             }
             __syncwarp();
         }
-        cp_wait<0>();
+        if (Q4 && X.bulk) {
+            copied += mine;
+            if (lost) {  // (a copy that never came: not a number, rather than a wrong one)
+#pragma unroll
+                for (int n = 0; n < NQ; n++) sum[n][0] = sum[n][1] = __int_as_float(0x7FC00000);
+            }
+        } else {
+            cp_wait<0>();
+        }
         __syncwarp();
 
         // ---- this warp's (m, l, o) to shared memory (over its ring)
@@ -890,6 +1035,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_split(const __grid_constan
                 if (d == 0) X.pml[slot * R + m] = make_float2(mm == -INFINITY ? mm : mm - BIAS, l);
             }
         }
+        // (bulk: the next pair's copies come after what was written and read here)
+        if (Q4 && X.bulk) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
     }
 }
