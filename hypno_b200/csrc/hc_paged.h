@@ -137,15 +137,20 @@ __host__ __device__ constexpr int q4_slots(int hd) { return hd <= 64 ? 2 : hd <=
 // is 1024 + c + 8.  The first takes the nibbles that lie there after no shift, or one
 // of the whole word by 8, the second the others: shifts and logic run at half the
 // rate of the multiply-add units (one shift a word in place of three).
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {  // one instruction (written with & and |, two)
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+    return y;
+}
 __device__ __forceinline__ void q4_pairs(uint32_t x, __half2 s, __half2 s72, uint32_t* out) {
     const __half2 back = __half2half2(__ushort_as_half(0xE408));  // -1032
     auto odd = [&](uint32_t y) {
-        const uint32_t b = (y & 0x00F000F0u) | 0x54005400u;
+        const uint32_t b = and_or(y, 0x00F000F0u, 0x54005400u);
         const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&b), s, s72);
         return *reinterpret_cast<const uint32_t*>(&v);
     };
     auto even = [&](uint32_t y) {
-        const uint32_t b = (y & 0x000F000Fu) | 0x64006400u;
+        const uint32_t b = and_or(y, 0x000F000Fu, 0x64006400u);
         const __half2 v = __hmul2(__hadd2(*reinterpret_cast<const __half2*>(&b), back), s);
         return *reinterpret_cast<const uint32_t*>(&v);
     };

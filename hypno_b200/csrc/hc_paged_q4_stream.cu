@@ -1,0 +1,538 @@
+// Attention of few rows, or of rows with lists of pages, over a pool in 4 bits
+// whose pages are runs of memory (k_paged_split takes the other layouts).
+//
+// The line of units, its runs, the join and the products are k_paged_split's.  A
+// fifth warp copies: a stage is 128 keys, eight tiles of 16, and each of its lanes
+// copies one tile's codes or scales of K or V as one run (cp.async.bulk, counted by
+// the stage's mbarrier), so a page's place is worked out once and the four warps that
+// compute spend nothing on it.  Each takes 32 keys of a stage: two tiles whose
+// chains of dependent steps (codes, products, maxima, weights, products) overlap.
+//
+// A key's codes become float16 in registers (q4_pairs, 11 instructions for eight
+// elements), which is most of what the kernel does: shifts, logic and float16
+// arithmetic run at half rate, so K and V of 16 keys of 128 elements take about 260
+// cycles of a scheduler's logic unit where their bytes take 400 at the memory's rate.
+#include "hc_paged_split.cuh"
+
+namespace hc {
+
+namespace {
+
+constexpr int QS_WARPS = 4, QS_THREADS = 32 * (QS_WARPS + 1), QS_TILES = 2 * QS_WARPS, QS_KEYS = SP_TK * QS_TILES;
+
+template <int HD, int NQ>
+struct StreamShape {
+    static constexpr int ROWB = HD / 2, SCB = 2 * q4_slots(HD);
+    static constexpr int CODES = QS_KEYS * ROWB, SCALES = QS_KEYS * SCB;  // of K or V
+    static constexpr int STAGE = 2 * (CODES + SCALES);                    // K codes, V codes, K scales, V scales
+    static constexpr int STAGES = HD <= 64 ? 4 : 3;
+    static constexpr int LDO = HD + 4;
+    static constexpr int OUT = 8 * NQ * LDO * 4;                          // a warp's outputs
+    static constexpr int SMEM = STAGES * STAGE + QS_WARPS * OUT + 128;
+};
+
+// One CTA's share of a pair.
+struct PairWork {
+    int seq, r0, first, kvh, m0, mrows;
+    int c0, c1;     // positions (LIST: places of the list)
+    bool cut;
+    int64_t slot;   // of the partial results
+    int p_own;      // LIST: position of the token
+    const int32_t* list;
+};
+template <bool LIST>
+__device__ __forceinline__ bool next_pair(const SplitArgs& X, int64_t& u, int64_t u_begin, int64_t u_end, Line& at, PairWork& w) {
+    const PagedAttnArgs& A = X.a;
+    if (u >= u_end || !advance<LIST>(X, u, X.whole != 0, at)) return false;
+    const int64_t rem = u - at.base;
+    const int pair = (int)(X.whole ? rem : rem / at.w.units);
+    const int unit = X.whole ? 0 : (int)(rem - (int64_t)pair * at.w.units);
+    const int nunits = X.whole ? at.w.units : (int)min((int64_t)(at.w.units - unit), u_end - u);
+    w.seq = at.b;
+    w.r0 = at.w.r0;
+    w.first = at.w.first;
+    w.cut = nunits < at.w.units;
+    w.slot = 2 * (int64_t)blockIdx.x + (u == u_begin ? 0 : 1);
+    u += X.whole ? 1 : nunits;
+    w.kvh = pair % A.p.nkv;
+    tile_rows<LIST>(X, pair / A.p.nkv, at.w.r1 - w.r0, w.m0, w.mrows);
+    int begin, end;
+    w.p_own = w.first + token_of(A, w.m0);
+    w.list = nullptr;
+    if constexpr (LIST) {
+        const int row = w.r0 + token_of(A, w.m0);
+        w.list = X.l.pages + row * X.l.row_stride + w.kvh * X.l.head_stride;
+        begin = 0;
+        end = (int)min((int64_t)min(list_count(X.l, row, w.kvh), pages_seen(A.p, w.p_own)) * A.p.page_size, (int64_t)0x7fffff00);
+    } else {
+        visible(A, w.first, w.m0, w.mrows, begin, end);
+        begin &= ~(SP_TK - 1);
+    }
+    w.c0 = (int)min((int64_t)end, begin + (int64_t)unit * UNIT);
+    w.c1 = (int)min((int64_t)end, w.c0 + (int64_t)nunits * UNIT);
+    return true;
+}
+
+template <int STAGES>
+struct StreamBars {
+    uint64_t full[STAGES], empty[STAGES];
+    uint32_t in[STAGES][QS_TILES];  // which keys of a tile are there
+    int abort;
+};
+
+// The copying warp.
+template <int HD, int NQ, bool LIST>
+__device__ __forceinline__ void stream_copies(const SplitArgs& X, StreamBars<StreamShape<HD, NQ>::STAGES>& B, uint32_t ring, int64_t u_begin, int64_t u_end) {
+    using Sh = StreamShape<HD, NQ>;
+    constexpr int S = Sh::STAGES;
+    const PagedAttnArgs& A = X.a;
+    const PagedArgs& P = A.p;
+    const int lane = threadIdx.x & 31, tile = lane >> 2;
+    const bool is_v = lane & 1, is_s = lane & 2;
+    const uint8_t* pool = (const uint8_t*)(is_s ? (is_v ? (const void*)X.c.v : (const void*)X.c.k) : is_v ? P.v : P.k);
+    const int64_t ps = is_s ? 2 * (is_v ? X.c.vps : X.c.kps) : is_v ? P.vps : P.kps;
+    const int64_t hs = is_s ? 2 * (is_v ? X.c.vhs : X.c.khs) : is_v ? P.vhs : P.khs;
+    const uint32_t pos_bytes = is_s ? Sh::SCB : Sh::ROWB, bytes = SP_TK * pos_bytes;
+    const uint32_t to = ring + (is_s ? 2 * Sh::CODES + (is_v ? Sh::SCALES : 0) : (is_v ? Sh::CODES : 0)) + tile * bytes;
+    int64_t u = u_begin;
+    Line at = {0, 0, {}};
+    PairWork w;
+    uint32_t n = 0;  // stages so far
+    bool ok = true;
+    while (ok && next_pair<LIST>(X, u, u_begin, u_end, at, w)) {
+        const uint8_t* from = pool + w.kvh * hs;
+        const int stages = (w.c1 - w.c0 + QS_KEYS - 1) / QS_KEYS;
+        auto entry_of = [&](int k) {  // LIST: the index that the list has for this lane's tile
+            const int64_t v = w.c0 + (int64_t)k * QS_KEYS + tile * SP_TK;
+            return LIST && v < w.c1 ? __ldg(w.list + page_of(P, (int)v)) : 0;
+        };
+        auto place_of_tile = [&](int k, int entry, uint32_t& place) {  // page, -1: none; slot << 16 | keys
+            place = 0;
+            const int64_t v = w.c0 + (int64_t)k * QS_KEYS + tile * SP_TK;
+            if (v >= w.c1) return -1;
+            int x = page_of(P, (int)v), have = min(SP_TK, w.c1 - (int)v), low = 0;
+            const int slot = (int)v - x * P.page_size;
+            if constexpr (LIST) {
+                x = entry;
+                if (x >= P.max_pages) return -1;
+                const int64_t pos = (int64_t)x * P.page_size + slot;
+                have = (int)min((int64_t)have, w.p_own - pos + 1);
+                if (A.window > 0) low = (int)min(max(w.p_own - A.window + 1 - pos, (int64_t)0), (int64_t)SP_TK);
+                if (have <= low) return -1;
+            }
+            const int g = __ldg(P.table + (int64_t)w.seq * P.table_stride + x);
+            if ((unsigned)g >= (unsigned)P.n_pages) return -1;
+            place = (uint32_t)slot << 16 | (((1u << have) - 1) & ~((1u << low) - 1));
+            return g;
+        };
+        uint32_t place;
+        int page = place_of_tile(0, entry_of(0), place);
+        int entry = entry_of(1);
+        for (int k = 0; k < stages; k++, n++) {
+            uint32_t next_place;
+            const int next_page = place_of_tile(k + 1, entry, next_place);
+            entry = entry_of(k + 2);
+            const uint32_t st = n % S;
+            if (n >= S && !mbar_wait(&B.empty[st], (n / S & 1) ^ 1, &B.abort)) {
+                ok = false;
+                break;
+            }
+            if ((lane & 3) == 0) B.in[st][tile] = place & 0xffffu;
+            const int copies = __popc(__ballot_sync(0xffffffffu, page >= 0)) >> 2;
+            __syncwarp();
+            if (lane == 0) {
+                if (copies) mbar_expect_tx(&B.full[st], copies * (Sh::STAGE / QS_TILES));
+                else mbar_arrive(&B.full[st]);
+            }
+            __syncwarp();
+            if (page >= 0) cp_run(to + st * Sh::STAGE, from + page * ps + (int64_t)(place >> 16) * pos_bytes, bytes, &B.full[st]);
+            page = next_page;
+            place = next_place;
+        }
+    }
+    // every copy has landed before the CTA ends: the rows' warps waited for all of
+    // them, unless a wait ran out
+    if (!ok) {
+        const long long start = clock64();
+        for (uint32_t k = n > S ? n - S : 0; k < n; k++)
+            while (!mbar_try_wait(&B.full[k % S], k / S & 1) && clock64() - start < WAIT_CYCLES) {}
+    }
+}
+
+template <typename QT, int HD, int NQ, bool LIST>
+__global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const __grid_constant__ SplitArgs X) {
+    using Sh = StreamShape<HD, NQ>;
+    constexpr int R = 8 * NQ, S = Sh::STAGES, ROWB = Sh::ROWB, SCB = Sh::SCB, LDO = Sh::LDO;
+    constexpr bool HILO = sizeof(QT) == 4;
+    constexpr int DT = HD / 16, KS = HD / 16, LE = HD / 4;
+    // the maximum stays until a score passes it by 2^TAU; weights are held times
+    // 2^BIAS in fp16, so that one of 2^-25 of the largest still has 11 bits
+    constexpr float BIAS = 11.0f, TAU = 4.0f;
+    const PagedAttnArgs& A = X.a;
+    const PagedArgs& P = A.p;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 127u);
+    __shared__ StreamBars<S> B;
+    __shared__ float s_m[QS_WARPS][R], s_l[QS_WARPS][R];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S; i++) {
+            mbar_init(&B.full[i], 1);
+            mbar_init(&B.empty[i], QS_WARPS);
+        }
+        B.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    pdl_trigger();  // the join may become resident; it waits for this grid's end
+    int64_t u = blockIdx.x, u_end = u + 1;
+    if (!X.whole) {
+        const int64_t run = run_of(all_units<LIST>(X), X.ctas);
+        u = blockIdx.x * run;
+        u_end = u + run;
+    }
+    const uint32_t ring = smem_u32(smem);
+    if (warp == QS_WARPS) {
+        stream_copies<HD, NQ, LIST>(X, B, ring, u, u_end);
+        return;
+    }
+    uint8_t* outs = smem + S * Sh::STAGE;
+    const int64_t u_begin = u;
+    Line at = {0, 0, {}};
+    PairWork w;
+    uint32_t st = 0, phase = 0;  // the next stage and the parity of its round
+    bool lost = false;
+    const int c = lane & 3, col = 2 * c, k0 = q4_key(lane >> 2);
+    while (next_pair<LIST>(X, u, u_begin, u_end, at, w)) {
+        // ---- queries as B fragments: column lane / 4 of each tile of eight rows
+        uint32_t qh[NQ][KS][2];
+        uint32_t ql[HILO ? NQ : 1][HILO ? KS : 1][2];
+        float cf[NQ][2];           // score factors of this thread's two columns, not negative
+        int ps[NQ][2], lo[NQ][2];  // their positions and first visible positions
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            const int m = n * 8 + (lane >> 2);
+            const bool in = m < w.mrows;
+            const int t = token_of(A, w.m0 + m);
+            const QT* q = (const QT*)A.q + (in ? (int64_t)(w.r0 + t) * A.q_rs + (w.kvh * A.G + (w.m0 + m) - t * A.G) * A.q_hs : 0);
+            // (a factor below zero turns the query's sign, one of zero its elements to zeros)
+            float f = fabsf(A.scale) * LOG2E;
+            const float sign = A.scale < 0.0f ? -1.0f : 1.0f;
+            const bool some = in && A.scale != 0.0f;
+            if (A.scale == 0.0f) f = 1.0f;
+            float x[LE / 8][8];
+            float top = 0.0f;
+#pragma unroll
+            for (int k = 0; k < LE / 8; k++) {
+                load_q8(q, some, A.qvec, q4_part<HD>(c, k), x[k]);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    x[k][i] *= sign;
+                    if constexpr (HILO) top = fmaxf(top, fabsf(x[k][i]));
+                }
+            }
+            float down = 1.0f;
+            if constexpr (HILO) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // 2^e <= max |q| < 2^(e + 1), e within what 2^e and 2^-e can be
+                const int e = min(max((int)(__float_as_uint(top) >> 23), 2), 252);
+                down = __uint_as_float((uint32_t)(254 - e) << 23);
+                f *= __uint_as_float((uint32_t)e << 23);
+            }
+#pragma unroll
+            for (int k = 0; k < LE / 8; k++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int s = (4 * k + j) / 2, i = j & 1;
+                    if constexpr (HILO) split2(x[k][j] * down, x[k][4 + j] * down, qh[n][s][i], ql[n][s][i]);
+                    else qh[n][s][i] = pack(x[k][j], x[k][4 + j]);
+                }
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                cf[n][y] = __shfl_sync(0xffffffffu, f, (col + y) * 4);
+                const int mm = n * 8 + col + y;
+                ps[n][y] = mm < w.mrows ? w.first + token_of(A, w.m0 + mm) : -1;
+                lo[n][y] = A.window > 0 ? ps[n][y] - A.window + 1 : 0;
+            }
+        }
+        // keys that every row of the tile sees
+        const int p_min = w.p_own, l_max = A.window > 0 ? w.first + token_of(A, w.m0 + w.mrows - 1) - A.window + 1 : 0;
+        const bool one_token = LIST || token_of(A, w.m0) == token_of(A, w.m0 + w.mrows - 1);
+
+        float o[NQ][DT][4];
+        float mx[NQ][2], sum[NQ][2];  // running maximum in log2 units; sum of this thread's keys only
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+#pragma unroll
+                for (int y = 0; y < 4; y++) o[n][t][y] = 0.0f;
+            mx[n][0] = mx[n][1] = -INFINITY;
+            sum[n][0] = sum[n][1] = 0.0f;
+        }
+        const int stages = (w.c1 - w.c0 + QS_KEYS - 1) / QS_KEYS;
+        for (int k = 0; k < stages; k++) {
+            if (!lost && !mbar_wait(&B.full[st], phase, &B.abort)) lost = true;
+            __syncwarp();
+            const uint32_t base = ring + st * Sh::STAGE;
+            const uint32_t kt = base + warp * 2 * SP_TK * ROWB, vt = kt + Sh::CODES;
+            const uint32_t ksc = base + 2 * Sh::CODES + warp * 2 * SP_TK * SCB, vsc = ksc + Sh::SCALES;
+            const uint2 in2 = *reinterpret_cast<const uint2*>(&B.in[st][2 * warp]);
+            const uint32_t in[2] = {in2.x, in2.y};
+            const int j0 = w.c0 + k * QS_KEYS + warp * 2 * SP_TK;
+            if ((in[0] | in[1]) && !lost) {
+                // ---- S^T = K Q^T: [0], [1] = key k0 and this thread's two columns, [2], [3] = key k0 + 8
+                float s[2][NQ][4];
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    uint32_t w0[LE / 8], w1[LE / 8];
+                    __half2 s0[1], s1[1], z0[1], z1[1];
+                    q4_key_words<HD>(kt + b * SP_TK * ROWB, ksc + b * SP_TK * SCB, k0, HD, w0, s0, z0);
+                    q4_key_words<HD>(kt + b * SP_TK * ROWB, ksc + b * SP_TK * SCB, k0 + 8, HD, w1, s1, z1);
+                    float sl[HILO ? NQ : 1][4];
+#pragma unroll
+                    for (int n = 0; n < NQ; n++)
+#pragma unroll
+                        for (int y = 0; y < 4; y++) {
+                            s[b][n][y] = 0.0f;
+                            if constexpr (HILO) sl[n][y] = 0.0f;
+                        }
+#pragma unroll
+                    for (int x = 0; x < LE / 8; x++) {
+                        uint32_t e[4], f[4];
+                        q4_pairs(w0[x], s0[0], z0[0], e);
+                        q4_pairs(w1[x], s1[0], z1[0], f);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const uint32_t a[4] = {e[2 * h], f[2 * h], e[2 * h + 1], f[2 * h + 1]};
+#pragma unroll
+                            for (int n = 0; n < NQ; n++) {
+                                mma16(s[b][n], a, qh[n][2 * x + h][0], qh[n][2 * x + h][1]);
+                                if constexpr (HILO) mma16(sl[n], a, ql[n][2 * x + h][0], ql[n][2 * x + h][1]);
+                            }
+                        }
+                    }
+                    if constexpr (HILO) {
+#pragma unroll
+                        for (int n = 0; n < NQ; n++)
+#pragma unroll
+                            for (int y = 0; y < 4; y++) s[b][n][y] += sl[n][y];
+                    }
+                }
+                // ---- weights
+                const bool full = (in[0] & in[1]) == 0xffffu && (LIST || (j0 + 2 * SP_TK - 1 <= p_min && j0 >= l_max));
+                if (!full) {
+#pragma unroll
+                    for (int b = 0; b < 2; b++)
+#pragma unroll
+                        for (int n = 0; n < NQ; n++)
+#pragma unroll
+                            for (int y = 0; y < 4; y++) {
+                                const int key = k0 + (y >> 1) * 8, j = j0 + b * SP_TK + key;
+                                if (!(in[b] >> key & 1u) || (!LIST && (j > ps[n][y & 1] || j < lo[n][y & 1]))) s[b][n][y] = -INFINITY;
+                            }
+                }
+#pragma unroll
+                for (int n = 0; n < NQ; n++) {
+                    float nm[2];
+#pragma unroll
+                    for (int y = 0; y < 2; y++) nm[y] = fmaxf(fmaxf(s[0][n][y], s[0][n][2 + y]), fmaxf(s[1][n][y], s[1][n][2 + y]));
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) {
+                        nm[0] = fmaxf(nm[0], __shfl_xor_sync(0xffffffffu, nm[0], d));
+                        nm[1] = fmaxf(nm[1], __shfl_xor_sync(0xffffffffu, nm[1], d));
+                    }
+                    nm[0] *= cf[n][0];
+                    nm[1] *= cf[n][1];
+                    if (__any_sync(0xffffffffu, nm[0] > mx[n][0] + TAU || nm[1] > mx[n][1] + TAU)) {
+#pragma unroll
+                        for (int y = 0; y < 2; y++) {
+                            const float m = nm[y] > mx[n][y] + TAU ? nm[y] : mx[n][y];
+                            const float f = m == mx[n][y] ? 1.0f : pow2<true>(mx[n][y] - m);
+                            mx[n][y] = m;
+                            sum[n][y] *= f;
+#pragma unroll
+                            for (int t = 0; t < DT; t++) {
+                                o[n][t][y] *= f;
+                                o[n][t][2 + y] *= f;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int y = 0; y < 2; y++) {
+                        const float b = mx[n][y] == -INFINITY ? 0.0f : mx[n][y] - BIAS;
+#pragma unroll
+                        for (int i = 0; i < 2; i++)
+#pragma unroll
+                            for (int z = 0; z < 2; z++) s[i][n][2 * z + y] = pow2<true>(fmaf(s[i][n][2 * z + y], cf[n][y], -b));
+                        sum[n][y] += (s[0][n][y] + s[0][n][2 + y]) + (s[1][n][y] + s[1][n][2 + y]);
+                    }
+                }
+                // ---- O^T += V^T P^T
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const uint32_t vt_b = vt + b * SP_TK * ROWB, vsc_b = vsc + b * SP_TK * SCB;
+                    // A key that some rows of the tile see and others do not must not
+                    // reach the latter through 0 * v where v is not finite: such a
+                    // tile adds its products one by one, masked keys left out.
+                    bool careful = false;
+                    if (!LIST && !full && !one_token) {
+                        uint32_t bad = 0;
+                        for (int x = lane; x < SP_TK * SCB / 4; x += 32) bad |= (lds_u32(vsc_b + 4 * x) & 0x7C007C00u) + 0x04000400u;
+                        careful = __any_sync(0xffffffffu, (bad & 0x80008000u) != 0);
+                    }
+                    if (!LIST && careful) {
+                        for (int key = 0; key < SP_TK; key++) {
+                            const int src = q4_key(key & 7) * 4 + c, j = j0 + b * SP_TK + key;
+                            const bool key_in = in[b] >> key & 1u;
+#pragma unroll
+                            for (int n = 0; n < NQ; n++)
+#pragma unroll
+                                for (int y = 0; y < 2; y++) {
+                                    const float p = __shfl_sync(0xffffffffu, key < 8 ? s[b][n][y] : s[b][n][2 + y], src);
+                                    if (!key_in || j > ps[n][y] || j < lo[n][y]) continue;
+#pragma unroll
+                                    for (int t = 0; t < DT; t++)
+#pragma unroll
+                                        for (int z = 0; z < 2; z++)
+                                            o[n][t][2 * z + y] = fmaf(p, q4_value<HD>(vt_b, vsc_b, key, (lane >> 2) * (HD / 8) + 2 * t + z), o[n][t][2 * z + y]);
+                                }
+                            __syncwarp();
+                        }
+                        continue;
+                    }
+                    uint32_t ph[NQ][2], pl[HILO ? NQ : 1][2];  // P^T as B fragments
+#pragma unroll
+                    for (int n = 0; n < NQ; n++)
+#pragma unroll
+                        for (int y = 0; y < 2; y++) {
+                            if constexpr (HILO) {
+                                split2(s[b][n][2 * y], s[b][n][2 * y + 1], ph[n][y], pl[n][y]);
+                                pl[n][y] = mov_trans(pl[n][y]);
+                            } else {
+                                ph[n][y] = pack(s[b][n][2 * y], s[b][n][2 * y + 1]);
+                            }
+                            ph[n][y] = mov_trans(ph[n][y]);
+                        }
+                    uint32_t vw[4][LE / 16];
+                    __half2 sv[2], sz[2];
+                    q4_value_words<HD>(vt_b, vsc_b, in[b], vw, sv, sz);
+#pragma unroll
+                    for (int h = 0; h < HD / 32; h++) {  // four columns
+                        uint32_t e[4], f[4];
+                        q4_pairs(__byte_perm(vw[0][h / 2], vw[1][h / 2], h & 1 ? 0x7632 : 0x5410), sv[0], sz[0], e);
+                        q4_pairs(__byte_perm(vw[2][h / 2], vw[3][h / 2], h & 1 ? 0x7632 : 0x5410), sv[1], sz[1], f);
+#pragma unroll
+                        for (int y = 0; y < 2; y++) {
+                            const uint32_t a[4] = {e[2 * y], e[2 * y + 1], f[2 * y], f[2 * y + 1]};
+                            const int t = 2 * h + y;
+#pragma unroll
+                            for (int n = 0; n < NQ; n++) {
+                                if constexpr (HILO) {
+                                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                    mma16(d, a, pl[n][0], pl[n][1]);
+                                    mma16(d, a, ph[n][0], ph[n][1]);
+#pragma unroll
+                                    for (int z = 0; z < 4; z++) o[n][t][z] += d[z];
+                                } else {
+                                    mma16(o[n][t], a, ph[n][0], ph[n][1]);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B.empty[st]);
+            if (++st == S) {
+                st = 0;
+                phase ^= 1;
+            }
+        }
+        if (lost) {  // (a copy that never came: not a number, rather than a wrong one)
+#pragma unroll
+            for (int n = 0; n < NQ; n++) sum[n][0] = sum[n][1] = __int_as_float(0x7FC00000);
+        }
+
+        // ---- this warp's (m, l, o) to shared memory, the four warps' joined
+        float* so = reinterpret_cast<float*>(outs + warp * Sh::OUT);
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) sum[n][y] += __shfl_xor_sync(0xffffffffu, sum[n][y], d);
+                if (lane < 4) {
+                    s_m[warp][n * 8 + col + y] = mx[n][y];
+                    s_l[warp][n * 8 + col + y] = sum[n][y];
+                }
+#pragma unroll
+                for (int t = 0; t < DT; t++)
+                    *reinterpret_cast<float2*>(so + (n * 8 + col + y) * LDO + (lane >> 2) * (HD / 8) + 2 * t) = make_float2(o[n][t][y], o[n][t][2 + y]);
+            }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        constexpr int HQ = HD >> 2;
+        for (int x = threadIdx.x; x < w.mrows * HQ; x += 32 * QS_WARPS) {
+            const int m = x / HQ, d = (x - m * HQ) * 4;
+            float mm = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < QS_WARPS; i++) mm = fmaxf(mm, s_m[i][m]);
+            float l = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < QS_WARPS; i++) {
+                if (s_l[i][m] == 0.0f) continue;  // saw nothing
+                const float f = exp2f(s_m[i][m] - mm);
+                const float4 y = *reinterpret_cast<const float4*>(outs + i * Sh::OUT + (m * LDO + d) * 4);
+                l = fmaf(f, s_l[i][m], l);
+                v.x = fmaf(f, y.x, v.x);
+                v.y = fmaf(f, y.y, v.y);
+                v.z = fmaf(f, y.z, v.z);
+                v.w = fmaf(f, y.w, v.w);
+            }
+            if (!w.cut) {
+                const int t = token_of(A, w.m0 + m), row = w.r0 + t, head = w.kvh * A.G + (w.m0 + m) - t * A.G;
+                store_row4<QT>(A, row, head, d, l, v);
+                if (A.lse && d == 0) A.lse[(int64_t)row * A.nh + head] = l == 0.0f ? -INFINITY : (mm - BIAS + log2f(l)) / LOG2E;
+            } else {
+                *reinterpret_cast<float4*>(X.po + (w.slot * R + m) * HD + d) = v;
+                if (d == 0) X.pml[w.slot * R + m] = make_float2(mm == -INFINITY ? mm : mm - BIAS, l);
+            }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+    }
+}
+
+template <typename QT, int HD, int NQ, bool LIST>
+int launch_stream_t(SplitArgs& X, cudaStream_t s) {
+    using Sh = StreamShape<HD, NQ>;
+    HC_CUDA(cudaFuncSetAttribute(k_paged_q4<QT, HD, NQ, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
+    static const int resident = [] {
+        int n = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_paged_q4<QT, HD, NQ, LIST>, QS_THREADS, Sh::SMEM) != cudaSuccess) n = 1;
+        return std::min(std::max(n, 1), SP_CTAS / 148);
+    }();
+    X.ctas = 148 * resident;
+    const int64_t pairs = pairs_bound(X);
+    HC_CHECK(pairs <= 0x7fffffff, HC_ERR_INVALID, "paged attention: %d rows of %d heads", X.a.p.n_rows, X.a.nh);
+    k_paged_q4<QT, HD, NQ, LIST><<<X.whole ? (unsigned)pairs : (unsigned)X.ctas, QS_THREADS, Sh::SMEM, s>>>(X);
+    HC_LAUNCH_CHECK();
+    return X.whole ? HC_OK : launch_join<QT, LIST>(X, pairs, s);
+}
+
+template <typename QT, bool LIST>
+int launch_stream_hd(SplitArgs& X, cudaStream_t s) {
+    if (X.rows == 8) return X.a.p.hd == 64 ? launch_stream_t<QT, 64, 1, LIST>(X, s) : launch_stream_t<QT, 128, 1, LIST>(X, s);
+    return X.a.p.hd == 64 ? launch_stream_t<QT, 64, 2, LIST>(X, s) : launch_stream_t<QT, 128, 2, LIST>(X, s);
+}
+
+}  // namespace
+
+int launch_q4_stream(SplitArgs& X, int q16, cudaStream_t s) {
+    if (X.l.width) return q16 ? launch_stream_hd<__half, true>(X, s) : launch_stream_hd<float, true>(X, s);
+    return q16 ? launch_stream_hd<__half, false>(X, s) : launch_stream_hd<float, false>(X, s);
+}
+
+}  // namespace hc

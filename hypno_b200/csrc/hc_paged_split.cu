@@ -59,6 +59,7 @@ int launch_paged_split(const PagedAttnArgs& A, const PagedScales& C, const Paged
              C.kss == sl && C.vss == sl && (C.kps | C.khs | C.vps | C.vhs) % 8 == 0 && ((uintptr_t)C.k | (uintptr_t)C.v) % 16 == 0;
     X.po = (float*)ws;
     X.pml = (float2*)((float*)ws + (size_t)2 * SP_CTAS * 16 * A.p.hd);
+    if (X.bulk && A.p.hd <= 128) return launch_q4_stream(X, q16, s);
     if (L.width) return launch_split_list(X, q16, kv, s);
     return kv == HC_KV_Q4 ? launch_split_q4(X, q16, s) : launch_split_dense(X, q16, kv, s);
 }

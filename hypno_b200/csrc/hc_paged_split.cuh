@@ -696,7 +696,11 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
             mx[n][0] = mx[n][1] = -INFINITY;
             sum[n][0] = sum[n][1] = 0.0f;
         }
-        constexpr float BIAS = C16 ? 14.0f : 0.0f;
+        // Planned forms: the maximum stays until a score passes it by 2^TAU, so that the
+        // outputs are rarely scaled (a tile in three raises one of its rows' maxima
+        // by a little); a weight is at most 2^(BIAS + TAU), one of 2^-25 of the largest
+        // still has 11 bits.
+        constexpr float BIAS = PLAN && C16 ? 11.0f : C16 ? 14.0f : 0.0f, TAU = PLAN ? 4.0f : 0.0f;
         const int mi = lane >> 3;
         // ldmatrix rows: K as A (keys x d), V transposed as A (d x keys)
         const int krow = (lane & 7) + (mi & 1) * 8, vrow = (lane & 7) + (mi >> 1) * 8;
@@ -809,10 +813,10 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
                     nm[0] = fmaxf(nm[0], __shfl_xor_sync(0xffffffffu, nm[0], d));
                     nm[1] = fmaxf(nm[1], __shfl_xor_sync(0xffffffffu, nm[1], d));
                 }
-                if (__any_sync(0xffffffffu, nm[0] > mx[n][0] || nm[1] > mx[n][1])) {
+                if (__any_sync(0xffffffffu, nm[0] > mx[n][0] + TAU || nm[1] > mx[n][1] + TAU)) {
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        const float m = fmaxf(nm[x], mx[n][x]);
+                        const float m = PLAN && !(nm[x] > mx[n][x] + TAU) ? mx[n][x] : fmaxf(nm[x], mx[n][x]);
                         const float f = m == mx[n][x] ? 1.0f : pow2<PLAN>(mx[n][x] - m);
                         mx[n][x] = m;
                         sum[n][x] *= f;
@@ -1092,6 +1096,14 @@ inline int64_t pairs_bound(const SplitArgs& X) {
     return ((int64_t)X.a.p.n_rows * X.a.G / X.rows + X.a.p.n_seqs) * X.a.p.nkv;
 }
 
+template <typename QT, bool LIST>
+int launch_join(const SplitArgs& X, int64_t pairs, cudaStream_t s) {
+    const int y = (std::min(X.rows, X.a.G) * X.a.p.hd / 4 + SP_THREADS - 1) / SP_THREADS;
+    HC_TRY(launch_pdl(k_paged_join<QT, LIST>, dim3((unsigned)pairs, std::max(y, 1)), dim3(SP_THREADS), 0, s, X));
+    HC_LAUNCH_CHECK();
+    return HC_OK;
+}
+
 template <typename QT, typename CT, int HD, int NQ, bool LIST>
 int launch_split_t(SplitArgs& X, cudaStream_t s) {
     using Sh = SplitShape<CT, HD>;
@@ -1107,12 +1119,7 @@ int launch_split_t(SplitArgs& X, cudaStream_t s) {
     HC_CHECK(pairs <= 0x7fffffff, HC_ERR_INVALID, "paged attention: %d rows of %d heads", P.n_rows, X.a.nh);
     k_paged_split<QT, CT, HD, NQ, LIST><<<X.whole ? (unsigned)pairs : (unsigned)X.ctas, SP_THREADS, Sh::SMEM, s>>>(X);
     HC_LAUNCH_CHECK();
-    if (!X.whole) {
-        const int y = (std::min(X.rows, X.a.G) * P.hd / 4 + SP_THREADS - 1) / SP_THREADS;
-        HC_TRY(launch_pdl(k_paged_join<QT, LIST>, dim3((unsigned)pairs, std::max(y, 1)), dim3(SP_THREADS), 0, s, X));
-        HC_LAUNCH_CHECK();
-    }
-    return HC_OK;
+    return X.whole ? HC_OK : launch_join<QT, LIST>(X, pairs, s);
 }
 
 template <typename QT, typename CT, bool LIST>
@@ -1132,5 +1139,6 @@ int launch_split_hd(SplitArgs& X, cudaStream_t s) {
 int launch_split_dense(SplitArgs& X, int q16, int kv, cudaStream_t s);
 int launch_split_q4(SplitArgs& X, int q16, cudaStream_t s);
 int launch_split_list(SplitArgs& X, int q16, int kv, cudaStream_t s);
+int launch_q4_stream(SplitArgs& X, int q16, cudaStream_t s);
 
 }  // namespace hc
