@@ -2,11 +2,12 @@
 // whose pages are runs of memory (k_paged_split takes the other layouts).
 //
 // The line of units, its runs, the join and the products are k_paged_split's.  A
-// fifth warp copies: a stage is 128 keys, eight tiles of 16, and each of its lanes
-// copies one tile's codes or scales of K or V as one run (cp.async.bulk, counted by
-// the stage's mbarrier), so a page's place is worked out once and the four warps that
-// compute spend nothing on it.  Each takes 32 keys of a stage: two tiles whose
-// chains of dependent steps (codes, products, maxima, weights, products) overlap.
+// fifth warp copies: a stage is 128 keys, eight tiles of 16 in a page each, so a
+// page's place is worked out once a tile and the four warps that compute spend
+// nothing on it.  Each takes 32 keys of a stage: two tiles whose chains of dependent
+// steps (codes, products, maxima, weights, products) overlap.  16 bytes a lane and
+// copy (one run a tile and pool, cp.async.bulk, took the copy engine's time: 391,000 runs
+// of 128 and 1,024 bytes 49 us where the same bytes in runs of four times that took 43).
 //
 // A key's codes become float16 in registers (q4_pairs, 11 instructions for eight
 // elements), which is most of what the kernel does: shifts, logic and float16
@@ -18,9 +19,9 @@ namespace hc {
 
 namespace {
 
-constexpr int QS_WARPS = 4, QS_THREADS = 32 * (QS_WARPS + 1), QS_TILES = 2 * QS_WARPS, QS_KEYS = SP_TK * QS_TILES;
+constexpr int QS_WARPS = 4, QS_ROWS = 32 * QS_WARPS, QS_THREADS = QS_ROWS + 32, QS_TILES = 2 * QS_WARPS, QS_KEYS = SP_TK * QS_TILES;
 
-template <int HD, int NQ>
+template <int HD, int NQ, bool HILO>
 struct StreamShape {
     static constexpr int ROWB = HD / 2, SCB = 2 * q4_slots(HD);
     static constexpr int CODES = QS_KEYS * ROWB, SCALES = QS_KEYS * SCB;  // of K or V
@@ -28,7 +29,9 @@ struct StreamShape {
     static constexpr int STAGES = HD <= 64 ? 4 : 3;
     static constexpr int LDO = HD + 4;
     static constexpr int OUT = 8 * NQ * LDO * 4;                          // a warp's outputs
+    static constexpr int QF = NQ * (HD / 16) * 32 * (HILO ? 4 : 2);       // the queries' fragments, in words
     static constexpr int SMEM = STAGES * STAGE + QS_WARPS * OUT + 128;
+    static_assert(QF * 4 <= QS_WARPS * OUT, "the queries' fragments lie where the outputs go later");
 };
 
 // One CTA's share of a pair.
@@ -80,91 +83,105 @@ struct StreamBars {
     int abort;
 };
 
+// Waits a bounded time; the whole warp.  (The clock is read when the first look fails.)
+__device__ __forceinline__ bool stream_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+// Arrives at the barrier when this thread's copies so far have landed.
+__device__ __forceinline__ void cp_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 // The copying warp.
-template <int HD, int NQ, bool LIST>
-__device__ __forceinline__ void stream_copies(const SplitArgs& X, StreamBars<StreamShape<HD, NQ>::STAGES>& B, uint32_t ring, int64_t u_begin, int64_t u_end) {
-    using Sh = StreamShape<HD, NQ>;
-    constexpr int S = Sh::STAGES;
+template <typename Sh, int HD, bool LIST>
+__device__ __forceinline__ void stream_copies(const SplitArgs& X, StreamBars<Sh::STAGES>& B, uint32_t ring, int64_t u_begin, int64_t u_end) {
+    constexpr int S = Sh::STAGES, CHUNKS = HD / 32, ROWS = 32 / CHUNKS;  // a row's 16-byte pieces, rows that the lanes copy at once
     const PagedAttnArgs& A = X.a;
     const PagedArgs& P = A.p;
-    const int lane = threadIdx.x & 31, tile = lane >> 2;
-    const bool is_v = lane & 1, is_s = lane & 2;
-    const uint8_t* pool = (const uint8_t*)(is_s ? (is_v ? (const void*)X.c.v : (const void*)X.c.k) : is_v ? P.v : P.k);
-    const int64_t ps = is_s ? 2 * (is_v ? X.c.vps : X.c.kps) : is_v ? P.vps : P.kps;
-    const int64_t hs = is_s ? 2 * (is_v ? X.c.vhs : X.c.khs) : is_v ? P.vhs : P.khs;
-    const uint32_t pos_bytes = is_s ? Sh::SCB : Sh::ROWB, bytes = SP_TK * pos_bytes;
-    const uint32_t to = ring + (is_s ? 2 * Sh::CODES + (is_v ? Sh::SCALES : 0) : (is_v ? Sh::CODES : 0)) + tile * bytes;
+    const int lane = threadIdx.x & 31, tile = lane & 7, kind = lane >> 3;  // what this lane works out: K, V codes, K, V scales
+    const int row = lane / CHUNKS, chunk = lane % CHUNKS, srow = lane & 15;
+    const bool sv = lane >= 16;  // this lane copies scales of V
+    const uint32_t to = ring + lane * 16, to_s = ring + 2 * Sh::CODES + (sv ? Sh::SCALES : 0) + srow * Sh::SCB;
     int64_t u = u_begin;
     Line at = {0, 0, {}};
     PairWork w;
     uint32_t n = 0;  // stages so far
     bool ok = true;
     while (ok && next_pair<LIST>(X, u, u_begin, u_end, at, w)) {
-        const uint8_t* from = pool + w.kvh * hs;
+        const uint8_t* kb = (const uint8_t*)P.k + w.kvh * P.khs + row * P.kss + chunk * 16;
+        const uint8_t* vb = (const uint8_t*)P.v + w.kvh * P.vhs + row * P.vss + chunk * 16;
+        const uint8_t* sb = (const uint8_t*)(sv ? X.c.v + w.kvh * X.c.vhs + srow * X.c.vss : X.c.k + w.kvh * X.c.khs + srow * X.c.kss);
+        // bytes from page to page and from position to position of this lane's kind
+        const int64_t page_bytes = kind == 0 ? P.kps : kind == 1 ? P.vps : 2 * (kind == 2 ? X.c.kps : X.c.vps);
+        const int64_t pos_bytes = kind == 0 ? P.kss : kind == 1 ? P.vss : 2 * (kind == 2 ? X.c.kss : X.c.vss);
+        const int64_t k_step = ROWS * P.kss, v_step = ROWS * P.vss;
         const int stages = (w.c1 - w.c0 + QS_KEYS - 1) / QS_KEYS;
         auto entry_of = [&](int k) {  // LIST: the index that the list has for this lane's tile
             const int64_t v = w.c0 + (int64_t)k * QS_KEYS + tile * SP_TK;
             return LIST && v < w.c1 ? __ldg(w.list + page_of(P, (int)v)) : 0;
         };
-        auto place_of_tile = [&](int k, int entry, uint32_t& place) {  // page, -1: none; slot << 16 | keys
-            place = 0;
+        auto place_of_tile = [&](int k, int entry, uint32_t& keys) {  // bytes from the pool's start, the keys that are there
+            keys = 0;
             const int64_t v = w.c0 + (int64_t)k * QS_KEYS + tile * SP_TK;
-            if (v >= w.c1) return -1;
+            if (v >= w.c1) return (int64_t)0;
             int x = page_of(P, (int)v), have = min(SP_TK, w.c1 - (int)v), low = 0;
             const int slot = (int)v - x * P.page_size;
             if constexpr (LIST) {
                 x = entry;
-                if (x >= P.max_pages) return -1;
+                if (x >= P.max_pages) return (int64_t)0;
                 const int64_t pos = (int64_t)x * P.page_size + slot;
                 have = (int)min((int64_t)have, w.p_own - pos + 1);
                 if (A.window > 0) low = (int)min(max(w.p_own - A.window + 1 - pos, (int64_t)0), (int64_t)SP_TK);
-                if (have <= low) return -1;
+                if (have <= low) return (int64_t)0;
             }
-            const int g = __ldg(P.table + (int64_t)w.seq * P.table_stride + x);
-            if ((unsigned)g >= (unsigned)P.n_pages) return -1;
-            place = (uint32_t)slot << 16 | (((1u << have) - 1) & ~((1u << low) - 1));
-            return g;
+            const int64_t g = __ldg(P.table + (int64_t)w.seq * P.table_stride + x);
+            if ((uint64_t)g >= (uint64_t)P.n_pages) return (int64_t)0;
+            keys = ((1u << have) - 1) & ~((1u << low) - 1);
+            return g * page_bytes + slot * pos_bytes;
         };
-        uint32_t place;
-        int page = place_of_tile(0, entry_of(0), place);
+        uint32_t keys;
+        int64_t from = place_of_tile(0, entry_of(0), keys);
         int entry = entry_of(1);
         for (int k = 0; k < stages; k++, n++) {
-            uint32_t next_place;
-            const int next_page = place_of_tile(k + 1, entry, next_place);
+            uint32_t next_keys;
+            const int64_t next_from = place_of_tile(k + 1, entry, next_keys);
             entry = entry_of(k + 2);
             const uint32_t st = n % S;
-            if (n >= S && !mbar_wait(&B.empty[st], (n / S & 1) ^ 1, &B.abort)) {
+            if (n >= S && !stream_wait(&B.empty[st], (n / S & 1) ^ 1, &B.abort)) {
                 ok = false;
                 break;
             }
-            if ((lane & 3) == 0) B.in[st][tile] = place & 0xffffu;
-            const int copies = __popc(__ballot_sync(0xffffffffu, page >= 0)) >> 2;
-            __syncwarp();
-            if (lane == 0) {
-                if (copies) mbar_expect_tx(&B.full[st], copies * (Sh::STAGE / QS_TILES));
-                else mbar_arrive(&B.full[st]);
+            if (kind == 0) B.in[st][tile] = keys;
+            const uint32_t base = st * Sh::STAGE, there = __ballot_sync(0xffffffffu, keys != 0);
+#pragma unroll
+            for (int x = 0; x < QS_TILES; x++) {
+                if (!(there >> x & 1u)) continue;
+                const uint8_t* kf = kb + __shfl_sync(0xffffffffu, from, x);
+                const uint8_t* vf = vb + __shfl_sync(0xffffffffu, from, 8 + x);
+                const uint8_t* sf = sb + __shfl_sync(0xffffffffu, from, (sv ? 24 : 16) + x);
+#pragma unroll
+                for (int y = 0; y < SP_TK / ROWS; y++) {
+                    const uint32_t d = to + base + x * SP_TK * Sh::ROWB + y * 512;
+                    cp16(d, kf + y * k_step, true);
+                    cp16(d + Sh::CODES, vf + y * v_step, true);
+                }
+                cp_small<Sh::SCB>(to_s + base + x * SP_TK * Sh::SCB, sf, true);
             }
-            __syncwarp();
-            if (page >= 0) cp_run(to + st * Sh::STAGE, from + page * ps + (int64_t)(place >> 16) * pos_bytes, bytes, &B.full[st]);
-            page = next_page;
-            place = next_place;
+            cp_arrive(&B.full[st]);
+            from = next_from;
+            keys = next_keys;
         }
     }
-    // every copy has landed before the CTA ends: the rows' warps waited for all of
-    // them, unless a wait ran out
-    if (!ok) {
-        const long long start = clock64();
-        for (uint32_t k = n > S ? n - S : 0; k < n; k++)
-            while (!mbar_try_wait(&B.full[k % S], k / S & 1) && clock64() - start < WAIT_CYCLES) {}
-    }
+    cp_commit();
+    cp_wait<0>();  // every copy has landed before the CTA ends
 }
 
 template <typename QT, int HD, int NQ, bool LIST>
 __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const __grid_constant__ SplitArgs X) {
-    using Sh = StreamShape<HD, NQ>;
+    using Sh = StreamShape<HD, NQ, sizeof(QT) == 4>;
     constexpr int R = 8 * NQ, S = Sh::STAGES, ROWB = Sh::ROWB, SCB = Sh::SCB, LDO = Sh::LDO;
     constexpr bool HILO = sizeof(QT) == 4;
-    constexpr int DT = HD / 16, KS = HD / 16, LE = HD / 4;
+    constexpr int DT = HD / 16, KS = HD / 16, LE = HD / 4, FW = HILO ? 4 : 2;
     // the maximum stays until a score passes it by 2^TAU; weights are held times
     // 2^BIAS in fp16, so that one of 2^-25 of the largest still has 11 bits
     constexpr float BIAS = 11.0f, TAU = 4.0f;
@@ -173,11 +190,11 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
     extern __shared__ __align__(128) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 127u);
     __shared__ StreamBars<S> B;
-    __shared__ float s_m[QS_WARPS][R], s_l[QS_WARPS][R];
+    __shared__ float s_m[QS_WARPS][R], s_l[QS_WARPS][R], s_cf[R];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; i++) {
-            mbar_init(&B.full[i], 1);
+            mbar_init(&B.full[i], 32);
             mbar_init(&B.empty[i], QS_WARPS);
         }
         B.abort = 0;
@@ -193,10 +210,12 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
     }
     const uint32_t ring = smem_u32(smem);
     if (warp == QS_WARPS) {
-        stream_copies<HD, NQ, LIST>(X, B, ring, u, u_end);
+        stream_copies<Sh, HD, LIST>(X, B, ring, u, u_end);
         return;
     }
     uint8_t* outs = smem + S * Sh::STAGE;
+    uint32_t* qf = reinterpret_cast<uint32_t*>(outs);  // until the outputs: [tile of rows][16 elements][lane][hi, hi (, lo, lo)]
+    const uint32_t qs = smem_u32(qf);
     const int64_t u_begin = u;
     Line at = {0, 0, {}};
     PairWork w;
@@ -204,58 +223,49 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
     bool lost = false;
     const int c = lane & 3, col = 2 * c, k0 = q4_key(lane >> 2);
     while (next_pair<LIST>(X, u, u_begin, u_end, at, w)) {
-        // ---- queries as B fragments: column lane / 4 of each tile of eight rows
-        uint32_t qh[NQ][KS][2];
-        uint32_t ql[HILO ? NQ : 1][HILO ? KS : 1][2];
-        float cf[NQ][2];           // score factors of this thread's two columns, not negative
-        int ps[NQ][2], lo[NQ][2];  // their positions and first visible positions
-#pragma unroll
-        for (int n = 0; n < NQ; n++) {
-            const int m = n * 8 + (lane >> 2);
+        // ---- queries as B fragments, once for all warps: eight elements a thread
+        constexpr int QW = HD / 8;
+        for (int i = threadIdx.x; i < R * QW; i += QS_ROWS) {  // (whole warps: R QW is a multiple of 32)
+            const int m = i / QW, kw = i % QW;
             const bool in = m < w.mrows;
             const int t = token_of(A, w.m0 + m);
             const QT* q = (const QT*)A.q + (in ? (int64_t)(w.r0 + t) * A.q_rs + (w.kvh * A.G + (w.m0 + m) - t * A.G) * A.q_hs : 0);
             // (a factor below zero turns the query's sign, one of zero its elements to zeros)
-            float f = fabsf(A.scale) * LOG2E;
-            const float sign = A.scale < 0.0f ? -1.0f : 1.0f;
-            const bool some = in && A.scale != 0.0f;
-            if (A.scale == 0.0f) f = 1.0f;
-            float x[LE / 8][8];
-            float top = 0.0f;
-#pragma unroll
-            for (int k = 0; k < LE / 8; k++) {
-                load_q8(q, some, A.qvec, q4_part<HD>(c, k), x[k]);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    x[k][i] *= sign;
-                    if constexpr (HILO) top = fmaxf(top, fabsf(x[k][i]));
-                }
-            }
-            float down = 1.0f;
+            float f = A.scale == 0.0f ? 1.0f : fabsf(A.scale) * LOG2E;
+            float x[8], top = 0.0f, by = A.scale < 0.0f ? -1.0f : 1.0f;
+            load_q8(q, in && A.scale != 0.0f, A.qvec, 8 * kw, x);
             if constexpr (HILO) {
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+#pragma unroll
+                for (int y = 0; y < 8; y++) top = fmaxf(top, fabsf(x[y]));
+#pragma unroll
+                for (int d = 1; d < QW; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                 // 2^e <= max |q| < 2^(e + 1), e within what 2^e and 2^-e can be
                 const int e = min(max((int)(__float_as_uint(top) >> 23), 2), 252);
-                down = __uint_as_float((uint32_t)(254 - e) << 23);
+                by *= __uint_as_float((uint32_t)(254 - e) << 23);
                 f *= __uint_as_float((uint32_t)e << 23);
             }
+            if (kw == 0) s_cf[m] = f;
+            const int part = kw / (LE / 8), k = kw % (LE / 8);  // word k of lane part's share of a key
+            uint32_t* to = qf + ((m >> 3) * KS * 32 + (m & 7) * 4 + part) * FW;
 #pragma unroll
-            for (int k = 0; k < LE / 8; k++)
+            for (int j = 0; j < 4; j++) {
+                uint32_t* z = to + (2 * k + (j >> 1)) * 32 * FW + (j & 1);
+                if constexpr (HILO) split2(x[j] * by, x[4 + j] * by, z[0], z[2]);
+                else z[0] = pack(x[j] * by, x[4 + j] * by);
+            }
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(QS_ROWS) : "memory");
+        float cf[NQ][2];           // score factors of this thread's two columns, not negative
+        int ps[NQ][2], lo[NQ][2];  // their positions and first visible positions
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int s = (4 * k + j) / 2, i = j & 1;
-                    if constexpr (HILO) split2(x[k][j] * down, x[k][4 + j] * down, qh[n][s][i], ql[n][s][i]);
-                    else qh[n][s][i] = pack(x[k][j], x[k][4 + j]);
-                }
+        for (int n = 0; n < NQ; n++)
 #pragma unroll
             for (int y = 0; y < 2; y++) {
-                cf[n][y] = __shfl_sync(0xffffffffu, f, (col + y) * 4);
                 const int mm = n * 8 + col + y;
+                cf[n][y] = s_cf[mm];
                 ps[n][y] = mm < w.mrows ? w.first + token_of(A, w.m0 + mm) : -1;
                 lo[n][y] = A.window > 0 ? ps[n][y] - A.window + 1 : 0;
             }
-        }
         // keys that every row of the tile sees
         const int p_min = w.p_own, l_max = A.window > 0 ? w.first + token_of(A, w.m0 + w.mrows - 1) - A.window + 1 : 0;
         const bool one_token = LIST || token_of(A, w.m0) == token_of(A, w.m0 + w.mrows - 1);
@@ -273,7 +283,7 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
         }
         const int stages = (w.c1 - w.c0 + QS_KEYS - 1) / QS_KEYS;
         for (int k = 0; k < stages; k++) {
-            if (!lost && !mbar_wait(&B.full[st], phase, &B.abort)) lost = true;
+            if (!lost && !stream_wait(&B.full[st], phase, &B.abort)) lost = true;
             __syncwarp();
             const uint32_t base = ring + st * Sh::STAGE;
             const uint32_t kt = base + warp * 2 * SP_TK * ROWB, vt = kt + Sh::CODES;
@@ -283,42 +293,55 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
             const int j0 = w.c0 + k * QS_KEYS + warp * 2 * SP_TK;
             if ((in[0] | in[1]) && !lost) {
                 // ---- S^T = K Q^T: [0], [1] = key k0 and this thread's two columns, [2], [3] = key k0 + 8
-                float s[2][NQ][4];
+                float s[2][NQ][4], sl[HILO ? 2 : 1][HILO ? NQ : 1][4];
 #pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    uint32_t w0[LE / 8], w1[LE / 8];
-                    __half2 s0[1], s1[1], z0[1], z1[1];
-                    q4_key_words<HD>(kt + b * SP_TK * ROWB, ksc + b * SP_TK * SCB, k0, HD, w0, s0, z0);
-                    q4_key_words<HD>(kt + b * SP_TK * ROWB, ksc + b * SP_TK * SCB, k0 + 8, HD, w1, s1, z1);
-                    float sl[HILO ? NQ : 1][4];
+                for (int b = 0; b < 2; b++)
 #pragma unroll
                     for (int n = 0; n < NQ; n++)
 #pragma unroll
                         for (int y = 0; y < 4; y++) {
                             s[b][n][y] = 0.0f;
-                            if constexpr (HILO) sl[n][y] = 0.0f;
+                            if constexpr (HILO) sl[b][n][y] = 0.0f;
                         }
+                {
+                    uint32_t w0[2][LE / 8], w1[2][LE / 8];
+                    __half2 s0[2], s1[2], z0[2], z1[2];
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        q4_key_words<HD>(kt + b * SP_TK * ROWB, ksc + b * SP_TK * SCB, k0, HD, w0[b], s0 + b, z0 + b);
+                        q4_key_words<HD>(kt + b * SP_TK * ROWB, ksc + b * SP_TK * SCB, k0 + 8, HD, w1[b], s1 + b, z1 + b);
+                    }
 #pragma unroll
                     for (int x = 0; x < LE / 8; x++) {
-                        uint32_t e[4], f[4];
-                        q4_pairs(w0[x], s0[0], z0[0], e);
-                        q4_pairs(w1[x], s1[0], z1[0], f);
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const uint32_t a[4] = {e[2 * h], f[2 * h], e[2 * h + 1], f[2 * h + 1]};
-#pragma unroll
-                            for (int n = 0; n < NQ; n++) {
-                                mma16(s[b][n], a, qh[n][2 * x + h][0], qh[n][2 * x + h][1]);
-                                if constexpr (HILO) mma16(sl[n], a, ql[n][2 * x + h][0], ql[n][2 * x + h][1]);
-                            }
-                        }
-                    }
-                    if constexpr (HILO) {
+                        uint32_t q[NQ][2][FW];
 #pragma unroll
                         for (int n = 0; n < NQ; n++)
 #pragma unroll
-                            for (int y = 0; y < 4; y++) s[b][n][y] += sl[n][y];
+                            for (int h = 0; h < 2; h++) lds_words<FW>(qs + ((n * KS + 2 * x + h) * 32 + lane) * FW * 4, q[n][h]);
+#pragma unroll
+                        for (int b = 0; b < 2; b++) {
+                            uint32_t e[4], f[4];
+                            q4_pairs(w0[b][x], s0[b], z0[b], e);
+                            q4_pairs(w1[b][x], s1[b], z1[b], f);
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const uint32_t a[4] = {e[2 * h], f[2 * h], e[2 * h + 1], f[2 * h + 1]};
+#pragma unroll
+                                for (int n = 0; n < NQ; n++) {
+                                    mma16(s[b][n], a, q[n][h][0], q[n][h][1]);
+                                    if constexpr (HILO) mma16(sl[b][n], a, q[n][h][2], q[n][h][3]);
+                                }
+                            }
+                        }
                     }
+                }
+                if constexpr (HILO) {
+#pragma unroll
+                    for (int b = 0; b < 2; b++)
+#pragma unroll
+                        for (int n = 0; n < NQ; n++)
+#pragma unroll
+                            for (int y = 0; y < 4; y++) s[b][n][y] += sl[b][n][y];
                 }
                 // ---- weights
                 const bool full = (in[0] & in[1]) == 0xffffu && (LIST || (j0 + 2 * SP_TK - 1 <= p_min && j0 >= l_max));
@@ -455,7 +478,8 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
             for (int n = 0; n < NQ; n++) sum[n][0] = sum[n][1] = __int_as_float(0x7FC00000);
         }
 
-        // ---- this warp's (m, l, o) to shared memory, the four warps' joined
+        // ---- this warp's (m, l, o) to shared memory (where the queries were), the four warps' joined
+        asm volatile("bar.sync 1, %0;" ::"n"(QS_ROWS) : "memory");
         float* so = reinterpret_cast<float*>(outs + warp * Sh::OUT);
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
@@ -472,9 +496,9 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
                     *reinterpret_cast<float2*>(so + (n * 8 + col + y) * LDO + (lane >> 2) * (HD / 8) + 2 * t) = make_float2(o[n][t][y], o[n][t][2 + y]);
             }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(QS_ROWS) : "memory");
         constexpr int HQ = HD >> 2;
-        for (int x = threadIdx.x; x < w.mrows * HQ; x += 32 * QS_WARPS) {
+        for (int x = threadIdx.x; x < w.mrows * HQ; x += QS_ROWS) {
             const int m = x / HQ, d = (x - m * HQ) * 4;
             float mm = -INFINITY;
 #pragma unroll
@@ -501,13 +525,13 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
                 if (d == 0) X.pml[w.slot * R + m] = make_float2(mm == -INFINITY ? mm : mm - BIAS, l);
             }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(QS_ROWS) : "memory");
     }
 }
 
 template <typename QT, int HD, int NQ, bool LIST>
 int launch_stream_t(SplitArgs& X, cudaStream_t s) {
-    using Sh = StreamShape<HD, NQ>;
+    using Sh = StreamShape<HD, NQ, sizeof(QT) == 4>;
     HC_CUDA(cudaFuncSetAttribute(k_paged_q4<QT, HD, NQ, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
     static const int resident = [] {
         int n = 0;
