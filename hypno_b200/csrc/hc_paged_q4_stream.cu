@@ -44,11 +44,11 @@ struct PairWork {
     const int32_t* list;
 };
 template <bool LIST>
-__device__ __forceinline__ bool next_pair(const SplitArgs& X, int64_t& u, int64_t u_begin, int64_t u_end, Line& at, PairWork& w) {
+__device__ __forceinline__ bool next_pair(const SplitArgs& X, const LineTable& line, int64_t& u, int64_t u_begin, int64_t u_end, Line& at, PairWork& w) {
     const PagedAttnArgs& A = X.a;
-    if (u >= u_end || !advance<LIST>(X, u, X.whole != 0, at)) return false;
+    if (u >= u_end || !(A.p.n_seqs <= 32 ? advance_by(line, u, at) : advance<LIST>(X, u, X.whole != 0, at))) return false;
     const int64_t rem = u - at.base;
-    const int pair = (int)(X.whole ? rem : rem / at.w.units);
+    const int pair = (int)(X.whole ? rem : quotient(rem, at.w.units));
     const int unit = X.whole ? 0 : (int)(rem - (int64_t)pair * at.w.units);
     const int nunits = X.whole ? at.w.units : (int)min((int64_t)(at.w.units - unit), u_end - u);
     w.seq = at.b;
@@ -94,7 +94,7 @@ __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
 
 // The copying warp.
 template <typename Sh, int HD, bool LIST>
-__device__ __forceinline__ void stream_copies(const SplitArgs& X, StreamBars<Sh::STAGES>& B, uint32_t ring, int64_t u_begin, int64_t u_end) {
+__device__ __forceinline__ void stream_copies(const SplitArgs& X, const LineTable& line, StreamBars<Sh::STAGES>& B, uint32_t ring, int64_t u_begin, int64_t u_end) {
     constexpr int S = Sh::STAGES, CHUNKS = HD / 32, ROWS = 32 / CHUNKS;  // a row's 16-byte pieces, rows that the lanes copy at once
     const PagedAttnArgs& A = X.a;
     const PagedArgs& P = A.p;
@@ -107,7 +107,7 @@ __device__ __forceinline__ void stream_copies(const SplitArgs& X, StreamBars<Sh:
     PairWork w;
     uint32_t n = 0;  // stages so far
     bool ok = true;
-    while (ok && next_pair<LIST>(X, u, u_begin, u_end, at, w)) {
+    while (ok && next_pair<LIST>(X, line, u, u_begin, u_end, at, w)) {
         const uint8_t* kb = (const uint8_t*)P.k + w.kvh * P.khs + row * P.kss + chunk * 16;
         const uint8_t* vb = (const uint8_t*)P.v + w.kvh * P.vhs + row * P.vss + chunk * 16;
         const uint8_t* sb = (const uint8_t*)(sv ? X.c.v + w.kvh * X.c.vhs + srow * X.c.vss : X.c.k + w.kvh * X.c.khs + srow * X.c.kss);
@@ -186,10 +186,10 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
     // 2^BIAS in fp16, so that one of 2^-25 of the largest still has 11 bits
     constexpr float BIAS = 11.0f, TAU = 4.0f;
     const PagedAttnArgs& A = X.a;
-    const PagedArgs& P = A.p;
     extern __shared__ __align__(128) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 127u);
     __shared__ StreamBars<S> B;
+    __shared__ LineTable line;
     __shared__ float s_m[QS_WARPS][R], s_l[QS_WARPS][R], s_cf[R];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
@@ -200,17 +200,18 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
         B.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == 1 && A.p.n_seqs <= 32) fill_table<LIST>(X, line);
     __syncthreads();
     pdl_trigger();  // the join may become resident; it waits for this grid's end
     int64_t u = blockIdx.x, u_end = u + 1;
     if (!X.whole) {
-        const int64_t run = run_of(all_units<LIST>(X), X.ctas);
+        const int64_t run = run_of(A.p.n_seqs <= 32 ? line.units : all_units<LIST>(X), X.ctas);
         u = blockIdx.x * run;
         u_end = u + run;
     }
     const uint32_t ring = smem_u32(smem);
     if (warp == QS_WARPS) {
-        stream_copies<Sh, HD, LIST>(X, B, ring, u, u_end);
+        stream_copies<Sh, HD, LIST>(X, line, B, ring, u, u_end);
         return;
     }
     uint8_t* outs = smem + S * Sh::STAGE;
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
     uint32_t st = 0, phase = 0;  // the next stage and the parity of its round
     bool lost = false;
     const int c = lane & 3, col = 2 * c, k0 = q4_key(lane >> 2);
-    while (next_pair<LIST>(X, u, u_begin, u_end, at, w)) {
+    while (next_pair<LIST>(X, line, u, u_begin, u_end, at, w)) {
         // ---- queries as B fragments, once for all warps: eight elements a thread
         constexpr int QW = HD / 8;
         for (int i = threadIdx.x; i < R * QW; i += QS_ROWS) {  // (whole warps: R QW is a multiple of 32)

@@ -133,7 +133,7 @@ __device__ __forceinline__ SeqWork seq_work(const SplitArgs& X, int b) {
         w.pairs = T * X.tg * A.p.nkv;
         return w;
     }
-    const int64_t tiles = ((int64_t)T * A.G + R - 1) / R;
+    const int64_t tiles = ((int64_t)T * A.G + R - 1) >> (R == 8 ? 3 : 4);
     // positions seen by any tile, at most: the last tile's end from the first tile's begin, per tile no
     // more than its window and its own tokens
     int len = min(max(0, w.first + T), A.p.reach);
@@ -141,6 +141,11 @@ __device__ __forceinline__ SeqWork seq_work(const SplitArgs& X, int b) {
     w.units = max(1, len / UNIT + (len % UNIT != 0));
     w.pairs = (int)(tiles * A.p.nkv);
     return w;
+}
+
+// a / b, neither negative: a 64-bit division takes some 500 cycles.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
 // A place on the line of units: sequence b, which begins at `base`.
@@ -194,7 +199,39 @@ __device__ __forceinline__ int64_t all_units(const SplitArgs& X) {
     return n;
 }
 __device__ __forceinline__ int64_t run_of(int64_t units, int ctas) {
-    return max((units + ctas - 1) / ctas, (int64_t)MIN_UNITS);
+    return max(quotient(units + ctas - 1, ctas), (int64_t)MIN_UNITS);
+}
+
+// The line of up to 32 sequences, worked out once a CTA (by its first warp).
+struct LineTable {
+    int64_t end[32];  // units (whole: pairs) up to each sequence's last
+    SeqWork w[32];
+    int64_t units;    // of all sequences
+};
+template <bool LIST>
+__device__ __forceinline__ void fill_table(const SplitArgs& X, LineTable& t) {
+    const int lane = threadIdx.x & 31;
+    SeqWork w = {0, 0, 0, 1, 0};
+    if (lane < X.a.p.n_seqs) w = seq_work<LIST>(X, lane);
+    int64_t incl = (int64_t)w.pairs * (X.whole ? 1 : w.units);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += x;
+    }
+    t.end[lane] = incl;
+    t.w[lane] = w;
+    if (lane == 31) t.units = incl;
+}
+// advance() by the table.
+__device__ __forceinline__ bool advance_by(const LineTable& t, int64_t u, Line& at) {
+    const int lane = threadIdx.x & 31;
+    const unsigned hit = __ballot_sync(0xffffffffu, t.end[lane] > u);
+    if (!hit) return false;
+    at.b = __ffs(hit) - 1;
+    at.base = at.b ? t.end[at.b - 1] : 0;
+    at.w = t.w[at.b];
+    return true;
 }
 
 // The packed rows of a tile: the first, and how many.
@@ -419,21 +456,27 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
     }
     pdl_trigger();  // the join may become resident; it waits for this grid's end
 
+    __shared__ LineTable s_line[1];
+    const bool table = PLAN && A.p.n_seqs <= 32;
+    if (table) {
+        if (warp == 0) fill_table<LIST>(X, s_line[0]);
+        __syncthreads();
+    }
     int64_t u, u_end;
     if (X.whole) {
         u = blockIdx.x;
         u_end = u + 1;
     } else {
-        const int64_t run = run_of(all_units<LIST>(X), X.ctas);
+        const int64_t run = run_of(table ? s_line[0].units : all_units<LIST>(X), X.ctas);
         u = blockIdx.x * run;
         u_end = u + run;
     }
     const int64_t u_begin = u;
     Line at = {0, 0, {}};
-    while (u < u_end && advance<LIST>(X, u, X.whole != 0, at)) {
+    while (u < u_end && (table ? advance_by(s_line[0], u, at) : advance<LIST>(X, u, X.whole != 0, at))) {
         const int seq = at.b, r0 = at.w.r0, first = at.w.first;
         const int64_t rem = u - at.base;
-        const int pair = (int)(X.whole ? rem : rem / at.w.units);
+        const int pair = (int)(X.whole ? rem : quotient(rem, at.w.units));
         const int unit = X.whole ? 0 : (int)(rem - (int64_t)pair * at.w.units);
         const int nunits = X.whole ? at.w.units : (int)min((int64_t)(at.w.units - unit), u_end - u);
         const bool cut = nunits < at.w.units;
@@ -1068,7 +1111,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_paged_join(const __grid_constant
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
     const int64_t p0 = before + (int64_t)pair * at.w.units, p1 = p0 + at.w.units;
-    const int c0 = (int)(p0 / run), c1 = (int)((p1 - 1) / run);
+    const int c0 = (int)quotient(p0, run), c1 = (int)quotient(p1 - 1, run);
     pdl_wait();  // (every CTA waits: the next kernel on the stream begins when this grid has ended)
     if (!any || c0 == c1) return;  // c0 == c1: one CTA took it whole
     const int kvh = pair % P.nkv, r0 = at.w.r0;
