@@ -165,7 +165,7 @@ SIGNATURES = {
     "hc_paged_values_dev": (_I, [_P, _P, _P, _P]),
     "hc_page_bounds_update_dev": (_I, [_P, _P, _P, _P]),
     "hc_page_bounds_values_dev": (_I, [_P, _P, _P, _P]),
-    "hc_page_select_workspace": (_I, [_P, _P, ctypes.POINTER(_SZ)]),
+    "hc_page_select_workspace": (_I, [_P, _P, _I, ctypes.POINTER(_SZ)]),
     "hc_page_select_dev": (_I, [_P, _P, _P, _I, _U32, _I, _I, _I, _P, _P, _SZ, _P]),
     "hc_rope_table_host": (_I, [_SZ, _SZ, _F, _P]),
     "hc_phase_name": (ctypes.c_char_p, [_I]),

@@ -46,77 +46,77 @@ __device__ __forceinline__ void key4(const PagedArgs& P, const PagedScales& C, i
     }
 }
 
-// A CTA takes one page and KV head at a time: a thread four elements of every
-// (threads / quads)-th slot, the slots' results joined in shared memory.
-constexpr int BD_THREADS = 128;
+// A warp takes one page and KV head at a time, four elements of a key a lane: heads
+// of up to 64 elements two or more keys at once, of more than 128 in two rounds.  Its
+// loads do not depend on one another, so a page's keys are requested together.
+constexpr int BD_WARPS = 4;
 
 template <typename CT, bool VEC>
-__global__ void __launch_bounds__(BD_THREADS) k_page_bounds(PagedArgs P, PagedScales C, Bounds B) {
-    __shared__ float s_lo[BD_THREADS * 4], s_hi[BD_THREADS * 4];
-    __shared__ uint32_t s_top[BD_THREADS / 32];
-    const int head = blockIdx.y, b = blockIdx.z;
+__global__ void __launch_bounds__(32 * BD_WARPS) k_page_bounds(PagedArgs P, PagedScales C, Bounds B) {
+    const int b = blockIdx.z, lane = threadIdx.x & 31;
     int r0, r1;
     seq_rows(P, b, r0, r1);
     const int n = min(seq_len(P, b), P.reach);
     const int begin = max(seq_len(P, b) - (r1 - r0), 0);
     if (r1 == r0 || begin >= n) return;
     const int i0 = page_of(P, begin), i1 = page_of(P, n - 1);
-    const int hq = P.hd >> 2, rows = BD_THREADS / hq, q = threadIdx.x % hq, r = threadIdx.x / hq;
-    for (int i = i0 + blockIdx.x; i <= i1; i += gridDim.x) {
+    const int hq = P.hd >> 2, across = min(hq, 32), rows = 32 / across, q = lane % across, r = lane / across;
+    const int head = blockIdx.y;
+    for (int i = i0 + blockIdx.x * BD_WARPS + (threadIdx.x >> 5); i <= i1; i += gridDim.x * BD_WARPS) {
         int slot;
         const int page = lookup(P, b, i * P.page_size, slot);
         if (page < 0) continue;
         const int filled = min(P.page_size, n - i * P.page_size);
-        float lo[4], hi[4];
+        float lo[2][4], hi[2][4];
         uint32_t top = 0;
 #pragma unroll
-        for (int k = 0; k < 4; k++) lo[k] = INFINITY, hi[k] = -INFINITY;
-        if (r < rows) {
-#pragma unroll 4
-            for (int s = r; s < filled; s += rows) {
-                float x[4];
-                key4<CT, VEC>(P, C, page, head, s, 4 * q, x);
+        for (int h = 0; h < 2; h++) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    lo[k] = fminf(lo[k], x[k]);
-                    hi[k] = fmaxf(hi[k], x[k]);
-                    top = max(top, __float_as_uint(x[k]) & 0x7FFFFFFFu);
+            for (int k = 0; k < 4; k++) lo[h][k] = INFINITY, hi[h][k] = -INFINITY;
+            if (q + 32 * h >= hq || (h && across < 32)) continue;
+            if (r < rows) {
+#pragma unroll 8
+                for (int s = r; s < filled; s += rows) {
+                    float x[4];
+                    key4<CT, VEC>(P, C, page, head, s, 4 * (q + 32 * h), x);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        lo[h][k] = fminf(lo[h][k], x[k]);
+                        hi[h][k] = fmaxf(hi[h][k], x[k]);
+                        top = max(top, __float_as_uint(x[k]) & 0x7FFFFFFFu);
+                    }
                 }
             }
+        }
+        __syncwarp();
+        for (int x = 1; x < rows; x++) {  // the other lanes of the same elements
+            const int from = (lane % across) + x * across;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                s_lo[r * P.hd + 4 * q + k] = lo[k];
-                s_hi[r * P.hd + 4 * q + k] = hi[k];
+                const float l = __shfl_sync(0xffffffffu, lo[0][k], from), h = __shfl_sync(0xffffffffu, hi[0][k], from);
+                if (r == 0) lo[0][k] = fminf(lo[0][k], l), hi[0][k] = fmaxf(hi[0][k], h);
             }
         }
         top = __reduce_max_sync(0xffffffffu, top);
-        if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < BD_THREADS / 32; w++) top = max(top, s_top[w]);
         const bool fine = top < 0x7F800000u;
         const int e = fine ? unit_exponent(top) : 255;
         const float inv = fine ? power(254 - e) : 0.0f;
         const int64_t at = (int64_t)page * P.nkv + head;
-        if (threadIdx.x == 0) B.scale[at] = power(e);  // 255: infinity
-        if (threadIdx.x < hq) {
-            uint32_t lw = 0, hw = 0;
+        if (lane == 0) B.scale[at] = power(e);  // 255: infinity
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                float l = s_lo[4 * q + k], h = s_hi[4 * q + k];
-                for (int x = 1; x < rows; x++) {
-                    l = fminf(l, s_lo[x * P.hd + 4 * q + k]);
-                    h = fmaxf(h, s_hi[x * P.hd + 4 * q + k]);
-                }
-                if (fine) {
-                    lw |= (uint32_t)((int)floorf(l * inv) & 255) << (8 * k);
-                    hw |= (uint32_t)((int)ceilf(h * inv) & 255) << (8 * k);
+        for (int h = 0; h < 2; h++) {
+            if (r != 0 || q + 32 * h >= hq || (h && across < 32)) continue;
+            uint32_t lw = 0, hw = 0;
+            if (fine) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    lw |= (uint32_t)((int)floorf(lo[h][k] * inv) & 255) << (8 * k);
+                    hw |= (uint32_t)((int)ceilf(hi[h][k] * inv) & 255) << (8 * k);
                 }
             }
-            reinterpret_cast<uint32_t*>(B.lo + at * P.hd)[q] = lw;
-            reinterpret_cast<uint32_t*>(B.hi + at * P.hd)[q] = hw;
+            reinterpret_cast<uint32_t*>(B.lo + at * P.hd)[q + 32 * h] = lw;
+            reinterpret_cast<uint32_t*>(B.hi + at * P.hd)[q + 32 * h] = hw;
         }
-        __syncthreads();
     }
 }
 
@@ -139,7 +139,7 @@ struct SelectArgs {
     Bounds b;
     const void* q;
     int64_t q_rs, q_hs;
-    int G;
+    int G, qvec;  // query heads a KV head; four elements of a query lie on 16 (f16: 8) bytes
     int budget, first, recent;
     int32_t* out;
     uint32_t* keys;  // [row][KV head][max_pages], score_key()
@@ -264,17 +264,116 @@ __global__ void __launch_bounds__(SC_THREADS) k_page_scores(const __grid_constan
     }
 }
 
-// One CTA per (row, KV head): the budget-th largest key by four passes of eight
-// bits, then what is above it and, of what equals it, the first by index.  A
-// thread's keys are a run, so that one scan over the threads places them all.
-constexpr int PK_THREADS = 256;
+// The pages of one row and KV head from their keys: the least key that is taken, by
+// histograms of 2,048 equal steps of the range that still holds it (so that the
+// keys of a row, which lie close together, spread over them: the shared counters
+// of equal digits would be added to one by one), then what is above it and, of what
+// equals it, the first by index.  A thread's keys are a run, so that one scan over
+// the threads places them all.
+constexpr int PK_THREADS = 256, PK_BINS = 2048;
+
+struct PickShared {
+    int hist[PK_BINS], sum[2][PK_THREADS / 32];
+    uint32_t least[PK_THREADS / 32], most[PK_THREADS / 32];
+    int bin, left, held;
+};
+
+__device__ __forceinline__ void pick_pages(const uint32_t* keys, int n, int budget, int first, int recent, int32_t* out, PickShared& S) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int begin = first, end = n - recent;  // the ones whose score counts (n > budget >= first + recent)
+    int left = budget - first - recent;         // and how many of them are taken
+    uint32_t least = 0xffffffffu, most = 0;
+    for (int i = begin + tid; i < end; i += PK_THREADS) {
+        const uint32_t k = keys[i];
+        least = min(least, k);
+        most = max(most, k);
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) S.least[warp] = least, S.most[warp] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < PK_THREADS / 32; w++) least = min(least, S.least[w]), most = max(most, S.most[w]);
+    uint32_t lo = least, hi = most, above = 0xffffffffu;  // the range; taken: keys above `above`, and the first `left` that equal it
+    int shift = max(32 - __clz(most - least) - 11, 0);
+    while (left > 0) {
+        for (int i = tid; i < PK_BINS; i += PK_THREADS) S.hist[i] = 0;
+        __syncthreads();
+        for (int i = begin + tid; i < end; i += PK_THREADS) {
+            const uint32_t k = keys[i];
+            if (k >= lo && k <= hi) atomicAdd(&S.hist[(k - lo) >> shift], 1);
+        }
+        __syncthreads();
+        // eight bins a thread, from the top
+        int c[PK_BINS / PK_THREADS], own = 0;
+#pragma unroll
+        for (int i = 0; i < PK_BINS / PK_THREADS; i++) own += c[i] = S.hist[PK_BINS - 1 - (tid * (PK_BINS / PK_THREADS) + i)];
+        int incl = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+        }
+        if (lane == 31) S.sum[0][warp] = incl;
+        __syncthreads();
+        for (int w = 0; w < warp; w++) incl += S.sum[0][w];
+        int before = incl - own;
+        if (before < left && incl >= left) {
+#pragma unroll
+            for (int i = 0; i < PK_BINS / PK_THREADS; i++) {
+                if (before < left && before + c[i] >= left) {
+                    S.bin = PK_BINS - 1 - (tid * (PK_BINS / PK_THREADS) + i);
+                    S.left = left - before;
+                    S.held = c[i];
+                }
+                before += c[i];
+            }
+        }
+        __syncthreads();
+        lo += (uint32_t)S.bin << shift;
+        hi = min(hi, lo + ((1u << shift) - 1));
+        left = S.left;
+        const int held = S.held;
+        __syncthreads();
+        if (shift == 0 || held == left) {  // one key's step, or all of the step is taken (a key is above 0)
+            above = held == left ? lo - 1 : lo;
+            if (held == left) left = 0;
+            break;
+        }
+        shift = max(shift - 11, 0);
+    }
+    // (the last step's upper end needs no mark: what lies above it is above `above`)
+    const int run = ((n + PK_THREADS - 1) / PK_THREADS) | 1, i0 = min(tid * run, n), i1 = min(i0 + run, n);
+    int more = 0, equal = 0;
+    for (int i = i0; i < i1; i++) {
+        const uint32_t k = keys[i];
+        const bool kept = i < begin || i >= end;
+        more += kept || k > above;
+        equal += !kept && k == above;
+    }
+    int a = more, e = equal;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, e, o);
+        if (lane >= o) a += x, e += y;
+    }
+    if (lane == 31) S.sum[0][warp] = a, S.sum[1][warp] = e;
+    __syncthreads();
+    for (int w = 0; w < warp; w++) a += S.sum[0][w], e += S.sum[1][w];
+    a -= more;
+    e -= equal;
+    int at = a + min(e, left);
+    for (int i = i0; i < i1; i++) {
+        const uint32_t k = keys[i];
+        const bool kept = i < begin || i >= end;
+        if (kept || k > above || (k == above && e++ < left)) out[at++] = i;
+    }
+}
 
 __global__ void __launch_bounds__(PK_THREADS) k_page_pick(const __grid_constant__ SelectArgs A) {
     const PagedArgs& P = A.p;
-    __shared__ int s_hist[256], s_sum[2][PK_THREADS / 32];
-    __shared__ uint32_t s_digit;
-    __shared__ int s_left;
-    const int row = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ PickShared S;
+    const int row = blockIdx.x, kvh = blockIdx.y;
     int seq, pos;
     const bool any = place_of(P, row, seq, pos);
     const int n = any ? pages_seen(P, pos) : 0;
@@ -282,71 +381,188 @@ __global__ void __launch_bounds__(PK_THREADS) k_page_pick(const __grid_constant_
     if (!any) return;
     int32_t* out = A.out + ((int64_t)row * P.nkv + kvh) * A.budget;
     if (n <= A.budget) {
+        for (int i = threadIdx.x; i < A.budget; i += PK_THREADS) out[i] = i < n ? i : -1;
+        return;
+    }
+    pick_pages(A.keys + ((int64_t)row * P.nkv + kvh) * P.max_pages, n, A.budget, A.first, A.recent, out, S);
+}
+
+// ---- both in one: a cluster of CTAs scores a row and KV head's pages, each a share
+// of them, into the first one's shared memory, which picks.  One launch and no
+// workspace.  Bound by latency: a cluster's start, the row's place, the queries, the
+// bounds, the pick, one after another.
+__device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// Four elements of a query row from d on.
+template <typename T>
+__device__ __forceinline__ void query4(const T* q, int vec, float* x) {
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(q));
+            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+        } else {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(q));
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+            x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = to_f32(q[i]);
+    }
+}
+
+// NX: 16-byte pieces of a head's bounds a lane (heads of 64 NX elements at most).
+template <typename T, int NX>
+__global__ void __launch_bounds__(PK_THREADS) k_page_select(const __grid_constant__ SelectArgs A) {
+    const PagedArgs& P = A.p;
+    extern __shared__ __align__(16) uint8_t sm[];
+    __shared__ PickShared S;
+    constexpr int STRIDE = 64 * NX;
+    const int hd = P.hd, G = A.G;
+    uint8_t* qp = sm;                       // [G][STRIDE]: codes above zero
+    uint8_t* qn = sm + (size_t)G * STRIDE;  // and below
+    int* unit = reinterpret_cast<int*>(sm + 2 * (size_t)G * STRIDE);
+    uint32_t* keys = reinterpret_cast<uint32_t*>(unit + (G + 3) / 4 * 4);
+    uint32_t rank, ctas, first_keys;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(first_keys) : "r"(smem_u32(keys)));
+    const int row = blockIdx.z, kvh = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int seq = 0, pos = -1;
+    const bool any = place_of(P, row, seq, pos);
+    const int n = any ? pages_seen(P, pos) : 0;
+    const bool score = any && n > A.budget;
+    const int share = ((n + (int)ctas - 1) / (int)ctas + 63) / 64 * 64, p0 = min((int)rank * share, n), p1 = min(p0 + share, n);
+    const int sub = tid & 3;
+    int slot, page = -1;
+    if (score && p0 + (tid >> 2) < p1) page = lookup(P, seq, (p0 + (tid >> 2)) * P.page_size, slot);
+    if (score && p0 < p1) {
+        for (int g = warp; g < G; g += PK_THREADS / 32) {
+            const T* q = (const T*)A.q + row * A.q_rs + (kvh * G + g) * A.q_hs;
+            float x[(NX + 1) / 2][4];
+            uint32_t top = 0;
+#pragma unroll
+            for (int h = 0; h < (NX + 1) / 2; h++) {
+                const int d = 4 * lane + 128 * h;
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[h][i] = 0.0f;
+                if (d < hd) query4(q + d, A.qvec, x[h]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) top = max(top, __float_as_uint(x[h][i]) & 0x7FFFFFFFu);
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            const bool fine = top < 0x7F800000u;
+            const int e = fine ? unit_exponent(top) : 0;
+            const float inv = fine ? power(254 - e) : 0.0f;
+#pragma unroll
+            for (int h = 0; h < (NX + 1) / 2; h++) {
+                const int d = 4 * lane + 128 * h;
+                uint32_t up = 0, down = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int c = fine ? __float2int_rn(x[h][i] * inv) : 0;
+                    up |= (uint32_t)max(c, 0) << (8 * i);
+                    down |= (uint32_t)(min(c, 0) & 255) << (8 * i);
+                }
+                if (d < STRIDE) {
+                    *reinterpret_cast<uint32_t*>(qp + g * STRIDE + d) = up;
+                    *reinterpret_cast<uint32_t*>(qn + g * STRIDE + d) = down;
+                }
+            }
+            if (lane == 0) unit[g] = e;
+        }
+    }
+    cluster_sync();  // (the codes are there, and the first CTA has begun)
+    for (int i0 = p0; i0 < p1 && score; i0 += PK_THREADS / 4) {
+        const int i = i0 + (tid >> 2);
+        const int64_t at = (int64_t)max(page, 0) * P.nkv + kvh;
+        int4 h[NX], l[NX];
+#pragma unroll
+        for (int x = 0; x < NX; x++) {
+            h[x] = l[x] = make_int4(0, 0, 0, 0);
+            if (page >= 0 && 16 * (sub + 4 * x) < hd) {
+                h[x] = __ldg(reinterpret_cast<const int4*>(A.b.hi + at * hd) + sub + 4 * x);
+                l[x] = __ldg(reinterpret_cast<const int4*>(A.b.lo + at * hd) + sub + 4 * x);
+            }
+        }
+        const uint32_t scale = page < 0 ? 0 : __float_as_uint(__ldg(A.b.scale + at)) >> 23;
+        const bool hole = page < 0;
+        page = -1;  // of the next round
+        if (i + PK_THREADS / 4 < p1) page = lookup(P, seq, (i + PK_THREADS / 4) * P.page_size, slot);
+        const int es = min(max((int)scale, 7), 249);
+        uint32_t best = 0;
+        for (int g0 = 0; g0 < G; g0 += SC_HEADS) {
+            int acc[SC_HEADS];
+#pragma unroll
+            for (int g = 0; g < SC_HEADS; g++) {
+                acc[g] = 0;
+                if (g0 + g >= G) continue;
+#pragma unroll
+                for (int x = 0; x < NX; x++) {
+                    const int4 p = *reinterpret_cast<const int4*>(qp + (g0 + g) * STRIDE + 16 * (sub + 4 * x));
+                    const int4 m = *reinterpret_cast<const int4*>(qn + (g0 + g) * STRIDE + 16 * (sub + 4 * x));
+                    acc[g] = __dp4a(h[x].x, p.x, __dp4a(h[x].y, p.y, __dp4a(h[x].z, p.z, __dp4a(h[x].w, p.w, acc[g]))));
+                    acc[g] = __dp4a(l[x].x, m.x, __dp4a(l[x].y, m.y, __dp4a(l[x].z, m.z, __dp4a(l[x].w, m.w, acc[g]))));
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < SC_HEADS; g++) {
+                acc[g] += __shfl_xor_sync(0xffffffffu, acc[g], 1);
+                acc[g] += __shfl_xor_sync(0xffffffffu, acc[g], 2);
+                if (g0 + g < G) best = max(best, score_key(acc[g], unit[g0 + g], es));
+            }
+        }
+        if (sub == 0 && i < p1) {
+            const uint32_t key = hole ? KEY_HOLE : scale == 255 ? KEY_INF : best;
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(first_keys + 4 * i), "r"(key) : "memory");
+        }
+    }
+    cluster_sync();
+    if (rank != 0 || !any) return;
+    int32_t* out = A.out + ((int64_t)row * P.nkv + kvh) * A.budget;
+    if (!score) {
         for (int i = tid; i < A.budget; i += PK_THREADS) out[i] = i < n ? i : -1;
         return;
     }
-    const uint32_t* keys = A.keys + ((int64_t)row * P.nkv + kvh) * P.max_pages;
-    uint32_t prefix = 0, mask = 0;
-    int left = A.budget;  // of the keys that share the prefix, so many are to be taken
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        s_hist[tid] = 0;
-        __syncthreads();
-        for (int i = tid; i < n; i += PK_THREADS) {
-            const uint32_t k = keys[i];
-            if ((k & mask) == prefix) atomicAdd(&s_hist[k >> shift & 255], 1);
-        }
-        __syncthreads();
-        // keys above digit tid: a scan from the top
-        const int c = s_hist[255 - tid];
-        int incl = c;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int t = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += t;
-        }
-        if (lane == 31) s_sum[0][warp] = incl;
-        __syncthreads();
-        for (int w = 0; w < warp; w++) incl += s_sum[0][w];
-        if (incl >= left && incl - c < left) {
-            s_digit = 255 - tid;
-            s_left = left - (incl - c);
-        }
-        __syncthreads();
-        prefix |= s_digit << shift;
-        mask |= 255u << shift;
-        left = s_left;
-        __syncthreads();
-    }
-    const int run = (n + PK_THREADS - 1) / PK_THREADS, i0 = min(tid * run, n), i1 = min(i0 + run, n);
-    int above = 0, equal = 0;
-    for (int i = i0; i < i1; i++) {
-        const uint32_t k = keys[i];
-        above += k > prefix;
-        equal += k == prefix;
-    }
-    int a = above, e = equal;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, e, o);
-        if (lane >= o) a += x, e += y;
-    }
-    if (lane == 31) s_sum[0][warp] = a, s_sum[1][warp] = e;
-    __syncthreads();
-    for (int w = 0; w < warp; w++) a += s_sum[0][w], e += s_sum[1][w];
-    a -= above;
-    e -= equal;
-    int at = a + min(e, left);
-    for (int i = i0; i < i1; i++) {
-        const uint32_t k = keys[i];
-        if (k > prefix || (k == prefix && e++ < left)) out[at++] = i;
-    }
+    pick_pages(keys, n, A.budget, A.first, A.recent, out, S);
+}
+
+template <typename T, int NX>
+int launch_select_t(const SelectArgs& A, int ctas, size_t smem, cudaStream_t s) {
+    HC_CUDA(cudaFuncSetAttribute(k_page_select<T, NX>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas, (unsigned)A.p.nkv, (unsigned)A.p.n_rows);
+    cfg.blockDim = dim3(PK_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    HC_CUDA(cudaLaunchKernelEx(&cfg, k_page_select<T, NX>, A));
+    HC_LAUNCH_CHECK();
+    return HC_OK;
+}
+
+// Shared memory of the form in one kernel; 0: two kernels, where a head's bounds are no
+// whole 16-byte pieces, a table's keys do not fit, or there are more rows than a
+// grid has places.
+size_t select_smem(int hd, int G, int max_pages, int n_rows) {
+    const size_t stride = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
+    const size_t bytes = 2 * (size_t)G * stride + 4 * (size_t)((G + 3) / 4 * 4) + 4 * (size_t)max_pages;
+    return hd % 16 == 0 && n_rows <= 65535 && bytes <= 200 * 1024 ? bytes : 0;
 }
 
 template <typename CT>
 int launch_bounds_t(const PagedArgs& P, const PagedScales& C, const Bounds& B, bool vec, int touched, cudaStream_t s) {
-    const dim3 grid((unsigned)touched, (unsigned)P.nkv, (unsigned)P.n_seqs);
-    if (vec) k_page_bounds<CT, true><<<grid, BD_THREADS, 0, s>>>(P, C, B);
-    else k_page_bounds<CT, false><<<grid, BD_THREADS, 0, s>>>(P, C, B);
+    const dim3 grid((unsigned)((touched + BD_WARPS - 1) / BD_WARPS), (unsigned)P.nkv, (unsigned)P.n_seqs);
+    if (vec) k_page_bounds<CT, true><<<grid, 32 * BD_WARPS, 0, s>>>(P, C, B);
+    else k_page_bounds<CT, false><<<grid, 32 * BD_WARPS, 0, s>>>(P, C, B);
     HC_LAUNCH_CHECK();
     return HC_OK;
 }
@@ -362,7 +578,8 @@ int bounds_ok(const char* who, const hc_page_bounds* b) {
     return HC_OK;
 }
 
-size_t key_bytes(const hc_page_bounds* b, const hc_paged_batch* batch) {
+size_t key_bytes(const hc_page_bounds* b, const hc_paged_batch* batch, int n_heads) {
+    if (select_smem(b->head_dim, n_heads / b->n_kv_heads, batch->max_pages, batch->n_rows)) return 0;
     return (size_t)std::max(batch->n_rows, 0) * b->n_kv_heads * std::max(batch->max_pages, 0) * 4;
 }
 
@@ -404,11 +621,12 @@ HC_EXPORT int hc_page_bounds_values_dev(const hc_page_bounds* b, float* lo_out, 
     return HC_OK;
 }
 
-HC_EXPORT int hc_page_select_workspace(const hc_page_bounds* b, const hc_paged_batch* batch, size_t* bytes) {
+HC_EXPORT int hc_page_select_workspace(const hc_page_bounds* b, const hc_paged_batch* batch, int n_heads, size_t* bytes) {
     const char* who = "hc_page_select_workspace";
     HC_TRY(hc::bounds_ok(who, b));
     HC_CHECK(batch && bytes, HC_ERR_INVALID, "%s: NULL batch or bytes", who);
-    *bytes = hc::key_bytes(b, batch);
+    HC_CHECK(n_heads >= 1 && n_heads % b->n_kv_heads == 0, HC_ERR_INVALID, "%s: %d query heads over %d KV heads", who, n_heads, b->n_kv_heads);
+    *bytes = hc::key_bytes(b, batch, n_heads);
     return HC_OK;
 }
 
@@ -431,7 +649,7 @@ HC_EXPORT int hc_page_select_dev(const hc_page_bounds* b, const hc_paged_batch* 
     if (batch->n_rows == 0) return HC_OK;
     HC_TRY(hc::page_rows_ok(who, "q", q, dtype));
     HC_CHECK(out && (uintptr_t)out % 4 == 0, HC_ERR_INVALID, "%s: NULL or misaligned out", who);
-    const size_t need = hc::key_bytes(b, batch);
+    const size_t need = hc::key_bytes(b, batch, n_heads);
     HC_CHECK(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 16 == 0)), HC_ERR_INVALID,
              "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, need, workspace_bytes);
     A.b = {b->lo, b->hi, b->scale};
@@ -444,11 +662,23 @@ HC_EXPORT int hc_page_select_dev(const hc_page_bounds* b, const hc_paged_batch* 
     A.out = out;
     A.keys = (uint32_t*)workspace;
     cudaStream_t s = (cudaStream_t)stream;
+    const bool f16 = dtype == HC_DTYPE_FP16;
+    A.qvec = (uintptr_t)q->data % (f16 ? 8 : 16) == 0 && (q->row_stride | q->head_stride) % 4 == 0;
+    const size_t one = hc::select_smem(A.p.hd, A.G, A.p.max_pages, A.p.n_rows);
+    if (one) {
+        // as many CTAs a row and KV head as fill the SMs, 64 pages each at least
+        const int64_t pairs = (int64_t)A.p.n_rows * A.p.nkv;
+        int ctas = 1;
+        while (ctas < 8 && ctas * pairs < 148 * 2 && ctas * 64 < A.p.max_pages) ctas *= 2;
+        if (A.p.hd <= 64) return f16 ? hc::launch_select_t<__half, 1>(A, ctas, one, s) : hc::launch_select_t<float, 1>(A, ctas, one, s);
+        if (A.p.hd <= 128) return f16 ? hc::launch_select_t<__half, 2>(A, ctas, one, s) : hc::launch_select_t<float, 2>(A, ctas, one, s);
+        return f16 ? hc::launch_select_t<__half, 4>(A, ctas, one, s) : hc::launch_select_t<float, 4>(A, ctas, one, s);
+    }
     if (A.p.max_pages > budget) {
         const int64_t pairs = (int64_t)A.p.n_rows * A.p.nkv, chunks = (A.p.max_pages + hc::SC_PAGES - 1) / hc::SC_PAGES;
         const dim3 grid((unsigned)std::max<int64_t>(1, std::min(chunks, (148 * 16 + pairs - 1) / pairs)), (unsigned)A.p.nkv,
                         (unsigned)std::min(A.p.n_rows, 65535));
-        if (dtype == HC_DTYPE_FP16) hc::k_page_scores<__half><<<grid, hc::SC_THREADS, smem, s>>>(A);
+        if (f16) hc::k_page_scores<__half><<<grid, hc::SC_THREADS, smem, s>>>(A);
         else hc::k_page_scores<float><<<grid, hc::SC_THREADS, smem, s>>>(A);
         HC_LAUNCH_CHECK();
         HC_TRY(hc::launch_pdl(hc::k_page_pick, dim3((unsigned)A.p.n_rows, (unsigned)A.p.nkv), dim3(hc::PK_THREADS), 0, s, A));

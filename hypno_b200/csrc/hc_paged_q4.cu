@@ -25,10 +25,10 @@ __device__ __forceinline__ void load8(const T* p, bool vec, float* x) {
         return;
     }
     if constexpr (sizeof(T) == 4) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
         x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
     } else {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
         const uint32_t u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -55,124 +55,88 @@ __device__ __forceinline__ void store8(T* p, bool vec, const float* x) {
 // Eight elements of a head a thread; the four threads of 32 elements find their
 // largest magnitude together.  The turned pairs are separately rounded products
 // (a c - b s, not contracted), so that a value at the border of two codes falls
-// the same way whatever kernel or host code computes it; q and k by the same
-// code.  A head's elements are read by the threads that need them: with half
-// pairs twice, from L1.
+// the same way whatever computes it.  A thread's loads are in flight before the
+// row's place in the cache (three dependent loads) is known.
 //
-// q may be turned in place: the eight elements of a pair's other run are read by
-// another thread too, so in-place queries with half pairs take one thread for
-// both runs (`both`).
+// Half pairs (HALVES): a thread reads its elements' partners too; of q, which may be
+// turned in place, the thread of the first elements turns both, and the one of the
+// second ones has nothing to do.
+// Bound by its bytes: q is read and written, k and v are read.
 template <typename T, bool HALVES>
-__device__ __forceinline__ void turned(const T* src, int i0, int rot, bool vec, const float2* cs, float* x) {
+__global__ void __launch_bounds__(Q4_THREADS) k_q4_append(AppendArgs A, PagedScales C, int vec) {
+    const PagedArgs& P = A.p;
+    const int row = blockIdx.x, hu = P.hd >> 3, half = A.rot >> 1;
+    const int unit = blockIdx.y * Q4_THREADS + threadIdx.x;
+    if (unit >= (A.nh + 2 * P.nkv) * hu) return;  // (the four threads of a block of 32 leave together)
+    int head = unit / hu;
+    const int i0 = 8 * (unit - head * hu);
+    const bool is_q = head < A.nh, is_v = head >= A.nh + P.nkv;
+    if (!is_q) head -= is_v ? A.nh + P.nkv : A.nh;
+    if (HALVES && is_q && i0 >= half && i0 + 8 <= A.rot) return;
+    const T* src = is_q   ? (const T*)A.q + row * A.q_rs + head * A.q_hs
+                   : is_v ? (const T*)A.v + row * A.v_rs + head * A.v_hs
+                          : (const T*)A.k + row * A.k_rs + head * A.k_hs;
+    const bool turns = !is_v && i0 < A.rot;
+    float x[8], y[8];  // the elements; HALVES: their partners
     load8(src + i0, vec, x);
-    if (i0 >= rot) return;
-    if constexpr (HALVES) {
-        const int half = rot >> 1;
-        float y[8];
+    if (HALVES && turns) {
         if (half % 8 == 0) {
             load8(src + (i0 < half ? i0 + half : i0 - half), vec, y);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int d = i0 + i;
-                y[i] = d < rot ? to_f32(src[d < half ? d + half : d - half]) : 0.0f;
+                y[i] = d < A.rot ? to_f32(src[d < half ? d + half : d - half]) : 0.0f;
             }
         }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int d = i0 + i;
-            if (d >= rot) break;
-            const float2 t = __ldg(cs + (d < half ? d : d - half));
-            x[i] = d < half ? __fsub_rn(__fmul_rn(x[i], t.x), __fmul_rn(y[i], t.y))
-                            : __fadd_rn(__fmul_rn(y[i], t.y), __fmul_rn(x[i], t.x));
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (i0 + 2 * i >= rot) break;
-            const float2 t = __ldg(cs + (i0 >> 1) + i);
-            const float a = x[2 * i], b = x[2 * i + 1];
-            x[2 * i] = __fsub_rn(__fmul_rn(a, t.x), __fmul_rn(b, t.y));
-            x[2 * i + 1] = __fadd_rn(__fmul_rn(a, t.y), __fmul_rn(b, t.x));
-        }
     }
-}
-
-template <typename T, bool HALVES>
-__global__ void __launch_bounds__(Q4_THREADS) k_q4_append(AppendArgs A, PagedScales C, int vec) {
-    const PagedArgs& P = A.p;
-    const int row = blockIdx.x, hu = P.hd >> 3;
-    const int unit = blockIdx.y * Q4_THREADS + threadIdx.x;
-    if (unit >= (A.nh + 2 * P.nkv) * hu) return;  // (the four threads of a block of 32 leave together)
-    int head = unit / hu;
-    const int i0 = 8 * (unit - head * hu);
     const int seq = seq_of_row(P, row);
     int r0, r1;
     seq_rows(P, seq, r0, r1);
     if (row < r0 || row >= r1) return;
     const int pos = seq_len(P, seq) - (r1 - r0) + (row - r0);
-    const float2* cs = A.rot ? A.rope + (int64_t)min(max(pos, 0), A.rope_rows - 1) * (A.rot >> 1) : nullptr;
-    float x[8];
-    if (head < A.nh) {
-        const T* src = (const T*)A.q + row * A.q_rs + head * A.q_hs;
-        T* dst = (T*)A.qo + row * A.o_rs + head * A.o_hs;
-        if constexpr (HALVES) {
-            // the thread of a pair's first element turns both: q_out may be q
-            const int half = A.rot >> 1;
-            if (i0 >= half) {
-                // elements past the pairs pass through; the second runs are the others' work
-                if (i0 + 8 <= A.rot) return;
-                load8(src + i0, vec, x);
-                if (i0 >= A.rot) {
-                    store8(dst + i0, vec, x);
-                } else {
+    if (turns) {
+        const float2* cs = A.rope + (int64_t)min(max(pos, 0), A.rope_rows - 1) * half;
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (i0 + i >= A.rot) dst[i0 + i] = from_f32<T>(x[i]);
-                }
-                return;
-            }
-            float y[8];
-            const bool even = half % 8 == 0;
-            load8(src + i0, vec, x);
-            if (even) {
-                load8(src + i0 + half, vec, y);
+        for (int i = 0; i < 8; i += HALVES ? 1 : 2) {
+            const int d = i0 + i;
+            if (d >= A.rot) break;
+            if constexpr (HALVES) {
+                const bool one = d < half;  // the pair's first element
+                const float2 t = __ldg(cs + (one ? d : d - half));
+                const float a = one ? x[i] : y[i], b = one ? y[i] : x[i];
+                const float u = __fsub_rn(__fmul_rn(a, t.x), __fmul_rn(b, t.y)), v = __fadd_rn(__fmul_rn(a, t.y), __fmul_rn(b, t.x));
+                x[i] = one ? u : v;
+                y[i] = one ? v : u;
             } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) y[i] = i0 + i < half ? to_f32(src[i0 + i + half]) : 0.0f;
+                const float2 t = __ldg(cs + (d >> 1));
+                const float a = x[i], b = x[i + 1];
+                x[i] = __fsub_rn(__fmul_rn(a, t.x), __fmul_rn(b, t.y));
+                x[i + 1] = __fadd_rn(__fmul_rn(a, t.y), __fmul_rn(b, t.x));
             }
+        }
+    }
+    if (is_q) {
+        T* dst = (T*)A.qo + row * A.o_rs + head * A.o_hs;
+        if (!HALVES || !turns) {
+            store8(dst + i0, vec, x);
+        } else if (half % 8 == 0) {
+            store8(dst + i0, vec, x);
+            store8(dst + i0 + half, vec, y);
+        } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                if (i0 + i >= half) break;
-                const float2 t = __ldg(cs + i0 + i);
-                const float a = x[i], b = y[i];
-                x[i] = __fsub_rn(__fmul_rn(a, t.x), __fmul_rn(b, t.y));
-                y[i] = __fadd_rn(__fmul_rn(a, t.y), __fmul_rn(b, t.x));
-            }
-            if (even) {
-                store8(dst + i0, vec, x);
-                store8(dst + i0 + half, vec, y);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if (i0 + i < half) {
-                        dst[i0 + i] = from_f32<T>(x[i]);
-                        dst[i0 + i + half] = from_f32<T>(y[i]);
-                    } else if (i0 + i >= A.rot) {
-                        dst[i0 + i] = from_f32<T>(x[i]);  // (a run of eight may hold all pairs and more)
-                    }
+                const int d = i0 + i;
+                if (d < half) {
+                    dst[d] = from_f32<T>(x[i]);
+                    dst[d + half] = from_f32<T>(y[i]);
+                } else if (d >= A.rot) {
+                    dst[d] = from_f32<T>(x[i]);  // (a run of eight may end past the pairs)
                 }
             }
-        } else {
-            turned<T, false>(src, i0, A.rot, vec, cs, x);
-            store8(dst + i0, vec, x);
         }
         return;
     }
-    const bool is_v = head >= A.nh + P.nkv;
-    head -= is_v ? A.nh + P.nkv : A.nh;
-    if (is_v) load8((const T*)A.v + row * A.v_rs + head * A.v_hs + i0, vec, x);
-    else turned<T, HALVES>((const T*)A.k + row * A.k_rs + head * A.k_hs, i0, A.rot, vec, cs, x);
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);

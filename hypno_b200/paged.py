@@ -146,8 +146,7 @@ class PagedKV4:
         if _lib.current_device() != self.index:
             with _lib.on_device(self.index):
                 return self.values()
-        shape = (self.n_pages, self.n_kv_heads, self.page_size, self.head_dim)
-        k, v = (torch.empty(shape, dtype=torch.float16, device=self.device) for _ in range(2))
+        k, v = torch.empty((2, self.n_pages, self.n_kv_heads, self.page_size, self.head_dim), dtype=torch.float16, device=self.device).unbind()
         check(load().hc_paged_values_dev(self.ref, k.data_ptr(), v.data_ptr(), raw_stream(self.index)))
         return k, v
 
@@ -368,7 +367,7 @@ class PageBounds:
         if _lib.current_device() != self.index:
             with _lib.on_device(self.index):
                 return self.values()
-        lo, hi = (torch.empty(self.lo.shape, dtype=torch.float32, device=self.device) for _ in range(2))
+        lo, hi = torch.empty((2, self.n_pages, self.n_kv_heads, self.head_dim), dtype=torch.float32, device=self.device).unbind()
         check(load().hc_page_bounds_values_dev(self.ref, lo.data_ptr(), hi.data_ptr(), raw_stream(self.index)))
         return lo, hi
 
@@ -417,7 +416,7 @@ def select_pages(bounds, batch, q, budget, first=1, recent=2, out=None):
         raise TypeError(f"out must be a contiguous {shape} int32 tensor on {bounds.device}")
     lib, ref = load(), batch.pack(n)
     need = ctypes.c_size_t()
-    check(lib.hc_page_select_workspace(bounds.ref, ref, ctypes.byref(need)))
+    check(lib.hc_page_select_workspace(bounds.ref, ref, heads, ctypes.byref(need)))
     ws = torch.empty(need.value, dtype=torch.uint8, device=bounds.device) if need.value else None
     check(lib.hc_page_select_dev(bounds.ref, ref, qs, heads, code, budget, first, recent, out.data_ptr(),
                                  ws.data_ptr() if ws is not None else None, need.value, raw_stream(bounds.index)))

@@ -428,7 +428,7 @@ int hc_page_bounds_values_dev(const hc_page_bounds* bounds, float* lo_out, float
  * infinite s scores +inf, a hole -inf.  out is [n_rows][n_kv_heads][budget], by
  * index, -1 behind the last; rows that belong to no sequence keep what they had.
  * workspace: hc_page_select_workspace bytes, 16-byte aligned. */
-int hc_page_select_workspace(const hc_page_bounds* bounds, const hc_paged_batch* batch, size_t* bytes);
+int hc_page_select_workspace(const hc_page_bounds* bounds, const hc_paged_batch* batch, int n_heads, size_t* bytes);
 int hc_page_select_dev(const hc_page_bounds* bounds, const hc_paged_batch* batch, const hc_rows* q, int n_heads, uint32_t dtype,
                        int budget, int first, int recent, int32_t* out, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -94,13 +94,21 @@ def test_refusals_at_the_c_entries(lib):
     def select(b, q=rows, heads=4, budget=4, first=1, recent=2, out=at, ws=(at, 1 << 20)):
         return lib.hc_page_select_dev(ctypes.addressof(b), batch, q, heads, 0, budget, first, recent, out, ws[0], ws[1], None)
 
-    assert lib.hc_page_select_workspace(ctypes.addressof(bounds()), batch, ctypes.byref(need)) == 0 and need.value == 1 * 2 * 8 * 4
+    def workspace(b=None, heads=4, pages=8):
+        batch = _lib.HC_PAGED_BATCH.pack(at, at, at, pages, 1, pages, 1, 1, 100, 0)
+        assert lib.hc_page_select_workspace(ctypes.addressof(b or bounds()), batch, heads, ctypes.byref(need)) == 0
+        return need.value
+
+    assert workspace() == 0 and workspace(pages=100000) == 2 * 100000 * 4 and workspace(bounds(at, at, at, 4, 16, 2, 68)) == 2 * 8 * 4
+    assert lib.hc_page_select_workspace(ctypes.addressof(bounds()), batch, 3, ctypes.byref(need)) == -1
     for b, want in ((bounds(at, at, at, 4, 16, 2, 66), -3), (bounds(at, at, at, 4, 16, 2, 260), -3), (bounds(at + 8, at, at, 4, 16, 2, 64), -1),
                     (bounds(at, at, None, 4, 16, 2, 64), -1), (bounds(at, at, at, 0, 16, 2, 64), -1)):
         assert select(b) == want and lib.hc_page_bounds_values_dev(ctypes.addressof(b), at, at, None) == want
         assert lib.hc_page_bounds_update_dev(ctypes.addressof(b), ctypes.addressof(kv()), batch, None) == want
+    for ws in ((None, 0), (at, 63), (at + 4, 64)):      # (heads of 68 elements take one)
+        assert select(bounds(at, at, at, 4, 16, 2, 68), q=_lib.HC_ROWS.pack(at, 272, 68), ws=ws) == -1
     for bad in (dict(heads=3), dict(budget=2), dict(first=-1), dict(recent=4), dict(budget=0, first=0, recent=0), dict(out=None), dict(out=at + 2),
-                dict(ws=(None, 0)), dict(ws=(at, 63)), dict(ws=(at + 4, 64)), dict(q=_lib.HC_ROWS.pack(0, 0, 0))):
+                dict(q=_lib.HC_ROWS.pack(0, 0, 0))):
         assert select(bounds(), **bad) == -1, bad
     assert lib.hc_page_bounds_update_dev(ctypes.addressof(bounds(at, at, at, 4, 32, 2, 64)), ctypes.addressof(kv()), batch, None) == -1
     assert lib.hc_page_bounds_values_dev(ctypes.addressof(bounds()), at, None, None) == -1
