@@ -62,13 +62,38 @@ __device__ __forceinline__ void store8(T* p, bool vec, const float* x) {
 // turned in place, the thread of the first elements turns both, and the one of the
 // second ones has nothing to do.
 // Bound by its bytes: q is read and written, k and v are read.
+//
+// Codes: with i = 1 / s, x i is x / s within 2^-22 of itself, so its nearest whole number
+// is that of the division unless it lies within 2^-19 of the middle of two; such a
+// block divides.  (Divisions alone took a third of the kernel's instructions, and those are
+// what it is bound by: 8,192 rows of 32 + 8 + 8 heads of 128, 80 us.)
+__device__ __forceinline__ uint32_t q4_codes(const float* x, float s) {
+    uint32_t code = 0;
+    const float inv = __frcp_rn(s);
+    constexpr float MID = 12582912.0f + 8.0f;  // 1.5 2^23: the sum's low bits are the whole number + 8
+    float off = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float y = __fmaf_rn(x[i], inv, MID);
+        off = fmaxf(off, fabsf(__fmaf_rn(x[i], inv, MID - y)));
+        code |= (__float_as_uint(y) & 15u) << (4 * i);
+    }
+    // (no scale, the largest one, where codes are held to 7, and what is not finite: by the division too)
+    if (!(s > 0.0f && s < Q4_TOP && off < 0.5f - 0x1p-19f)) {
+        code = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) code |= q4_code(x[i], s) << (4 * i);
+    }
+    return code;
+}
+
 template <typename T, bool HALVES>
-__global__ void __launch_bounds__(Q4_THREADS) k_q4_append(AppendArgs A, PagedScales C, int vec) {
+__global__ void __launch_bounds__(Q4_THREADS) k_q4_append(AppendArgs A, PagedScales C, int vec, int hu_shift) {
     const PagedArgs& P = A.p;
     const int row = blockIdx.x, hu = P.hd >> 3, half = A.rot >> 1;
     const int unit = blockIdx.y * Q4_THREADS + threadIdx.x;
     if (unit >= (A.nh + 2 * P.nkv) * hu) return;  // (the four threads of a block of 32 leave together)
-    int head = unit / hu;
+    int head = hu_shift >= 0 ? unit >> hu_shift : unit / hu;
     const int i0 = 8 * (unit - head * hu);
     const bool is_q = head < A.nh, is_v = head >= A.nh + P.nkv;
     if (!is_q) head -= is_v ? A.nh + P.nkv : A.nh;
@@ -95,7 +120,18 @@ __global__ void __launch_bounds__(Q4_THREADS) k_q4_append(AppendArgs A, PagedSca
     seq_rows(P, seq, r0, r1);
     if (row < r0 || row >= r1) return;
     const int pos = seq_len(P, seq) - (r1 - r0) + (row - r0);
-    if (turns) {
+    if (!HALVES && turns && vec && i0 + 8 <= A.rot && half % 2 == 0) {
+        // four whole pairs, their angles in 16-byte pieces
+        const float4* cs = reinterpret_cast<const float4*>(A.rope + (int64_t)min(max(pos, 0), A.rope_rows - 1) * half + (i0 >> 1));
+        const float4 t[2] = {__ldg(cs), __ldg(cs + 1)};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float c = i & 1 ? t[i >> 1].z : t[i >> 1].x, s = i & 1 ? t[i >> 1].w : t[i >> 1].y;
+            const float a = x[2 * i], b = x[2 * i + 1];
+            x[2 * i] = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+            x[2 * i + 1] = __fadd_rn(__fmul_rn(a, s), __fmul_rn(b, c));
+        }
+    } else if (turns) {
         const float2* cs = A.rope + (int64_t)min(max(pos, 0), A.rope_rows - 1) * half;
 #pragma unroll
         for (int i = 0; i < 8; i += HALVES ? 1 : 2) {
@@ -148,9 +184,7 @@ __global__ void __launch_bounds__(Q4_THREADS) k_q4_append(AppendArgs A, PagedSca
     const int page = lookup(P, seq, pos, slot);
     if (page < 0) return;
     const float s = q4_scale(top);
-    uint32_t code = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) code |= q4_code(x[i], s) << (4 * i);
+    const uint32_t code = q4_codes(x, s);
     uint8_t* dst = is_v ? (uint8_t*)P.v + page * P.vps + head * P.vhs + slot * P.vss : (uint8_t*)P.k + page * P.kps + head * P.khs + slot * P.kss;
     *reinterpret_cast<uint32_t*>(dst + (i0 >> 1)) = code;
     if ((i0 & 31) == 0) {
@@ -199,13 +233,16 @@ template <typename T>
 int launch_append_t(const AppendArgs& A, const PagedScales& C, cudaStream_t s) {
     const PagedArgs& P = A.p;
     const int64_t et = 16 / (int64_t)sizeof(T);
-    const int vec = ((uintptr_t)A.k | (uintptr_t)A.v | (uintptr_t)A.q | (uintptr_t)A.qo) % 16 == 0 &&
+    const int vec = ((uintptr_t)A.k | (uintptr_t)A.v | (uintptr_t)A.q | (uintptr_t)A.qo | (uintptr_t)A.rope) % 16 == 0 &&
                     (A.k_rs | A.k_hs | A.v_rs | A.v_hs | (A.nh ? A.q_rs | A.q_hs | A.o_rs | A.o_hs : 0)) % et == 0;
     const int64_t units = (int64_t)(A.nh + 2 * P.nkv) * (P.hd / 8);
     HC_CHECK(units <= 65535ll * Q4_THREADS, HC_ERR_INVALID, "hc_paged_append_dev: %d + %d heads of %d", A.nh, P.nkv, P.hd);
     const dim3 grid((unsigned)P.n_rows, (unsigned)((units + Q4_THREADS - 1) / Q4_THREADS));
-    if (A.halves) k_q4_append<T, true><<<grid, Q4_THREADS, 0, s>>>(A, C, vec);
-    else k_q4_append<T, false><<<grid, Q4_THREADS, 0, s>>>(A, C, vec);
+    int shift = -1;
+    for (int i = 0; i < 6; i++)
+        if (P.hd / 8 == 1 << i) shift = i;
+    if (A.halves) k_q4_append<T, true><<<grid, Q4_THREADS, 0, s>>>(A, C, vec, shift);
+    else k_q4_append<T, false><<<grid, Q4_THREADS, 0, s>>>(A, C, vec, shift);
     HC_LAUNCH_CHECK();
     return HC_OK;
 }
