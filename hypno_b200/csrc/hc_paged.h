@@ -86,11 +86,20 @@ __device__ __forceinline__ int seq_len(const PagedArgs& P, int b) { return max(_
 __device__ __forceinline__ int list_count(const PagedList& L, int row, int kvh) {
     const int lane = threadIdx.x & 31;
     const int32_t* e = L.pages + row * L.row_stride + kvh * L.head_stride;
-    for (int i0 = 0; i0 < L.width; i0 += 32) {
-        const int i = i0 + lane;
-        const int here = i < L.width ? __ldg(e + i) : -1, before = i > 0 && i < L.width ? __ldg(e + i - 1) : -1;
-        const unsigned end = __ballot_sync(0xffffffffu, here <= before);
-        if (end) return i0 + __ffs(end) - 1;
+    constexpr int N = 4;  // so many times 32 entries are requested at once
+    int last = -1;
+    for (int i0 = 0; i0 < L.width; i0 += 32 * N) {
+        int here[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) here[k] = i0 + 32 * k + lane < L.width ? __ldg(e + i0 + 32 * k + lane) : -1;
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            int before = __shfl_up_sync(0xffffffffu, here[k], 1);
+            if (lane == 0) before = last;
+            const unsigned end = __ballot_sync(0xffffffffu, here[k] <= before);
+            if (end) return i0 + 32 * k + __ffs(end) - 1;
+            last = __shfl_sync(0xffffffffu, here[k], 31);
+        }
     }
     return L.width;
 }

@@ -40,8 +40,11 @@ struct PairWork {
     int c0, c1;     // positions (LIST: places of the list)
     bool cut;
     int64_t slot;   // of the partial results
-    int p_own;      // LIST: position of the token
+    int p_own;      // position of the first row's token
     const int32_t* list;
+    int stages;     // -1: no more pairs
+    int lost;       // its copies were given up
+    int p_min, l_max, one_token;  // keys that every row sees lie in [l_max, p_min]; LIST: not used
 };
 template <bool LIST>
 __device__ __forceinline__ bool next_pair(const SplitArgs& X, const LineTable& line, int64_t& u, int64_t u_begin, int64_t u_end, Line& at, PairWork& w) {
@@ -73,6 +76,11 @@ __device__ __forceinline__ bool next_pair(const SplitArgs& X, const LineTable& l
     }
     w.c0 = (int)min((int64_t)end, begin + (int64_t)unit * UNIT);
     w.c1 = (int)min((int64_t)end, w.c0 + (int64_t)nunits * UNIT);
+    w.stages = (w.c1 - w.c0 + QS_KEYS - 1) / QS_KEYS;
+    const int last = token_of(A, w.m0 + w.mrows - 1);
+    w.p_min = w.p_own;
+    w.l_max = A.window > 0 ? w.first + last - A.window + 1 : 0;
+    w.one_token = LIST || token_of(A, w.m0) == last;
     return true;
 }
 
@@ -80,12 +88,27 @@ template <int STAGES>
 struct StreamBars {
     uint64_t full[STAGES], empty[STAGES];
     uint32_t in[STAGES][QS_TILES];  // which keys of a tile are there
-    int abort;
+    uint64_t told[2], read[2];      // the pairs that the copying warp has told of, that the others have done with
+    PairWork work[2];
+    int abort, stuck;  // a wait for copies or stages, for pairs ran out
 };
 
 // Waits a bounded time; the whole warp.  (The clock is read when the first look fails.)
 __device__ __forceinline__ bool stream_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
     return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+// Whether a condition holds for all threads of the rows' warps, which meet here.
+__device__ __forceinline__ bool all_rows(bool p) {
+    int r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.s32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, 1, %2, p;\n\t"
+        "selp.s32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((int)p), "n"(QS_ROWS)
+        : "memory");
+    return r != 0;
 }
 // Arrives at the barrier when this thread's copies so far have landed.
 __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
@@ -105,9 +128,21 @@ __device__ __forceinline__ void stream_copies(const SplitArgs& X, const LineTabl
     int64_t u = u_begin;
     Line at = {0, 0, {}};
     PairWork w;
-    uint32_t n = 0;  // stages so far
-    bool ok = true;
-    while (ok && next_pair<LIST>(X, line, u, u_begin, u_end, at, w)) {
+    uint32_t n = 0, pairs = 0;  // stages, pairs so far
+    bool ok = true;  // false: a wait ran out, and the pairs from there on are told of without copies
+    for (;;) {
+        const bool more = next_pair<LIST>(X, line, u, u_begin, u_end, at, w);
+        w.lost = !ok;
+        if (!ok) w.stages = 0;
+        if (!more) w.stages = -1;
+        if (pairs >= 2 && !stream_wait(&B.read[pairs & 1], (pairs >> 1 & 1) ^ 1, &B.stuck)) break;
+        if (lane == 0) {
+            B.work[pairs & 1] = w;
+            mbar_arrive(&B.told[pairs & 1]);
+        }
+        pairs++;
+        if (!more) break;
+        if (!ok) continue;
         const uint8_t* kb = (const uint8_t*)P.k + w.kvh * P.khs + row * P.kss + chunk * 16;
         const uint8_t* vb = (const uint8_t*)P.v + w.kvh * P.vhs + row * P.vss + chunk * 16;
         const uint8_t* sb = (const uint8_t*)(sv ? X.c.v + w.kvh * X.c.vhs + srow * X.c.vss : X.c.k + w.kvh * X.c.khs + srow * X.c.kss);
@@ -115,7 +150,6 @@ __device__ __forceinline__ void stream_copies(const SplitArgs& X, const LineTabl
         const int64_t page_bytes = kind == 0 ? P.kps : kind == 1 ? P.vps : 2 * (kind == 2 ? X.c.kps : X.c.vps);
         const int64_t pos_bytes = kind == 0 ? P.kss : kind == 1 ? P.vss : 2 * (kind == 2 ? X.c.kss : X.c.vss);
         const int64_t k_step = ROWS * P.kss, v_step = ROWS * P.vss;
-        const int stages = (w.c1 - w.c0 + QS_KEYS - 1) / QS_KEYS;
         auto entry_of = [&](int k) {  // LIST: the index that the list has for this lane's tile
             const int64_t v = w.c0 + (int64_t)k * QS_KEYS + tile * SP_TK;
             return LIST && v < w.c1 ? __ldg(w.list + page_of(P, (int)v)) : 0;
@@ -142,7 +176,7 @@ __device__ __forceinline__ void stream_copies(const SplitArgs& X, const LineTabl
         uint32_t keys;
         int64_t from = place_of_tile(0, entry_of(0), keys);
         int entry = entry_of(1);
-        for (int k = 0; k < stages; k++, n++) {
+        for (int k = 0; k < w.stages; k++, n++) {
             uint32_t next_keys;
             const int64_t next_from = place_of_tile(k + 1, entry, next_keys);
             entry = entry_of(k + 2);
@@ -197,33 +231,42 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
             mbar_init(&B.full[i], 32);
             mbar_init(&B.empty[i], QS_WARPS);
         }
-        B.abort = 0;
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&B.told[i], 1);
+            mbar_init(&B.read[i], QS_WARPS);
+        }
+        B.abort = B.stuck = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1 && A.p.n_seqs <= 32) fill_table<LIST>(X, line);
     __syncthreads();
     pdl_trigger();  // the join may become resident; it waits for this grid's end
-    int64_t u = blockIdx.x, u_end = u + 1;
-    if (!X.whole) {
-        const int64_t run = run_of(A.p.n_seqs <= 32 ? line.units : all_units<LIST>(X), X.ctas);
-        u = blockIdx.x * run;
-        u_end = u + run;
-    }
     const uint32_t ring = smem_u32(smem);
     if (warp == QS_WARPS) {
+        int64_t u = blockIdx.x, u_end = u + 1;
+        if (!X.whole) {
+            const int64_t run = run_of(A.p.n_seqs <= 32 ? line.units : all_units<LIST>(X), X.ctas);
+            u = blockIdx.x * run;
+            u_end = u + run;
+        }
         stream_copies<Sh, HD, LIST>(X, line, B, ring, u, u_end);
         return;
     }
     uint8_t* outs = smem + S * Sh::STAGE;
     uint32_t* qf = reinterpret_cast<uint32_t*>(outs);  // until the outputs: [tile of rows][16 elements][lane][hi, hi (, lo, lo)]
     const uint32_t qs = smem_u32(qf);
-    const int64_t u_begin = u;
-    Line at = {0, 0, {}};
-    PairWork w;
     uint32_t st = 0, phase = 0;  // the next stage and the parity of its round
     bool lost = false;
     const int c = lane & 3, col = 2 * c, k0 = q4_key(lane >> 2);
-    while (next_pair<LIST>(X, line, u, u_begin, u_end, at, w)) {
+    for (uint32_t pairs = 0;; pairs++) {
+        // (read where it is needed: kept in registers it would cost a warp's worth of them)
+        const bool told = stream_wait(&B.told[pairs & 1], pairs >> 1 & 1, &B.stuck);
+        // (all warps go on together, or none; and the outputs before have been read)
+        if (!all_rows(told)) break;
+        const volatile PairWork& w = B.work[pairs & 1];
+        const int stages = w.stages, c0 = w.c0;
+        if (stages < 0) break;
+        lost |= w.lost != 0;
         // ---- queries as B fragments, once for all warps: eight elements a thread
         constexpr int QW = HD / 8;
         for (int i = threadIdx.x; i < R * QW; i += QS_ROWS) {  // (whole warps: R QW is a multiple of 32)
@@ -256,21 +299,11 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
             }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(QS_ROWS) : "memory");
-        float cf[NQ][2];           // score factors of this thread's two columns, not negative
-        int ps[NQ][2], lo[NQ][2];  // their positions and first visible positions
+        float cf[NQ][2];  // score factors of this thread's two columns, not negative
 #pragma unroll
         for (int n = 0; n < NQ; n++)
 #pragma unroll
-            for (int y = 0; y < 2; y++) {
-                const int mm = n * 8 + col + y;
-                cf[n][y] = s_cf[mm];
-                ps[n][y] = mm < w.mrows ? w.first + token_of(A, w.m0 + mm) : -1;
-                lo[n][y] = A.window > 0 ? ps[n][y] - A.window + 1 : 0;
-            }
-        // keys that every row of the tile sees
-        const int p_min = w.p_own, l_max = A.window > 0 ? w.first + token_of(A, w.m0 + w.mrows - 1) - A.window + 1 : 0;
-        const bool one_token = LIST || token_of(A, w.m0) == token_of(A, w.m0 + w.mrows - 1);
-
+            for (int y = 0; y < 2; y++) cf[n][y] = s_cf[n * 8 + col + y];
         float o[NQ][DT][4];
         float mx[NQ][2], sum[NQ][2];  // running maximum in log2 units; sum of this thread's keys only
 #pragma unroll
@@ -282,7 +315,6 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
             mx[n][0] = mx[n][1] = -INFINITY;
             sum[n][0] = sum[n][1] = 0.0f;
         }
-        const int stages = (w.c1 - w.c0 + QS_KEYS - 1) / QS_KEYS;
         for (int k = 0; k < stages; k++) {
             if (!lost && !stream_wait(&B.full[st], phase, &B.abort)) lost = true;
             __syncwarp();
@@ -291,7 +323,7 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
             const uint32_t ksc = base + 2 * Sh::CODES + warp * 2 * SP_TK * SCB, vsc = ksc + Sh::SCALES;
             const uint2 in2 = *reinterpret_cast<const uint2*>(&B.in[st][2 * warp]);
             const uint32_t in[2] = {in2.x, in2.y};
-            const int j0 = w.c0 + k * QS_KEYS + warp * 2 * SP_TK;
+            const int j0 = c0 + k * QS_KEYS + warp * 2 * SP_TK;
             if ((in[0] | in[1]) && !lost) {
                 // ---- S^T = K Q^T: [0], [1] = key k0 and this thread's two columns, [2], [3] = key k0 + 8
                 float s[2][NQ][4], sl[HILO ? 2 : 1][HILO ? NQ : 1][4];
@@ -345,17 +377,28 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
                             for (int y = 0; y < 4; y++) s[b][n][y] += sl[b][n][y];
                 }
                 // ---- weights
-                const bool full = (in[0] & in[1]) == 0xffffu && (LIST || (j0 + 2 * SP_TK - 1 <= p_min && j0 >= l_max));
+                const bool full = (in[0] & in[1]) == 0xffffu && (LIST || (j0 + 2 * SP_TK - 1 <= w.p_min && j0 >= w.l_max));
+                // (position of a column's row, and the first one that it sees)
+                auto row_of = [&](int n, int y, int& p, int& first) {
+                    const int m = n * 8 + col + y;
+                    p = m < w.mrows ? w.first + token_of(A, w.m0 + m) : -1;
+                    first = A.window > 0 ? p - A.window + 1 : 0;
+                };
                 if (!full) {
 #pragma unroll
-                    for (int b = 0; b < 2; b++)
+                    for (int n = 0; n < NQ; n++)
 #pragma unroll
-                        for (int n = 0; n < NQ; n++)
+                        for (int y = 0; y < 2; y++) {
+                            int p = 0, lo = 0;
+                            if (!LIST) row_of(n, y, p, lo);
 #pragma unroll
-                            for (int y = 0; y < 4; y++) {
-                                const int key = k0 + (y >> 1) * 8, j = j0 + b * SP_TK + key;
-                                if (!(in[b] >> key & 1u) || (!LIST && (j > ps[n][y & 1] || j < lo[n][y & 1]))) s[b][n][y] = -INFINITY;
-                            }
+                            for (int b = 0; b < 2; b++)
+#pragma unroll
+                                for (int z = 0; z < 2; z++) {
+                                    const int key = k0 + z * 8, j = j0 + b * SP_TK + key;
+                                    if (!(in[b] >> key & 1u) || (!LIST && (j > p || j < lo))) s[b][n][2 * z + y] = -INFINITY;
+                                }
+                        }
                 }
 #pragma unroll
                 for (int n = 0; n < NQ; n++) {
@@ -401,7 +444,7 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
                     // reach the latter through 0 * v where v is not finite: such a
                     // tile adds its products one by one, masked keys left out.
                     bool careful = false;
-                    if (!LIST && !full && !one_token) {
+                    if (!LIST && !full && !w.one_token) {
                         uint32_t bad = 0;
                         for (int x = lane; x < SP_TK * SCB / 4; x += 32) bad |= (lds_u32(vsc_b + 4 * x) & 0x7C007C00u) + 0x04000400u;
                         careful = __any_sync(0xffffffffu, (bad & 0x80008000u) != 0);
@@ -415,7 +458,9 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
 #pragma unroll
                                 for (int y = 0; y < 2; y++) {
                                     const float p = __shfl_sync(0xffffffffu, key < 8 ? s[b][n][y] : s[b][n][2 + y], src);
-                                    if (!key_in || j > ps[n][y] || j < lo[n][y]) continue;
+                                    int row_p, row_lo;
+                                    row_of(n, y, row_p, row_lo);
+                                    if (!key_in || j > row_p || j < row_lo) continue;
 #pragma unroll
                                     for (int t = 0; t < DT; t++)
 #pragma unroll
@@ -526,7 +571,8 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
                 if (d == 0) X.pml[w.slot * R + m] = make_float2(mm == -INFINITY ? mm : mm - BIAS, l);
             }
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(QS_ROWS) : "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.read[pairs & 1]);
     }
 }
 

@@ -35,7 +35,8 @@ static int tile_height(const PagedAttnArgs& A, const PagedList& L, int max_q_len
 bool paged_split_whole(const PagedAttnArgs& A, const PagedList& L, int max_q_len, int max_kv_len) {
     if (L.width) {
         const int R = tile_height(A, L, max_q_len);
-        if ((int64_t)A.p.n_rows * ((A.G + R - 1) / R) * A.p.nkv >= 4 * SP_CTAS) return true;
+        const int64_t pairs = (int64_t)A.p.n_rows * ((A.G + R - 1) / R) * A.p.nkv, rounds = (pairs + 147) / 148;
+        if (5 * pairs >= 4 * 148 * rounds) return true;
         return (int64_t)L.width * A.p.page_size <= MIN_UNITS * UNIT;
     }
     if ((int64_t)max_q_len * A.G > 64 && (int64_t)A.p.n_rows * A.G / 16 * A.p.nkv >= 2 * SP_CTAS) return true;
