@@ -547,9 +547,12 @@ __global__ void __launch_bounds__(PK_THREADS) k_page_select(const __grid_constan
     pick_pages(keys, n, A.budget, A.first, A.recent, out, S);
 }
 
+constexpr int SELECT_SMEM = 200 * 1024;
+
 template <typename T, int NX>
 int launch_select_t(const SelectArgs& A, int ctas, size_t smem, cudaStream_t s) {
-    HC_CUDA(cudaFuncSetAttribute(k_page_select<T, NX>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // (the same for every call: calls of several threads may come between this and the launch)
+    HC_CUDA(cudaFuncSetAttribute(k_page_select<T, NX>, cudaFuncAttributeMaxDynamicSharedMemorySize, SELECT_SMEM));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas, (unsigned)A.p.nkv, (unsigned)A.p.n_rows);
     cfg.blockDim = dim3(PK_THREADS);
@@ -572,7 +575,7 @@ int launch_select_t(const SelectArgs& A, int ctas, size_t smem, cudaStream_t s) 
 size_t select_smem(int hd, int G, int max_pages, int n_rows) {
     const size_t stride = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
     const size_t bytes = 2 * (size_t)G * stride + 4 * (size_t)((G + 3) / 4 * 4) + 4 * (size_t)max_pages;
-    return hd % 16 == 0 && n_rows <= 65535 && bytes <= 200 * 1024 ? bytes : 0;
+    return hd % 16 == 0 && n_rows <= 65535 && bytes <= SELECT_SMEM ? bytes : 0;
 }
 
 template <typename CT>
@@ -662,7 +665,8 @@ HC_EXPORT int hc_page_select_dev(const hc_page_bounds* b, const hc_paged_batch* 
              "%s: a budget of %d pages with the first %d and the last %d", who, budget, first, recent);
     A.G = n_heads / A.p.nkv;
     const size_t smem = 2 * (size_t)A.G * ((A.p.hd + 15) / 16 * 16) + 4 * (size_t)A.G;
-    HC_CHECK(smem <= 48 * 1024, HC_ERR_UNSUPPORTED, "%s: %d query heads of %d a KV head", who, A.G, A.p.hd);
+    HC_CHECK(smem <= 48 * 1024 || hc::select_smem(A.p.hd, A.G, A.p.max_pages, A.p.n_rows), HC_ERR_UNSUPPORTED,
+             "%s: %d query heads of %d a KV head", who, A.G, A.p.hd);
     if (batch->n_rows == 0) return HC_OK;
     HC_TRY(hc::page_rows_ok(who, "q", q, dtype));
     HC_CHECK(out && (uintptr_t)out % 4 == 0, HC_ERR_INVALID, "%s: NULL or misaligned out", who);

@@ -574,7 +574,7 @@ AttnPlan attn_plan(const AttnCall& X, const hc_paged_batch* b, int kv) {
         if (kv == HC_KV_Q4 && A.p.max_pages > 0) {
             // (sized by the table, not by the host's bound of the lengths, which chooses no results)
             const size_t page = (size_t)A.p.page_size * A.p.nkv * A.p.hd * 2, each = page * A.p.max_pages;
-            plan.at_once = (int)std::min<size_t>(A.p.n_seqs, std::max<size_t>(1, VALUES_AT_ONCE / (2 * each)));
+            plan.at_once = (int)std::min<size_t>(std::min(A.p.n_seqs, 65535), std::max<size_t>(1, VALUES_AT_ONCE / (2 * each)));
             plan.of_k = aligned(each * plan.at_once);
             plan.values = 2 * plan.of_k + aligned((size_t)4 * plan.at_once * A.p.max_pages);
             const hc::PagedAttnArgs B = over_values(A, 0, plan.at_once, nullptr, plan);

@@ -210,8 +210,7 @@ __global__ void __launch_bounds__(Q4_THREADS) k_q4_values(PagedArgs P, PagedScal
         if (src < 0) return;
     }
     const int units = P.nkv * P.page_size * hu;
-    const int unit = blockIdx.y * Q4_THREADS + threadIdx.x;
-    if (unit >= units) return;
+    for (int unit = blockIdx.y * Q4_THREADS + threadIdx.x; unit < units; unit += gridDim.y * Q4_THREADS) {
     const int u = unit % hu, at = unit / hu, slot = at % P.page_size, head = at / P.page_size;
     const int64_t kb = src * P.kps + head * P.khs + slot * P.kss + 4 * u, vb = src * P.vps + head * P.vhs + slot * P.vss + 4 * u;
     const uint32_t kw = __ldg(reinterpret_cast<const uint32_t*>((const uint8_t*)P.k + kb));
@@ -226,6 +225,7 @@ __global__ void __launch_bounds__(Q4_THREADS) k_q4_values(PagedArgs P, PagedScal
         q4_pairs(x ? vw : kw, s, z, e);  // (0, 4), (1, 5), (2, 6), (3, 7)
         *reinterpret_cast<uint4*>((x ? v : k) + to) = make_uint4(__byte_perm(e[0], e[1], 0x5410), __byte_perm(e[2], e[3], 0x5410),
                                                                 __byte_perm(e[0], e[1], 0x7632), __byte_perm(e[2], e[3], 0x7632));
+    }
     }
 }
 
@@ -255,8 +255,8 @@ int launch_append_q4(const AppendArgs& A, const PagedScales& C, int x16, cudaStr
 
 int launch_q4_values(const PagedArgs& P, const PagedScales& C, bool of_batch, __half* k, __half* v, int32_t* numbers, cudaStream_t s) {
     const int64_t units = (int64_t)P.nkv * P.page_size * (P.hd / 8), y = (units + Q4_THREADS - 1) / Q4_THREADS;
-    HC_CHECK(y <= 65535 && (!of_batch || P.n_seqs <= 65535), HC_ERR_INVALID, "pages of %d positions of %d heads, %d sequences", P.page_size, P.nkv, P.n_seqs);
-    const dim3 grid((unsigned)(of_batch ? P.max_pages : P.n_pages), (unsigned)y, of_batch ? (unsigned)P.n_seqs : 1u);
+    HC_CHECK(units <= 0x7fffffff - 65535ll * Q4_THREADS, HC_ERR_INVALID, "pages of %d positions of %d heads", P.page_size, P.nkv);
+    const dim3 grid((unsigned)(of_batch ? P.max_pages : P.n_pages), (unsigned)std::min<int64_t>(y, 65535), of_batch ? (unsigned)P.n_seqs : 1u);
     if (grid.x == 0) return HC_OK;
     k_q4_values<<<grid, Q4_THREADS, 0, s>>>(P, C, of_batch, k, v, numbers);
     HC_LAUNCH_CHECK();

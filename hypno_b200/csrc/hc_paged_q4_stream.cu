@@ -1,5 +1,6 @@
 // Attention of few rows, or of rows with lists of pages, over a pool in 4 bits
-// whose pages are runs of memory (k_paged_split takes the other layouts).
+// with heads of 64 or 128 elements and pages of whole tiles of 16 keys
+// (k_paged_split takes the others).
 //
 // The line of units, its runs, the join and the products are k_paged_split's.  A
 // fifth warp copies: a stage is 128 keys, eight tiles of 16 in a page each, so a

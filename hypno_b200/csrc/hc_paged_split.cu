@@ -55,12 +55,9 @@ int launch_paged_split(const PagedAttnArgs& A, const PagedScales& C, const Paged
     X.tg = (A.G + X.rows - 1) / X.rows;
     // one page a tile: pages of whole tiles, at most what 16 bits count
     X.uni = (kv == HC_KV_Q4 || L.width) && A.p.page_size % SP_TK == 0 && A.p.page_size <= 65536;
-    const int64_t row = A.p.hd / 2, sl = q4_slots(A.p.hd);
-    X.bulk = kv == HC_KV_Q4 && X.uni && (A.p.hd == 64 || A.p.hd == 128 || A.p.hd == 256) && A.p.kss == row && A.p.vss == row &&
-             C.kss == sl && C.vss == sl && (C.kps | C.khs | C.vps | C.vhs) % 8 == 0 && ((uintptr_t)C.k | (uintptr_t)C.v) % 16 == 0;
     X.po = (float*)ws;
     X.pml = (float2*)((float*)ws + (size_t)2 * SP_CTAS * 16 * A.p.hd);
-    if (X.bulk && A.p.hd <= 128) return launch_q4_stream(X, q16, s);
+    if (kv == HC_KV_Q4 && X.uni && (A.p.hd == 64 || A.p.hd == 128)) return launch_q4_stream(X, q16, s);
     if (L.width) return launch_split_list(X, q16, kv, s);
     return kv == HC_KV_Q4 ? launch_split_q4(X, q16, s) : launch_split_dense(X, q16, kv, s);
 }

@@ -63,7 +63,6 @@ struct SplitArgs {
     PagedList l;    // LIST only
     int tg;         // LIST: tiles of a token
     int uni;        // 4 bits, LIST: a tile of 16 keys lies in one page
-    int bulk;       // 4 bits: and its codes, and its scales, are one run of memory each
     int whole;
     int ctas;     // CTAs of the line (cut)
     int rows;     // R, rows of a tile
@@ -369,19 +368,6 @@ __device__ __forceinline__ float q4_value(uint32_t tile, uint32_t scales, int ke
     const uint32_t word = lds_u32(tile + key * ROWB + (d >> 3) * 4);
     return (float)((int)(word >> (4 * (d & 7)) & 15) - 8) * __half2float(lds_f16(scales + key * SCB + 2 * (d >> 5)));
 }
-// A copy of one run of memory, counted by an mbarrier.
-__device__ __forceinline__ void cp_run(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
-}
-// Waits for a stage's copies, a bounded time; the whole warp.
-__device__ __forceinline__ bool run_there(uint64_t* bar, uint32_t parity) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    const long long start = clock64();
-    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
-        if (__any_sync(0xffffffffu, clock64() - start > WAIT_CYCLES)) return false;
-    return true;
-}
 // 2^x; results below 2^-126 are zeros.
 template <bool FAST>
 __device__ __forceinline__ float pow2(float x) {
@@ -442,18 +428,8 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
     uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 511u);
     __shared__ float s_m[SP_WARPS][R], s_l[SP_WARPS][R];
     __shared__ uint32_t s_in[SP_WARPS][S];
-    __shared__ uint64_t s_full[Q4 ? SP_WARPS : 1][S];  // bulk: the copies of a warp's stages
     constexpr bool PLAN = Q4 || LIST;  // forms with one page a tile
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    [[maybe_unused]] uint32_t copied = 0;  // bulk: tiles of this warp so far
-    [[maybe_unused]] bool lost = false;    // bulk: a wait ran out
-    if constexpr (Q4) {
-        if (X.bulk) {
-            if (lane < S) mbar_init(&s_full[warp][lane], 1);
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-            __syncwarp();
-        }
-    }
     pdl_trigger();  // the join may become resident; it waits for this grid's end
 
     __shared__ LineTable s_line[1];
@@ -557,22 +533,6 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
         } else {
             look(0);
         }
-        // bulk: lanes 0 to 3 copy the codes of K and V and their scales
-        [[maybe_unused]] const uint8_t* run_from = nullptr;
-        [[maybe_unused]] int64_t run_page = 0, run_pos = 0;
-        [[maybe_unused]] uint32_t run_bytes = 0, run_to = 0;
-        if constexpr (Q4) {
-            if (X.bulk) {
-                const bool is_v = lane & 1, is_s = lane & 2;
-                const int64_t ps = is_s ? 2 * (is_v ? X.c.vps : X.c.kps) : is_v ? P.vps : P.kps;
-                const int64_t hs = is_s ? 2 * (is_v ? X.c.vhs : X.c.khs) : is_v ? P.vhs : P.khs;
-                run_from = (const uint8_t*)(is_s ? (is_v ? (const void*)X.c.v : (const void*)X.c.k) : is_v ? P.v : P.k) + kvh * hs;
-                run_page = ps;
-                run_pos = is_s ? SCB : ROWB;
-                run_bytes = SP_TK * (is_s ? SCB : ROWB);
-                run_to = ring + (is_s ? SC : 0) + (is_v ? run_bytes : 0);
-            }
-        }
         auto issue = [&](int i) {
             if (plan) {
                 if (i < mine) {
@@ -585,20 +545,6 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
                     }
                     const int page = __shfl_sync(0xffffffffu, now_page, i & 31);
                     const uint32_t at = __shfl_sync(0xffffffffu, now_place, i & 31), in = at & 0xffffu;
-                    if constexpr (Q4) {
-                        if (X.bulk) {
-                            if (lost) return;
-                            const uint32_t st = (copied + i) % S;
-                            if (lane == 0) {
-                                s_in[warp][st] = in;
-                                if (page < 0) mbar_arrive(&s_full[warp][st]);
-                                else mbar_expect_tx(&s_full[warp][st], Sh::STAGE);
-                            }
-                            if (lane < 4 && page >= 0)
-                                cp_run(run_to + st * Sh::STAGE, run_from + page * run_page + (int64_t)(at >> 16) * run_pos, run_bytes, &s_full[warp][st]);
-                            return;
-                        }
-                    }
                     page0 = in >> kr & 1u ? page : -1;  // (a key that no row sees is zeros)
                     page1 = in >> (kr + 8) & 1u ? page : -1;
                     slot0 = (int)(at >> 16) + kr;
@@ -751,16 +697,8 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
         const uint32_t vget = (uint32_t)(vrow * ROWB + (((mi & 1) ^ (vrow & 7)) << 4));
 
         for (int i = 0; i < mine; i++) {
-            uint32_t st = i % S;
-            if (Q4 && X.bulk) {
-                st = (copied + i) % S;
-                if (!lost && !run_there(&s_full[warp][st], (copied + i) / S & 1)) {
-                    lost = true;  // nothing is issued from here on; what is under way gets its time
-                    for (int k = 1; k < S - 1 && i + k < mine; k++) run_there(&s_full[warp][(copied + i + k) % S], (copied + i + k) / S & 1);
-                }
-            } else {
-                cp_wait<S - 2>();
-            }
+            const uint32_t st = i % S;
+            cp_wait<S - 2>();
             __syncwarp();
             issue(i + S - 1);
             const uint32_t kt = ring + st * Sh::STAGE, vt = kt + SP_TK * ROWB;
@@ -1022,15 +960,7 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
             }
             __syncwarp();
         }
-        if (Q4 && X.bulk) {
-            copied += mine;
-            if (lost) {  // (a copy that never came: not a number, rather than a wrong one)
-#pragma unroll
-                for (int n = 0; n < NQ; n++) sum[n][0] = sum[n][1] = __int_as_float(0x7FC00000);
-            }
-        } else {
-            cp_wait<0>();
-        }
+        cp_wait<0>();
         __syncwarp();
 
         // ---- this warp's (m, l, o) to shared memory (over its ring)
@@ -1082,8 +1012,6 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
                 if (d == 0) X.pml[slot * R + m] = make_float2(mm == -INFINITY ? mm : mm - BIAS, l);
             }
         }
-        // (bulk: the next pair's copies come after what was written and read here)
-        if (Q4 && X.bulk) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
     }
 }
@@ -1182,6 +1110,6 @@ int launch_split_hd(SplitArgs& X, cudaStream_t s) {
 int launch_split_dense(SplitArgs& X, int q16, int kv, cudaStream_t s);
 int launch_split_q4(SplitArgs& X, int q16, cudaStream_t s);
 int launch_split_list(SplitArgs& X, int q16, int kv, cudaStream_t s);
-int launch_q4_stream(SplitArgs& X, int q16, cudaStream_t s);
+int launch_q4_stream(SplitArgs& X, int q16, cudaStream_t s);  // heads of 64 or 128, X.uni
 
 }  // namespace hc

@@ -200,6 +200,13 @@ class PagedBatch:
             self.n_rows = n_rows
         return self.blob
 
+    def open(self):
+        """The same for a call that reads no rows: however many the row starts name."""
+        t, starts, lengths = self._tensors
+        n, pages = t.shape
+        return HC_PAGED_BATCH.pack(t.data_ptr(), starts.data_ptr(), lengths.data_ptr(), t.stride(0), n, pages, 2 ** 31 - 1 if n else 0,
+                                   *self._bounds, 0)
+
 
 def _rows(t, name, kv, dtype, n):
     shape = t.shape
@@ -381,9 +388,7 @@ def update_bounds(bounds, kv, batch):
     _same_device(kv, batch)
     if bounds.index != kv.index:
         raise ValueError(f"the bounds are on {bounds.device}, the pool on {kv.device}")
-    # no row is read, so their number may stay open where no call has named it yet
-    rows = batch.n_rows if batch.n_rows >= 0 else 2 ** 31 - 1 if batch.block_table.shape[0] else 0
-    check(load().hc_page_bounds_update_dev(bounds.ref, kv.ref, batch.pack(rows), raw_stream(kv.index)))
+    check(load().hc_page_bounds_update_dev(bounds.ref, kv.ref, batch.open(), raw_stream(kv.index)))
 
 
 def select_pages(bounds, batch, q, budget, first=1, recent=2, out=None):

@@ -75,6 +75,9 @@ class PagedModel:
         self.keep_pages = keep_pages
         man = hf.Manifest(np.frombuffer(image, np.uint8) if isinstance(image, (bytes, bytearray)) else image)
         meta = man.metadata
+        dim = int(meta["hidden_size"]) // int(meta["num_attention_heads"])
+        if cache_dtype == "q4" and (dim % 32 or dim > 256) or keep_pages is not None and (dim % 4 or dim > 256):
+            raise ValueError(f"heads of {dim} elements: 4 bits take a multiple of 32, keep_pages of 4, at most 256")
         self.device = torch.device("cuda", torch.cuda.current_device()) if str(device) == "cuda" else torch.device(device)
         self.workspace = ctypes.c_void_p()  # of this model's products
         with on_device(self.device.index):

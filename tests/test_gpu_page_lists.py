@@ -252,6 +252,43 @@ def test_select_ties_and_odd_values(cuda_device):
         check_select(c, cuda_device, d, 9)
 
 
+def test_select_with_a_wide_table_and_many_rows(cuda_device):
+    """Tables whose keys do not fit one CTA's memory, and more rows than a grid's third dimension takes: the form in two kernels."""
+    c = case("f32", [1, 3], [700, 333], 4, 2, 16, 16, 34)
+    b = all_bounds(c)
+    want = long.select(c, *b, 9)
+    kv, batch, q, _, _ = on_device(c, cuda_device)
+    h = paged.PageBounds(*(torch.from_numpy(t).to(cuda_device) for t in b), page_size=16)
+    wide = torch.full((2, 60000), -1, dtype=torch.int32, device=cuda_device)
+    wide[:, :c.table.shape[1]] = torch.from_numpy(c.table).to(cuda_device)
+    other = paged.PagedBatch(wide, batch.q_start, batch.kv_len, 3, 700)
+    assert np.array_equal(paged.select_pages(h, other, q, 9).cpu().numpy(), want)
+    n = 70000
+    i32 = dict(dtype=torch.int32, device=cuda_device)
+    many = paged.PagedBatch(batch.block_table[:1].repeat(n, 1), torch.arange(n + 1, **i32), torch.full((n,), 700, **i32), 1, 700)
+    got = paged.select_pages(h, many, q[:1].expand(n, -1, -1), 9)
+    assert torch.equal(got, torch.from_numpy(want[:1]).to(cuda_device).expand(n, -1, -1))
+
+
+def test_select_of_many_heads(cuda_device):
+    """A group of 130 query heads."""
+    c = case("f32", [2], [400], 130, 1, 256, 16, 35)
+    check_select(c, cuda_device, all_bounds(c), 9)
+
+
+def test_bounds_after_a_call_with_fewer_rows(cuda_device):
+    """update_bounds goes by the row starts, whatever other calls with the batch have read."""
+    c = case("f16", [1, 1, 33], [20, 40, 60], 4, 2, 64, 16, 36)
+    kv, batch, q, _, _ = on_device(c, cuda_device)
+    b = paged.PageBounds.alloc(kv)
+    paged.select_pages(b, batch, q[:2], 4)
+    paged.update_bounds(b, kv, batch)
+    want = [torch.zeros_like(t).cpu().numpy() for t in (b.lo, b.hi, b.scale)]
+    for g, filled in long.touched(c):
+        want[0][g], want[1][g], want[2][g] = long.bounds(c.k[g], filled)
+    assert all(np.array_equal(t.cpu().numpy(), w) for t, w in zip((b.lo, b.hi, b.scale), want))
+
+
 def test_rows_of_no_sequence_keep_their_lists(cuda_device):
     c = case("f32", [2, 1], [300, 200], 4, 2, 64, 16, 33)
     kv, batch, q, _, _ = on_device(c, cuda_device)
@@ -266,6 +303,37 @@ def test_rows_of_no_sequence_keep_their_lists(cuda_device):
 
 
 # ---------------------------------------------------------------- together
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_many_sequences(cuda_device, cache):
+    """More than the 32 whose places are worked out together."""
+    n = 75
+    c = case(cache, [1 + (i % 7 == 3) for i in range(n)], [2 + (131 * i) % 900 for i in range(n)], 8, 2, 64, 16, 46)
+    check_lists(c, cuda_device, some_pages(c, 11, 47))
+    kv, batch, q, _, _ = on_device(c, cuda_device)
+    lse = torch.empty((c.rows, 8), device=cuda_device)
+    out = paged.attention(kv, batch, q, lse=lse)
+    compare(c, out, lse, *ref.attention(c))
+    b = all_bounds(c)
+    check_select(c, cuda_device, b, 5)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_calls_on_two_streams_at_once(cuda_device, cache):
+    c = case(cache, [1, 2], [3000, 1700], 8, 2, 128, 16, 48)
+    kv, batch, q, _, _ = on_device(c, cuda_device)
+    pages = torch.from_numpy(some_pages(c, 90, 49)).to(cuda_device)
+    want = paged.attention(kv, batch, q, pages=pages), paged.attention(kv, batch, q)
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((paged.attention(kv, batch, q, pages=pages), paged.attention(kv, batch, q)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
 
 @pytest.mark.parametrize("cache", CACHES)
 def test_a_captured_step(cuda_device, cache):

@@ -223,8 +223,14 @@ def test_wide_tables_take_several_rounds(cuda_device):
     check_attention(c, cuda_device)
 
 
+def test_large_pages(cuda_device):
+    """Pages whose elements' eighths are more than a grid's second dimension takes, for a chunk and single tokens."""
+    for new in (1, 60):
+        check_attention(long.Case([new], [100], 8, 8, 128, 140000, 31, x=np.float16), cuda_device)
+
+
 def test_long_cache_offsets(cuda_device):
-    """Codes beyond 2^31 bytes of the pool, and scales beyond 2^31 bytes of theirs are not reached by it: a page stride of its own."""
+    """Codes beyond 2^31 bytes of the pool."""
     dim, page, heads, dev = 128, 16, 8, cuda_device
     n_pages = (1 << 31) // (heads * page * dim // 2) + 700
     codes = torch.zeros((n_pages, heads, page, dim // 2), dtype=torch.uint8, device=dev)
