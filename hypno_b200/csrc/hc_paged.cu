@@ -570,7 +570,13 @@ AttnPlan attn_plan(const AttnCall& X, const hc_paged_batch* b, int kv) {
     // tokens 207 / 147, 227 / 226; 32 tokens 702 / 148, 817 / 234.  One sequence
     // of 6 tokens: 26 / 19, 25 / 25.)
     const int64_t few = hc::paged_tiles(A, b->max_q_len, 16), many = hc::paged_tiles(A, b->max_q_len, 256);
-    if (!X.l.width && 2 * few > 3 * many) {
+    // Over 4 bits the values' way through memory comes on top (32 sequences as above: 230 us
+    // of it), so from more than five small tiles a large one on.  (Small tiles / large ones,
+    // us, those: 8 tokens, f16 129 / 307, f32 184 / 384; 16 tokens 235 / 308, 341 / 389; 32
+    // tokens 439 / 309, 644 / 393.  One sequence of 16,384 keys: 16 tokens 54 / 58, 68 /
+    // 72; 32 tokens 74 / 65, 100 / 78.  8 sequences of 1,024, 32 heads over 4 of 64: 16 tokens
+    // 25 / 27, 27 / 29; 32 tokens 36 / 32, 40 / 36.)
+    if (!X.l.width && (kv == HC_KV_Q4 ? few > 5 * many : 2 * few > 3 * many)) {
         if (kv == HC_KV_Q4 && A.p.max_pages > 0) {
             // (sized by the table, not by the host's bound of the lengths, which chooses no results)
             const size_t page = (size_t)A.p.page_size * A.p.nkv * A.p.hd * 2, each = page * A.p.max_pages;

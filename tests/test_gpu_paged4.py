@@ -210,7 +210,7 @@ def test_scales_of_the_scores(cuda_device, x, new):
 
 def test_wide_tables_take_several_rounds(cuda_device):
     """Prompts whose values do not fit the workspace together: 3 tables of 20,000 pages of 16."""
-    c = long.Case([40, 70, 33], [100, 70, 333], 8, 8, 128, 16, 30, x=np.float16)
+    c = long.Case([140, 170, 133], [200, 170, 333], 8, 8, 128, 16, 30, x=np.float16)
     wide = np.full((3, 20000), -1, np.int32)
     wide[:, :c.table.shape[1]] = c.table
     c.table = wide
