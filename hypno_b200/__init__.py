@@ -11,7 +11,8 @@ engine's interfaces:
     hypno_b200.convert     safetensors -> .hypno with Q4_0 packed on the GPU
                            (sft_convert.rs)
     hypno_b200.paged       paged KV cache: append with rotation, attention of
-                           ragged batches of chunks and single tokens, page owner
+                           ragged batches of chunks and single tokens, page owner;
+                           the cache in 4 bits, pages selected by score
     hypno_b200.sampling    tokens from given uniforms: temperature, top-k, top-p,
                            min-p
     hypno_b200.paged_model a .hypno model over a paged cache, and the continuous

@@ -46,6 +46,10 @@ __device__ __forceinline__ void key4(const PagedArgs& P, const PagedScales& C, i
     }
 }
 
+// Bounds.  Read from the keys that are stored, so that they hold whatever the cache
+// rounds.  Bound by latency (places, page, keys, one after another): 4 prompts of
+// 2,048 positions, 8 heads of 128, pages of 16, FP16: 12 us, 1.8 TB/s (17 us with a CTA
+// and shared memory a page).
 // A warp takes one page and KV head at a time, four elements of a key a lane: heads
 // of up to 64 elements two or more keys at once, of more than 128 in two rounds.  Its
 // loads do not depend on one another, so a page's keys are requested together.
@@ -393,7 +397,9 @@ __global__ void __launch_bounds__(PK_THREADS) k_page_pick(const __grid_constant_
 // bounds, the pick, one after another.  Scores by mma.sync on bytes, 16 pages a warp
 // against eight heads (the order of a head's elements is free, so a lane's operands
 // are its 16-byte pieces of a page's bounds): by dp4a, 8 rows of 64 heads over 2,048
-// pages took 17,000 to 27,000 cycles for the scores of a CTA's 256 pages.
+// pages took 17,000 to 27,000 cycles for the scores of a CTA's 256 pages, now 9,000.
+// That call: 19.5 us with the host's part (two kernels 28.7), of a cluster's 22,000
+// cycles some 3,000 for the queries and 8,000 for the pick.
 __device__ __forceinline__ void cluster_sync() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");

@@ -61,12 +61,12 @@ __device__ __forceinline__ void store8(T* p, bool vec, const float* x) {
 // Half pairs (HALVES): a thread reads its elements' partners too; of q, which may be
 // turned in place, the thread of the first elements turns both, and the one of the
 // second ones has nothing to do.
-// Bound by its bytes: q is read and written, k and v are read.
+// 8,192 rows of 32 + 8 + 8 heads of 128, f32: 67 us, 5.2 TB/s; 32 rows: 5.4.
 //
 // Codes: with i = 1 / s, x i is x / s within 2^-22 of itself, so its nearest whole number
 // is that of the division unless it lies within 2^-19 of the middle of two; such a
-// block divides.  (Divisions alone took a third of the kernel's instructions, and those are
-// what it is bound by: 8,192 rows of 32 + 8 + 8 heads of 128, 80 us.)
+// block divides.  (Divisions alone, and angles pair by pair, took a third of the kernel's
+// instructions: 8,192 rows 80 us.)
 __device__ __forceinline__ uint32_t q4_codes(const float* x, float s) {
     uint32_t code = 0;
     const float inv = __frcp_rn(s);
@@ -193,39 +193,41 @@ __global__ void __launch_bounds__(Q4_THREADS) k_q4_append(AppendArgs A, PagedSca
     }
 }
 
-// Values as float16, exactly: eight elements of K and of V a thread, positions of
-// a page side by side in both layouts.  Bound by its writes.
+// Values as float16, exactly: a CTA takes one page of one KV head, a thread eight
+// elements of K and of V of every (threads / eights)-th position.  Bound by its writes
+// (with a thread's place worked out from one index for all of a pool it was bound by
+// the divisions: 16,384 positions of 8 heads of 128, 25 us).
 __global__ void __launch_bounds__(Q4_THREADS) k_q4_values(PagedArgs P, PagedScales C, int of_batch, __half* k, __half* v,
                                                           int32_t* numbers) {
-    const int hu = P.hd >> 3;
-    int64_t page = blockIdx.x;
-    int src = blockIdx.x;
+    const int hu = P.hd >> 3, head = blockIdx.y;
+    int64_t page = blockIdx.x, src = blockIdx.x;
     if (of_batch) {
         const int b = blockIdx.z;
         page += (int64_t)b * P.max_pages;
         src = __ldg(P.table + (int64_t)b * P.table_stride + blockIdx.x);
         const int64_t begin = (int64_t)blockIdx.x * P.page_size;
-        if ((unsigned)src >= (unsigned)P.n_pages || begin >= seq_len(P, b)) src = -1;
-        if (blockIdx.y == 0 && threadIdx.x == 0) numbers[page] = src < 0 ? -1 : (int32_t)page;
+        if ((uint64_t)src >= (uint64_t)P.n_pages || begin >= seq_len(P, b)) src = -1;
+        if (head == 0 && threadIdx.x == 0) numbers[page] = src < 0 ? -1 : (int32_t)page;
         if (src < 0) return;
     }
-    const int units = P.nkv * P.page_size * hu;
-    for (int unit = blockIdx.y * Q4_THREADS + threadIdx.x; unit < units; unit += gridDim.y * Q4_THREADS) {
-    const int u = unit % hu, at = unit / hu, slot = at % P.page_size, head = at / P.page_size;
-    const int64_t kb = src * P.kps + head * P.khs + slot * P.kss + 4 * u, vb = src * P.vps + head * P.vhs + slot * P.vss + 4 * u;
-    const uint32_t kw = __ldg(reinterpret_cast<const uint32_t*>((const uint8_t*)P.k + kb));
-    const uint32_t vw = __ldg(reinterpret_cast<const uint32_t*>((const uint8_t*)P.v + vb));
-    const __half ks = C.k[src * C.kps + head * C.khs + slot * C.kss + (u >> 2)];
-    const __half vs = C.v[src * C.vps + head * C.vhs + slot * C.vss + (u >> 2)];
-    const int64_t to = (page * P.nkv * P.page_size + at) * P.hd + 8 * u;
+    const int u = threadIdx.x % hu, rows = Q4_THREADS / hu, r = threadIdx.x / hu;
+    if (r >= rows) return;
+    const uint8_t* kp = (const uint8_t*)P.k + src * P.kps + head * P.khs + 4 * u;
+    const uint8_t* vp = (const uint8_t*)P.v + src * P.vps + head * P.vhs + 4 * u;
+    const __half *ks = C.k + src * C.kps + head * C.khs + (u >> 2), *vs = C.v + src * C.vps + head * C.vhs + (u >> 2);
+    const int64_t to = (page * P.nkv + head) * P.page_size * P.hd + 8 * u;
+#pragma unroll 2
+    for (int slot = r; slot < P.page_size; slot += rows) {
+        const uint32_t w[2] = {__ldg(reinterpret_cast<const uint32_t*>(kp + slot * P.kss)), __ldg(reinterpret_cast<const uint32_t*>(vp + slot * P.vss))};
+        const __half sc[2] = {ks[slot * C.kss], vs[slot * C.vss]};
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
-        const __half2 s = __half2half2(x ? vs : ks), z = __hmul2(s, __half2half2(__float2half_rn(-72.0f)));
-        uint32_t e[4];
-        q4_pairs(x ? vw : kw, s, z, e);  // (0, 4), (1, 5), (2, 6), (3, 7)
-        *reinterpret_cast<uint4*>((x ? v : k) + to) = make_uint4(__byte_perm(e[0], e[1], 0x5410), __byte_perm(e[2], e[3], 0x5410),
-                                                                __byte_perm(e[0], e[1], 0x7632), __byte_perm(e[2], e[3], 0x7632));
-    }
+        for (int x = 0; x < 2; x++) {
+            const __half2 s = __half2half2(sc[x]), z = __hmul2(s, __half2half2(__float2half_rn(-72.0f)));
+            uint32_t e[4];
+            q4_pairs(w[x], s, z, e);  // (0, 4), (1, 5), (2, 6), (3, 7)
+            *reinterpret_cast<uint4*>((x ? v : k) + to + (int64_t)slot * P.hd) =
+                make_uint4(__byte_perm(e[0], e[1], 0x5410), __byte_perm(e[2], e[3], 0x5410), __byte_perm(e[0], e[1], 0x7632), __byte_perm(e[2], e[3], 0x7632));
+        }
     }
 }
 
@@ -254,9 +256,7 @@ int launch_append_q4(const AppendArgs& A, const PagedScales& C, int x16, cudaStr
 }
 
 int launch_q4_values(const PagedArgs& P, const PagedScales& C, bool of_batch, __half* k, __half* v, int32_t* numbers, cudaStream_t s) {
-    const int64_t units = (int64_t)P.nkv * P.page_size * (P.hd / 8), y = (units + Q4_THREADS - 1) / Q4_THREADS;
-    HC_CHECK(units <= 0x7fffffff - 65535ll * Q4_THREADS, HC_ERR_INVALID, "pages of %d positions of %d heads", P.page_size, P.nkv);
-    const dim3 grid((unsigned)(of_batch ? P.max_pages : P.n_pages), (unsigned)std::min<int64_t>(y, 65535), of_batch ? (unsigned)P.n_seqs : 1u);
+    const dim3 grid((unsigned)(of_batch ? P.max_pages : P.n_pages), (unsigned)P.nkv, of_batch ? (unsigned)P.n_seqs : 1u);
     if (grid.x == 0) return HC_OK;
     k_q4_values<<<grid, Q4_THREADS, 0, s>>>(P, C, of_batch, k, v, numbers);
     HC_LAUNCH_CHECK();

@@ -35,6 +35,9 @@ static int tile_height(const PagedAttnArgs& A, const PagedList& L, int max_q_len
 bool paged_split_whole(const PagedAttnArgs& A, const PagedList& L, int max_q_len, int max_kv_len) {
     if (L.width) {
         const int R = tile_height(A, L, max_q_len);
+        // lists are about as long as one another, so whole pairs are cut no worse than equal runs
+        // from four fifths of the last round of SMs on (256 pairs of 2,048 keys in 4 bits: 41.0 us
+        // cut, 40.4 whole)
         const int64_t pairs = (int64_t)A.p.n_rows * ((A.G + R - 1) / R) * A.p.nkv, rounds = (pairs + 147) / 148;
         if (5 * pairs >= 4 * 148 * rounds) return true;
         return (int64_t)L.width * A.p.page_size <= MIN_UNITS * UNIT;

@@ -41,7 +41,10 @@
 // makes of two keys' words, and its columns are a run of its bytes again.
 //
 // Lists of pages (LIST): a tile holds rows of one token, whose keys are the
-// positions of its listed pages one after another.
+// positions of its listed pages one after another; in pages of whole tiles a tile's
+// place is worked out once, by a lane, 16 tiles ahead.  8 tokens over 64 FP16 pages of 64
+// each, 64 heads over 8 of 128: 39 us with the join, 3.4 TB/s; bound by the latency of the start
+// (the list, its pages, their keys, one after another), not by its bytes.
 #pragma once
 
 #include "hc_paged.h"
