@@ -557,8 +557,8 @@ constexpr int SELECT_SMEM = 200 * 1024;
 
 template <typename T, int NX>
 int launch_select_t(const SelectArgs& A, int ctas, size_t smem, cudaStream_t s) {
-    // (the same for every call: calls of several threads may come between this and the launch)
-    HC_CUDA(cudaFuncSetAttribute(k_page_select<T, NX>, cudaFuncAttributeMaxDynamicSharedMemorySize, SELECT_SMEM));
+    static std::atomic<uint64_t> asked{0};
+    HC_TRY(ask_smem((const void*)k_page_select<T, NX>, SELECT_SMEM, asked));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas, (unsigned)A.p.nkv, (unsigned)A.p.n_rows);
     cfg.blockDim = dim3(PK_THREADS);

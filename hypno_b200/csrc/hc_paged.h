@@ -6,6 +6,7 @@
 #include "hc_internal.h"
 
 #include <algorithm>
+#include <atomic>
 
 namespace hc {
 
@@ -354,6 +355,18 @@ __device__ __forceinline__ void join_runs(int n, RowOf row_of, const float* po, 
             v.w = fmaf(f, y[i].w, v.w);
         }
     }
+}
+
+// Shared memory beyond 48 KB has to be asked for, once a kernel and device (asking takes
+// some 4 us of a call's 10 to 14); `asked` is the kernel's own.
+inline int ask_smem(const void* kernel, int bytes, std::atomic<uint64_t>& asked) {
+    int dev = 0;
+    HC_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (asked.load(std::memory_order_acquire) & bit) return HC_OK;
+    HC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    asked.fetch_or(bit, std::memory_order_release);
+    return HC_OK;
 }
 
 // Row tiles of all sequences, at most, from what the host knows.

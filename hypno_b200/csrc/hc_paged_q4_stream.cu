@@ -584,7 +584,8 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
 template <typename QT, int HD, int NQ, bool LIST>
 int launch_stream_t(SplitArgs& X, cudaStream_t s) {
     using Sh = StreamShape<HD, NQ, sizeof(QT) == 4>;
-    HC_CUDA(cudaFuncSetAttribute(k_paged_q4<QT, HD, NQ, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
+    static std::atomic<uint64_t> asked{0};
+    HC_TRY(ask_smem((const void*)k_paged_q4<QT, HD, NQ, LIST>, Sh::SMEM, asked));
     static const int resident = [] {
         int n = 0;
         if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_paged_q4<QT, HD, NQ, LIST>, QS_THREADS, Sh::SMEM) != cudaSuccess) n = 1;

@@ -405,9 +405,9 @@ __device__ __forceinline__ void load_q8(const QT* q, bool in, int vec, int d, fl
 }
 
 // CTAs an SM is to hold at least, for the forms whose copies are planned ahead (their
-// state would take the registers of the third).
+// state would take the registers of the third); 0: as the compiler likes it.
 template <typename CT, int HD, int NQ, bool LIST>
-constexpr int split_ctas() { return (LIST || std::is_same<CT, q4x>::value) && NQ == 1 && HD <= 128 ? 3 : 1; }
+constexpr int split_ctas() { return (LIST || std::is_same<CT, q4x>::value) && NQ == 1 && HD <= 128 ? 3 : 0; }
 
 template <typename QT, typename CT, int HD, int NQ, bool LIST>
 __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_paged_split(const __grid_constant__ SplitArgs X) {
@@ -1081,7 +1081,8 @@ int launch_join(const SplitArgs& X, int64_t pairs, cudaStream_t s) {
 template <typename QT, typename CT, int HD, int NQ, bool LIST>
 int launch_split_t(SplitArgs& X, cudaStream_t s) {
     using Sh = SplitShape<CT, HD>;
-    HC_CUDA(cudaFuncSetAttribute(k_paged_split<QT, CT, HD, NQ, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
+    static std::atomic<uint64_t> asked{0};
+    HC_TRY(ask_smem((const void*)k_paged_split<QT, CT, HD, NQ, LIST>, Sh::SMEM, asked));
     const PagedArgs& P = X.a.p;
     static const int resident = [] {  // CTAs an SM holds: the kernel's registers and shared memory decide
         int n = 0;
