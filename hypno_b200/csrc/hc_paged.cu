@@ -586,7 +586,11 @@ AttnPlan attn_plan(const AttnCall& X, const hc_paged_batch* b, int kv) {
             const hc::PagedAttnArgs B = over_values(A, 0, plan.at_once, nullptr, plan);
             if ((int64_t)plan.at_once * A.p.max_pages <= INT_MAX && hc::paged_tc_ok(B, 1)) {
                 plan.kernel = ATTN_TC;
-                plan.bytes = plan.values + hc::paged_tc_bytes(B, b->max_q_len, b->max_kv_len);
+                // (the last round may have fewer sequences, and so more runs of keys)
+                const int rest = A.p.n_seqs % plan.at_once;
+                size_t runs = hc::paged_tc_bytes(B, b->max_q_len, b->max_kv_len);
+                if (rest) runs = std::max(runs, hc::paged_tc_bytes(over_values(A, 0, rest, nullptr, plan), b->max_q_len, b->max_kv_len));
+                plan.bytes = plan.values + runs;
                 return plan;
             }
         } else if (hc::paged_tc_ok(A, kv == HC_KV_FP16)) {

@@ -223,6 +223,32 @@ def test_wide_tables_take_several_rounds(cuda_device):
     check_attention(c, cuda_device)
 
 
+def test_a_smaller_last_round(cuda_device):
+    """Three sequences' values at a time, then the fourth's; the fourth's keys are cut into more runs."""
+    c = long.Case([140, 170, 133, 100], [200, 170, 333, 1200], 2, 2, 128, 16, 32, x=np.float16)
+    wide = np.full((4, 20000), -1, np.int32)
+    wide[:, :c.table.shape[1]] = c.table
+    c.table = wide
+    check_attention(c, cuda_device, batch_edit=lambda b: paged.PagedBatch(b.block_table, b.q_start, b.kv_len, 170, 320000))
+
+
+def test_rows_behind_the_last_sequence(cuda_device):
+    """A padded batch: outputs, queries and pages of rows that belong to no sequence stay as they were."""
+    for new in ([1, 2], [140, 30]):
+        c = long.Case(new, [n + 60 for n in new], 4, 2, 128, 16, 33)
+        kv, batch, q, kn, vn = on_device(c, cuda_device)
+        q2, k2, v2 = (torch.cat([t, torch.full_like(t[:1], 9).repeat(5, 1, 1)]) for t in (q, kn, vn))
+        out, turned = torch.full_like(q2, 3.0), torch.full_like(q2, 4.0)
+        want = paged.attention(kv, batch, q)
+        paged.attention(kv, batch, q2, out=out)
+        assert torch.equal(out[:-5], want) and bool((out[-5:] == 3.0).all())
+        rope = paged.rope_table(256, 128, 1e4, cuda_device)
+        want = paged.append(kv, batch, kn, vn, q=q, rope=rope)
+        held = kv.values()
+        paged.append(kv, batch, k2, v2, q=q2, rope=rope, q_out=turned)
+        assert torch.equal(turned[:-5], want) and bool((turned[-5:] == 4.0).all()) and all(torch.equal(a, b) for a, b in zip(kv.values(), held))
+
+
 def test_large_pages(cuda_device):
     """Pages whose elements' eighths are more than a grid's second dimension takes, for a chunk and single tokens."""
     for new in (1, 60):

@@ -114,6 +114,22 @@ def test_refusals_at_the_c_entries(lib):
     assert lib.hc_page_bounds_values_dev(ctypes.addressof(bounds()), at, None, None) == -1
 
 
+def test_the_workspace_fits_the_last_round_of_a_chunk_over_4_bits(lib):
+    """Four sequences whose values fit three at a time: the last one alone is cut into more runs than the three together."""
+    at, need = 1 << 20, ctypes.c_size_t()
+    kv = _lib.HcPagedKV4(_lib.HcPagedKV(at, at, 1024, 1024, 64, 1024, 1024, 64, _lib.KV_Q4, 4, 16, 1, 128, 0), at, at, 64, 64, 4, 64, 64, 4)
+    pages, each = 40000, 40000 * 16 * 128 * 2
+
+    def bytes_of(seqs):
+        batch = _lib.HC_PAGED_BATCH.pack(at, at, at, pages, seqs, pages, 800, 200, 640000, 0)
+        assert lib.hc_paged_attention_workspace(ctypes.addressof(kv), batch, 1, 1, 0, ctypes.byref(need)) == 0
+        return need.value
+
+    runs = lambda seqs, together: bytes_of(seqs) - 2 * together * each - 4 * together * pages  # noqa: E731  (each part a multiple of 256)
+    assert 2 * each * 3 <= 2 ** 30 < 2 * each * 4 and runs(1, 1) > runs(3, 3) > 0
+    assert runs(4, 3) >= runs(1, 1)
+
+
 def test_a_step_refuses_rows_that_are_not_single():
     m = PagedModel.__new__(PagedModel)
     m.vocab, m.device, m.keep_pages = 50, None, 4
