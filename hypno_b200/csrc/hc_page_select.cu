@@ -335,7 +335,7 @@ __device__ __forceinline__ void pick_pages(const uint32_t* keys, int n, int budg
         }
         __syncthreads();
         lo += (uint32_t)S.bin << shift;
-        hi = min(hi, lo + ((1u << shift) - 1));
+        hi = lo + min(hi - lo, (1u << shift) - 1);  // (lo + a step may pass 32 bits: KEY_INF lies there)
         left = S.left;
         const int held = S.held;
         __syncthreads();
@@ -370,7 +370,7 @@ __device__ __forceinline__ void pick_pages(const uint32_t* keys, int n, int budg
     for (int i = i0; i < i1; i++) {
         const uint32_t k = keys[i];
         const bool kept = i < begin || i >= end;
-        if (kept || k > above || (k == above && e++ < left)) out[at++] = i;
+        if ((kept || k > above || (k == above && e++ < left)) && at < budget) out[at++] = i;
     }
 }
 

@@ -270,6 +270,29 @@ def test_select_with_a_wide_table_and_many_rows(cuda_device):
     assert torch.equal(got, torch.from_numpy(want[:1]).to(cuda_device).expand(n, -1, -1))
 
 
+@pytest.mark.parametrize("dim", [16, 12])      # in one kernel, in two
+@pytest.mark.parametrize("x", [np.float32, np.float16], ids=["qf32", "qf16"])
+@pytest.mark.parametrize("infinite", [1, 10, 37, 40])
+@pytest.mark.parametrize("holes", [0, 1, 25])
+def test_select_with_more_infinite_pages_than_places(cuda_device, dim, x, infinite, holes):
+    """Beside finite pages, one or many, and holes; nothing behind the lists is written."""
+    c = case("f32", [1, 2], [640, 635], 4, 2, dim, 16, 37, x=x)
+    b = all_bounds(c)
+    g = np.random.default_rng(infinite + holes)
+    for s in range(2):
+        at = g.permutation(40)
+        b[2][c.table[s, at[:infinite]]] = np.inf
+        c.table[s, at[max(40 - holes, 1):]] = -1
+    kv, batch, q, _, _ = on_device(c, cuda_device)
+    h = paged.PageBounds(*(torch.from_numpy(t).to(cuda_device) for t in b), page_size=16)
+    for budget, first, recent in ((6, 1, 2), (3, 0, 0), (16, 1, 2), (39, 1, 1), (4, 2, 2)):
+        room = torch.full((3 * 2 * budget + 256,), 77, dtype=torch.int32, device=cuda_device)
+        out = room[:3 * 2 * budget].view(3, 2, budget)
+        paged.select_pages(h, batch, q, budget, first, recent, out=out)
+        assert np.array_equal(out.cpu().numpy(), long.select(c, *b, budget, first, recent))
+        assert bool((room[3 * 2 * budget:] == 77).all())
+
+
 def test_select_of_many_heads(cuda_device):
     """A group of 130 query heads."""
     c = case("f32", [2], [400], 130, 1, 256, 16, 35)
