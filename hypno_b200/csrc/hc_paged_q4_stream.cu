@@ -172,6 +172,10 @@ __device__ __forceinline__ void stream_copies(const SplitArgs& X, const LineTabl
                 have = (int)min((int64_t)have, w.p_own - pos + 1);
                 if (A.window > 0) low = (int)min(max(w.p_own - A.window + 1 - pos, (int64_t)0), (int64_t)SP_TK);
                 if (have <= low) return (int64_t)0;
+            } else if (A.window > 0 && w.one_token) {
+                // (a lone token's first tile begins in front of its window: what lies there, it
+                // may not be finite, is not there; tiles of several tokens look for that by themselves)
+                low = min(max(w.p_own - A.window + 1 - (int)v, 0), SP_TK);
             }
             const int64_t g = __ldg(P.table + (int64_t)w.seq * P.table_stride + x);
             if ((uint64_t)g >= (uint64_t)P.n_pages) return (int64_t)0;

@@ -465,7 +465,8 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
         int m0, mrows;
         tile_rows<LIST>(X, pair / P.nkv, at.w.r1 - r0, m0, mrows);
         int begin, end;
-        const int p_own = first + token_of(A, m0);  // LIST: position of the tile's token
+        const int p_own = first + token_of(A, m0);  // position of the tile's first token; LIST: of its only one
+        const bool one_token = token_of(A, m0) == token_of(A, m0 + mrows - 1);
         const int32_t* list = nullptr;
         if constexpr (LIST) {
             const int row = r0 + token_of(A, m0);
@@ -523,6 +524,8 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
                 n = (int)min((int64_t)n, p_own - pos + 1);
                 if (A.window > 0) low = (int)min(max(p_own - A.window + 1 - pos, (int64_t)0), (int64_t)SP_TK);
                 if (n <= low) return;
+            } else if (A.window > 0 && one_token) {  // (begins at a tile's first key: what lies in front of the window is not there)
+                low = min(max(p_own - A.window + 1 - v, 0), SP_TK);
             }
             const int g = __ldg(P.table + (int64_t)seq * P.table_stride + x);
             if ((unsigned)g >= (unsigned)P.n_pages) return;
@@ -675,7 +678,6 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
         }
         // keys that every row of the tile sees
         const int p_min = first + token_of(A, m0), l_max = A.window > 0 ? first + token_of(A, m0 + mrows - 1) - A.window + 1 : 0;
-        const bool one_token = token_of(A, m0) == token_of(A, m0 + mrows - 1);
 
         float o[NQ][DT][4];
         float mx[NQ][2], sum[NQ][2];  // running maximum; sum of this thread's keys only

@@ -155,6 +155,27 @@ def test_later_tokens_do_not_reach_a_row(cuda_device, x, dim, new):
 
 
 @pytest.mark.parametrize("x", X, ids=IDS)
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (8, 1), (16, 1), (24, 1)])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (64, 32), (96, 16), (160, 16), (128, 20)])
+@pytest.mark.parametrize("new", [1, 2, 3])
+def test_what_has_left_the_window_does_not_reach_a_row(cuda_device, x, heads, kv_heads, dim, page, new):
+    """Everything in front of the windows of a sequence's rows is not finite, up to the key before the first one's, for
+    tiles of one token and of several, windows that begin at every place of a tile."""
+    lens = [40, 47, 48, 49, 63, 300, 1111]
+    c = long.Case([new] * len(lens), lens, heads, kv_heads, dim, page, 34, x=x)
+    for window in (1, 15, 16, 30, 37):
+        d = [t.copy() for t in c.pools]
+        for b, n in enumerate(lens):
+            for j in range(max(n - new - window + 1, 0)):
+                for t in (d[1], d[3]):
+                    t[c.page_of(b, j), :, j % page, :dim // 32] = np.nan
+        held, c.pools = c.pools, d
+        out = check_attention(c, cuda_device, window=window)
+        assert bool(torch.isfinite(out).all())
+        c.pools = held
+
+
+@pytest.mark.parametrize("x", X, ids=IDS)
 @pytest.mark.parametrize("order", ["head", "page"])
 def test_strides(cuda_device, x, order):
     check_attention(long.Case([1, 9, 140], [33, 65, 200], 8, 2, 64, 16, 8, x=x), cuda_device, order=order, fused=True)
