@@ -283,10 +283,10 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
             const bool in = m < w.mrows;
             const int t = token_of(A, w.m0 + m);
             const QT* q = (const QT*)A.q + (in ? (int64_t)(w.r0 + t) * A.q_rs + (w.kvh * A.G + (w.m0 + m) - t * A.G) * A.q_hs : 0);
-            // (a factor below zero turns the query's sign, one of zero its elements to zeros)
-            float f = A.scale == 0.0f ? 1.0f : fabsf(A.scale) * LOG2E;
+            // (a factor below zero turns the query's sign)
+            float f = fabsf(A.scale) * LOG2E;
             float x[8], top = 0.0f, by = A.scale < 0.0f ? -1.0f : 1.0f;
-            load_q8(q, in && A.scale != 0.0f, A.qvec, 8 * kw, x);
+            load_q8(q, in, A.qvec, 8 * kw, x);
             if constexpr (HILO) {
 #pragma unroll
                 for (int y = 0; y < 8; y++) top = fmaxf(top, fabsf(x[y]));
@@ -297,7 +297,9 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
                 by *= __uint_as_float((uint32_t)(254 - e) << 23);
                 f *= __uint_as_float((uint32_t)e << 23);
             }
-            if (kw == 0) s_cf[m] = f;
+            // Scores are masked with -inf before they are multiplied, so the factor is above zero: a
+            // product with 2^-126 of a score below 2^90 is as good as zero, one that is not finite stays so.
+            if (kw == 0) s_cf[m] = f < 0x1p-126f ? 0x1p-126f : f;
             const int part = kw / (LE / 8), k = kw % (LE / 8);  // word k of lane part's share of a key
             uint32_t* to = qf + ((m >> 3) * KS * 32 + (m & 7) * 4 + part) * FW;
 #pragma unroll
@@ -308,7 +310,7 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
             }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(QS_ROWS) : "memory");
-        float cf[NQ][2];  // score factors of this thread's two columns, not negative
+        float cf[NQ][2];  // score factors of this thread's two columns, above zero
 #pragma unroll
         for (int n = 0; n < NQ; n++)
 #pragma unroll

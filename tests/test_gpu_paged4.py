@@ -229,6 +229,25 @@ def test_scales_of_the_scores(cuda_device, x, new):
         check_attention(c, cuda_device, scale=1e-6)
 
 
+@pytest.mark.parametrize("x", X, ids=IDS)
+@pytest.mark.parametrize("dim", [64, 128, 96])
+@pytest.mark.parametrize("new", [1, 3])
+def test_scales_that_vanish(cuda_device, x, dim, new):
+    """A scale of zero, or one that leaves nothing of a row's scores: every key weighs the same, of rows of zeros, of the
+    smallest and of ordinary elements, over whole tiles and cut ones; rows that are not finite stay so."""
+    c = long.Case([new] * 5, [32, 40, 75, 131, 500], 4, 2, dim, 16, 35, x=x)
+    c.q[0], c.q[1, :2], c.q[-1, 1], c.q[2] = 0, 0, 0, np.finfo(x).tiny
+    for scale in (0.0, 1e-45, 1e-38, 1e-30, -1e-30, 1e-8, None):
+        check_attention(c, cuda_device, scale=scale)
+        check_attention(c, cuda_device, scale=scale, window=21)
+    kv, batch, q, _, _ = on_device(c, cuda_device)
+    q[0, 1, 5], q[-1, 2, 0] = float("nan"), float("inf")
+    for scale in (0.0, 1e-30, None):
+        got = paged.attention(kv, batch, q, scale=scale)
+        nan = torch.isnan(got).all(-1)
+        assert bool(nan[0, 1]) and bool(nan[-1, 2]) and int(nan.sum()) == 2 and bool(torch.isfinite(got[~nan]).all())
+
+
 def test_wide_tables_take_several_rounds(cuda_device):
     """Prompts whose values do not fit the workspace together: 3 tables of 20,000 pages of 16."""
     c = long.Case([140, 170, 133], [200, 170, 333], 8, 8, 128, 16, 30, x=np.float16)
