@@ -93,27 +93,29 @@ template <int STAGES>
 struct StreamBars {
     uint64_t full[STAGES], empty[STAGES];
     uint32_t in[STAGES][QS_TILES];  // which keys of a tile are there
-    uint64_t told[2], read[2];      // the pairs that the copying warp has told of, that the others have done with
     PairWork work[2];
-    int abort, stuck;  // a wait for copies or stages, for pairs ran out
+    int abort;  // a wait for copies or stages ran out
 };
+// The copying warp tells of a pair by one barrier of the CTA, and the others that they have
+// done with it by another, in turn for even and odd pairs.  (Barriers of all threads: what
+// they wait for always comes, because the waits for copies and stages are bounded, and a
+// warp that gave one up goes on to the CTA's last pair.)  The numbers are the instructions'
+// own: taken from a register, 32 tokens over listed pages took 39.5 us in place of 39.0.
+constexpr int QS_TOLD = 2, QS_READ = 4;
+template <int ID>
+__device__ __forceinline__ void pair_sync(bool odd) {
+    if (odd) asm volatile("bar.sync %0, %1;" ::"n"(ID + 1), "n"(QS_THREADS) : "memory");
+    else asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(QS_THREADS) : "memory");
+}
+template <int ID>
+__device__ __forceinline__ void pair_arrive(bool odd) {
+    if (odd) asm volatile("bar.arrive %0, %1;" ::"n"(ID + 1), "n"(QS_THREADS) : "memory");
+    else asm volatile("bar.arrive %0, %1;" ::"n"(ID), "n"(QS_THREADS) : "memory");
+}
 
 // Waits a bounded time; the whole warp.  (The clock is read when the first look fails.)
 __device__ __forceinline__ bool stream_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
     return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
-}
-// Whether a condition holds for all threads of the rows' warps, which meet here.
-__device__ __forceinline__ bool all_rows(bool p) {
-    int r;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.s32 p, %1, 0;\n\t"
-        "barrier.cta.red.and.pred q, 1, %2, p;\n\t"
-        "selp.s32 %0, 1, 0, q;\n\t}"
-        : "=r"(r)
-        : "r"((int)p), "n"(QS_ROWS)
-        : "memory");
-    return r != 0;
 }
 // Arrives at the barrier when this thread's copies so far have landed.
 __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
@@ -140,11 +142,10 @@ __device__ __forceinline__ void stream_copies(const SplitArgs& X, const LineTabl
         w.lost = !ok;
         if (!ok) w.stages = 0;
         if (!more) w.stages = -1;
-        if (pairs >= 2 && !stream_wait(&B.read[pairs & 1], (pairs >> 1 & 1) ^ 1, &B.stuck)) break;
-        if (lane == 0) {
-            B.work[pairs & 1] = w;
-            mbar_arrive(&B.told[pairs & 1]);
-        }
+        if (pairs >= 2) pair_sync<QS_READ>(pairs & 1);
+        if (lane == 0) B.work[pairs & 1] = w;
+        __syncwarp();
+        pair_arrive<QS_TOLD>(pairs & 1);
         pairs++;
         if (!more) break;
         if (!ok) continue;
@@ -217,6 +218,7 @@ __device__ __forceinline__ void stream_copies(const SplitArgs& X, const LineTabl
     }
     cp_commit();
     cp_wait<0>();  // every copy has landed before the CTA ends
+    if (pairs >= 2) pair_sync<QS_READ>(pairs & 1);  // (the last pair's, so that no barrier is left half full)
 }
 
 template <typename QT, int HD, int NQ, bool LIST>
@@ -240,11 +242,7 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
             mbar_init(&B.full[i], 32);
             mbar_init(&B.empty[i], QS_WARPS);
         }
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&B.told[i], 1);
-            mbar_init(&B.read[i], QS_WARPS);
-        }
-        B.abort = B.stuck = 0;
+        B.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1 && A.p.n_seqs <= 32) fill_table<LIST>(X, line);
@@ -268,10 +266,8 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
     bool lost = false;
     const int c = lane & 3, col = 2 * c, k0 = q4_key(lane >> 2);
     for (uint32_t pairs = 0;; pairs++) {
+        pair_sync<QS_TOLD>(pairs & 1);  // (by then the outputs before have been read, too)
         // (read where it is needed: kept in registers it would cost a warp's worth of them)
-        const bool told = stream_wait(&B.told[pairs & 1], pairs >> 1 & 1, &B.stuck);
-        // (all warps go on together, or none; and the outputs before have been read)
-        if (!all_rows(told)) break;
         const volatile PairWork& w = B.work[pairs & 1];
         const int stages = w.stages, c0 = w.c0;
         if (stages < 0) break;
@@ -583,7 +579,7 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
             }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&B.read[pairs & 1]);
+        pair_arrive<QS_READ>(pairs & 1);
     }
 }
 
