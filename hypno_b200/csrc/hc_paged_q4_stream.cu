@@ -212,6 +212,9 @@ __device__ __forceinline__ void stream_copies(const SplitArgs& X, const LineTabl
                 cp_small<Sh::SCB>(to_s + base + x * SP_TK * Sh::SCB, sf, true);
             }
             cp_arrive(&B.full[st]);
+            // (that arrival orders a lane's copies alone: its stores are published by one of their own)
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B.full[st]);
             from = next_from;
             keys = next_keys;
         }
@@ -239,7 +242,7 @@ __global__ void __launch_bounds__(QS_THREADS, NQ == 1 ? 3 : 2) k_paged_q4(const 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; i++) {
-            mbar_init(&B.full[i], 32);
+            mbar_init(&B.full[i], 33);  // 32 lanes' copies, and the keys' masks
             mbar_init(&B.empty[i], QS_WARPS);
         }
         B.abort = 0;
