@@ -162,8 +162,10 @@ def _int32(t, name, dim, index):
 class PagedBatch:
     """The new tokens of a step.  block_table [n_seqs, max_pages] (an entry
     outside the pool is a hole), q_start [n_seqs + 1] (the packed rows of
-    sequence b are q_start[b] .. q_start[b + 1] - 1), kv_len [n_seqs] (its
-    positions, the new ones included), all int32 on the pool's device.
+    sequence b are q_start[b] .. q_start[b + 1] - 1; rows in front of the first
+    and behind the last belong to no sequence, and their places in outputs keep what
+    they had), kv_len [n_seqs] (its positions, the new ones included), all int32 on
+    the pool's device.
     max_q_len and max_kv_len are the host's upper bounds on a sequence's rows
     and positions: they choose launches, not results.  The tensors' contents may
     change between calls; other tensors or bounds are another batch."""

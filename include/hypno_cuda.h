@@ -308,9 +308,12 @@ typedef struct hc_paged_kv_q4 {
 } hc_paged_kv_q4;
 
 /* The new tokens of a step, packed: sequence b owns the rows q_start[b] ..
- * q_start[b + 1] - 1 (q_start[0] = 0, non-decreasing, q_start[n_seqs] =
- * n_rows), and its kv_len[b] positions end with them, so its i-th row stands
- * at position kv_len[b] - (q_start[b + 1] - q_start[b]) + i.  Position p of
+ * q_start[b + 1] - 1 (non-decreasing, from 0 to n_rows), and its kv_len[b]
+ * positions end with them, so its i-th row stands at position kv_len[b] -
+ * (q_start[b + 1] - q_start[b]) + i.  Rows in front of q_start[0] and from
+ * q_start[n_seqs] on belong to no sequence: nothing is stored for them, and their
+ * places in outputs keep what they had (so a part of a step's sequences is a
+ * batch over the step's rows, and a batch may be padded).  Position p of
  * sequence b lives in page block_table[b * table_stride + p / page_size]; an
  * entry outside [0, n_pages) and a position beyond max_pages * page_size is a
  * hole, whatever kv_len[b] is (below 0: no positions).  All arrays are device memory.  max_q_len and max_kv_len are the

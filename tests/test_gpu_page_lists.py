@@ -325,6 +325,43 @@ def test_rows_of_no_sequence_keep_their_lists(cuda_device):
     assert bool((res[3:] == 3.0).all()) and torch.equal(res[:3], paged.attention(kv, batch, q, pages=out[:3]))
 
 
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("new", [[1, 1, 2], [1, 70, 200]])
+def test_a_part_of_a_steps_sequences(cuda_device, cache, new):
+    """A batch whose rows begin behind others and end before others: the ones that belong to no sequence keep what they
+    had, store nothing, and the rest is as without them."""
+    c = case(cache, new, [n + 300 for n in new], 8, 2, 64, 16, 50)
+    kv, batch, q, kn, vn = on_device(c, cuda_device)
+    rope = paged.rope_table(512, 64, 1e4, cuda_device)
+    b = paged.PageBounds(*(torch.from_numpy(t).to(cuda_device) for t in all_bounds(c)), page_size=16)
+    pools = list(kv.pools) if cache == "q4" else [kv.k, kv.v]
+    held = [t.clone() for t in pools]
+
+    def step(batch, q, kn, vn, outs):
+        for t, was in zip(pools, held):
+            t.copy_(was)
+        paged.append(kv, batch, kn, vn, q=q, rope=rope, q_out=outs[0])
+        paged.update_bounds(b, kv, batch)
+        paged.select_pages(b, batch, outs[0], 9, out=outs[1])
+        paged.attention(kv, batch, outs[0], out=outs[2], lse=outs[3])
+        paged.attention(kv, batch, outs[0], out=outs[4], pages=outs[1])
+        return [t.clone() for t in (*pools, b.lo, b.hi, b.scale)]
+
+    def empty(n):
+        return [torch.full((n, 8, 64), 5.0, device=cuda_device), torch.full((n, 2, 9), 5, dtype=torch.int32, device=cuda_device),
+                torch.full((n, 8, 64), 5.0, device=cuda_device), torch.full((n, 8), 5.0, device=cuda_device), torch.full((n, 8, 64), 5.0, device=cuda_device)]
+
+    want = empty(c.rows)
+    state = step(batch, q, kn, vn, want)
+    wide = [torch.cat([torch.full_like(t[:1], 9).repeat(7, 1, 1), t, torch.full_like(t[:1], 9).repeat(4, 1, 1)]) for t in (q, kn, vn)]
+    got = empty(c.rows + 11)
+    part = paged.PagedBatch(batch.block_table, batch.q_start + 7, batch.kv_len, batch.max_q_len, batch.max_kv_len)
+    again = step(part, *wide, got)
+    for a, w in zip(got, want):
+        assert torch.equal(a[7:-4], w) and bool((a[:7] == 5).all()) and bool((a[-4:] == 5).all())
+    assert all(torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8)) for x, y in zip(again, state))
+
+
 # ---------------------------------------------------------------- together
 
 @pytest.mark.parametrize("cache", CACHES)
