@@ -393,8 +393,8 @@ __global__ void __launch_bounds__(PK_THREADS) k_page_pick(const __grid_constant_
 
 // ---- both in one: a cluster of CTAs scores a row and KV head's pages, each a share
 // of them, into the first one's shared memory, which picks.  One launch and no
-// workspace.  Bound by latency: a cluster's start, the row's place, the queries, the
-// bounds, the pick, one after another.  Scores by mma.sync on bytes, 16 pages a warp
+// workspace.  Bound by steps that follow one another: a cluster's start, the row's place, the
+// queries, the bounds, and the pick, which the first CTA does alone.  Scores by mma.sync on bytes, 16 pages a warp
 // against eight heads (the order of a head's elements is free, so a lane's operands
 // are its 16-byte pieces of a page's bounds): by dp4a, 8 rows of 64 heads over 2,048
 // pages took 17,000 to 27,000 cycles for the scores of a CTA's 256 pages, now 9,000.

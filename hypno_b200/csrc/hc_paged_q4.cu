@@ -63,9 +63,9 @@ __device__ __forceinline__ void store8(T* p, bool vec, const float* x) {
 // second ones has nothing to do.
 // 8,192 rows of 32 + 8 + 8 heads of 128, f32: 67 us, 5.2 TB/s; 32 rows: 5.4.
 //
-// Codes: with i = 1 / s, x i is x / s within 2^-22 of itself, so its nearest whole number
-// is that of the division unless it lies within 2^-19 of the middle of two; such a
-// block divides.  (Divisions alone, and angles pair by pair, took a third of the kernel's
+// Codes: with i = 1 / s rounded, x i is within 7 2^-24 < 2^-21 of x / s, which is 7 at most,
+// and the difference to its nearest whole number rounds by less than 2^-24, so that number is
+// the division's unless it lies within 2^-19 of the middle of two; such a block divides.  (Divisions alone, and angles pair by pair, took a third of the kernel's
 // instructions: 8,192 rows 80 us.)
 __device__ __forceinline__ uint32_t q4_codes(const float* x, float s) {
     uint32_t code = 0;

@@ -14,9 +14,9 @@
 // elements), half of the 405 instructions that 16 keys of a head of 128 cost.  Bound by
 // them: shifts, logic and float16 arithmetic run at half rate, and what depends on
 // what leaves a scheduler's three or four warps idle on 40% of the cycles.  8 sequences
-// of up to 32,768 keys, 64 heads over 8 of 128, f16: 69 us, 3.3 TB/s (the copies alone 46;
-// issue slots 59%, logic 43%); 32 of up to 2,304, 32 heads over 8, f32: 31 us with the
-// join; 32 tokens over 128 listed pages of 16 each: 39 us.  (Five warps a scheduler at 96 registers
+// of up to 32,768 keys, 64 heads over 8 of 128, f16: 70 us, 3.2 TB/s (the copies alone 46;
+// issue slots 59%, logic 43%, so neither is at its limit); 32 of up to 2,304, 32 heads over 8,
+// f32: 31 us with the join; 32 tokens over 128 listed pages of 16 each: 39 us.  (Five warps a scheduler at 96 registers
 // for the first: 73 us; eight warps of 16 keys each: 84.)
 #include "hc_paged_split.cuh"
 

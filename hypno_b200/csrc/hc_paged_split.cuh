@@ -44,7 +44,9 @@
 // positions of its listed pages one after another; in pages of whole tiles a tile's
 // place is worked out once, by a lane, 16 tiles ahead.  8 tokens over 64 FP16 pages of 64
 // each, 64 heads over 8 of 128: 39 us with the join, 3.4 TB/s; bound by the latency of the start
-// (the list, its pages, their keys, one after another), not by its bytes.
+// (the list, its pages, their keys, one after another) and of the copies, which the warps
+// that compute issue themselves, two tiles ahead.  FP32 pages, the caches cold: 121 us where
+// FP16 ones take 47, by the three products and the splitting of both operands.
 #pragma once
 
 #include "hc_paged.h"
@@ -465,7 +467,7 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
         int m0, mrows;
         tile_rows<LIST>(X, pair / P.nkv, at.w.r1 - r0, m0, mrows);
         int begin, end;
-        const int p_own = first + token_of(A, m0);  // position of the tile's first token; LIST: of its only one
+        const int p_own = first + token_of(A, m0);  // position of the tile's first token (LIST: its only one)
         const bool one_token = token_of(A, m0) == token_of(A, m0 + mrows - 1);
         const int32_t* list = nullptr;
         if constexpr (LIST) {
@@ -690,10 +692,13 @@ __global__ void __launch_bounds__(SP_THREADS, split_ctas<CT, HD, NQ, LIST>()) k_
             mx[n][0] = mx[n][1] = -INFINITY;
             sum[n][0] = sum[n][1] = 0.0f;
         }
-        // Planned forms: the maximum stays until a score passes it by 2^TAU, so that the
-        // outputs are rarely scaled (a tile in three raises one of its rows' maxima
-        // by a little); a weight is at most 2^(BIAS + TAU), one of 2^-25 of the largest
-        // still has 11 bits.
+        // Planned forms (4 bits, and lists over every pool): the maximum stays until a score
+        // passes it by 2^TAU, so that the outputs are rarely scaled (a tile in three raises
+        // one of its rows' maxima by a little); a weight is at most 2^(BIAS + TAU), one of
+        // 2^-25 of the largest still has 11 bits (2^-28 in the dense form over FP16), a smaller
+        // one is off by 2^-36 of the largest at most.  Their exponential is the special
+        // function alone (2^-22 of the weight at most, as much as the two-part products
+        // leave; weights below 2^-126 are zeros), over FP32 pages too.
         constexpr float BIAS = PLAN && C16 ? 11.0f : C16 ? 14.0f : 0.0f, TAU = PLAN ? 4.0f : 0.0f;
         const int mi = lane >> 3;
         // ldmatrix rows: K as A (keys x d), V transposed as A (d x keys)

@@ -104,7 +104,10 @@ class PagedKV4:
     k_scales and v_scales [n_pages, n_kv_heads, page_size, slots] float16 with 2, 4
     or 8 slots for heads of up to 64, 128 or 256 elements, the first head_dim / 32 in
     use.  The last dimensions are contiguous and begin on multiples of 16 bytes
-    (codes) and of their slots (scales); head_dim is a multiple of 32."""
+    (codes) and of their slots (scales); head_dim is a multiple of 32.
+
+    attention() of chunks takes a workspace for the float16 values of their
+    sequences' tables: as many sequences as fit 1 GiB, one at least."""
 
     __slots__ = ("_pools", "struct", "ref", "device", "index", "n_kv_heads", "head_dim", "page_size", "n_pages")
 

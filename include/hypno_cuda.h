@@ -359,8 +359,8 @@ int hc_paged_append_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, cons
  * j > p - window), holes left out; a row that sees nothing gives zeros.  Query
  * head h reads KV head h / (n_heads / n_kv_heads).  The softmax is the exact
  * exponential's (the flat-cache forward passes keep the reference's
- * polynomial).  Scores and sums are f32.  With FP16 queries over an FP16 cache
- * the weights are rounded to 11 bits for their product with V, which adds about
+ * polynomial).  Scores and sums are f32.  With FP16 queries over an FP16 or 4-bit
+ * cache the weights are rounded to 11 bits for their product with V, which adds about
  * as much error as the rounding of an FP16 output does, at most; FP32 queries
  * or caches keep 22 bits.  What a row does not see cannot reach it, whatever it
  * holds; a row that sees a key or value that is not finite may be NaN where the
@@ -368,8 +368,9 @@ int hc_paged_append_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, cons
  * log of each row's sum of exponentials, [n_rows][n_heads], -inf for a row
  * that sees nothing.  The call needs hc_paged_attention_workspace bytes of
  * device memory (16-byte aligned; contents do not matter, and calls on
- * different streams need one each).  Stream-ordered, no synchronization.
- * head_dim <= 256. */
+ * different streams need one each).  Chunks over a cache in 4 bits take the float16
+ * values of their sequences' tables there, as many sequences as fit 1 GiB, one at
+ * least.  Stream-ordered, no synchronization.  head_dim <= 256. */
 int hc_paged_attention_workspace(const hc_paged_kv* kv, const hc_paged_batch* batch, int n_heads, uint32_t dtype,
                                  int window, size_t* bytes);
 int hc_paged_attention_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_rows* q, const hc_rows* out,
@@ -393,7 +394,8 @@ typedef struct hc_page_lists {
     int32_t reserved;
 } hc_page_lists;
 
-/* hc_paged_attention_dev over the positions of the listed pages alone. */
+/* hc_paged_attention_dev over the positions of the listed pages alone.  With FP16
+ * queries over an FP16 or 4-bit cache the weights are rounded to 11 bits, too. */
 int hc_paged_list_attention_workspace(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_page_lists* lists,
                                       int n_heads, uint32_t dtype, int window, size_t* bytes);
 int hc_paged_list_attention_dev(const hc_paged_kv* kv, const hc_paged_batch* batch, const hc_page_lists* lists,
