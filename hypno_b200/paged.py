@@ -400,12 +400,13 @@ def select_pages(bounds, batch, q, budget, first=1, recent=2, out=None):
     """The pages that each row is to read, per KV head, as attention() takes them:
     an [n_rows, n_kv_heads, budget] int32 tensor (out, if given).  Of the pages that
     hold positions up to the row's own, all if they are `budget` or fewer; else the
-    first `first`, the last `recent`, and of the others those with the largest
-    scores, the lower index first among equals; by index, -1 behind the last.  A
-    page's score is the largest, over the group's query heads, of
+    first `first`, the last `recent` (`budget` together, at most), and of the others
+    those with the largest scores, the lower index first among equals; by index, -1
+    behind the last.  A page's score is the largest, over the group's query heads, of
     t sum_d max(c_d lo_d, c_d hi_d) s, with c = round(q / t) and t the least power of
     two of which the head's largest |q| is at most 127: a bound of the scores of the
-    page's keys, but for the rounding of q.  Scores are exact, so the choice depends
+    page's keys, but for the rounding of q; a page of infinite scale comes before all
+    others, a hole behind them.  Scores are exact, so the choice depends
     on no order of additions.  q is as attention() takes it."""
     if _lib.current_device() != bounds.index:
         with _lib.on_device(bounds.index):
